@@ -230,6 +230,50 @@ int kf_argmax(kf_ctx* ctx, int32_t* out_tokens_dev, const void* logits_bf16_dev,
 int kf_sample(kf_ctx* ctx, int32_t* out_tokens_dev, const void* logits_bf16_dev, int M, int vocab, float temperature, int top_k, float top_p,
               uint64_t* rng_state_dev, int selection);
 
+/* ---- a cache in pages, and steps that mix sequences with any number of new tokens (paged_append.cu, attn_paged.cu, attn_paged_tc.cu; no reference
+ *      equivalents: the reference keeps one contiguous cache and feeds a prompt token by token).
+ *      The step's tokens lie one after the other in the rows of a panel: sequence s has rows q_start[s] .. q_start[s + 1] - 1 and, these included, len[s]
+ *      positions; its last row is position len[s] - 1.  Position p lies in row p % page_size of page table[s][p / page_size].  Everything per sequence is
+ *      read on the device, so a captured step serves other lengths, tables and mixtures of the same panel.
+ *      A table entry outside 0 .. n_pages - 1 is a page that is not there (given back behind a window, say): nothing is written to it, and no query sees its
+ *      positions.  Entries behind a sequence's last position are not read.  Pages may be shared by sequences as long as no new token falls into them.
+ *      Rows outside q_start[0] .. q_start[n_seq] - 1 are padding: not read, and left as they are in every output. ---- */
+typedef struct kf_paged_kv {
+    void* k_dev;            /* bf16 [n_pages][page_size][n_kv][head_dim], 16-byte aligned */
+    void* v_dev;
+    size_t page_stride;     /* elements from one page to the next, a multiple of 8 (0: pages are dense); K and V side by side in one pool: twice a page's */
+    int n_pages, page_size; /* page_size: a multiple of 8 */
+    int n_kv, head_dim;     /* head_dim 64 or 128 */
+    const int32_t* table_dev; /* [n_seq][table_cols] */
+    int table_cols;
+    int n_seq;              /* up to 8192 */
+    const int32_t* q_start_dev; /* [n_seq + 1], not decreasing */
+    const int32_t* len_dev; /* [n_seq], at most table_cols * page_size (more is cut) */
+} kf_paged_kv;
+/* Rotation of the first rot_dims entries of a head: pair j turns by t = pos[axis[j]][row] * inv_freq[j], (a, b) -> amp * (a cos t - b sin t, b cos t + a sin t).
+ * layout 0: pairs (2j, 2j + 1); 1: (j, j + rot_dims / 2).  Angles are formed and reduced in 64 bits. */
+typedef struct kf_rotation {
+    const double* inv_freq_dev; /* [rot_dims / 2] */
+    int rot_dims, layout;       /* rot_dims even, 0: no rotation */
+    float amp;
+    int n_axes;                 /* position axes (time, height, width), 1 .. 8 */
+    const int32_t* axis_dev;    /* [rot_dims / 2] axis of every pair, NULL: axis 0; a pair whose axis is outside 0 .. n_axes - 1 does not turn */
+    const int32_t* pos_dev;     /* [n_axes][pos_stride] positions by row of the panel */
+    size_t pos_stride;          /* 0: as many as the panel has rows */
+} kf_rotation;
+/* New tokens into their pages: q and k get an RMS norm per head (weights bf16 [head_dim], NULL: none) and the rotation (rot NULL: none; rot->pos_dev NULL: the
+ * position in the sequence on every axis), k and v go to the sequence's pages as bf16, the finished q to q_out (bf16 [M][ldqo]; q itself when the panel is bf16).
+ * All in fp32 with one rounding at the end.  q [M][n_head * head_dim], k and v [M][n_kv * head_dim], bf16 or (src_f32) float, rows ldq / ldk / ldv elements apart.
+ * A token whose page is not there or whose position is outside the table keeps its finished q only. */
+int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, void* q_out_dev, int ldqo, const void* q_dev, int ldq, const void* k_dev, int ldk,
+                    const void* v_dev, int ldv, int src_f32, int M, int n_head, const void* qnorm_w_dev, const void* knorm_w_dev, float eps);
+/* Causal attention of the panel's rows over the pages: a row at position p sees the positions j <= p of its sequence, with window > 0 only j > p - window.
+ * out [M][ldo], q [M][ldq] bf16, n_head * head_dim entries a row; softmax(scale * q . k) in fp32.  A row that sees nothing gets zeros.  n_head / n_kv at most 64;
+ * q 16-byte aligned, ldq a multiple of 8.  max_q: the largest number of new tokens of a sequence, as a hint: it chooses the kernels, results do not depend on it. */
+int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int max_q);
+/* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x. */
+int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out_dev, int ldo, const void* x_dev, int ldx, int f32, int M, int n_head, int head_dim);
+
 /* ---- tensor parallel: no reference equivalent (multi_gpu.cuh is dead code).  One process per GPU;
  *      the unique id is exchanged by the caller (torch.distributed / MPI) ---- */
 int kf_nccl_unique_id(void* id_out_128_bytes);

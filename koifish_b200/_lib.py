@@ -41,6 +41,16 @@ class DytStep(C.Structure):
                 ("plane", C.c_size_t), ("tail", C.c_void_p), ("tail_stride", C.c_size_t), ("pos", C.c_void_p), ("slot", C.c_void_p)]
 
 
+class PagedKVDesc(C.Structure):
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("page_stride", C.c_size_t), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv", C.c_int),
+                ("head_dim", C.c_int), ("table_dev", C.c_void_p), ("table_cols", C.c_int), ("n_seq", C.c_int), ("q_start_dev", C.c_void_p), ("len_dev", C.c_void_p)]
+
+
+class RotationDesc(C.Structure):
+    _fields_ = [("inv_freq_dev", C.c_void_p), ("rot_dims", C.c_int), ("layout", C.c_int), ("amp", C.c_float), ("n_axes", C.c_int), ("axis_dev", C.c_void_p),
+                ("pos_dev", C.c_void_p), ("pos_stride", C.c_size_t)]
+
+
 # every symbol include/*.h declares, with its signature: (restype, [argtypes])
 _P, _I, _SZ, _U64, _F = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_float
 _DESCP = C.POINTER(TensorDesc)
@@ -167,6 +177,9 @@ SIGNATURES = {
     "kf_linear_batch": (_I, [_P, _I, C.POINTER(_P), _DESCP, C.POINTER(_P), C.POINTER(_I), _I, _I, _I]),
     "kf_wkv_scan": (_I, [_P, _P, _I, _P, _I, _P, _I, _P, _I, _P, _I, _P, _P, _P, _SZ, _P, _P, _I, _I, _I, _I, _I]),
     "kf_qk_heads_prepare_ex": (_I, [_P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _F, _I, _P, _F, _I, _P, _I, _P, _P, _I, _SZ, _I, _I, _I, _P, _P, _P, _I]),
+    "kf_paged_append": (_I, [_P, C.POINTER(PagedKVDesc), C.POINTER(RotationDesc), _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _F]),
+    "kf_paged_attention": (_I, [_P, C.POINTER(PagedKVDesc), _P, _I, _P, _I, _I, _I, _F, _I, _I]),
+    "kf_rope_axes": (_I, [_P, C.POINTER(RotationDesc), _P, _I, _P, _I, _I, _I, _I, _I]),
     "kf_nccl_unique_id": (_I, [_P]),
     "kf_ctx_init_nccl": (_I, [_P, _P, _I, _I]),
     "kf_allreduce_bf16": (_I, [_P, _P, _SZ]),

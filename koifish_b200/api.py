@@ -314,6 +314,55 @@ def qkv_attention(ctx, q, k, v, qw, kw, kcache, vcache, table, pos, M, n_head, n
     return out
 
 
+class PagedKV:
+    """A layer's keys and values in pages and the step over them (kf_paged_kv); keeps what it was given alive."""
+
+    def __init__(self, k, v, n_pages, page_size, n_kv, head_dim, table, table_cols, n_seq, q_start, lens, page_stride=0):
+        self.keep = (k, v, table, q_start, lens)
+        self.n_kv, self.head_dim = n_kv, head_dim
+        self.desc = L.PagedKVDesc(k.ptr, v.ptr, page_stride, n_pages, page_size, n_kv, head_dim, table.ptr, table_cols, n_seq, q_start.ptr, lens.ptr)
+        self.ref = C.byref(self.desc)
+
+
+class Rotation:
+    """Frequencies, axes and positions of a rotation (kf_rotation)."""
+
+    def __init__(self, inv_freq, rot_dims, layout=1, amp=1.0, n_axes=1, pair_axis=None, pos=None, pos_stride=0):
+        self.keep = (inv_freq, pair_axis, pos)
+        self.desc = L.RotationDesc(inv_freq.ptr if inv_freq is not None else None, rot_dims, layout, amp, n_axes, pair_axis.ptr if pair_axis is not None else None,
+                                   pos.ptr if pos is not None else None, pos_stride)
+        self.ref = C.byref(self.desc)
+
+
+def paged_append(ctx, kv, rot, q, k, v, M, n_head, q_norm=None, k_norm=None, eps=1e-6, ldq=0, ldk=0, ldv=0, out=None, ldo=0, src_f32=False):
+    """a step's keys and values into the pages of their sequences, norm and rotation on the way; returns the finished queries"""
+    wide, kvw = n_head * kv.head_dim, kv.n_kv * kv.head_dim
+    if out is None:
+        out = ctx.empty(M * (ldo or wide) * 2)
+    ctx.check(ctx.lib.kf_paged_append(ctx.h, kv.ref, rot.ref if rot is not None else None, out.ptr, ldo or wide, q.ptr, ldq or wide, k.ptr, ldk or kvw, v.ptr, ldv or kvw,
+                                      int(src_f32), M, n_head, q_norm.ptr if q_norm is not None else None, k_norm.ptr if k_norm is not None else None, eps), "kf_paged_append")
+    return out
+
+
+def paged_attention(ctx, kv, q, M, n_head, max_q, scale=None, window=0, ldq=0, out=None, ldo=0):
+    """causal attention of a step's rows (one token, a few or a chunk for each sequence) over the pages; max_q is a hint"""
+    wide = n_head * kv.head_dim
+    if out is None:
+        out = ctx.empty(M * (ldo or wide) * 2)
+    ctx.check(ctx.lib.kf_paged_attention(ctx.h, kv.ref, out.ptr, ldo or wide, q.ptr, ldq or wide, M, n_head, kv.head_dim ** -0.5 if scale is None else scale, window, max_q),
+              "kf_paged_attention")
+    return out
+
+
+def rope_axes(ctx, rot, x, M, n_head, head_dim, ldx=0, out=None, ldo=0, f32=False):
+    """the heads of a panel rotated by positions with one or several axes; out may be x"""
+    wide = n_head * head_dim
+    if out is None:
+        out = ctx.empty(M * (ldo or wide) * (4 if f32 else 2))
+    ctx.check(ctx.lib.kf_rope_axes(ctx.h, rot.ref, out.ptr, ldo or (ldx if out is x and ldx else wide), x.ptr, ldx or wide, int(f32), M, n_head, head_dim), "kf_rope_axes")
+    return out
+
+
 def swiglu(ctx, g, u, n):
     out = ctx.empty(n * 2)
     ctx.check(ctx.lib.kf_swiglu(ctx.h, out.ptr, g.ptr, u.ptr, n), "kf_swiglu")

@@ -1,0 +1,420 @@
+// attn_paged.cu -- attention of a step's rows over a cache in pages (kf_paged_attention): the kernel for sequences with up to 16 rows (new tokens x heads of a kv group),
+// and the choice between it and the one for more (attn_paged_tc.cu).
+//
+//   out = sum_j w_j v_j / sum_j w_j,  w_j = 2^(c q.k_j - m),  c = scale * log2(e),  m the largest c q.k_j so far, over the positions j that the row sees
+//
+// Every cached row is read once per kv head for all rows of a block, so the bytes of the cache bound it; what matters is how many of them are on their way and that no SM
+// runs dry.
+//   * A team of n_kv CTAs takes a run of tiles of 64 positions, a kv head each, so that the rows of a position, which lie side by side, are read at about the same time.
+//     The runs are equal whatever the sequences' lengths are (PagedWalk).
+//   * One warp looks the pages up and loads tiles of K and V by TMA into a ring of stages; a tile is as many boxes as pages (or parts of 8, 16, 32 or 64 positions of
+//     them) meet in it, each asked for by a lane of its own.  Boxes of pages that are not there are out of the tensor map's range and arrive as zeros.
+//   * Four computing warps take a tile, 16 positions each; scores and P V on mma.sync with the block's rows as the 16 rows of the A operand.
+//   * The piece that arrives last at its block merges all of them in order.
+// Values behind a block's last position or before its window need not be numbers: their rows of V are zeroed in shared memory.
+#include <algorithm>
+
+#include "kf_paged.cuh"
+#include "kf_tc.cuh"
+
+namespace {
+constexpr int kTok = 64;
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(tm), "r"(c0),
+                 "r"(c1), "r"(c2), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void put4(uint16_t* p, float4 v, bool vec) {
+    if (vec) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    else p[0] = f32_to_bf16_bits(v.x), p[1] = f32_to_bf16_bits(v.y), p[2] = f32_to_bf16_bits(v.z), p[3] = f32_to_bf16_bits(v.w);
+}
+
+// Shared memory: a ring of stages (K and V tiles in turn) and the computing warps' sums.  SETS 1: two CTAs per SM.  A stage always comes back to the same warps, which
+// wait for each of its uses; with SETS 2, whose tiles alternate, that needs a number of stages that is a multiple of 4 (a wait tells a phase of a barrier from the one
+// before by one bit), and pieces begin behind a meeting of all warps.
+constexpr int rows_area(int hd, int sets, int rb) { return 4 * sets * rb * hd * 4; }
+constexpr int ring_stages(int hd, int sets, int rb) {
+    const int fit = ((sets == 1 ? 108 : 216) * 1024 - rows_area(hd, sets, rb)) / (kTok * hd * 2), most = fit < 10 * sets ? fit : 10 * sets;
+    return sets == 1 ? most & ~1 : most & ~3;
+}
+constexpr bool rings_fit() {
+    for (int hd = 64; hd <= 128; hd += 64)
+        for (int sets = 1; sets <= 2; sets++)
+            for (int rb = 1; rb <= 16; rb++)
+                if (ring_stages(hd, sets, rb) < 4 * sets) return false;
+    return true;
+}
+static_assert(rings_fit(), "two tiles of every set in flight");
+
+template <int HD, int SETS>
+__global__ void __launch_bounds__((4 * SETS + 1) * 32, 3 - SETS)
+    kf_attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, uint16_t* out, float* ws, float2* ws_ml, unsigned* cnt, const uint16_t* q,
+                         const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, long long ldo, long long ldq, int n_kv, int min_run, int box /* positions */, int stages,
+                         float sc2 /* scale * log2(e) */, const __grid_constant__ KfBound bound) {
+    constexpr int HALVES = HD / 64, TILE = kTok * HD * 2, HALF = kTok * 128;  // a tile lies as halves of 64 dims: 64 rows of 128 bytes (SWIZZLE_128B)
+    constexpr int kWarps = 4 * SETS, kComp = kWarps * 32, kMaxStages = 20;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    float* s_o    = reinterpret_cast<float*>(ring + (size_t)stages * TILE);  // [kWarps][rb][HD]
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], meet_bar;
+    __shared__ volatile int dead;
+    __shared__ int s_there[kMaxStages], s_last;  // bit i: positions 8 i .. 8 i + 7 of the stage's K tile are there
+    __shared__ long long s_sum[256];
+    __shared__ float s_m[kWarps][16], s_l[kWarps][16], s_M[16], s_i[16];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    if (tid == 0) {
+        for (int s = 0; s < stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 4);
+        mbar_init(&meet_bar, kWarps);
+        dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    kf_grid_launch_dependents();
+    kf_grid_dependency_wait();  // queries, the new positions' rows, lengths and tables, workspace
+    const KfPaged pg = behind_wait(pg_);
+    q                = behind_wait(q);
+    PagedWalk<kTok> walk(pg, pl, lane);
+    const long long W = walk.count(s_sum, warp, kWarps + 1);
+    __syncthreads();
+    const int teams = (int)gridDim.x / n_kv, team = (int)blockIdx.x / n_kv, kvh = (int)blockIdx.x % n_kv;
+    const long long run = max((long long)min_run, (W + teams - 1) / teams), u0 = team * run, u1 = min(W, u0 + run);
+    if (u0 >= u1) return;
+    walk.seek(s_sum, u0);
+    uint32_t st = 0, ph = 0;  // ring position and its phase
+    if (warp == kWarps) {
+        if (bound.drop == (int)blockIdx.x + 1) return;
+        bool live = true;
+        uint32_t asked = 0;
+        const int n_box = kTok / box, bx = lane / HALVES, hf = lane % HALVES;  // a lane per box and half; bx >= n_box: none
+        for (long long u = u0; live && u < u1;) {
+            const PagedPiece pc = walk.at(u, u1);
+            u += pc.t1 - pc.t0;
+            auto page_of = [&](int t) {  // the page of this lane's box of tile t
+                const int p = t * kTok + bx * box;
+                return t < pc.t1 && bx < n_box && p < pc.hi && p + box > pc.lo ? paged_page(pg, pc.s, p) : -1;
+            };
+            int next = page_of(pc.t0);
+            for (int t = pc.t0; live && t < pc.t1; t++) {
+                const int page = next, row = (t * kTok + bx * box) % pg.page;
+                next = page_of(t + 1);  // a tile ahead: the look-up takes as long as a tile
+                const unsigned lanes = __ballot_sync(0xffffffffu, page >= 0);
+                for (int kv = 0; kv < 2; kv++) {
+                    if (!(live = mbar_wait_warp(smem_u32(&empty[st]), ph ^ 1, &dead, bound))) break;
+                    if (lane == 0) {
+                        unsigned there = 0;
+                        for (int i = 0; i < kTok / 8; i++) there |= (lanes >> (i * 8 / box * HALVES) & 1) << i;
+                        s_there[st] = (int)there;
+                        mbar_arrive_expect_tx(&full[st], TILE);
+                    }
+                    __syncwarp();
+                    if (bx < n_box)
+                        tma_load_3d(ring + (size_t)st * TILE + hf * HALF + bx * box * 128, kv ? &tm_v : &tm_k, kvh * HD + hf * 64, page >= 0 ? row : 0, page >= 0 ? page : pg.n_pages,
+                                    &full[st]);
+                    __syncwarp();
+                    asked++;
+                    if (++st == (uint32_t)stages) st = 0, ph ^= 1;
+                }
+            }
+        }
+        if (!live)  // copies in flight write shared memory
+            for (uint32_t k = asked > (uint32_t)stages ? asked - stages : 0; k < asked; k++) mbar_drain(smem_u32(&full[k % stages]), (k / stages) & 1, bound);
+        return;
+    }
+    const int set = warp >> 2, w4 = warp & 3, group = pl.group, rb = pl.rb;
+    const bool vec = ((uintptr_t)out & 7) == 0 && ldo % 4 == 0;
+    uint32_t mph = 0, done = 0;  // done: tiles of this CTA before the current piece
+    bool live = true;
+    auto meet = [&]() {  // all computing warps; bounded like every wait
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&meet_bar);
+        live = mbar_wait_warp(smem_u32(&meet_bar), mph, &dead, bound) && live;
+        mph ^= 1;
+    };
+    // 16-byte chunk c (0 .. HD / 8 - 1) of a row: half c / 8, chunk c % 8 swizzled by the row
+    auto at = [](uint32_t base, int row, int c) { return base + (uint32_t)((c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)); };
+    for (long long u = u0; live && u < u1;) {
+        const PagedPiece pc = walk.at(u, u1);
+        u += pc.t1 - pc.t0;
+        const int ntiles = pc.t1 - pc.t0, rows = (int)min((long long)rb, (long long)pc.n * group - (long long)pc.b * rb);
+        // the block's queries as A fragments (rows past its end are zero), and what its rows see: positions above `low` up to `lim`
+        uint32_t qa[HD / 16][4];
+        int lim[2], low[2];
+        const uint32_t* qp[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = pc.b * rb + g + 8 * e, tok = r / group;
+            lim[e] = min(pc.len - pc.n + tok, pg.cap - 1), low[e] = pl.window > 0 ? pc.len - pc.n + tok - pl.window : -1;
+            qp[e]  = reinterpret_cast<const uint32_t*>(q + (pc.q0 + tok) * ldq + (long long)(kvh * group + r % group) * HD);
+        }
+#pragma unroll
+        for (int kc = 0; kc < HD / 16; kc++) {
+            qa[kc][0] = g < rows ? qp[0][kc * 8 + t4] : 0u, qa[kc][2] = g < rows ? qp[0][kc * 8 + t4 + 4] : 0u;
+            qa[kc][1] = g + 8 < rows ? qp[1][kc * 8 + t4] : 0u, qa[kc][3] = g + 8 < rows ? qp[1][kc * 8 + t4 + 4] : 0u;
+        }
+        // positions that all rows see: below the first row's, above the last row's window
+        const int sure_hi = min(pc.len - pc.n + pc.b * rb / group + 1, pg.cap), sure_lo = pl.window > 0 ? pc.len - pc.n + (pc.b * rb + rows - 1) / group - pl.window + 1 : 0;
+        float o[HD / 8][4];
+#pragma unroll
+        for (int j = 0; j < HD / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
+        for (int kt = set; kt < ntiles; kt += SETS) {
+            const uint32_t n = 2 * (done + kt);
+            const uint32_t sk = n % stages, pk = (n / stages) & 1, sv = (n + 1) % stages, pv = ((n + 1) / stages) & 1;
+            if (!(live = mbar_wait_warp(smem_u32(&full[sk]), pk, &dead, bound))) break;
+            const uint32_t kb = smem_u32(ring + (size_t)sk * TILE), vb = smem_u32(ring + (size_t)sv * TILE);
+            const int tok0 = (pc.t0 + kt) * kTok + w4 * 16;  // this warp's 16 positions
+            const unsigned there = ((unsigned)*(volatile int*)&s_there[sk] >> (w4 * 2)) & 3u;
+            const bool mine = tok0 < pc.hi && tok0 + 16 > pc.lo && there;
+            float sc[2][4];
+#pragma unroll
+            for (int j = 0; j < 2; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+            if (mine) {
+#pragma unroll
+                for (int kc = 0; kc < HD / 16; kc++) {
+                    uint32_t b[4];
+                    ldsm4(b, at(kb, w4 * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
+                    mma16816(sc[0], qa[kc], b[0], b[1]);
+                    mma16816(sc[1], qa[kc], b[2], b[3]);
+                }
+            }
+            // a stage goes back when every ldmatrix of it has delivered: the matrix instructions behind them were issued with its registers
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[sk]);
+            if (!(live = mbar_wait_warp(smem_u32(&full[sv]), pv, &dead, bound))) break;
+            if (mine) {
+                if (tok0 + 16 > sure_hi || tok0 < sure_lo || there != 3u) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int p = tok0 + j * 8 + 2 * t4 + (e & 1);
+                            if (p > lim[e >> 1] || p <= low[e >> 1] || !(there >> j & 1)) sc[j][e] = -INFINITY;
+                        }
+                }
+                if (tok0 + 16 > pc.hi || tok0 < pc.lo) {  // positions that no row sees: no value that might not be a number
+                    for (int c = lane; c < 16 * (HD / 8); c += 32) {
+                        const int r = c / (HD / 8), ch = c % (HD / 8), row = w4 * 16 + r;
+                        if (tok0 + r >= pc.hi || tok0 + r < pc.lo)
+                            *reinterpret_cast<uint4*>(ring + (size_t)sv * TILE + (ch >> 3) * HALF + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    // the stage is refilled by the asynchronous proxy later: these writes come before that
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                float mx_lo = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])), mx_hi = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+                mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, 1)), mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, 2));
+                mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 1)), mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 2));
+                const float mn_lo = fmaxf(m_lo, mx_lo * sc2), mn_hi = fmaxf(m_hi, mx_hi * sc2);
+                // where all scores so far are -inf their weights are 0
+                const float b_lo = mn_lo == -INFINITY ? 0.f : mn_lo, b_hi = mn_hi == -INFINITY ? 0.f : mn_hi;
+                const float c_lo = exp2f(m_lo - b_lo), c_hi = exp2f(m_hi - b_hi);
+                m_lo = mn_lo, m_hi = mn_hi;
+                float rs_lo = 0.f, rs_hi = 0.f;
+                uint32_t pa[4];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float p0 = exp2f(fmaf(sc[j][0], sc2, -b_lo)), p1 = exp2f(fmaf(sc[j][1], sc2, -b_lo));
+                    const float p2 = exp2f(fmaf(sc[j][2], sc2, -b_hi)), p3 = exp2f(fmaf(sc[j][3], sc2, -b_hi));
+                    rs_lo += p0 + p1, rs_hi += p2 + p3;
+                    pa[j * 2 + 0] = pack_bf16x2(p0, p1), pa[j * 2 + 1] = pack_bf16x2(p2, p3);
+                }
+                l_lo = l_lo * c_lo + rs_lo, l_hi = l_hi * c_hi + rs_hi;
+                if (__any_sync(0xffffffffu, c_lo != 1.f || c_hi != 1.f)) {
+#pragma unroll
+                    for (int j = 0; j < HD / 8; j++) o[j][0] *= c_lo, o[j][1] *= c_lo, o[j][2] *= c_hi, o[j][3] *= c_hi;
+                }
+#pragma unroll
+                for (int jp = 0; jp < HD / 16; jp++) {
+                    uint32_t b[4];
+                    ldsm4_t(b, at(vb, w4 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, jp * 2 + (lane >> 4)));
+                    mma16816(o[2 * jp], pa, b[0], b[1]);
+                    mma16816(o[2 * jp + 1], pa, b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[sv]);
+        }
+        done += (uint32_t)ntiles;
+        if (!live) break;
+        // ---- merge the warps (fixed order) through shared memory ----
+        l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 1), l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 2);
+        l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 1), l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 2);
+#pragma unroll
+        for (int j = 0; j < HD / 8; j++) {
+            float* r0 = s_o + ((size_t)warp * rb + g) * HD + j * 8 + 2 * t4;
+            if (g < rows) *reinterpret_cast<float2*>(r0) = make_float2(o[j][0], o[j][1]);
+            if (g + 8 < rows) *reinterpret_cast<float2*>(r0 + 8 * HD) = make_float2(o[j][2], o[j][3]);
+        }
+        if (t4 == 0) s_m[warp][g] = m_lo, s_m[warp][g + 8] = m_hi, s_l[warp][g] = l_lo, s_l[warp][g + 8] = l_hi;
+        meet();
+        if (!live) break;
+        const bool whole = ntiles == pc.tiles;
+        auto out_row = [&](int r) {
+            const int R = pc.b * rb + r;
+            return out + (pc.q0 + R / group) * ldo + (long long)(kvh * group + R % group) * HD;
+        };
+        // partial sums: a CTA has at most one piece that others have begun (slot 0) and one that others go on with (slot 1)
+        const int first = (int)(pc.u / run), last = (int)((pc.u + pc.tiles - 1) / run);  // teams
+        const size_t slot = (size_t)blockIdx.x * 2 + (first == team);
+        for (int idx = tid; idx < rows * (HD / 4); idx += kComp) {
+            const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
+            float M_ = -INFINITY, L_ = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) M_ = fmaxf(M_, s_m[w][r]);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float f  = s_m[w][r] == -INFINITY ? 0.f : exp2f(s_m[w][r] - M_);
+                const float4 v = *reinterpret_cast<const float4*>(s_o + ((size_t)w * rb + r) * HD + c);
+                L_ += s_l[w][r] * f;
+                a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+            }
+            if (whole) {
+                const float i = L_ == 0.f ? 0.f : 1.f / L_;
+                put4(out_row(r) + c, make_float4(a.x * i, a.y * i, a.z * i, a.w * i), vec);
+            } else {
+                __stcg(reinterpret_cast<float4*>(ws + (slot * rb + r) * HD + c), a);
+                if (c == 0) __stcg(ws_ml + slot * rb + r, make_float2(M_, L_));
+            }
+        }
+        if (!whole) {
+            // ---- the piece that arrives last at its block merges all of them in order ----
+            const int pieces = last - first + 1;
+            auto slot_of = [&](int i) { return ((size_t)(first + i) * n_kv + kvh) * 2 + (i == 0); };
+            __threadfence();
+            meet();
+            if (live && tid == 0) {
+                unsigned* c = cnt + (size_t)first * n_kv + kvh;
+                s_last      = atomicAdd(c, 1u) == (unsigned)(pieces - 1);
+                if (s_last) *c = 0u;  // self-reset for the next launch
+            }
+            meet();
+            if (live && s_last) {
+                __threadfence();
+                for (int r = warp; r < rows; r += kWarps) {
+                    float M_ = -INFINITY, L_ = 0.f;
+                    for (int i = lane; i < pieces; i += 32) M_ = fmaxf(M_, __ldcg(ws_ml + slot_of(i) * rb + r).x);
+                    M_ = warp_max(M_);
+                    if (M_ != -INFINITY)
+                        for (int i = lane; i < pieces; i += 32) {
+                            const float2 ml = __ldcg(ws_ml + slot_of(i) * rb + r);
+                            L_ += ml.y * exp2f(ml.x - M_);
+                        }
+                    L_ = warp_sum(L_);
+                    if (lane == 0) s_M[r] = M_, s_i[r] = L_ == 0.f ? 0.f : 1.f / L_;
+                }
+                meet();
+                // a slice of HD / 4 threads adds every kSlices-th piece of a row, then the slices are added
+                constexpr int VEC = HD / 4, kSlices = kComp / VEC;
+                static_assert(kSlices <= 2 * kWarps, "slices fit the warps' area for half the rows at a time");
+                const int slice = tid / VEC, c = tid % VEC * 4, per = HD == 128 ? rb : (rb + 1) / 2;  // rows at a time
+                for (int r0 = 0; live && r0 < rows; r0 += per) {
+                    for (int r = r0; r < min(rows, r0 + per); r++) {
+                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float M_ = s_M[r];
+#pragma unroll 8
+                        for (int i = slice; i < pieces; i += kSlices) {
+                            const size_t row = slot_of(i) * rb + r;
+                            const float4 v   = __ldcg(reinterpret_cast<const float4*>(ws + row * HD + c));
+                            const float m    = __ldcg(ws_ml + row).x, f = m == -INFINITY ? 0.f : exp2f(m - M_);
+                            a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+                        }
+                        *reinterpret_cast<float4*>(s_o + ((size_t)slice * per + (r - r0)) * HD + c) = a;
+                    }
+                    meet();
+                    for (int idx = tid; live && idx < min(per, rows - r0) * VEC; idx += kComp) {
+                        const int r = idx / VEC, d = idx % VEC * 4;
+                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int sl = 0; sl < kSlices; sl++) {
+                            const float4 v = *reinterpret_cast<const float4*>(s_o + ((size_t)sl * per + r) * HD + d);
+                            a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+                        }
+                        const float i = s_i[r0 + r];
+                        put4(out_row(r0 + r) + d, make_float4(a.x * i, a.y * i, a.z * i, a.w * i), vec);
+                    }
+                    meet();
+                }
+            }
+        }
+        meet();  // the area belongs to the next piece
+    }
+}
+
+// positions of a box: the largest power of two that divides a page, at most `most`
+int box_of(int page, int most) {
+    int b = 8;
+    while (b < most && page % (2 * b) == 0) b *= 2;
+    return b;
+}
+
+template <int HD, int SETS>
+int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, const PagedPlan& pl, void* out, long long ldo, const void* q, long long ldq, float scale) {
+    const int n_kv = kv->n_kv, teams = std::max(1, (3 - SETS) * ctx->sm_count / n_kv), grid = teams * n_kv, box = box_of(kv->page_size, kTok);
+    const size_t rows = (size_t)grid * 2 * pl.rb;
+    int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
+    if (!rc) rc = kf_ensure_attn_cnt(ctx, grid);
+    if (rc) return rc;
+    CUtensorMap tk, tv;
+    const uint64_t stride = kf_paged_stride(kv) * 2;
+    rc = kf_tmap_rows(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
+    if (!rc) rc = kf_tmap_rows(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
+    if (rc) return rc;
+    const int stages  = ring_stages(HD, SETS, pl.rb);
+    const size_t smem = (size_t)stages * kTok * HD * 2 + rows_area(HD, SETS, pl.rb) + 1024;
+    auto kern         = kf_attn_paged_kernel<HD, SETS>;
+    static bool set[kf_ctx::kMaxDevices] = {};  // function attributes are per device
+    if (!set[ctx->device]) {
+        KF_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (SETS == 1 ? 109 : 217) * 1024));
+        set[ctx->device] = true;
+    }
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((4 * SETS + 1) * 32), smem, tk, tv, (uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD),
+                               ctx->attn_cnt, (const uint16_t*)q, pg, pl, ldo, ldq, n_kv, 2, box, stages, scale * 1.4426950408889634f,
+                               KfBound{ctx->wait_flags + 1, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+    KF_LAUNCH_CHECK(ctx);
+    return KF_OK;
+}
+}  // namespace
+
+static int check_args(kf_ctx* ctx, const kf_paged_kv* kv, const void* out, int ldo, const void* q, int ldq, int M, int n_head, float scale, int max_q, KfPaged* pg) {
+    if (!kv || !out || !q) return KF_ERR_BAD_ARG;
+    const int rc = kf_paged_check(ctx, kv, M, pg);
+    if (rc) return rc;
+    KF_REQUIRE(ctx, n_head >= 1 && n_head % kv->n_kv == 0 && n_head / kv->n_kv <= 64, "n_head a multiple of n_kv, at most 64 heads to a kv head");
+    KF_REQUIRE(ctx, (long long)n_head * kv->head_dim <= ldq && (long long)n_head * kv->head_dim <= ldo, "rows as long as their heads");
+    KF_REQUIRE(ctx, ((uintptr_t)q & 15) == 0 && ldq % 8 == 0, "q at 16 bytes, ldq a multiple of 8");
+    KF_REQUIRE(ctx, scale > 0.f && scale < INFINITY && max_q >= 0, "scale above 0, max_q not negative");
+    return KF_OK;
+}
+extern "C" int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out, int ldo, const void* q, int ldq, int M, int n_head, float scale, int window, int max_q) {
+    if (!ctx) return KF_ERR_BAD_ARG;
+    KfPaged pg;
+    int rc = check_args(ctx, kv, out, ldo, q, ldq, M, n_head, scale, max_q, &pg);
+    if (!rc) rc = kf_wait_status(ctx);
+    if (rc || M == 0) return rc;
+    const int group = n_head / kv->n_kv;
+    const PagedPlan pl{(int)std::min(16ll, std::max(1ll, (long long)max_q * group)), group, window, 0, 0x7fffffff};
+    const int few = 1;
+    if (kv->head_dim == 128)
+        return few ? launch_few<128, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<128, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
+    return few ? launch_few<64, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<64, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
+}
+// The checks and the blocks' arithmetic for tests on a host without a device
+extern "C" int kf_paged_attention_args(const kf_paged_kv* kv, const void* out, int ldo, const void* q, int ldq, int M, int n_head, float scale, int max_q) {
+    KfPaged pg;
+    return check_args(nullptr, kv, out, ldo, q, ldq, M, n_head, scale, max_q, &pg);
+}
+extern "C" int kf_paged_attention_block(int tile, int cap, int rb, int group, int window, int n, int len, int b, int* lo_hi_first) {
+    return paged_block(tile, cap, PagedPlan{rb, group, window, 0, 0}, n, len, b, lo_hi_first[0], lo_hi_first[1], lo_hi_first[2]);
+}
