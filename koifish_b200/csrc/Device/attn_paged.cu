@@ -20,22 +20,6 @@
 namespace {
 constexpr int kTok = 64;
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, int c0, int c1, int c2, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(tm), "r"(c0),
-                 "r"(c1), "r"(c2), "r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void put4(uint16_t* p, float4 v, bool vec) {
     if (vec) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
     else p[0] = f32_to_bf16_bits(v.x), p[1] = f32_to_bf16_bits(v.y), p[2] = f32_to_bf16_bits(v.z), p[3] = f32_to_bf16_bits(v.w);
@@ -404,11 +388,15 @@ extern "C" int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out,
     if (!rc) rc = kf_wait_status(ctx);
     if (rc || M == 0) return rc;
     const int group = n_head / kv->n_kv;
-    const PagedPlan pl{(int)std::min(16ll, std::max(1ll, (long long)max_q * group)), group, window, 0, 0x7fffffff};
+    const bool many = (long long)max_q * group > 16;
+    const PagedPlan pl{(int)std::min(16ll, std::max(1ll, (long long)max_q * group)), group, window, 0, many ? 16 : 0x7fffffff, 1};
     const int few = 1;
     if (kv->head_dim == 128)
-        return few ? launch_few<128, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<128, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
-    return few ? launch_few<64, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<64, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
+        rc = few ? launch_few<128, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<128, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
+    else
+        rc = few ? launch_few<64, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<64, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
+    if (!rc && many) rc = kf_attn_paged_tc(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, 16);
+    return rc;
 }
 // The checks and the blocks' arithmetic for tests on a host without a device
 extern "C" int kf_paged_attention_args(const kf_paged_kv* kv, const void* out, int ldo, const void* q, int ldq, int M, int n_head, float scale, int max_q) {
@@ -416,5 +404,5 @@ extern "C" int kf_paged_attention_args(const kf_paged_kv* kv, const void* out, i
     return check_args(nullptr, kv, out, ldo, q, ldq, M, n_head, scale, max_q, &pg);
 }
 extern "C" int kf_paged_attention_block(int tile, int cap, int rb, int group, int window, int n, int len, int b, int* lo_hi_first) {
-    return paged_block(tile, cap, PagedPlan{rb, group, window, 0, 0}, n, len, b, lo_hi_first[0], lo_hi_first[1], lo_hi_first[2]);
+    return paged_block(tile, cap, PagedPlan{rb, group, window, 0, 0, 1}, n, len, b, lo_hi_first[0], lo_hi_first[1], lo_hi_first[2]);
 }

@@ -1,0 +1,513 @@
+// attn_paged_tc.cu -- attention of sequences with many rows (chunks of prompts, drafts) over a cache in pages, on tcgen05 / TMEM / TMA.  Formulas: attn_paged.cu.
+//
+// A row tile is 128 rows: as many tokens as fit with all heads of their kv group, so that a tile of K and V serves all of them and few tokens still fill a tile.  A block
+// is two row tiles.  Its visible positions go by in tiles of 128, and the two chains of scores -> weights -> sums fill each other's gaps: while the softmax warps of one turn
+// scores into weights, the tensor cores work for the other.  The chains are the block's two row tiles, which share every tile of K and V -- or, where the block has one
+// row tile only, its even and odd tiles of positions, whose sums meet in shared memory at the end.
+//   warps 0-3 / 4-7  softmax of chain 0 / 1, thread = row: scores from tensor memory, running maximum, weights as bf16 back over the scores of the second half
+//   warp 8           matrix instructions: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory, V as it lies: MN-major)
+//   warp 9 / 10      Q and K / V: page look-up and TMA, a box per page (or part of 8 .. 128 positions of it) and 64 dims, each asked for by a lane of its own
+// The tiles of all blocks and kv heads are cut into equal runs, one CTA each (PagedWalk).  Blocks that several CTAs share leave their sums in the workspace; a second
+// kernel, launched behind, merges them in order.
+// The output is rescaled whenever a maximum of the warp's rows grows, so the largest weight of a row is 1 and has no rounding error; the denominator adds the unrounded
+// weights.  Rows of V that no row of the block sees are zeroed in shared memory, since they need not hold numbers; boxes of pages that are not there arrive as zeros.
+// Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
+#include <algorithm>
+
+#include "kf_paged.cuh"
+#include "kf_tc.cuh"
+
+namespace {
+constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kThreads = 11 * 32, kMasks = 8;
+template <int HD>
+struct Cfg {
+    static constexpr int kHalves = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStages = HD == 128 ? 2 : 4;  // a tile lies as halves of 64 dims, 128 rows of 128 bytes each
+    static constexpr size_t kSmem = (2 + 2 * kStages) * (size_t)kTile + 1024;
+};
+struct TcArgs {  // kernel parameter
+    uint16_t* out;
+    float* ws;      // [CTA][2][256][HD] sums, then as many (maximum, denominator) pairs
+    float2* ws_ml;
+    long long ldo;
+    int tokens, n_kv, min_run, box;  // tokens of a row tile; positions of a box
+    float sc2;                       // scale * log2(e)
+};
+
+// shared-memory descriptor of a V tile: MN-major (64 dims side by side, then the next position's 128-byte row), SWIZZLE_128B; the dims' second half lies 128 rows
+// behind the first (leading byte offset), eight positions 1024 bytes behind the eight before (stride byte offset)
+__device__ __forceinline__ uint64_t make_desc_v(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(kKV * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void store_row(uint16_t* p, const uint32_t (&o)[32], float f, bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = pack_bf16x2(__uint_as_float(o[8 * j + 2 * e]) * f, __uint_as_float(o[8 * j + 2 * e + 1]) * f);
+            *reinterpret_cast<uint4*>(p + 8 * j) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++) p[j] = f32_to_bf16_bits(__uint_as_float(o[j]) * f);
+    }
+}
+// the tiles of a piece as the chains take them
+struct Steps {
+    bool pair;      // two row tiles, which share the tiles; otherwise chain t takes every second one
+    int n, steps;   // tiles, steps
+    __device__ __forceinline__ Steps(const PagedPiece& pc, const PagedPlan& pl, int tokens) {
+        pair  = pc.n - pc.b * (pl.rb / pl.group) > tokens;
+        n     = pc.t1 - pc.t0;
+        steps = pair ? n : (n + 1) / 2;
+    }
+    __device__ __forceinline__ int wide(int j) const { return pair ? 1 : min(2, n - 2 * j); }         // tiles of step j
+    __device__ __forceinline__ bool active(int t, int j) const { return j < steps && (pair || 2 * j + t < n); }
+    __device__ __forceinline__ int of(int t) const { return pair ? n : (n + 1 - t) / 2; }              // steps of chain t
+    __device__ __forceinline__ int tile(int t, int j) const { return pair ? j : 2 * j + t; }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    kf_attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                            const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a, const __grid_constant__ KfBound bound) {
+    using C = Cfg<HD>;
+    constexpr int kTile = C::kTile, kHalf = C::kHalf, kHalves = C::kHalves, kStages = C::kStages;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sk = sq + 2 * kTile;
+    uint8_t* sv = sk + kStages * kTile;
+    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][2], o_done[2], x_full, x_free, x_done, done_bar;
+    __shared__ uint32_t tmem_base_smem;
+    __shared__ volatile int dead;
+    __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
+    __shared__ long long s_sum[256];
+    __shared__ float s_m[kQ], s_l[kQ];  // chain 1's maximum and denominator, where the chains share a row tile
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 8);
+        for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
+        for (int t = 0; t < 2; t++) mbar_init(&s_full[t], 2), mbar_init(&p_full[t][0], 4), mbar_init(&p_full[t][1], 4), mbar_init(&o_done[t], 1);
+        dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaW) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    kf_grid_launch_dependents();
+    kf_grid_dependency_wait();  // queries, cache rows, lengths and tables, workspace
+    const KfPaged pg = behind_wait(pg_);
+    PagedWalk<kKV> walk(pg, pl, lane);
+    const long long W = walk.count(s_sum, warp, kThreads / 32);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_smem;
+    const int grid = (int)gridDim.x, cta = (int)blockIdx.x;
+    const long long run = max((long long)a.min_run, (W + grid - 1) / grid), u0 = cta * run, u1 = min(W, u0 + run);
+    if (u0 < u1) walk.seek(s_sum, u0);
+
+    if (u0 >= u1) {
+    } else if (warp < 8) {
+        const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t s_row = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(t * 128), o_row = tmem + ((uint32_t)(quad * 32) << 16) + 256u + (uint32_t)(t * HD);
+        const uint32_t sfull = smem_u32(&s_full[t]), pfull = smem_u32(&p_full[t][0]), odone = smem_u32(&o_done[t]);
+        const bool vec = ((uintptr_t)a.out & 15) == 0 && a.ldo % 8 == 0;
+        const float sc2 = a.sc2;
+        uint32_t cnt = 0, tile0 = 0, xph = 0;  // steps of this chain, tiles of this CTA before the piece, phases of the exchange
+        bool live = true;
+        for (long long u = u0; live && u < u1;) {
+            const PagedPiece pc = walk.at(u, u1);
+            u += pc.t1 - pc.t0;
+            const Steps st(pc, pl, a.tokens);
+            const int steps = st.of(t), tok0 = pc.b * 2 * a.tokens + (st.pair ? t * a.tokens : 0);  // the row tile's first token
+            const int tok = tok0 + row / pl.group;
+            const bool mine = row < a.tokens * pl.group && tok < pc.n;
+            const int pos = mine ? min(pc.len - pc.n + tok, pg.cap - 1) : -1, low = pl.window > 0 ? pc.len - pc.n + tok - pl.window : -1;  // sees (low, pos]
+            // positions that all rows of the row tile see
+            const int last = min(pc.n, tok0 + a.tokens) - 1, sure_hi = min(pc.len - pc.n + tok0 + 1, pg.cap), sure_lo = pl.window > 0 ? pc.len - pc.n + last - pl.window + 1 : 0;
+            float m = -INFINITY;           // the maximum that the weights and O refer to
+            unsigned long long l2 = 0ull;  // the denominator, even and odd positions apart
+            for (int j = 0; j < steps; j++) {
+                if (!(live = mbar_wait_warp(sfull, cnt & 1, &dead, bound))) break;
+                tc_fence_after();
+                // The scores are read twice, 64 positions at a time: 128 of them beside the weights do not fit the registers.  The second half is still there when the
+                // maximum is known, so it goes first.
+                const int p0 = (pc.t0 + st.tile(t, j)) * kKV;
+                const unsigned there = (unsigned)s_there[(tile0 + st.tile(t, j)) % kMasks];
+                const bool part = p0 + kKV > sure_hi || p0 < sure_lo || there != 0xffffu;
+                const int hi = pos - p0, lo = low - p0;
+                uint32_t s[64];
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto fetch = [&](int c) {
+                    ld32_async(s_row + 64 * c, s), ld32_async(s_row + 64 * c + 32, s + 32);
+                    wait_ld();
+                    if (part) {
+#pragma unroll
+                        for (int i = 0; i < 64; i++)
+                            if (64 * c + i > hi || 64 * c + i <= lo || !(there >> (8 * c + i / 8) & 1)) s[i] = 0xff800000u;
+                    }
+                };
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    fetch(c);
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(s[i + e]));
+                }
+                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (j == 0) {
+                    m = mn;
+                } else if (__any_sync(0xffffffffu, mn > m)) {
+                    const float n = fmaxf(m, mn), f = ex2((m - finite_or_0(n)) * sc2);
+                    if (!(live = mbar_wait_warp(odone, (cnt - 1) & 1, &dead, bound))) break;  // the last O += P V is through
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t o[32];
+                        ld32_async(o_row + 32 * c, o);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        st32(o_row + 32 * c, o);
+                    }
+                    wait_st();
+                    l2 = mul2(l2, pack2(f, f)), m = n;
+                }
+                const float base = finite_or_0(m) * sc2;
+                const unsigned long long sc22 = pack2(sc2, sc2), nm2 = pack2(-base, -base);
+#pragma unroll
+                for (int c = 1; c >= 0; c--) {  // one half's O += P V runs while the other half's weights are formed
+                    if (c == 0) fetch(0);
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const float2 x = unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc22, nm2));
+                        const float e = ex2(x.x), f = ex2(x.y);
+                        l2   = add2(l2, pack2(e, f));
+                        p[i] = pack_bf16x2(e, f);
+                    }
+                    st32(s_row + 64 + 32 * c, p);  // over scores of the second half, which are in registers
+                    wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_a(pfull + 8 * c);
+                }
+                cnt++;
+            }
+            if (live && steps > 0) live = mbar_wait_warp(odone, (cnt - 1) & 1, &dead, bound);
+            if (!live) break;
+            tc_fence_after();
+            const float2 ll = unpack2(l2);
+            float l = ll.x + ll.y, m2 = m == -INFINITY ? -INFINITY : m * sc2;
+            const bool whole = st.n == pc.tiles, meet = !st.pair && st.n > 1;
+            const long long first = pc.u / run;
+            const size_t slot = ((size_t)cta * 2 + (first == cta)) * 256 + (st.pair ? t * kQ : 0) + row;
+            uint16_t* op = a.out + (pc.q0 + tok) * a.ldo + (long long)((pl.heads > 1 ? pc.head : 0) * pl.group + row % pl.group) * HD;
+            if (meet && t == 1) s_m[row] = m2, s_l[row] = l;
+            float f0 = 1.f, f1 = 0.f;
+            constexpr int kCols = HD / 2;  // columns of an exchange: as many as the second Q tile, which such a block does not have, holds of 128 rows
+            float4* xb = reinterpret_cast<float4*>(sq + kTile);
+            for (int c0 = 0; live && c0 < HD; c0 += kCols) {
+                if (meet && t == 1) {
+                    if (c0 > 0 && !(live = mbar_wait_warp(smem_u32(&x_free), xph & 1, &dead, bound))) break;
+                    if (c0 > 0) xph++;
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 32) {
+                        uint32_t o[32];
+                        ld32_async(o_row + c0 + c, o);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 8; i++) xb[(c / 4 + i) * kQ + row] = *reinterpret_cast<const float4*>(&o[4 * i]);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&x_full);
+                    continue;
+                }
+                if (st.pair || t == 0) {
+                    if (meet) {
+                        if (!(live = mbar_wait_warp(smem_u32(&x_full), xph & 1, &dead, bound))) break;
+                        xph++;
+                        if (c0 == 0) {
+                            const float mb = s_m[row], mm = fmaxf(m2, mb);
+                            f0 = m2 == -INFINITY ? 0.f : ex2(m2 - mm), f1 = mb == -INFINITY ? 0.f : ex2(mb - mm);
+                            l = l * f0 + s_l[row] * f1, m2 = mm;
+                        }
+                    }
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 32) {
+                        uint32_t o[32];
+                        ld32_async(o_row + c0 + c, o);
+                        wait_ld();
+                        if (meet) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                const float4 b = xb[(c / 4 + i) * kQ + row];
+                                o[4 * i]     = __float_as_uint(fmaf(b.x, f1, __uint_as_float(o[4 * i]) * f0));
+                                o[4 * i + 1] = __float_as_uint(fmaf(b.y, f1, __uint_as_float(o[4 * i + 1]) * f0));
+                                o[4 * i + 2] = __float_as_uint(fmaf(b.z, f1, __uint_as_float(o[4 * i + 2]) * f0));
+                                o[4 * i + 3] = __float_as_uint(fmaf(b.w, f1, __uint_as_float(o[4 * i + 3]) * f0));
+                            }
+                        }
+                        if (!mine) continue;
+                        if (whole) store_row(op + c0 + c, o, inv, vec);
+                        else {
+                            float4* w = reinterpret_cast<float4*>(a.ws + slot * HD + c0 + c);
+#pragma unroll
+                            for (int i = 0; i < 8; i++) __stcg(w + i, *reinterpret_cast<const float4*>(&o[4 * i]));
+                        }
+                    }
+                    if (mine && !whole && c0 == 0) __stcg(a.ws_ml + slot, make_float2(m2, l));
+                    if (meet && c0 + kCols < HD) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&x_free);
+                    }
+                }
+            }
+            if (!live) break;
+            if (meet) {  // the second Q tile is the loader's again
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&x_done);
+            }
+            tc_fence_before();
+            tile0 += st.n;
+        }
+    } else if (warp == kMmaW) {
+        constexpr uint32_t id_s = make_idesc_bf16(128), id_o = make_idesc_bf16(HD) | (1u << 16);  // bit 16: B is MN-major
+        const uint32_t q_addr = smem_u32(sq), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
+        uint32_t kpos = 0, vpos = 0, qph = 0, cnt[2] = {0, 0};  // tiles whose scores / sums have been issued, Q tiles, steps of the chains
+        bool live = true;
+        auto score = [&](const Steps& st, int j, int t) {  // S_t = Q K^T, 16 dims per instruction
+            const uint32_t i = kpos + (st.pair ? 0 : t), stage = i % kStages;
+            if (!(live = live && mbar_wait_warp(smem_u32(&k_full[stage]), (i / kStages) & 1, &dead, bound))) return;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++) {
+                const uint32_t off = (uint32_t)((k >> 2) * kHalf + (k & 3) * 32);
+                umma_ss(tmem + t * 128, make_desc_sw128(q_addr + (st.pair ? t * kTile : 0) + off), make_desc_sw128(k_addr + stage * kTile + off), id_s, k > 0);
+            }
+            umma_commit_a(smem_u32(&s_full[t]));
+            if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
+        };
+        auto scored = [&](const Steps& st, int j) {  // the K tiles of step j, and behind the last the queries, go back when these have been read
+            for (int i = 0; i < st.wide(j); i++) umma_commit_a(smem_u32(&k_empty[(kpos + i) % kStages]));
+            kpos += st.wide(j);
+            if (j + 1 == st.steps) umma_commit_a(smem_u32(&q_empty));
+        };
+        auto queries = [&]() {
+            live = live && mbar_wait_warp(smem_u32(&q_full), qph & 1, &dead, bound);
+            qph++;
+            tc_fence_after();
+        };
+        long long u   = u0;
+        PagedPiece pc = walk.at(u, u1);
+        u += pc.t1 - pc.t0;
+        Steps cur(pc, pl, a.tokens);
+        int j = 0;
+        queries();
+        for (int t = 0; t < 2; t++)
+            if (live && cur.active(t, 0)) score(cur, 0, t);
+        if (live) scored(cur, 0);
+        bool more = true;
+        while (live && more) {
+            Steps nxt = cur;
+            int jn    = j + 1;
+            if (jn == cur.steps) {  // on to the next piece
+                more = u < u1;
+                if (more) {
+                    pc = walk.at(u, u1);
+                    u += pc.t1 - pc.t0;
+                    nxt = Steps(pc, pl, a.tokens), jn = 0;
+                }
+            }
+            // the scores of a new piece come behind both sums of the old one: its queries may wait for these (the chains' meeting in the second Q tile)
+            const bool same = more && jn > 0;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                if (live && cur.active(t, j)) {
+                    const uint32_t i = vpos + (cur.pair ? 0 : t), stage = i % kStages;
+                    live = mbar_wait_warp(smem_u32(&v_full[stage]), (i / kStages) & 1, &dead, bound);
+#pragma unroll
+                    for (int i8 = 0; i8 < 8; i8++) {  // O_t += P_t V, 16 positions per instruction, the second half of the positions first
+                        const int k = i8 ^ 4;
+                        if (i8 % 4 == 0) {
+                            live = live && mbar_wait_warp(smem_u32(&p_full[t][k / 4]), cnt[t] & 1, &dead, bound);
+                            tc_fence_after();
+                        }
+                        if (live) umma_ts(tmem + 256 + t * HD, tmem + t * 128 + 64 + k * 8, make_desc_v(v_addr + stage * kTile + k * 2048), id_o, j > 0 || i8 > 0);
+                    }
+                    cnt[t]++;
+                    if (live) umma_commit_a(smem_u32(&o_done[t]));
+                }
+                if (live && same && nxt.active(t, jn)) score(nxt, jn, t);  // behind the O above, which reads the weights from the same columns
+            }
+            if (live && more && !same) {
+                queries();
+                for (int t = 0; t < 2; t++)
+                    if (live && nxt.active(t, 0)) score(nxt, 0, t);
+            }
+            if (!live) break;
+            for (int i = 0; i < cur.wide(j); i++) umma_commit_a(smem_u32(&v_empty[(vpos + i) % kStages]));
+            vpos += cur.wide(j);
+            if (more) scored(nxt, jn);
+            cur = nxt, j = jn;
+        }
+        if (!live) {
+            umma_commit_a(smem_u32(&done_bar));
+            mbar_drain(smem_u32(&done_bar), 0, bound);
+        }
+    } else if (bound.drop != cta + 1) {
+        // Q and K, or V
+        const bool isv = warp == kLoadV;
+        const int n_box = kKV / a.box, bx = lane / kHalves, hf = lane % kHalves;  // a lane per box and half; bx >= n_box: none
+        uint32_t pos = 0, landed = 0, qn = 0, xn = 0;  // tiles, ragged tiles, pieces, pieces with an exchange
+        bool live = true, met = false;
+        for (long long u = u0; live && u < u1;) {
+            const PagedPiece pc = walk.at(u, u1);
+            u += pc.t1 - pc.t0;
+            const Steps st(pc, pl, a.tokens);
+            const int head = pl.heads > 1 ? pc.head : 0;
+            auto page_of = [&](int t) {  // the page of this lane's box of tile t
+                const int p = t * kKV + bx * a.box;
+                return t < pc.t1 && bx < n_box && p < pc.hi && p + a.box > pc.lo ? paged_page(pg, pc.s, p) : -1;
+            };
+            int next = page_of(pc.t0);
+            if (!isv) {
+                if (qn > 0) live = mbar_wait_warp(smem_u32(&q_empty), (qn - 1) & 1, &dead, bound);
+                if (live && met) live = mbar_wait_warp(smem_u32(&x_done), xn++ & 1, &dead, bound);
+                if (!live) break;
+                met = !st.pair && st.n > 1;
+                if (lane == 0) {
+                    const int tiles = st.pair ? 2 : 1;
+                    mbar_arrive_expect_tx(&q_full, (uint32_t)(tiles * kHalves * a.tokens * pl.group * 128));
+                    for (int i = 0; i < tiles * kHalves; i++) {
+                        const int t = i / kHalves, h = i % kHalves;
+                        tma_load_3d(sq + t * kTile + h * kHalf, &tm_q, h * 64, head * pl.group, pc.q0 + (pc.b * 2 + t) * a.tokens, &q_full);
+                    }
+                }
+                __syncwarp();
+                qn++;
+            }
+            for (int t = pc.t0; t < pc.t1; t++) {
+                const uint32_t stage = pos % kStages;
+                const int page = next, row = (t * kKV + bx * a.box) % pg.page;
+                next = page_of(t + 1);  // a tile ahead: the look-up takes its time
+                const unsigned lanes = __ballot_sync(0xffffffffu, page >= 0);
+                if (!(live = mbar_wait_warp(smem_u32(isv ? &v_empty[stage] : &k_empty[stage]), ((pos / kStages) & 1) ^ 1, &dead, bound))) break;
+                const bool ragged = isv && (t * kKV < pc.lo || (t + 1) * kKV > pc.hi);
+                uint64_t* bar = !isv ? &k_full[stage] : ragged ? &v_land : &v_full[stage];
+                uint8_t* dst  = (isv ? sv : sk) + stage * kTile;
+                if (lane == 0) {
+                    if (!isv) {
+                        unsigned there = 0;
+                        for (int i = 0; i < kKV / 8; i++) there |= (lanes >> (i * 8 / a.box * kHalves) & 1) << i;
+                        s_there[pos % kMasks] = (int)there;
+                    }
+                    mbar_arrive_expect_tx(bar, kTile);
+                }
+                __syncwarp();
+                if (bx < n_box) tma_load_3d(dst + hf * kHalf + bx * a.box * 128, isv ? &tm_v : &tm_k, head * HD + hf * 64, page >= 0 ? row : 0, page >= 0 ? page : pg.n_pages, bar);
+                __syncwarp();
+                pos++;
+                if (ragged) {
+                    if (!(live = mbar_wait_warp(smem_u32(&v_land), landed++ & 1, &dead, bound))) break;
+                    for (int i = lane; i < kKV * (HD / 8); i += 32) {
+                        const int r = i / (HD / 8), c = i % (HD / 8), p = t * kKV + r;
+                        if (p < pc.lo || p >= pc.hi) *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[stage]);
+                }
+            }
+        }
+        if (!live) {  // copies in flight write shared memory: wait for what was asked for
+            if (!isv && qn > 0) mbar_drain(smem_u32(&q_full), (qn - 1) & 1, bound);
+            for (uint32_t k = pos > (uint32_t)kStages ? pos - kStages : 0; k < pos; k++) mbar_drain(smem_u32(isv ? &v_full[k % kStages] : &k_full[k % kStages]), (k / kStages) & 1, bound);
+            if (isv && landed > 0) mbar_drain(smem_u32(&v_land), (landed - 1) & 1, bound);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaW) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Blocks that several CTAs share: block (c, s) takes rows 32 s .. 32 s + 31 of the one that begins in run c and goes on behind it, if there is one.
+constexpr int kMergeRows = 32;
+template <int HD>
+__global__ void __launch_bounds__(256) kf_attn_paged_merge_kernel(const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a, int runs) {
+    __shared__ long long s_sum[256];
+    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x;
+    kf_grid_launch_dependents();
+    kf_grid_dependency_wait();
+    const KfPaged pg = behind_wait(pg_);
+    PagedWalk<kKV> walk(pg, pl, lane);
+    const long long W = walk.count(s_sum, tid >> 5, 8), run = max((long long)a.min_run, (W + runs - 1) / runs), end = min(W, (cta + 1) * run);
+    if (end >= W || cta * run >= W) return;  // nothing behind this run
+    walk.seek(s_sum, end - 1);
+    const PagedPiece pc = walk.at(end - 1, end);
+    if (pc.u < cta * run || pc.u + pc.tiles <= end) return;  // begun before, or ends with the run
+    const Steps st(pc, pl, a.tokens);
+    const int pieces = (int)((pc.u + pc.tiles - 1) / run) - cta + 1, c = tid % (HD / 4) * 4;
+    for (int rr = tid / (HD / 4); rr < kMergeRows; rr += 256 / (HD / 4)) {
+        const int r = blockIdx.y * kMergeRows + rr, t = r / kQ, row = r % kQ, tok = pc.b * 2 * a.tokens + t * a.tokens + row / pl.group;
+        if ((t > 0 && !st.pair) || row >= a.tokens * pl.group || tok >= pc.n) continue;
+        float m = -INFINITY, l = 0.f;
+        auto at = [&](int i) { return ((size_t)(cta + i) * 2 + (i == 0)) * 256 + r; };
+        for (int i = 0; i < pieces; i++) m = fmaxf(m, __ldcg(a.ws_ml + at(i)).x);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < pieces; i++) {
+            const float2 ml = __ldcg(a.ws_ml + at(i));
+            const float4 v  = __ldcg(reinterpret_cast<const float4*>(a.ws + at(i) * HD + c));
+            const float f   = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+            l = fmaf(ml.y, f, l);
+            o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* op    = a.out + (pc.q0 + tok) * a.ldo + (long long)((pl.heads > 1 ? pc.head : 0) * pl.group + row % pl.group) * HD + c;
+        if (((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0) *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        else op[0] = f32_to_bf16_bits(o.x * inv), op[1] = f32_to_bf16_bits(o.y * inv), op[2] = f32_to_bf16_bits(o.z * inv), op[3] = f32_to_bf16_bits(o.w * inv);
+    }
+}
+
+template <int HD>
+int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_rows) {
+    const int n_kv = kv->n_kv, group = n_head / n_kv, tokens = kQ / group, grid = ctx->sm_count;
+    int box = 8;
+    while (box < kKV && kv->page_size % (2 * box) == 0) box *= 2;
+    const PagedPlan pl{2 * tokens * group, group, window, min_rows, 0x7fffffff, n_kv};
+    const size_t rows = (size_t)grid * 2 * 256;
+    int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
+    CUtensorMap tq, tk, tv;
+    const uint64_t stride = kf_paged_stride(kv) * 2;
+    if (!rc) rc = kf_tmap_heads(ctx, &tq, q, HD, n_head, (uint64_t)pg.M, (uint64_t)ldq * 2, 64, group, tokens);
+    if (!rc) rc = kf_tmap_rows(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
+    if (!rc) rc = kf_tmap_rows(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
+    if (rc) return rc;
+    auto kern = kf_attn_paged_tc_kernel<HD>;
+    static bool set[kf_ctx::kMaxDevices] = {};  // function attributes are per device
+    if (!set[ctx->device]) {
+        KF_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::kSmem));
+        set[ctx->device] = true;
+    }
+    const TcArgs a{(uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD), ldo, tokens, n_kv, 4, box, scale * 1.4426950408889634f};
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, tq, tk, tv, pg, pl, a, KfBound{ctx->wait_flags, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+    KF_LAUNCH_CHECK(ctx);
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_paged_merge_kernel<HD>, dim3(grid, 256 / kMergeRows), dim3(256), 0, pg, pl, a, grid));
+    KF_LAUNCH_CHECK(ctx);
+    return KF_OK;
+}
+}  // namespace
+
+int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_rows) {
+    return kv->head_dim == 128 ? launch_tc<128>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_rows)
+                               : launch_tc<64>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_rows);
+}

@@ -974,9 +974,10 @@ struct TmapKey {
     uint64_t inner, outer;
     uint32_t box_inner, box_outer, dt, sw, esize;
     uint64_t planes, plane_stride;  // third dimension (1: a matrix)
+    uint32_t box_planes;
     bool operator<(const TmapKey& o) const {
-        return std::tie(base, inner, outer, box_inner, box_outer, dt, sw, esize, planes, plane_stride) <
-               std::tie(o.base, o.inner, o.outer, o.box_inner, o.box_outer, o.dt, o.sw, o.esize, o.planes, o.plane_stride);
+        return std::tie(base, inner, outer, box_inner, box_outer, dt, sw, esize, planes, plane_stride, box_planes) <
+               std::tie(o.base, o.inner, o.outer, o.box_inner, o.box_outer, o.dt, o.sw, o.esize, o.planes, o.plane_stride, o.box_planes);
     }
 };
 // Maps of weights apart from those of what changes from call to call (activations and queries by their number of tokens, the cache by the number of sequences): a
@@ -996,10 +997,10 @@ EncodeTiledFn encode_fn() {
 }
 }  // namespace
 static int tmap_encode(kf_ctx* ctx, CUtensorMap* tm, CUtensorMapDataType dt, int esize, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner,
-                       uint32_t box_outer, CUtensorMapSwizzle sw, uint64_t planes, uint64_t plane_stride, bool weight) {
+                       uint32_t box_outer, CUtensorMapSwizzle sw, uint64_t planes, uint64_t plane_stride, bool weight, uint32_t box_planes = 1) {
     // a tensor map depends only on (address, geometry, box, swizzle): encode each once per context and reuse it (weights and the context's
     // activation scratch keep their addresses from token to token)
-    TmapKey key = {base, inner, outer, box_inner, box_outer, (uint32_t)dt, (uint32_t)sw, (uint32_t)esize, planes, plane_stride};
+    TmapKey key = {base, inner, outer, box_inner, box_outer, (uint32_t)dt, (uint32_t)sw, (uint32_t)esize, planes, plane_stride, box_planes};
     if (!ctx->tmap_cache) ctx->tmap_cache = new TmapCache();
     auto& cache = reinterpret_cast<TmapCache*>(ctx->tmap_cache)->maps[weight ? 0 : 1];
     auto hit    = cache.find(key);
@@ -1012,7 +1013,7 @@ static int tmap_encode(kf_ctx* ctx, CUtensorMap* tm, CUtensorMapDataType dt, int
     KF_REQUIRE(ctx, ((uintptr_t)base & 15) == 0 && (inner * esize) % 16 == 0, "TMA needs 16-byte aligned rows");
     cuuint64_t dims[3]    = {inner, outer, planes};
     cuuint64_t strides[2] = {inner * (uint64_t)esize, plane_stride};
-    cuuint32_t box[3]     = {box_inner, box_outer, 1};
+    cuuint32_t box[3]     = {box_inner, box_outer, box_planes};
     cuuint32_t estr[3]    = {1, 1, 1};
     CUresult r = fn(tm, dt, plane_stride ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1037,6 +1038,10 @@ int kf_tmap_rows(kf_ctx* ctx, CUtensorMap* tm, const void* base, uint64_t inner,
                  uint32_t box_rows) {
     return tmap_encode(ctx, tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, inner, rows, box_inner, box_rows, CU_TENSOR_MAP_SWIZZLE_128B, planes, plane_stride,
                        false);
+}
+int kf_tmap_heads(kf_ctx* ctx, CUtensorMap* tm, const void* base, uint64_t hd, uint64_t heads, uint64_t rows, uint64_t row_stride, uint32_t box_inner, uint32_t box_heads,
+                  uint32_t box_rows) {
+    return tmap_encode(ctx, tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, hd, heads, box_inner, box_heads, CU_TENSOR_MAP_SWIZZLE_128B, rows, row_stride, false, box_rows);
 }
 namespace {
 

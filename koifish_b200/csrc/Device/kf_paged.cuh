@@ -6,6 +6,8 @@ struct KfPaged {  // kernel parameter
     const int32_t *table, *q_start, *len;
     int table_cols, n_seq, n_pages, page, cap /* positions a table holds */, M /* rows of the panel */;
 };
+// attn_paged_tc.cu: sequences with more than min_rows rows on tcgen05
+int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_rows);
 int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out);  // paged_append.cu: arguments that all of them share
 static inline size_t kf_paged_stride(const kf_paged_kv* kv) { return kv->page_stride ? kv->page_stride : (size_t)kv->page_size * kv->n_kv * kv->head_dim; }
 
@@ -14,6 +16,7 @@ static inline size_t kf_paged_stride(const kf_paged_kv* kv) { return kv->page_st
 // A block that two or more runs share is a piece in each and is merged afterwards.
 struct PagedPlan {  // kernel parameter
     int rb, group, window, min_rows, max_rows;  // sequences with min_rows < rows <= max_rows
+    int heads;                                  // kv heads that lie one after the other in the order of tiles (1: every CTA of a team has its own)
 };
 // the positions [lo, hi) that a row of block b may see, their first tile and how many tiles they touch
 static inline __host__ __device__ int paged_block(int tile, int cap, const PagedPlan& pl, int n, int len, int b, int& lo, int& hi, int& kt0) {
@@ -48,14 +51,15 @@ __device__ __forceinline__ void paged_seq(const KfPaged& pg, int s, int& q0, int
 
 struct PagedPiece {
     int s, q0, n, len, b;     // sequence, its rows in the panel, its positions; block
+    int head;                 // of plan.heads
     int lo, hi;               // positions that a row of the block may see
     int t0, t1;               // tiles of this piece
-    long long u;              // first tile of the block in the order of all, and how many the block has
+    long long u;              // first tile of the block and head in the order of all, and how many there are
     int tiles;
 };
 // One warp's way through the sequences, 32 at a time: every lane holds one.
 template <int TILE>
-struct PagedWalk {
+struct PagedWalk {  // plan.heads is counted in
     const KfPaged pg;
     const PagedPlan pl;
     const int lane;
@@ -90,6 +94,7 @@ struct PagedWalk {
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (lane == l) units = sum;
         }
+        units *= pl.heads;
         inc = scan(units, lane);
     }
     __device__ __forceinline__ long long total() const { return __shfl_sync(0xffffffffu, inc, 31); }
@@ -140,11 +145,11 @@ struct PagedWalk {
         PagedPiece p;
         p.s = base + l, p.q0 = __shfl_sync(0xffffffffu, q0, l), p.n = __shfl_sync(0xffffffffu, n, l), p.len = __shfl_sync(0xffffffffu, len, l);
         const int nb_ = __shfl_sync(0xffffffffu, nb, l);
-        int off       = (int)(u - before - __shfl_sync(0xffffffffu, inc - units, l));
+        long long off = u - before - __shfl_sync(0xffffffffu, inc - units, l);
         p.b           = 0;
         if (nb_ > 1)
             for (int b0 = 0; b0 < nb_; b0 += 32) {
-                const int t = b0 + lane < nb_ ? tiles(p.n, p.len, b0 + lane) : 0, c = (int)scan(t, lane);
+                const long long t = b0 + lane < nb_ ? (long long)tiles(p.n, p.len, b0 + lane) * pl.heads : 0, c = scan(t, lane);
                 const unsigned in = __ballot_sync(0xffffffffu, c > off);
                 if (in) {
                     const int f = __ffs(in) - 1;
@@ -155,8 +160,10 @@ struct PagedWalk {
             }
         int kt0;
         p.tiles = paged_block(TILE, pg.cap, pl, p.n, p.len, p.b, p.lo, p.hi, kt0);
-        p.u     = u - off;
-        p.t0 = kt0 + off, p.t1 = kt0 + (int)min((long long)p.tiles, off + (end - u));
+        p.head  = pl.heads > 1 ? (int)(off / p.tiles) : 0;
+        off -= (long long)p.head * p.tiles;
+        p.u  = u - off;
+        p.t0 = kt0 + (int)off, p.t1 = kt0 + (int)min((long long)p.tiles, off + (end - u));
         return p;
     }
 };

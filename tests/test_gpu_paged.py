@@ -127,7 +127,7 @@ class Step:
     def check(self, ctx, window=0, scale=None, **kw):
         scale = self.hd ** -0.5 if scale is None else scale
         out = self.attend(ctx, scale, window, **kw)
-        torch.cuda.synchronize()
+        ctx.sync()
         ref, tol = self.expect(scale, window)
         a, b = self.start[0], self.start[-1]
         got = out[:, :self.heads * self.hd].double()
@@ -207,7 +207,7 @@ def test_scores_of_minus_infinity(ctx):
     for j in (0, 1):
         s.k[int(s.table[1, j])] = float("-inf")
     out = s.attend(ctx, 64 ** -0.5)
-    torch.cuda.synchronize()
+    ctx.sync()
     t = Step([1, 1], [200, 30], 4, 1, 64, 16, seed=10, drop=[(0, 0, -1), (0, 3, -1), (0, 12, -1), (1, 0, -1), (1, 1, -1)])
     t.k, t.v, t.q, t.table = s.k, s.v, s.q, np.where(t.table == -1, -1, s.table)
     ref, tol = t.expect(64 ** -0.5, 0)
@@ -241,7 +241,7 @@ def test_chunks_before_the_first_position(ctx):
     """More new tokens than positions: the first rows stand before position 0 and see nothing."""
     s = Step([20, 40], [8, 33], 4, 1, 128, 8, seed=4)
     out = s.attend(ctx, 0.1)
-    torch.cuda.synchronize()
+    ctx.sync()
     assert torch.all(out[:12] == 0) and torch.all(out[20:27] == 0)
     t = Step([8, 33], [8, 33], 4, 1, 128, 8, seed=4)
     t.k, t.v, t.table = s.k, s.v, s.table
@@ -463,7 +463,7 @@ def serve(ctx, heads, kv, hd, page, chunks, seed=0, graph=False):
             ctx.sync()
         else:
             step()
-        torch.cuda.synchronize()
+            ctx.sync()
         assert torch.all(out[n:] == 7)
         row = 0
         for i in range(n_seq):
@@ -514,7 +514,7 @@ def test_same_bits(ctx):
     a = s.attend(ctx, 0.1)
     for _ in range(5):
         b = s.attend(ctx, 0.1)
-        torch.cuda.synchronize()
+        ctx.sync()
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
@@ -528,7 +528,7 @@ def test_against_the_contiguous_cache(ctx):
     pos = i32([n - 1 for n in s.length])
     ctx.check(ctx.lib.kf_attn_decode_gqa(ctx.h, out.data_ptr(), s.q.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), 4, 16, 4, 128, 512, 511, 512 * 4 * 128), "gqa")
     got = s.attend(ctx, 128 ** -0.5)
-    torch.cuda.synchronize()
+    ctx.sync()
     assert torch.all((out.double() - got.double()).abs() <= 2 * tol)
 
 
