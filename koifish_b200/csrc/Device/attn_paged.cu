@@ -14,8 +14,7 @@
 // Values behind a block's last position or before its window need not be numbers: their rows of V are zeroed in shared memory.
 #include <algorithm>
 
-#include "kf_paged.cuh"
-#include "kf_tc.cuh"
+#include "kf_paged_walk.cuh"
 
 namespace {
 constexpr int kTok = 64;
@@ -43,11 +42,11 @@ constexpr bool rings_fit() {
 static_assert(rings_fit(), "two tiles of every set in flight");
 
 template <int HD, int SETS>
-__global__ void __launch_bounds__((4 * SETS + 1) * 32, 3 - SETS)
+__global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
     kf_attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, uint16_t* out, float* ws, float2* ws_ml, unsigned* cnt, const uint16_t* q,
                          const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, long long ldo, long long ldq, int n_kv, int min_run, int box /* positions */, int stages,
                          float sc2 /* scale * log2(e) */, const __grid_constant__ KfBound bound) {
-    constexpr int HALVES = HD / 64, TILE = kTok * HD * 2, HALF = kTok * 128;  // a tile lies as halves of 64 dims: 64 rows of 128 bytes (SWIZZLE_128B)
+    constexpr int PARTS = HD / 64, TILE = kTok * HD * 2, GROUP8 = PARTS * 1024;  // a tile lies as groups of 8 rows, each in parts of 64 dims (kf_tmap_pages)
     constexpr int kWarps = 4 * SETS, kComp = kWarps * 32, kMaxStages = 20;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -55,35 +54,40 @@ __global__ void __launch_bounds__((4 * SETS + 1) * 32, 3 - SETS)
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], meet_bar;
     __shared__ volatile int dead;
     __shared__ int s_there[kMaxStages], s_last;  // bit i: positions 8 i .. 8 i + 7 of the stage's K tile are there
-    __shared__ long long s_sum[256];
+    __shared__ PagedQueue qu;
     __shared__ float s_m[kWarps][16], s_l[kWarps][16], s_M[16], s_i[16];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     if (tid == 0) {
         for (int s = 0; s < stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 4);
         mbar_init(&meet_bar, kWarps);
+        qu.init(kWarps + 1);
         dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma_prefetch_map(&tm_k), tma_prefetch_map(&tm_v);
     }
+    __syncthreads();
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();  // queries, the new positions' rows, lengths and tables, workspace
     const KfPaged pg = behind_wait(pg_);
     q                = behind_wait(q);
-    PagedWalk<kTok> walk(pg, pl, lane);
-    const long long W = walk.count(s_sum, warp, kWarps + 1);
-    __syncthreads();
     const int teams = (int)gridDim.x / n_kv, team = (int)blockIdx.x / n_kv, kvh = (int)blockIdx.x % n_kv;
-    const long long run = max((long long)min_run, (W + teams - 1) / teams), u0 = team * run, u1 = min(W, u0 + run);
-    if (u0 >= u1) return;
-    walk.seek(s_sum, u0);
+    if (pg.n_seq > 32) {
+        paged_sums<kTok>(pg, pl, qu.s_sum, warp, kWarps + 2, lane);
+        __syncthreads();
+    }
+    if (warp == kWarps + 1) {
+        paged_plan<kTok>(qu, pg, pl, teams, min_run, team, lane, &dead, bound);
+        return;
+    }
+    PagedReader reader;
+    PagedPiece pc;
+    bool live = true;
     uint32_t st = 0, ph = 0;  // ring position and its phase
     if (warp == kWarps) {
         if (bound.drop == (int)blockIdx.x + 1) return;
-        bool live = true;
         uint32_t asked = 0;
-        const int n_box = kTok / box, bx = lane / HALVES, hf = lane % HALVES;  // a lane per box and half; bx >= n_box: none
-        for (long long u = u0; live && u < u1;) {
-            const PagedPiece pc = walk.at(u, u1);
-            u += pc.t1 - pc.t0;
+        const int n_box = kTok / box, bx = lane;  // a lane per box; bx >= n_box: none
+        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             auto page_of = [&](int t) {  // the page of this lane's box of tile t
                 const int p = t * kTok + bx * box;
                 return t < pc.t1 && bx < n_box && p < pc.hi && p + box > pc.lo ? paged_page(pg, pc.s, p) : -1;
@@ -97,14 +101,12 @@ __global__ void __launch_bounds__((4 * SETS + 1) * 32, 3 - SETS)
                     if (!(live = mbar_wait_warp(smem_u32(&empty[st]), ph ^ 1, &dead, bound))) break;
                     if (lane == 0) {
                         unsigned there = 0;
-                        for (int i = 0; i < kTok / 8; i++) there |= (lanes >> (i * 8 / box * HALVES) & 1) << i;
+                        for (int i = 0; i < kTok / 8; i++) there |= (lanes >> (i * 8 / box) & 1) << i;
                         s_there[st] = (int)there;
                         mbar_arrive_expect_tx(&full[st], TILE);
                     }
                     __syncwarp();
-                    if (bx < n_box)
-                        tma_load_3d(ring + (size_t)st * TILE + hf * HALF + bx * box * 128, kv ? &tm_v : &tm_k, kvh * HD + hf * 64, page >= 0 ? row : 0, page >= 0 ? page : pg.n_pages,
-                                    &full[st]);
+                    if (bx < n_box) tma_load_page(ring + (size_t)st * TILE + bx * box * (HD * 2), kv ? &tm_v : &tm_k, kvh * PARTS, page >= 0 ? row / 8 : 0, page >= 0 ? page : pg.n_pages, &full[st]);
                     __syncwarp();
                     asked++;
                     if (++st == (uint32_t)stages) st = 0, ph ^= 1;
@@ -118,19 +120,16 @@ __global__ void __launch_bounds__((4 * SETS + 1) * 32, 3 - SETS)
     const int set = warp >> 2, w4 = warp & 3, group = pl.group, rb = pl.rb;
     const bool vec = ((uintptr_t)out & 7) == 0 && ldo % 4 == 0;
     uint32_t mph = 0, done = 0;  // done: tiles of this CTA before the current piece
-    bool live = true;
     auto meet = [&]() {  // all computing warps; bounded like every wait
         __syncwarp();
         if (lane == 0) mbar_arrive(&meet_bar);
         live = mbar_wait_warp(smem_u32(&meet_bar), mph, &dead, bound) && live;
         mph ^= 1;
     };
-    // 16-byte chunk c (0 .. HD / 8 - 1) of a row: half c / 8, chunk c % 8 swizzled by the row
-    auto at = [](uint32_t base, int row, int c) { return base + (uint32_t)((c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)); };
-    for (long long u = u0; live && u < u1;) {
-        const PagedPiece pc = walk.at(u, u1);
-        u += pc.t1 - pc.t0;
-        const int ntiles = pc.t1 - pc.t0, rows = (int)min((long long)rb, (long long)pc.n * group - (long long)pc.b * rb);
+    // 16-byte chunk c (0 .. HD / 8 - 1) of a row: part c / 8, chunk c % 8 swizzled by the row
+    auto at = [](uint32_t base, int row, int c) { return base + (uint32_t)((row >> 3) * GROUP8 + (c >> 3) * 1024 + (row & 7) * 128 + (((c & 7) ^ (row & 7)) << 4)); };
+    while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
+        const int ntiles = pc.t1 - pc.t0, rows = min(rb, pc.n * group - pc.b * rb);
         // the block's queries as A fragments (rows past its end are zero), and what its rows see: positions above `low` up to `lim`
         uint32_t qa[HD / 16][4];
         int lim[2], low[2];
@@ -190,7 +189,7 @@ __global__ void __launch_bounds__((4 * SETS + 1) * 32, 3 - SETS)
                     for (int c = lane; c < 16 * (HD / 8); c += 32) {
                         const int r = c / (HD / 8), ch = c % (HD / 8), row = w4 * 16 + r;
                         if (tok0 + r >= pc.hi || tok0 + r < pc.lo)
-                            *reinterpret_cast<uint4*>(ring + (size_t)sv * TILE + (ch >> 3) * HALF + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(ring + (size_t)sv * TILE + (row >> 3) * GROUP8 + (ch >> 3) * 1024 + (row & 7) * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     // the stage is refilled by the asynchronous proxy later: these writes come before that
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -249,7 +248,7 @@ __global__ void __launch_bounds__((4 * SETS + 1) * 32, 3 - SETS)
             return out + (pc.q0 + R / group) * ldo + (long long)(kvh * group + R % group) * HD;
         };
         // partial sums: a CTA has at most one piece that others have begun (slot 0) and one that others go on with (slot 1)
-        const int first = (int)(pc.u / run), last = (int)((pc.u + pc.tiles - 1) / run);  // teams
+        const int first = reader.first, last = reader.last;  // teams
         const size_t slot = (size_t)blockIdx.x * 2 + (first == team);
         for (int idx = tid; idx < rows * (HD / 4); idx += kComp) {
             const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
@@ -347,13 +346,14 @@ template <int HD, int SETS>
 int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, const PagedPlan& pl, void* out, long long ldo, const void* q, long long ldq, float scale) {
     const int n_kv = kv->n_kv, teams = std::max(1, (3 - SETS) * ctx->sm_count / n_kv), grid = teams * n_kv, box = box_of(kv->page_size, kTok);
     const size_t rows = (size_t)grid * 2 * pl.rb;
+    KF_REQUIRE(ctx, paged_most(kTok, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
     int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
     if (!rc) rc = kf_ensure_attn_cnt(ctx, grid);
     if (rc) return rc;
     CUtensorMap tk, tv;
     const uint64_t stride = kf_paged_stride(kv) * 2;
-    rc = kf_tmap_rows(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
-    if (!rc) rc = kf_tmap_rows(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
+    rc = kf_tmap_pages(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
+    if (!rc) rc = kf_tmap_pages(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
     if (rc) return rc;
     const int stages  = ring_stages(HD, SETS, pl.rb);
     const size_t smem = (size_t)stages * kTok * HD * 2 + rows_area(HD, SETS, pl.rb) + 1024;
@@ -363,7 +363,7 @@ int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, const Page
         KF_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (SETS == 1 ? 109 : 217) * 1024));
         set[ctx->device] = true;
     }
-    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((4 * SETS + 1) * 32), smem, tk, tv, (uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD),
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((4 * SETS + 2) * 32), smem, tk, tv, (uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD),
                                ctx->attn_cnt, (const uint16_t*)q, pg, pl, ldo, ldq, n_kv, 2, box, stages, scale * 1.4426950408889634f,
                                KfBound{ctx->wait_flags + 1, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
@@ -378,6 +378,7 @@ static int check_args(kf_ctx* ctx, const kf_paged_kv* kv, const void* out, int l
     KF_REQUIRE(ctx, n_head >= 1 && n_head % kv->n_kv == 0 && n_head / kv->n_kv <= 64, "n_head a multiple of n_kv, at most 64 heads to a kv head");
     KF_REQUIRE(ctx, (long long)n_head * kv->head_dim <= ldq && (long long)n_head * kv->head_dim <= ldo, "rows as long as their heads");
     KF_REQUIRE(ctx, ((uintptr_t)q & 15) == 0 && ldq % 8 == 0, "q at 16 bytes, ldq a multiple of 8");
+    KF_REQUIRE(ctx, (long long)M * (n_head / kv->n_kv) < 0x7fffff00, "rows");
     KF_REQUIRE(ctx, scale > 0.f && scale < INFINITY && max_q >= 0, "scale above 0, max_q not negative");
     return KF_OK;
 }

@@ -14,14 +14,14 @@
 // Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
 #include <algorithm>
 
-#include "kf_paged.cuh"
-#include "kf_tc.cuh"
+#include "kf_paged_walk.cuh"
 
 namespace {
-constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kThreads = 11 * 32, kMasks = 8;
+constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kPlanW = 11, kThreads = 12 * 32, kMasks = 8;
 template <int HD>
 struct Cfg {
-    static constexpr int kHalves = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStages = HD == 128 ? 2 : 4;  // a tile lies as halves of 64 dims, 128 rows of 128 bytes each
+    static constexpr int kParts = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStages = HD == 128 ? 2 : 4;
+    static constexpr int kGroup = kParts * 1024;  // tiles of K and V lie as groups of 8 rows, each in parts of 64 dims (kf_tmap_pages); of Q as halves of 64 dims
     static constexpr size_t kSmem = (2 + 2 * kStages) * (size_t)kTile + 1024;
 };
 struct TcArgs {  // kernel parameter
@@ -33,10 +33,11 @@ struct TcArgs {  // kernel parameter
     float sc2;                       // scale * log2(e)
 };
 
-// shared-memory descriptor of a V tile: MN-major (64 dims side by side, then the next position's 128-byte row), SWIZZLE_128B; the dims' second half lies 128 rows
-// behind the first (leading byte offset), eight positions 1024 bytes behind the eight before (stride byte offset)
-__device__ __forceinline__ uint64_t make_desc_v(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(kKV * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// shared-memory descriptors of a K tile (K-major) and a V tile (MN-major: 64 dims side by side, then the next position's 128-byte row), SWIZZLE_128B: eight positions lie
+// kGroup behind the eight before (stride byte offset), V's second 64 dims 1024 bytes behind the first (leading byte offset)
+template <int HD>
+__device__ __forceinline__ uint64_t make_desc_kv(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(1024 >> 4) << 16) | ((uint64_t)(Cfg<HD>::kGroup >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ void store_row(uint16_t* p, const uint32_t (&o)[32], float f, bool vec) {
     if (vec) {
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     kf_attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                             const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a, const __grid_constant__ KfBound bound) {
     using C = Cfg<HD>;
-    constexpr int kTile = C::kTile, kHalf = C::kHalf, kHalves = C::kHalves, kStages = C::kStages;
+    constexpr int kTile = C::kTile, kHalf = C::kHalf, kParts = C::kParts, kGroup = C::kGroup, kStages = C::kStages;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sk = sq + 2 * kTile;
@@ -81,45 +82,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t tmem_base_smem;
     __shared__ volatile int dead;
     __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
-    __shared__ long long s_sum[256];
+    __shared__ PagedQueue qu;
     __shared__ float s_m[kQ], s_l[kQ];  // chain 1's maximum and denominator, where the chains share a row tile
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 8);
         for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
         for (int t = 0; t < 2; t++) mbar_init(&s_full[t], 2), mbar_init(&p_full[t][0], 4), mbar_init(&p_full[t][1], 4), mbar_init(&o_done[t], 1);
+        qu.init(11);
         dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma_prefetch_map(&tm_q), tma_prefetch_map(&tm_k), tma_prefetch_map(&tm_v);
     }
     if (warp == kMmaW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    kf_grid_launch_dependents();
-    kf_grid_dependency_wait();  // queries, cache rows, lengths and tables, workspace
-    const KfPaged pg = behind_wait(pg_);
-    PagedWalk<kKV> walk(pg, pl, lane);
-    const long long W = walk.count(s_sum, warp, kThreads / 32);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_smem;
-    const int grid = (int)gridDim.x, cta = (int)blockIdx.x;
-    const long long run = max((long long)a.min_run, (W + grid - 1) / grid), u0 = cta * run, u1 = min(W, u0 + run);
-    if (u0 < u1) walk.seek(s_sum, u0);
+    const int cta       = (int)blockIdx.x;
+    kf_grid_launch_dependents();
+    kf_grid_dependency_wait();  // queries, cache rows, lengths and tables, workspace
+    const KfPaged pg = behind_wait(pg_);
+    if (pg.n_seq > 32) {
+        paged_sums<kKV>(pg, pl, qu.s_sum, warp, kThreads / 32, lane);
+        __syncthreads();
+    }
+    PagedReader reader;
+    PagedPiece pc;
+    bool live = true;
 
-    if (u0 >= u1) {
-    } else if (warp < 8) {
+    if (warp < 8) {
         const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t s_row = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(t * 128), o_row = tmem + ((uint32_t)(quad * 32) << 16) + 256u + (uint32_t)(t * HD);
         const uint32_t sfull = smem_u32(&s_full[t]), pfull = smem_u32(&p_full[t][0]), odone = smem_u32(&o_done[t]);
         const bool vec = ((uintptr_t)a.out & 15) == 0 && a.ldo % 8 == 0;
         const float sc2 = a.sc2;
         uint32_t cnt = 0, tile0 = 0, xph = 0;  // steps of this chain, tiles of this CTA before the piece, phases of the exchange
-        bool live = true;
-        for (long long u = u0; live && u < u1;) {
-            const PagedPiece pc = walk.at(u, u1);
-            u += pc.t1 - pc.t0;
+        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
             const int steps = st.of(t), tok0 = pc.b * 2 * a.tokens + (st.pair ? t * a.tokens : 0);  // the row tile's first token
             const int tok = tok0 + row / pl.group;
@@ -203,8 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float2 ll = unpack2(l2);
             float l = ll.x + ll.y, m2 = m == -INFINITY ? -INFINITY : m * sc2;
             const bool whole = st.n == pc.tiles, meet = !st.pair && st.n > 1;
-            const long long first = pc.u / run;
-            const size_t slot = ((size_t)cta * 2 + (first == cta)) * 256 + (st.pair ? t * kQ : 0) + row;
+            const size_t slot = ((size_t)cta * 2 + (reader.first == cta)) * 256 + (st.pair ? t * kQ : 0) + row;
             uint16_t* op = a.out + (pc.q0 + tok) * a.ldo + (long long)((pl.heads > 1 ? pc.head : 0) * pl.group + row % pl.group) * HD;
             if (meet && t == 1) s_m[row] = m2, s_l[row] = l;
             float f0 = 1.f, f1 = 0.f;
@@ -280,7 +281,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t id_s = make_idesc_bf16(128), id_o = make_idesc_bf16(HD) | (1u << 16);  // bit 16: B is MN-major
         const uint32_t q_addr = smem_u32(sq), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
         uint32_t kpos = 0, vpos = 0, qph = 0, cnt[2] = {0, 0};  // tiles whose scores / sums have been issued, Q tiles, steps of the chains
-        bool live = true;
         auto score = [&](const Steps& st, int j, int t) {  // S_t = Q K^T, 16 dims per instruction
             const uint32_t i = kpos + (st.pair ? 0 : t), stage = i % kStages;
             if (!(live = live && mbar_wait_warp(smem_u32(&k_full[stage]), (i / kStages) & 1, &dead, bound))) return;
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < HD / 16; k++) {
                 const uint32_t off = (uint32_t)((k >> 2) * kHalf + (k & 3) * 32);
-                umma_ss(tmem + t * 128, make_desc_sw128(q_addr + (st.pair ? t * kTile : 0) + off), make_desc_sw128(k_addr + stage * kTile + off), id_s, k > 0);
+                umma_ss(tmem + t * 128, make_desc_sw128(q_addr + (st.pair ? t * kTile : 0) + off), make_desc_kv<HD>(k_addr + stage * kTile + (k >> 2) * 1024 + (k & 3) * 32), id_s, k > 0);
             }
             umma_commit_a(smem_u32(&s_full[t]));
             if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
@@ -303,26 +303,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             qph++;
             tc_fence_after();
         };
-        long long u   = u0;
-        PagedPiece pc = walk.at(u, u1);
-        u += pc.t1 - pc.t0;
+        bool more = reader.next(qu, pc, lane, &dead, bound, live);
         Steps cur(pc, pl, a.tokens);
         int j = 0;
-        queries();
-        for (int t = 0; t < 2; t++)
-            if (live && cur.active(t, 0)) score(cur, 0, t);
-        if (live) scored(cur, 0);
-        bool more = true;
+        if (more) {
+            queries();
+            for (int t = 0; t < 2; t++)
+                if (live && cur.active(t, 0)) score(cur, 0, t);
+            if (live) scored(cur, 0);
+        }
         while (live && more) {
             Steps nxt = cur;
             int jn    = j + 1;
             if (jn == cur.steps) {  // on to the next piece
-                more = u < u1;
-                if (more) {
-                    pc = walk.at(u, u1);
-                    u += pc.t1 - pc.t0;
-                    nxt = Steps(pc, pl, a.tokens), jn = 0;
-                }
+                more = reader.next(qu, pc, lane, &dead, bound, live);
+                if (more) nxt = Steps(pc, pl, a.tokens), jn = 0;
             }
             // the scores of a new piece come behind both sums of the old one: its queries may wait for these (the chains' meeting in the second Q tile)
             const bool same = more && jn > 0;
@@ -338,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             live = live && mbar_wait_warp(smem_u32(&p_full[t][k / 4]), cnt[t] & 1, &dead, bound);
                             tc_fence_after();
                         }
-                        if (live) umma_ts(tmem + 256 + t * HD, tmem + t * 128 + 64 + k * 8, make_desc_v(v_addr + stage * kTile + k * 2048), id_o, j > 0 || i8 > 0);
+                        if (live) umma_ts(tmem + 256 + t * HD, tmem + t * 128 + 64 + k * 8, make_desc_kv<HD>(v_addr + stage * kTile + k * 2 * kGroup), id_o, j > 0 || i8 > 0);
                     }
                     cnt[t]++;
                     if (live) umma_commit_a(smem_u32(&o_done[t]));
@@ -360,15 +355,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit_a(smem_u32(&done_bar));
             mbar_drain(smem_u32(&done_bar), 0, bound);
         }
+    } else if (warp == kPlanW) {
+        paged_plan<kKV>(qu, pg, pl, (int)gridDim.x, a.min_run, cta, lane, &dead, bound);
     } else if (bound.drop != cta + 1) {
         // Q and K, or V
         const bool isv = warp == kLoadV;
-        const int n_box = kKV / a.box, bx = lane / kHalves, hf = lane % kHalves;  // a lane per box and half; bx >= n_box: none
+        const int n_box = kKV / a.box, bx = lane;  // a lane per box; bx >= n_box: none
         uint32_t pos = 0, landed = 0, qn = 0, xn = 0;  // tiles, ragged tiles, pieces, pieces with an exchange
-        bool live = true, met = false;
-        for (long long u = u0; live && u < u1;) {
-            const PagedPiece pc = walk.at(u, u1);
-            u += pc.t1 - pc.t0;
+        bool met = false;
+        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
             const int head = pl.heads > 1 ? pc.head : 0;
             auto page_of = [&](int t) {  // the page of this lane's box of tile t
@@ -383,9 +378,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 met = !st.pair && st.n > 1;
                 if (lane == 0) {
                     const int tiles = st.pair ? 2 : 1;
-                    mbar_arrive_expect_tx(&q_full, (uint32_t)(tiles * kHalves * a.tokens * pl.group * 128));
-                    for (int i = 0; i < tiles * kHalves; i++) {
-                        const int t = i / kHalves, h = i % kHalves;
+                    mbar_arrive_expect_tx(&q_full, (uint32_t)(tiles * kParts * a.tokens * pl.group * 128));
+                    for (int i = 0; i < tiles * kParts; i++) {
+                        const int t = i / kParts, h = i % kParts;
                         tma_load_3d(sq + t * kTile + h * kHalf, &tm_q, h * 64, head * pl.group, pc.q0 + (pc.b * 2 + t) * a.tokens, &q_full);
                     }
                 }
@@ -404,20 +399,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) {
                     if (!isv) {
                         unsigned there = 0;
-                        for (int i = 0; i < kKV / 8; i++) there |= (lanes >> (i * 8 / a.box * kHalves) & 1) << i;
+                        for (int i = 0; i < kKV / 8; i++) there |= (lanes >> (i * 8 / a.box) & 1) << i;
                         s_there[pos % kMasks] = (int)there;
                     }
                     mbar_arrive_expect_tx(bar, kTile);
                 }
                 __syncwarp();
-                if (bx < n_box) tma_load_3d(dst + hf * kHalf + bx * a.box * 128, isv ? &tm_v : &tm_k, head * HD + hf * 64, page >= 0 ? row : 0, page >= 0 ? page : pg.n_pages, bar);
+                if (bx < n_box) tma_load_page(dst + bx * a.box * (HD * 2), isv ? &tm_v : &tm_k, head * kParts, page >= 0 ? row / 8 : 0, page >= 0 ? page : pg.n_pages, bar);
                 __syncwarp();
                 pos++;
                 if (ragged) {
                     if (!(live = mbar_wait_warp(smem_u32(&v_land), landed++ & 1, &dead, bound))) break;
                     for (int i = lane; i < kKV * (HD / 8); i += 32) {
                         const int r = i / (HD / 8), c = i % (HD / 8), p = t * kKV + r;
-                        if (p < pc.lo || p >= pc.hi) *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        if (p < pc.lo || p >= pc.hi) *reinterpret_cast<uint4*>(dst + (r >> 3) * kGroup + (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
@@ -443,19 +438,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kMergeRows = 32;
 template <int HD>
 __global__ void __launch_bounds__(256) kf_attn_paged_merge_kernel(const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a, int runs) {
-    __shared__ long long s_sum[256];
+    __shared__ int s_sum[256];
     const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x;
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();
     const KfPaged pg = behind_wait(pg_);
     PagedWalk<kKV> walk(pg, pl, lane);
-    const long long W = walk.count(s_sum, tid >> 5, 8), run = max((long long)a.min_run, (W + runs - 1) / runs), end = min(W, (cta + 1) * run);
-    if (end >= W || cta * run >= W) return;  // nothing behind this run
+    if (pg.n_seq > 32) {
+        paged_sums<kKV>(pg, pl, s_sum, tid >> 5, 8, lane);
+        __syncthreads();
+    }
+    const int W = walk.count(s_sum), run = max(a.min_run, (W + runs - 1) / runs), end = (int)min((long long)W, (long long)(cta + 1) * run);
+    if (end >= W) return;  // nothing behind this run
     walk.seek(s_sum, end - 1);
     const PagedPiece pc = walk.at(end - 1, end);
     if (pc.u < cta * run || pc.u + pc.tiles <= end) return;  // begun before, or ends with the run
     const Steps st(pc, pl, a.tokens);
-    const int pieces = (int)((pc.u + pc.tiles - 1) / run) - cta + 1, c = tid % (HD / 4) * 4;
+    const int pieces = (pc.u + pc.tiles - 1) / run - cta + 1, c = tid % (HD / 4) * 4;
     for (int rr = tid / (HD / 4); rr < kMergeRows; rr += 256 / (HD / 4)) {
         const int r = blockIdx.y * kMergeRows + rr, t = r / kQ, row = r % kQ, tok = pc.b * 2 * a.tokens + t * a.tokens + row / pl.group;
         if ((t > 0 && !st.pair) || row >= a.tokens * pl.group || tok >= pc.n) continue;
@@ -485,12 +484,13 @@ int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, 
     while (box < kKV && kv->page_size % (2 * box) == 0) box *= 2;
     const PagedPlan pl{2 * tokens * group, group, window, min_rows, 0x7fffffff, n_kv};
     const size_t rows = (size_t)grid * 2 * 256;
+    KF_REQUIRE(ctx, paged_most(kKV, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
     int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
     CUtensorMap tq, tk, tv;
     const uint64_t stride = kf_paged_stride(kv) * 2;
     if (!rc) rc = kf_tmap_heads(ctx, &tq, q, HD, n_head, (uint64_t)pg.M, (uint64_t)ldq * 2, 64, group, tokens);
-    if (!rc) rc = kf_tmap_rows(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
-    if (!rc) rc = kf_tmap_rows(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, 64, box);
+    if (!rc) rc = kf_tmap_pages(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
+    if (!rc) rc = kf_tmap_pages(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
     if (rc) return rc;
     auto kern = kf_attn_paged_tc_kernel<HD>;
     static bool set[kf_ctx::kMaxDevices] = {};  // function attributes are per device

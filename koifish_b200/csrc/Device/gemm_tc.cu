@@ -1043,6 +1043,35 @@ int kf_tmap_heads(kf_ctx* ctx, CUtensorMap* tm, const void* base, uint64_t hd, u
                   uint32_t box_rows) {
     return tmap_encode(ctx, tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, hd, heads, box_inner, box_heads, CU_TENSOR_MAP_SWIZZLE_128B, rows, row_stride, false, box_rows);
 }
+// Five dimensions: 64 dims, 8 rows, the 64-dim parts of a row, the page's groups of 8 rows, pages -- so that a box lies in shared memory as groups of 8 rows with their parts
+// one after the other, the same for every page size that is a multiple of 8
+int kf_tmap_pages(kf_ctx* ctx, CUtensorMap* tm, const void* base, uint64_t row, uint64_t page, uint64_t pages, uint64_t page_stride, uint32_t parts, uint32_t box_rows) {
+    TmapKey key = {base, row, page, 64 * parts, box_rows, (uint32_t)CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint32_t)CU_TENSOR_MAP_SWIZZLE_128B, 2, pages, page_stride, 0};
+    if (!ctx->tmap_cache) ctx->tmap_cache = new TmapCache();
+    auto& cache = reinterpret_cast<TmapCache*>(ctx->tmap_cache)->maps[1];
+    auto hit    = cache.find(key);
+    if (hit != cache.end()) {
+        *tm = hit->second;
+        return KF_OK;
+    }
+    EncodeTiledFn fn = encode_fn();
+    KF_REQUIRE(ctx, fn != nullptr, "cuTensorMapEncodeTiled not available from the driver");
+    cuuint64_t dims[5]    = {64, 8, row / 64, page / 8, pages};
+    cuuint64_t strides[4] = {row * 2, 128, row * 16, page_stride};
+    cuuint32_t box[5]     = {64, 8, parts, box_rows / 8, 1};
+    cuuint32_t estr[5]    = {1, 1, 1, 1, 1};
+    CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        char b[128];
+        snprintf(b, sizeof(b), "cuTensorMapEncodeTiled failed for a cache in pages (%d)", (int)r);
+        ctx->last_error = b;
+        return KF_ERR_CUDA;
+    }
+    if (cache.size() >= kTmapMost[1]) cache.clear();
+    cache[key] = *tm;
+    return KF_OK;
+}
 namespace {
 
 // Row tiles of a launch: 128 rows of one weight each, or (SwiGLU) 64 rows of gate and the same 64 of up

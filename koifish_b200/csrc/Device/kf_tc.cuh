@@ -15,6 +15,9 @@ int kf_tmap_rows(kf_ctx* ctx, CUtensorMap* tm, const void* base, uint64_t inner,
 // bf16 rows of `heads` dense heads, row_stride bytes apart, box [box_rows][box_heads][box_inner], SWIZZLE_128B
 int kf_tmap_heads(kf_ctx* ctx, CUtensorMap* tm, const void* base, uint64_t hd, uint64_t heads, uint64_t rows, uint64_t row_stride, uint32_t box_inner, uint32_t box_heads,
                   uint32_t box_rows);
+// bf16 pages of `page` rows of `row` elements, page_stride bytes apart; a box is box_rows rows (within a page, from a multiple of 8) of parts x 64 elements, SWIZZLE_128B: in
+// shared memory [box_rows / 8][parts][8 rows of 128 bytes].  Coordinates: 0, 0, part, row / 8, page (gemm_tc.cu)
+int kf_tmap_pages(kf_ctx* ctx, CUtensorMap* tm, const void* base, uint64_t row, uint64_t page, uint64_t pages, uint64_t page_stride, uint32_t parts, uint32_t box_rows);
 
 namespace {
 // ---- PTX helpers ------------------------------------------------------------------------------------------------------------------
@@ -255,6 +258,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, in
                  "r"(c1), "r"(c2), "r"(smem_u32(bar))
                  : "memory");
 }
+// a box of a cache in pages (kf_tmap_pages)
+__device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* tm, int part, int group, int page, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)), "l"(tm), "r"(0),
+                 "r"(part), "r"(group), "r"(page), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* tm) { asm volatile("prefetch.tensormap [%0];" ::"l"(tm) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
