@@ -44,7 +44,7 @@ static_assert(rings_fit(), "two tiles of every set in flight");
 template <int HD, int SETS>
 __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
     kf_attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, uint16_t* out, float* ws, float2* ws_ml, unsigned* cnt, const uint16_t* q,
-                         const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, long long ldo, long long ldq, int n_kv, int min_run, int box /* positions */, int stages,
+                         const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, long long ldo, long long ldq, int n_kv, int box /* positions */, int stages,
                          float sc2 /* scale * log2(e) */, const __grid_constant__ KfBound bound) {
     constexpr int PARTS = HD / 64, TILE = kTok * HD * 2, GROUP8 = PARTS * 1024;  // a tile lies as groups of 8 rows, each in parts of 64 dims (kf_tmap_pages)
     constexpr int kWarps = 4 * SETS, kComp = kWarps * 32, kMaxStages = 20;
@@ -70,13 +70,13 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
     kf_grid_dependency_wait();  // queries, the new positions' rows, lengths and tables, workspace
     const KfPaged pg = behind_wait(pg_);
     q                = behind_wait(q);
-    const int teams = (int)gridDim.x / n_kv, team = (int)blockIdx.x / n_kv, kvh = (int)blockIdx.x % n_kv;
+    const int team = (int)blockIdx.x / n_kv, kvh = (int)blockIdx.x % n_kv;
     if (pg.n_seq > 32) {
-        paged_sums<kTok>(pg, pl, qu.s_sum, warp, kWarps + 2, lane);
+        paged_plan<kTok>(false, qu, pg, pl, team, warp, kWarps + 2, lane, nullptr, &dead, bound);
         __syncthreads();
     }
     if (warp == kWarps + 1) {
-        paged_plan<kTok>(qu, pg, pl, teams, min_run, team, lane, &dead, bound);
+        paged_plan<kTok>(true, qu, pg, pl, team, warp, kWarps + 2, lane, nullptr, &dead, bound);
         return;
     }
     PagedReader reader;
@@ -88,13 +88,14 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
         uint32_t asked = 0;
         const int n_box = kTok / box, bx = lane;  // a lane per box; bx >= n_box: none
         while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
+            int next_row = 0;
             auto page_of = [&](int t) {  // the page of this lane's box of tile t
                 const int p = t * kTok + bx * box;
-                return t < pc.t1 && bx < n_box && p < pc.hi && p + box > pc.lo ? paged_page(pg, pc.s, p) : -1;
+                return t < pc.t1 && bx < n_box && p < pc.hi && p + box > pc.lo ? paged_page(pg, pc.s, p, next_row) : -1;
             };
             int next = page_of(pc.t0);
             for (int t = pc.t0; live && t < pc.t1; t++) {
-                const int page = next, row = (t * kTok + bx * box) % pg.page;
+                const int page = next, row = next_row;
                 next = page_of(t + 1);  // a tile ahead: the look-up takes as long as a tile
                 const unsigned lanes = __ballot_sync(0xffffffffu, page >= 0);
                 for (int kv = 0; kv < 2; kv++) {
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
             for (uint32_t k = asked > (uint32_t)stages ? asked - stages : 0; k < asked; k++) mbar_drain(smem_u32(&full[k % stages]), (k / stages) & 1, bound);
         return;
     }
-    const int set = warp >> 2, w4 = warp & 3, group = pl.group, rb = pl.rb;
+    const int set = warp >> 2, w4 = warp & 3, group = pl.group, rb = pl.tb * group;
     const bool vec = ((uintptr_t)out & 7) == 0 && ldo % 4 == 0;
     uint32_t mph = 0, done = 0;  // done: tiles of this CTA before the current piece
     auto meet = [&]() {  // all computing warps; bounded like every wait
@@ -129,14 +130,14 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
     // 16-byte chunk c (0 .. HD / 8 - 1) of a row: part c / 8, chunk c % 8 swizzled by the row
     auto at = [](uint32_t base, int row, int c) { return base + (uint32_t)((row >> 3) * GROUP8 + (c >> 3) * 1024 + (row & 7) * 128 + (((c & 7) ^ (row & 7)) << 4)); };
     while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
-        const int ntiles = pc.t1 - pc.t0, rows = min(rb, pc.n * group - pc.b * rb);
+        const int ntiles = pc.t1 - pc.t0, rows = min(pl.tb, pc.n - pc.b * pl.tb) * group;
         // the block's queries as A fragments (rows past its end are zero), and what its rows see: positions above `low` up to `lim`
         uint32_t qa[HD / 16][4];
         int lim[2], low[2];
         const uint32_t* qp[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int r = pc.b * rb + g + 8 * e, tok = r / group;
+            const int r = g + 8 * e, tok = pc.b * pl.tb + r / group;
             lim[e] = min(pc.len - pc.n + tok, pg.cap - 1), low[e] = pl.window > 0 ? pc.len - pc.n + tok - pl.window : -1;
             qp[e]  = reinterpret_cast<const uint32_t*>(q + (pc.q0 + tok) * ldq + (long long)(kvh * group + r % group) * HD);
         }
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
             qa[kc][1] = g + 8 < rows ? qp[1][kc * 8 + t4] : 0u, qa[kc][3] = g + 8 < rows ? qp[1][kc * 8 + t4 + 4] : 0u;
         }
         // positions that all rows see: below the first row's, above the last row's window
-        const int sure_hi = min(pc.len - pc.n + pc.b * rb / group + 1, pg.cap), sure_lo = pl.window > 0 ? pc.len - pc.n + (pc.b * rb + rows - 1) / group - pl.window + 1 : 0;
+        const int sure_hi = min(pc.len - pc.n + pc.b * pl.tb + 1, pg.cap), sure_lo = pl.window > 0 ? pc.len - pc.n + min(pc.n, (pc.b + 1) * pl.tb) - pl.window : 0;
         float o[HD / 8][4];
 #pragma unroll
         for (int j = 0; j < HD / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -242,13 +243,12 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
         if (t4 == 0) s_m[warp][g] = m_lo, s_m[warp][g + 8] = m_hi, s_l[warp][g] = l_lo, s_l[warp][g + 8] = l_hi;
         meet();
         if (!live) break;
-        const bool whole = ntiles == pc.tiles;
+        const bool whole = pc.whole;
         auto out_row = [&](int r) {
-            const int R = pc.b * rb + r;
-            return out + (pc.q0 + R / group) * ldo + (long long)(kvh * group + R % group) * HD;
+            return out + (pc.q0 + pc.b * pl.tb + r / group) * ldo + (long long)(kvh * group + r % group) * HD;
         };
         // partial sums: a CTA has at most one piece that others have begun (slot 0) and one that others go on with (slot 1)
-        const int first = reader.first, last = reader.last;  // teams
+        const int first = pc.first, last = pc.last;  // teams
         const size_t slot = (size_t)blockIdx.x * 2 + (first == team);
         for (int idx = tid; idx < rows * (HD / 4); idx += kComp) {
             const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
@@ -343,9 +343,10 @@ int box_of(int page, int most) {
 }
 
 template <int HD, int SETS>
-int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, const PagedPlan& pl, void* out, long long ldo, const void* q, long long ldq, float scale) {
-    const int n_kv = kv->n_kv, teams = std::max(1, (3 - SETS) * ctx->sm_count / n_kv), grid = teams * n_kv, box = box_of(kv->page_size, kTok);
-    const size_t rows = (size_t)grid * 2 * pl.rb;
+int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, PagedPlan pl, void* out, long long ldo, const void* q, long long ldq, float scale) {
+    const int n_kv = kv->n_kv, teams = std::max(1, (3 - SETS) * ctx->sm_count / n_kv), grid = teams * n_kv, box = box_of(kv->page_size, kTok), rb = pl.tb * pl.group;
+    const size_t rows = (size_t)grid * 2 * rb;
+    pl.runs = teams, pl.min_run = 2;
     KF_REQUIRE(ctx, paged_most(kTok, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
     int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
     if (!rc) rc = kf_ensure_attn_cnt(ctx, grid);
@@ -355,8 +356,8 @@ int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, const Page
     rc = kf_tmap_pages(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
     if (!rc) rc = kf_tmap_pages(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
     if (rc) return rc;
-    const int stages  = ring_stages(HD, SETS, pl.rb);
-    const size_t smem = (size_t)stages * kTok * HD * 2 + rows_area(HD, SETS, pl.rb) + 1024;
+    const int stages  = ring_stages(HD, SETS, rb);
+    const size_t smem = (size_t)stages * kTok * HD * 2 + rows_area(HD, SETS, rb) + 1024;
     auto kern         = kf_attn_paged_kernel<HD, SETS>;
     static bool set[kf_ctx::kMaxDevices] = {};  // function attributes are per device
     if (!set[ctx->device]) {
@@ -364,7 +365,7 @@ int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, const Page
         set[ctx->device] = true;
     }
     KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((4 * SETS + 2) * 32), smem, tk, tv, (uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD),
-                               ctx->attn_cnt, (const uint16_t*)q, pg, pl, ldo, ldq, n_kv, 2, box, stages, scale * 1.4426950408889634f,
+                               ctx->attn_cnt, (const uint16_t*)q, pg, pl, ldo, ldq, n_kv, box, stages, scale * 1.4426950408889634f,
                                KfBound{ctx->wait_flags + 1, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
@@ -389,14 +390,13 @@ extern "C" int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out,
     if (!rc) rc = kf_wait_status(ctx);
     if (rc || M == 0) return rc;
     const int group = n_head / kv->n_kv;
-    const bool many = (long long)max_q * group > 16;
-    const PagedPlan pl{(int)std::min(16ll, std::max(1ll, (long long)max_q * group)), group, window, 0, many ? 16 : 0x7fffffff, 1};
-    const int few = 1;
-    if (kv->head_dim == 128)
-        rc = few ? launch_few<128, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<128, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
-    else
-        rc = few ? launch_few<64, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<64, 2>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
-    if (!rc && many) rc = kf_attn_paged_tc(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, 16);
+    // sequences with up to 16 rows a kv head here, the others on tcgen05
+    const int few = 16 / group, tokens = std::max(1, max_q);
+    if (few > 0) {
+        const PagedPlan pl{std::min(few, tokens), group, window, 0, tokens > few ? few : 0x7fffffff, 1, 0, 0};
+        rc = kv->head_dim == 128 ? launch_few<128, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<64, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
+    }
+    if (!rc && tokens > few) rc = kf_attn_paged_tc(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, few);
     return rc;
 }
 // The checks and the blocks' arithmetic for tests on a host without a device
@@ -404,6 +404,12 @@ extern "C" int kf_paged_attention_args(const kf_paged_kv* kv, const void* out, i
     KfPaged pg;
     return check_args(nullptr, kv, out, ldo, q, ldq, M, n_head, scale, max_q, &pg);
 }
-extern "C" int kf_paged_attention_block(int tile, int cap, int rb, int group, int window, int n, int len, int b, int* lo_hi_first) {
-    return paged_block(tile, cap, PagedPlan{rb, group, window, 0, 0, 1}, n, len, b, lo_hi_first[0], lo_hi_first[1], lo_hi_first[2]);
+extern "C" int kf_paged_attention_block(int tile, int cap, int tb, int window, int n, int len, int b, int* lo_hi_first) {
+    return paged_block(tile, cap, tb, window, n, len, b, lo_hi_first[0], lo_hi_first[1], lo_hi_first[2]);
+}
+extern "C" int kf_paged_page_of(int page, int p) {
+    KfPaged pg = {};
+    pg.page    = page;
+    kf_paged_divisor(&pg);
+    return (int)((uint64_t)(uint32_t)p * pg.page_mul >> 32 >> pg.page_shift);
 }

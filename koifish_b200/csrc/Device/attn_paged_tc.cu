@@ -17,6 +17,7 @@
 #include "kf_paged_walk.cuh"
 
 namespace {
+constexpr float kSlack = 8.f;
 constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kPlanW = 11, kThreads = 12 * 32, kMasks = 8;
 template <int HD>
 struct Cfg {
@@ -26,18 +27,54 @@ struct Cfg {
 };
 struct TcArgs {  // kernel parameter
     uint16_t* out;
-    float* ws;      // [CTA][2][256][HD] sums, then as many (maximum, denominator) pairs
+    float* ws;        // [CTA][2][256][HD] sums, then as many (maximum, denominator) pairs, then what begins in a run and goes on behind it, per run
     float2* ws_ml;
+    PagedPiece* rec;
     long long ldo;
-    int tokens, n_kv, min_run, box;  // tokens of a row tile; positions of a box
-    float sc2;                       // scale * log2(e)
+    int tokens, box;  // tokens of a row tile; positions of a box
+    float sc2;        // scale * log2(e)
 };
-
 // shared-memory descriptors of a K tile (K-major) and a V tile (MN-major: 64 dims side by side, then the next position's 128-byte row), SWIZZLE_128B: eight positions lie
 // kGroup behind the eight before (stride byte offset), V's second 64 dims 1024 bytes behind the first (leading byte offset)
 template <int HD>
 __device__ __forceinline__ uint64_t make_desc_kv(uint32_t smem_addr) {
     return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(1024 >> 4) << 16) | ((uint64_t)(Cfg<HD>::kGroup >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// four steps of 16 dims of scores: 32 bytes on in the swizzled rows of both operands each; one election for all of them
+__device__ __forceinline__ void umma_scores_x4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "add.u64 a1, %1, 2;\n\tadd.u64 a2, %1, 4;\n\tadd.u64 a3, %1, 6;\n\t"
+        "add.u64 b1, %2, 2;\n\tadd.u64 b2, %2, 4;\n\tadd.u64 b3, %2, 6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, 1;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// four steps of 16 positions of sums: 8 tensor-memory columns of weights, 2 groups of 8 rows of V on each
+template <int GROUP>
+__device__ __forceinline__ void umma_sums_x4(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+        "add.u64 b1, %2, %5;\n\tadd.u64 b2, b1, %5;\n\tadd.u64 b3, b2, %5;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(2 * GROUP / 16)
+        : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ void store_row(uint16_t* p, const uint32_t (&o)[32], float f, bool vec) {
     if (vec) {
@@ -58,7 +95,7 @@ struct Steps {
     bool pair;      // two row tiles, which share the tiles; otherwise chain t takes every second one
     int n, steps;   // tiles, steps
     __device__ __forceinline__ Steps(const PagedPiece& pc, const PagedPlan& pl, int tokens) {
-        pair  = pc.n - pc.b * (pl.rb / pl.group) > tokens;
+        pair  = pc.n - pc.b * pl.tb > tokens;
         n     = pc.t1 - pc.t0;
         steps = pair ? n : (n + 1) / 2;
     }
@@ -107,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     kf_grid_dependency_wait();  // queries, cache rows, lengths and tables, workspace
     const KfPaged pg = behind_wait(pg_);
     if (pg.n_seq > 32) {
-        paged_sums<kKV>(pg, pl, qu.s_sum, warp, kThreads / 32, lane);
+        paged_plan<kKV>(false, qu, pg, pl, cta, warp, kThreads / 32, lane, nullptr, &dead, bound);
         __syncthreads();
     }
     PagedReader reader;
@@ -123,79 +160,75 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t cnt = 0, tile0 = 0, xph = 0;  // steps of this chain, tiles of this CTA before the piece, phases of the exchange
         while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
-            const int steps = st.of(t), tok0 = pc.b * 2 * a.tokens + (st.pair ? t * a.tokens : 0);  // the row tile's first token
+            const int steps = st.of(t), tok0 = pc.b * pl.tb + (st.pair ? t * a.tokens : 0);  // the row tile's first token
             const int tok = tok0 + row / pl.group;
             const bool mine = row < a.tokens * pl.group && tok < pc.n;
             const int pos = mine ? min(pc.len - pc.n + tok, pg.cap - 1) : -1, low = pl.window > 0 ? pc.len - pc.n + tok - pl.window : -1;  // sees (low, pos]
             // positions that all rows of the row tile see
             const int last = min(pc.n, tok0 + a.tokens) - 1, sure_hi = min(pc.len - pc.n + tok0 + 1, pg.cap), sure_lo = pl.window > 0 ? pc.len - pc.n + last - pl.window + 1 : 0;
-            float m = -INFINITY;           // the maximum that the weights and O refer to
+            float m = -INFINITY;           // the maximum, times sc2, that the weights and O refer to
             unsigned long long l2 = 0ull;  // the denominator, even and odd positions apart
             for (int j = 0; j < steps; j++) {
                 if (!(live = mbar_wait_warp(sfull, cnt & 1, &dead, bound))) break;
                 tc_fence_after();
-                // The scores are read twice, 64 positions at a time: 128 of them beside the weights do not fit the registers.  The second half is still there when the
-                // maximum is known, so it goes first.
+                uint32_t s[kKV];
+#pragma unroll
+                for (int c = 0; c < 4; c++) ld32_async(s_row + 32 * c, s + 32 * c);
                 const int p0 = (pc.t0 + st.tile(t, j)) * kKV;
                 const unsigned there = (unsigned)s_there[(tile0 + st.tile(t, j)) % kMasks];
-                const bool part = p0 + kKV > sure_hi || p0 < sure_lo || there != 0xffffu;
-                const int hi = pos - p0, lo = low - p0;
-                uint32_t s[64];
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                auto fetch = [&](int c) {
-                    ld32_async(s_row + 64 * c, s), ld32_async(s_row + 64 * c + 32, s + 32);
-                    wait_ld();
-                    if (part) {
+                wait_ld();
+                if (p0 + kKV > sure_hi || p0 < sure_lo || there != 0xffffu) {
 #pragma unroll
-                        for (int i = 0; i < 64; i++)
-                            if (64 * c + i > hi || 64 * c + i <= lo || !(there >> (8 * c + i / 8) & 1)) s[i] = 0xff800000u;
+                    for (int c = 0; c < 4; c++) {  // what the row sees of 32 positions, a bit each
+                        const int hi = pos - p0 - 32 * c, lo = low - p0 - 32 * c;
+                        uint32_t see = ((there >> (4 * c) & 15u) * 0x00204081u & 0x01010101u) * 255u;
+                        see &= hi < 0 ? 0u : hi > 30 ? 0xffffffffu : (2u << hi) - 1u;
+                        see &= lo < 0 ? 0xffffffffu : lo > 30 ? 0u : ~((2u << lo) - 1u);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) s[32 * c + i] = see >> i & 1 ? s[32 * c + i] : 0xff800000u;
                     }
-                };
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    fetch(c);
-#pragma unroll
-                    for (int i = 0; i < 64; i += 4)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(s[i + e]));
                 }
-                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < kKV; i += 4)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) mx[e] = max3(mx[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+                const float mn = fmaxf(mx[0], mx[1]) * sc2;
                 if (j == 0) {
                     m = mn;
-                } else if (__any_sync(0xffffffffu, mn > m)) {
-                    const float n = fmaxf(m, mn), f = ex2((m - finite_or_0(n)) * sc2);
+                } else if (__any_sync(0xffffffffu, mn > m + kSlack)) {
+                    const float n = fmaxf(m, mn), f = ex2(m - finite_or_0(n));
                     if (!(live = mbar_wait_warp(odone, (cnt - 1) & 1, &dead, bound))) break;  // the last O += P V is through
                     tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_row + c, o);
 #pragma unroll
-                    for (int c = 0; c < HD / 32; c++) {
-                        uint32_t o[32];
-                        ld32_async(o_row + 32 * c, o);
-                        wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        st32(o_row + 32 * c, o);
+                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(o_row + c, o);
                     }
                     wait_st();
                     l2 = mul2(l2, pack2(f, f)), m = n;
                 }
-                const float base = finite_or_0(m) * sc2;
+                const float base = finite_or_0(m);
                 const unsigned long long sc22 = pack2(sc2, sc2), nm2 = pack2(-base, -base);
 #pragma unroll
-                for (int c = 1; c >= 0; c--) {  // one half's O += P V runs while the other half's weights are formed
-                    if (c == 0) fetch(0);
-                    uint32_t p[32];
+                for (int c = 0; c < 4; c++) {  // one half's O += P V runs while the other half's weights are formed
+                    uint32_t p[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const float2 x = unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc22, nm2));
-                        const float e = ex2(x.x), f = ex2(x.y);
-                        l2   = add2(l2, pack2(e, f));
-                        p[i] = pack_bf16x2(e, f);
+                    for (int i = 0; i < 16; i++) {
+                        const float2 x = unpack2(fma2(pack2(__uint_as_float(s[32 * c + 2 * i]), __uint_as_float(s[32 * c + 2 * i + 1])), sc22, nm2));
+                        p[i] = pack_bf16x2(ex2(x.x), ex2(x.y));
+                        l2   = add2(l2, pack2(bf16lo(p[i]), bf16hi(p[i])));  // the weights as they are used: a rounding that numerator and denominator share
                     }
-                    st32(s_row + 64 + 32 * c, p);  // over scores of the second half, which are in registers
-                    wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_a(pfull + 8 * c);
+                    tmem_st16(s_row + 16 * c, p);  // over scores, which are in registers
+                    if (c & 1) {
+                        wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_a(pfull + 8 * (c >> 1));
+                    }
                 }
                 cnt++;
             }
@@ -203,10 +236,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!live) break;
             tc_fence_after();
             const float2 ll = unpack2(l2);
-            float l = ll.x + ll.y, m2 = m == -INFINITY ? -INFINITY : m * sc2;
-            const bool whole = st.n == pc.tiles, meet = !st.pair && st.n > 1;
-            const size_t slot = ((size_t)cta * 2 + (reader.first == cta)) * 256 + (st.pair ? t * kQ : 0) + row;
-            uint16_t* op = a.out + (pc.q0 + tok) * a.ldo + (long long)((pl.heads > 1 ? pc.head : 0) * pl.group + row % pl.group) * HD;
+            float l = ll.x + ll.y, m2 = m;
+            const bool whole = pc.whole, meet = !st.pair && st.n > 1;
+            const size_t slot = ((size_t)cta * 2 + (pc.first == cta)) * 256 + (st.pair ? t * kQ : 0) + row;
+            uint16_t* op = a.out + (pc.q0 + tok) * a.ldo + (long long)(pc.head * pl.group + row % pl.group) * HD;
             if (meet && t == 1) s_m[row] = m2, s_l[row] = l;
             float f0 = 1.f, f1 = 0.f;
             constexpr int kCols = HD / 2;  // columns of an exchange: as many as the second Q tile, which such a block does not have, holds of 128 rows
@@ -215,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (meet && t == 1) {
                     if (c0 > 0 && !(live = mbar_wait_warp(smem_u32(&x_free), xph & 1, &dead, bound))) break;
                     if (c0 > 0) xph++;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < kCols; c += 32) {
                         uint32_t o[32];
                         ld32_async(o_row + c0 + c, o);
@@ -238,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < kCols; c += 32) {
                         uint32_t o[32];
                         ld32_async(o_row + c0 + c, o);
@@ -286,10 +319,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(live = live && mbar_wait_warp(smem_u32(&k_full[stage]), (i / kStages) & 1, &dead, bound))) return;
             tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < HD / 16; k++) {
-                const uint32_t off = (uint32_t)((k >> 2) * kHalf + (k & 3) * 32);
-                umma_ss(tmem + t * 128, make_desc_sw128(q_addr + (st.pair ? t * kTile : 0) + off), make_desc_kv<HD>(k_addr + stage * kTile + (k >> 2) * 1024 + (k & 3) * 32), id_s, k > 0);
-            }
+            for (int k = 0; k < kParts; k++)
+                umma_scores_x4(tmem + t * 128, make_desc_sw128(q_addr + (st.pair ? t * kTile : 0) + k * kHalf), make_desc_kv<HD>(k_addr + stage * kTile + k * 1024), id_s, k > 0);
             umma_commit_a(smem_u32(&s_full[t]));
             if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
         };
@@ -327,13 +358,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t i = vpos + (cur.pair ? 0 : t), stage = i % kStages;
                     live = mbar_wait_warp(smem_u32(&v_full[stage]), (i / kStages) & 1, &dead, bound);
 #pragma unroll
-                    for (int i8 = 0; i8 < 8; i8++) {  // O_t += P_t V, 16 positions per instruction, the second half of the positions first
-                        const int k = i8 ^ 4;
-                        if (i8 % 4 == 0) {
-                            live = live && mbar_wait_warp(smem_u32(&p_full[t][k / 4]), cnt[t] & 1, &dead, bound);
-                            tc_fence_after();
-                        }
-                        if (live) umma_ts(tmem + 256 + t * HD, tmem + t * 128 + 64 + k * 8, make_desc_kv<HD>(v_addr + stage * kTile + k * 2 * kGroup), id_o, j > 0 || i8 > 0);
+                    for (int k = 0; k < 2; k++) {  // O_t += P_t V, 64 positions at a time
+                        live = live && mbar_wait_warp(smem_u32(&p_full[t][k]), cnt[t] & 1, &dead, bound);
+                        tc_fence_after();
+                        if (live) umma_sums_x4<kGroup>(tmem + 256 + t * HD, tmem + t * 128 + k * 32, make_desc_kv<HD>(v_addr + stage * kTile + k * 8 * kGroup), id_o, j > 0 || k > 0);
                     }
                     cnt[t]++;
                     if (live) umma_commit_a(smem_u32(&o_done[t]));
@@ -356,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_drain(smem_u32(&done_bar), 0, bound);
         }
     } else if (warp == kPlanW) {
-        paged_plan<kKV>(qu, pg, pl, (int)gridDim.x, a.min_run, cta, lane, &dead, bound);
+        paged_plan<kKV>(true, qu, pg, pl, cta, warp, kThreads / 32, lane, a.rec, &dead, bound);
     } else if (bound.drop != cta + 1) {
         // Q and K, or V
         const bool isv = warp == kLoadV;
@@ -365,10 +393,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool met = false;
         while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
-            const int head = pl.heads > 1 ? pc.head : 0;
+            const int head = pc.head;
+            int next_row = 0;
             auto page_of = [&](int t) {  // the page of this lane's box of tile t
                 const int p = t * kKV + bx * a.box;
-                return t < pc.t1 && bx < n_box && p < pc.hi && p + a.box > pc.lo ? paged_page(pg, pc.s, p) : -1;
+                return t < pc.t1 && bx < n_box && p < pc.hi && p + a.box > pc.lo ? paged_page(pg, pc.s, p, next_row) : -1;
             };
             int next = page_of(pc.t0);
             if (!isv) {
@@ -389,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             for (int t = pc.t0; t < pc.t1; t++) {
                 const uint32_t stage = pos % kStages;
-                const int page = next, row = (t * kKV + bx * a.box) % pg.page;
+                const int page = next, row = next_row;
                 next = page_of(t + 1);  // a tile ahead: the look-up takes its time
                 const unsigned lanes = __ballot_sync(0xffffffffu, page >= 0);
                 if (!(live = mbar_wait_warp(smem_u32(isv ? &v_empty[stage] : &k_empty[stage]), ((pos / kStages) & 1) ^ 1, &dead, bound))) break;
@@ -437,55 +466,58 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Blocks that several CTAs share: block (c, s) takes rows 32 s .. 32 s + 31 of the one that begins in run c and goes on behind it, if there is one.
 constexpr int kMergeRows = 32;
 template <int HD>
-__global__ void __launch_bounds__(256) kf_attn_paged_merge_kernel(const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a, int runs) {
-    __shared__ int s_sum[256];
-    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x;
+__global__ void __launch_bounds__(256) kf_attn_paged_merge_kernel(const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a) {
+    const int tid = threadIdx.x, cta = blockIdx.x;
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();
-    const KfPaged pg = behind_wait(pg_);
-    PagedWalk<kKV> walk(pg, pl, lane);
-    if (pg.n_seq > 32) {
-        paged_sums<kKV>(pg, pl, s_sum, tid >> 5, 8, lane);
-        __syncthreads();
-    }
-    const int W = walk.count(s_sum), run = max(a.min_run, (W + runs - 1) / runs), end = (int)min((long long)W, (long long)(cta + 1) * run);
-    if (end >= W) return;  // nothing behind this run
-    walk.seek(s_sum, end - 1);
-    const PagedPiece pc = walk.at(end - 1, end);
-    if (pc.u < cta * run || pc.u + pc.tiles <= end) return;  // begun before, or ends with the run
-    const Steps st(pc, pl, a.tokens);
-    const int pieces = (pc.u + pc.tiles - 1) / run - cta + 1, c = tid % (HD / 4) * 4;
+    const PagedPiece pc = *behind_wait(a.rec + cta);
+    if (pc.last == 0) return;
+    const bool pair  = pc.n - pc.b * pl.tb > a.tokens;
+    const int pieces = pc.last - cta + 1, c = tid % (HD / 4) * 4;
+    const bool vec   = ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0;
+#pragma unroll 1
     for (int rr = tid / (HD / 4); rr < kMergeRows; rr += 256 / (HD / 4)) {
-        const int r = blockIdx.y * kMergeRows + rr, t = r / kQ, row = r % kQ, tok = pc.b * 2 * a.tokens + t * a.tokens + row / pl.group;
-        if ((t > 0 && !st.pair) || row >= a.tokens * pl.group || tok >= pc.n) continue;
+        const int r = blockIdx.y * kMergeRows + rr, t = r / kQ, row = r % kQ, tok = pc.b * pl.tb + t * a.tokens + row / pl.group;
+        if ((t > 0 && !pair) || row >= a.tokens * pl.group || tok >= pc.n) continue;
         float m = -INFINITY, l = 0.f;
         auto at = [&](int i) { return ((size_t)(cta + i) * 2 + (i == 0)) * 256 + r; };
-        for (int i = 0; i < pieces; i++) m = fmaxf(m, __ldcg(a.ws_ml + at(i)).x);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int i = 0; i < pieces; i++) {
-            const float2 ml = __ldcg(a.ws_ml + at(i));
-            const float4 v  = __ldcg(reinterpret_cast<const float4*>(a.ws + at(i) * HD + c));
-            const float f   = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-            l = fmaf(ml.y, f, l);
-            o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+        // in order, four at a time: what they hold is asked for at once
+#pragma unroll 1
+        for (int i0 = 0; i0 < pieces; i0 += 4) {
+            float2 ml[4];
+            float4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool in = i0 + i < pieces;
+                ml[i] = in ? __ldcg(a.ws_ml + at(i0 + i)) : make_float2(-INFINITY, 0.f);
+                v[i]  = in ? __ldcg(reinterpret_cast<const float4*>(a.ws + at(i0 + i) * HD + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            const float n = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m), f = ex2(m - finite_or_0(n));
+            m = n, l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float g = ex2(ml[i].x - finite_or_0(m));
+                l = fmaf(ml[i].y, g, l);
+                o.x = fmaf(v[i].x, g, o.x), o.y = fmaf(v[i].y, g, o.y), o.z = fmaf(v[i].z, g, o.z), o.w = fmaf(v[i].w, g, o.w);
+            }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* op    = a.out + (pc.q0 + tok) * a.ldo + (long long)((pl.heads > 1 ? pc.head : 0) * pl.group + row % pl.group) * HD + c;
-        if (((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0) *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        uint16_t* op    = a.out + (pc.q0 + tok) * a.ldo + (long long)(pc.head * pl.group + row % pl.group) * HD + c;
+        if (vec) *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
         else op[0] = f32_to_bf16_bits(o.x * inv), op[1] = f32_to_bf16_bits(o.y * inv), op[2] = f32_to_bf16_bits(o.z * inv), op[3] = f32_to_bf16_bits(o.w * inv);
     }
 }
 
 template <int HD>
-int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_rows) {
+int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_n) {
     const int n_kv = kv->n_kv, group = n_head / n_kv, tokens = kQ / group, grid = ctx->sm_count;
     int box = 8;
     while (box < kKV && kv->page_size % (2 * box) == 0) box *= 2;
-    const PagedPlan pl{2 * tokens * group, group, window, min_rows, 0x7fffffff, n_kv};
+    const PagedPlan pl{2 * tokens, group, window, min_n, 0x7fffffff, n_kv, grid, 4};
     const size_t rows = (size_t)grid * 2 * 256;
     KF_REQUIRE(ctx, paged_most(kKV, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
-    int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
+    int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float) + grid * sizeof(PagedPiece));
     CUtensorMap tq, tk, tv;
     const uint64_t stride = kf_paged_stride(kv) * 2;
     if (!rc) rc = kf_tmap_heads(ctx, &tq, q, HD, n_head, (uint64_t)pg.M, (uint64_t)ldq * 2, 64, group, tokens);
@@ -498,16 +530,17 @@ int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, 
         KF_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::kSmem));
         set[ctx->device] = true;
     }
-    const TcArgs a{(uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD), ldo, tokens, n_kv, 4, box, scale * 1.4426950408889634f};
+    const TcArgs a{(uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD), reinterpret_cast<PagedPiece*>(ctx->attn_ws + rows * (HD + 2)), ldo, tokens, box,
+                   scale * 1.4426950408889634f};
     KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, tq, tk, tv, pg, pl, a, KfBound{ctx->wait_flags, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
-    KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_paged_merge_kernel<HD>, dim3(grid, 256 / kMergeRows), dim3(256), 0, pg, pl, a, grid));
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_paged_merge_kernel<HD>, dim3(grid, 256 / kMergeRows), dim3(256), 0, pl, a));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
 }
 }  // namespace
 
-int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_rows) {
-    return kv->head_dim == 128 ? launch_tc<128>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_rows)
-                               : launch_tc<64>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_rows);
+int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_n) {
+    return kv->head_dim == 128 ? launch_tc<128>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_n)
+                               : launch_tc<64>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_n);
 }

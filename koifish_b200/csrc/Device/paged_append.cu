@@ -101,8 +101,9 @@ __global__ void __launch_bounds__(kThreads) kf_rows_kernel(const __grid_constant
         int q0, n, len;
         paged_seq(pg, s, q0, n, len);
         at = len - n + (m - q0);
-        const int page = at >= 0 ? paged_page(pg, s, at) : -1;
-        if (page >= 0) row = page * p.page_stride + (long long)(at % pg.page) * p.nkv * p.hd;
+        int in         = 0;
+        const int page = at >= 0 ? paged_page(pg, s, at, in) : -1;
+        if (page >= 0) row = page * p.page_stride + (long long)in * p.nkv * p.hd;
     }
     for (int j = tid; j < p.rot / 2; j += kThreads) {
         const int ax = p.axis ? p.axis[j] : 0;
@@ -240,7 +241,8 @@ int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out) {
     KF_REQUIRE(ctx, kv->n_seq >= 1 && kv->n_seq <= 8192 && M >= 0, "n_seq 1 .. 8192");
     KF_REQUIRE(ctx, kv->page_stride == 0 || (kv->page_stride % 8 == 0 && kv->page_stride >= (size_t)kv->page_size * kv->n_kv * kv->head_dim), "page_stride: a multiple of 8, at least a page");
     KF_REQUIRE(ctx, (((uintptr_t)kv->k_dev | (uintptr_t)kv->v_dev) & 15) == 0, "pages at 16 bytes");
-    *out = KfPaged{kv->table_dev, kv->q_start_dev, kv->len_dev, kv->table_cols, kv->n_seq, kv->n_pages, kv->page_size, kv->table_cols * kv->page_size, M};
+    *out = KfPaged{kv->table_dev, kv->q_start_dev, kv->len_dev, kv->table_cols, kv->n_seq, kv->n_pages, kv->page_size, kv->table_cols * kv->page_size, M, 0, 0};
+    kf_paged_divisor(out);
     return KF_OK;
 }
 

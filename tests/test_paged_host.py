@@ -103,20 +103,28 @@ def test_blocks(lib):
     r = np.random.RandomState(0)
     got = (C.c_int * 3)()
     for _ in range(4000):
-        tile = int(r.choice([64, 128]))
-        group = int(r.choice([1, 2, 4, 5, 7, 8, 16, 40, 64]))
-        rb = int(r.choice([1, 4, 8, 16, 128 // group * group, 2 * (128 // group) * group]))
-        n, len_ = int(r.randint(1, 60)), int(r.choice([0, r.randint(0, 80), r.randint(0, 700)]))
+        tile, tb = int(r.choice([64, 128])), int(r.choice([1, 2, 3, 16, 36, 50, 256]))
+        n, len_ = int(r.randint(1, 400)), int(r.choice([0, r.randint(0, 80), r.randint(0, 700)]))
         cap = int(r.choice([8, 64, 200, 800]))
         window = int(r.choice([0, 1, 5, 64, 300, 2 ** 31 - 1]))
-        for b in range(-(-n * group // rb)):
-            tiles = lib.kf_paged_attention_block(tile, cap, rb, group, window, n, len_, b, got)
+        for b in range(-(-n // tb)):
+            tiles = lib.kf_paged_attention_block(tile, cap, tb, window, n, len_, b, got)
             seen = set()
-            for row in range(b * rb, min(n * group, (b + 1) * rb)):
-                p = len_ - n + row // group
-                seen |= {j for j in range(max(0, p - window + 1) if window else 0, min(p + 1, cap))}
+            for tok in range(b * tb, min(n, (b + 1) * tb)):
+                p = len_ - n + tok
+                seen |= set(range(max(0, p - window + 1) if window else 0, min(p + 1, cap)))
             if not seen:
                 assert tiles == 1 and list(got) == [0, 0, 0]
                 continue
             assert (got[0], got[1]) == (min(seen), max(seen) + 1) and got[1] <= cap
             assert got[2] == min(seen) // tile and tiles == max(seen) // tile - min(seen) // tile + 1
+
+
+def test_page_of_a_position(lib):
+    """The division by a page size as the kernels do it, up to the largest position."""
+    r = np.random.RandomState(1)
+    for page in [8, 16, 24, 40, 48, 56, 64, 120, 128, 136, 1000, 4096, 65528, 1 << 20, (1 << 20) + 8, (1 << 30) - 8, 1 << 30]:
+        near = [k * page + d for k in [0, 1, 2, 3, (2 ** 31 - 1) // page] for d in (-1, 0, 1)]
+        for p in near + r.randint(0, 2 ** 31 - 1, 200).tolist():
+            if 0 <= p < 2 ** 31:
+                assert lib.kf_paged_page_of(page, p) == p // page
