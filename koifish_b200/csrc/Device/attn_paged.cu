@@ -72,11 +72,13 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
     q                = behind_wait(q);
     const int team = (int)blockIdx.x / n_kv, kvh = (int)blockIdx.x % n_kv;
     if (pg.n_seq > 32) {
-        paged_plan<kTok>(false, qu, pg, pl, team, warp, kWarps + 2, lane, nullptr, &dead, bound);
+        PagedPlanner<kTok>::count(pg, pl, qu.s_sum, warp, kWarps + 2, lane);
         __syncthreads();
     }
     if (warp == kWarps + 1) {
-        paged_plan<kTok>(true, qu, pg, pl, team, warp, kWarps + 2, lane, nullptr, &dead, bound);
+        PagedPlanner<kTok> plan(pg, pl, lane);
+        plan.start(qu, team);
+        while (plan.push(qu, team, nullptr, &dead, bound)) {}
         return;
     }
     PagedReader reader;

@@ -5,8 +5,8 @@
 // scores into weights, the tensor cores work for the other.  The chains are the block's two row tiles, which share every tile of K and V -- or, where the block has one
 // row tile only, its even and odd tiles of positions, whose sums meet in shared memory at the end.
 //   warps 0-3 / 4-7  softmax of chain 0 / 1, thread = row: scores from tensor memory, running maximum, weights as bf16 back over the scores of the second half
-//   warp 8           matrix instructions: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory, V as it lies: MN-major)
-//   warp 9 / 10      Q and K / V: page look-up and TMA, a box per page (or part of 8 .. 128 positions of it) and 64 dims, each asked for by a lane of its own
+//   warp 8 / 9       matrix instructions of chain 0 / 1: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory, V as it lies: MN-major)
+//   warp 10 / 11     Q and K / V: page look-up and TMA, a box per page (or part of 8 .. 128 positions of it), each asked for by a lane of its own; warp 11 plans the pieces
 // The tiles of all blocks and kv heads are cut into equal runs, one CTA each (PagedWalk).  Blocks that several CTAs share leave their sums in the workspace; a second
 // kernel, launched behind, merges them in order.
 // The output is rescaled whenever a maximum of the warp's rows grows, so the largest weight of a row is 1 and has no rounding error; the denominator adds the unrounded
@@ -18,7 +18,7 @@
 
 namespace {
 constexpr float kSlack = 8.f;
-constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kPlanW = 11, kThreads = 12 * 32, kMasks = 8;
+constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 10, kLoadV = 11, kThreads = 12 * 32, kMasks = 8, kParts4 = 4 /* parts of a tile's weights */;
 template <int HD>
 struct Cfg {
     static constexpr int kParts = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStages = HD == 128 ? 2 : 4;
@@ -55,19 +55,16 @@ __device__ __forceinline__ void umma_scores_x4(uint32_t tmem_d, uint64_t adesc, 
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// four steps of 16 positions of sums: 8 tensor-memory columns of weights, 2 groups of 8 rows of V on each
+// two steps of 16 positions of sums: 8 tensor-memory columns of weights, 2 groups of 8 rows of V on
 template <int GROUP>
-__device__ __forceinline__ void umma_sums_x4(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_sums_x2(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 a1;\n\t.reg .b64 b1;\n\t"
         "elect.sync _|q, 0xffffffff;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
-        "add.u64 b1, %2, %5;\n\tadd.u64 b2, b1, %5;\n\tadd.u64 b3, b2, %5;\n\t"
+        "add.u32 a1, %1, 8;\n\tadd.u64 b1, %2, %5;\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(tmem_d),
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t}" ::"r"(tmem_d),
         "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(2 * GROUP / 16)
         : "memory");
 }
@@ -92,15 +89,12 @@ __device__ __forceinline__ void store_row(uint16_t* p, const uint32_t (&o)[32], 
 }
 // the tiles of a piece as the chains take them
 struct Steps {
-    bool pair;      // two row tiles, which share the tiles; otherwise chain t takes every second one
-    int n, steps;   // tiles, steps
+    bool pair;  // two row tiles, which share the tiles; otherwise chain t takes every second one
+    int n;      // tiles
     __device__ __forceinline__ Steps(const PagedPiece& pc, const PagedPlan& pl, int tokens) {
-        pair  = pc.n - pc.b * pl.tb > tokens;
-        n     = pc.t1 - pc.t0;
-        steps = pair ? n : (n + 1) / 2;
+        pair = pc.n - pc.b * pl.tb > tokens;
+        n    = pc.t1 - pc.t0;
     }
-    __device__ __forceinline__ int wide(int j) const { return pair ? 1 : min(2, n - 2 * j); }         // tiles of step j
-    __device__ __forceinline__ bool active(int t, int j) const { return j < steps && (pair || 2 * j + t < n); }
     __device__ __forceinline__ int of(int t) const { return pair ? n : (n + 1 - t) / 2; }              // steps of chain t
     __device__ __forceinline__ int tile(int t, int j) const { return pair ? j : 2 * j + t; }
 };
@@ -115,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sk = sq + 2 * kTile;
     uint8_t* sv = sk + kStages * kTile;
-    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][2], o_done[2], x_full, x_free, x_done, done_bar;
+    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts4], o_done[2], x_full, x_free, x_done, done_bar[2];
     __shared__ uint32_t tmem_base_smem;
     __shared__ volatile int dead;
     __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
@@ -123,10 +117,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ float s_m[kQ], s_l[kQ];  // chain 1's maximum and denominator, where the chains share a row tile
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 8);
-        for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
-        for (int t = 0; t < 2; t++) mbar_init(&s_full[t], 2), mbar_init(&p_full[t][0], 4), mbar_init(&p_full[t][1], 4), mbar_init(&o_done[t], 1);
-        qu.init(11);
+        mbar_init(&q_full, 1), mbar_init(&q_empty, 2), mbar_init(&v_land, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 8);
+        for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 2), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 2);
+        for (int t = 0; t < 2; t++) {
+            mbar_init(&s_full[t], 2), mbar_init(&o_done[t], 1), mbar_init(&done_bar[t], 1);
+            for (int k = 0; k < kParts4; k++) mbar_init(&p_full[t][k], 4);
+        }
+        qu.init(12);
         dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&tm_q), tma_prefetch_map(&tm_k), tma_prefetch_map(&tm_v);
@@ -144,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     kf_grid_dependency_wait();  // queries, cache rows, lengths and tables, workspace
     const KfPaged pg = behind_wait(pg_);
     if (pg.n_seq > 32) {
-        paged_plan<kKV>(false, qu, pg, pl, cta, warp, kThreads / 32, lane, nullptr, &dead, bound);
+        PagedPlanner<kKV>::count(pg, pl, qu.s_sum, warp, kThreads / 32, lane);
         __syncthreads();
     }
     PagedReader reader;
@@ -188,12 +185,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < 32; i++) s[32 * c + i] = see >> i & 1 ? s[32 * c + i] : 0xff800000u;
                     }
                 }
-                float mx[2] = {-INFINITY, -INFINITY};
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < kKV; i += 4)
+                for (int i = 0; i < kKV; i += 8)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) mx[e] = max3(mx[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
-                const float mn = fmaxf(mx[0], mx[1]) * sc2;
+                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+                const float mn = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sc2;
                 if (j == 0) {
                     m = mn;
                 } else if (__any_sync(0xffffffffu, mn > m + kSlack)) {
@@ -214,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float base = finite_or_0(m);
                 const unsigned long long sc22 = pack2(sc2, sc2), nm2 = pack2(-base, -base);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {  // one half's O += P V runs while the other half's weights are formed
+                for (int c = 0; c < kParts4; c++) {  // a part's O += P V runs while the next one's weights are formed
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -223,12 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         l2   = add2(l2, pack2(bf16lo(p[i]), bf16hi(p[i])));  // the weights as they are used: a rounding that numerator and denominator share
                     }
                     tmem_st16(s_row + 16 * c, p);  // over scores, which are in registers
-                    if (c & 1) {
-                        wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_a(pfull + 8 * (c >> 1));
-                    }
+                    wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_a(pfull + 8 * c);
                 }
                 cnt++;
             }
@@ -310,88 +305,78 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             tile0 += st.n;
         }
-    } else if (warp == kMmaW) {
+    } else if (warp < kLoadK) {
+        const int t = warp - kMmaW;
         constexpr uint32_t id_s = make_idesc_bf16(128), id_o = make_idesc_bf16(HD) | (1u << 16);  // bit 16: B is MN-major
+        const uint32_t s_t = tmem + t * 128, o_t = tmem + 256 + t * HD, sfull = smem_u32(&s_full[t]), odone = smem_u32(&o_done[t]), pfull = smem_u32(&p_full[t][0]);
         const uint32_t q_addr = smem_u32(sq), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
-        uint32_t kpos = 0, vpos = 0, qph = 0, cnt[2] = {0, 0};  // tiles whose scores / sums have been issued, Q tiles, steps of the chains
-        auto score = [&](const Steps& st, int j, int t) {  // S_t = Q K^T, 16 dims per instruction
-            const uint32_t i = kpos + (st.pair ? 0 : t), stage = i % kStages;
-            if (!(live = live && mbar_wait_warp(smem_u32(&k_full[stage]), (i / kStages) & 1, &dead, bound))) return;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < kParts; k++)
-                umma_scores_x4(tmem + t * 128, make_desc_sw128(q_addr + (st.pair ? t * kTile : 0) + k * kHalf), make_desc_kv<HD>(k_addr + stage * kTile + k * 1024), id_s, k > 0);
-            umma_commit_a(smem_u32(&s_full[t]));
-            if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
-        };
-        auto scored = [&](const Steps& st, int j) {  // the K tiles of step j, and behind the last the queries, go back when these have been read
-            for (int i = 0; i < st.wide(j); i++) umma_commit_a(smem_u32(&k_empty[(kpos + i) % kStages]));
-            kpos += st.wide(j);
-            if (j + 1 == st.steps) umma_commit_a(smem_u32(&q_empty));
-        };
-        auto queries = [&]() {
-            live = live && mbar_wait_warp(smem_u32(&q_full), qph & 1, &dead, bound);
-            qph++;
-            tc_fence_after();
-        };
-        bool more = reader.next(qu, pc, lane, &dead, bound, live);
-        Steps cur(pc, pl, a.tokens);
-        int j = 0;
-        if (more) {
-            queries();
-            for (int t = 0; t < 2; t++)
-                if (live && cur.active(t, 0)) score(cur, 0, t);
-            if (live) scored(cur, 0);
-        }
-        while (live && more) {
-            Steps nxt = cur;
-            int jn    = j + 1;
-            if (jn == cur.steps) {  // on to the next piece
-                more = reader.next(qu, pc, lane, &dead, bound, live);
-                if (more) nxt = Steps(pc, pl, a.tokens), jn = 0;
+        uint32_t pos = 0, qn = 0, cnt = 0;     // tiles of the CTA before the piece, pieces, steps of the chain
+        uint32_t seen[2] = {0, 0};             // tiles of K and V passed or taken
+        // To tile i of K or V.  Those before it are the other chain's: every tile is seen, and given back, by both, so that no stage gets a phase ahead of a warp's wait.
+        auto come = [&](int v, uint32_t i, bool take) {
+            while (live && seen[v] < i + take) {
+                const uint32_t x = seen[v]++, stage = x % kStages;
+                live = mbar_wait_warp(smem_u32(v ? &v_full[stage] : &k_full[stage]), (x / kStages) & 1, &dead, bound);
+                if (x < i && lane == 0) mbar_arrive(v ? &v_empty[stage] : &k_empty[stage]);
             }
-            // the scores of a new piece come behind both sums of the old one: its queries may wait for these (the chains' meeting in the second Q tile)
-            const bool same = more && jn > 0;
+            return live;
+        };
+        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
+            const Steps st(pc, pl, a.tokens);
+            const int steps = st.of(t);
+            const uint32_t q_t = q_addr + (st.pair ? t * kTile : 0);
+            if (!(live = mbar_wait_warp(smem_u32(&q_full), qn & 1, &dead, bound))) break;
+            if (steps == 0 && lane == 0) mbar_arrive(&q_empty);
+            for (int j = -1; j < steps; j++) {  // the sums of step j, the scores of step j + 1
+                const uint32_t iv = pos + st.tile(t, max(j, 0)), ik = pos + st.tile(t, j + 1), sv_ = iv % kStages, sk_ = ik % kStages;
+                // what the loaders bring is waited for first: the weights come last
+                if (j + 1 < steps && !come(0, ik, true)) break;
+                if (j >= 0) {
+                    if (!come(1, iv, true)) break;
+                    const uint64_t vd = make_desc_kv<HD>(v_addr + sv_ * kTile);
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                if (live && cur.active(t, j)) {
-                    const uint32_t i = vpos + (cur.pair ? 0 : t), stage = i % kStages;
-                    live = mbar_wait_warp(smem_u32(&v_full[stage]), (i / kStages) & 1, &dead, bound);
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {  // O_t += P_t V, 64 positions at a time
-                        live = live && mbar_wait_warp(smem_u32(&p_full[t][k]), cnt[t] & 1, &dead, bound);
+                    for (int k = 0; k < kParts4; k++) {  // O_t += P_t V, 32 positions at a time
+                        live = live && mbar_wait_warp(pfull + 8 * k, cnt & 1, &dead, bound);
                         tc_fence_after();
-                        if (live) umma_sums_x4<kGroup>(tmem + 256 + t * HD, tmem + t * 128 + k * 32, make_desc_kv<HD>(v_addr + stage * kTile + k * 8 * kGroup), id_o, j > 0 || k > 0);
+                        if (live) umma_sums_x2<kGroup>(o_t, s_t + k * 16, vd + k * (4 * kGroup / 16), id_o, j > 0 || k > 0);
                     }
-                    cnt[t]++;
-                    if (live) umma_commit_a(smem_u32(&o_done[t]));
+                    if (!live) break;
+                    umma_commit_a(odone);
+                    umma_commit_a(smem_u32(&v_empty[sv_]));
+                    cnt++;
                 }
-                if (live && same && nxt.active(t, jn)) score(nxt, jn, t);  // behind the O above, which reads the weights from the same columns
+                if (j + 1 < steps) {  // S_t = Q K^T, behind the O above, which reads the weights from the same columns
+                    tc_fence_after();
+                    const uint32_t kd = k_addr + sk_ * kTile;
+#pragma unroll
+                    for (int k = 0; k < kParts; k++) umma_scores_x4(s_t, make_desc_sw128(q_t + k * kHalf), make_desc_kv<HD>(kd + k * 1024), id_s, k > 0);
+                    umma_commit_a(sfull);
+                    if (lane == 0) mbar_arrive_a(sfull);  // for what the loader wrote beside the tile
+                    umma_commit_a(smem_u32(&k_empty[sk_]));
+                    if (j + 2 == steps) umma_commit_a(smem_u32(&q_empty));
+                }
             }
-            if (live && more && !same) {
-                queries();
-                for (int t = 0; t < 2; t++)
-                    if (live && nxt.active(t, 0)) score(nxt, 0, t);
-            }
-            if (!live) break;
-            for (int i = 0; i < cur.wide(j); i++) umma_commit_a(smem_u32(&v_empty[(vpos + i) % kStages]));
-            vpos += cur.wide(j);
-            if (more) scored(nxt, jn);
-            cur = nxt, j = jn;
+            pos += st.n, qn++;
+            come(0, pos, false), come(1, pos, false);
         }
         if (!live) {
-            umma_commit_a(smem_u32(&done_bar));
-            mbar_drain(smem_u32(&done_bar), 0, bound);
+            umma_commit_a(smem_u32(&done_bar[t]));
+            mbar_drain(smem_u32(&done_bar[t]), 0, bound);
         }
-    } else if (warp == kPlanW) {
-        paged_plan<kKV>(true, qu, pg, pl, cta, warp, kThreads / 32, lane, a.rec, &dead, bound);
     } else if (bound.drop != cta + 1) {
         // Q and K, or V
         const bool isv = warp == kLoadV;
         const int n_box = kKV / a.box, bx = lane;  // a lane per box; bx >= n_box: none
         uint32_t pos = 0, landed = 0, qn = 0, xn = 0;  // tiles, ragged tiles, pieces, pieces with an exchange
         bool met = false;
-        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
+        PagedPlanner<kKV> plan(pg, pl, lane);
+        if (isv) {
+            plan.start(qu, cta);
+            plan.push(qu, cta, a.rec, &dead, bound);
+        }
+        while (live) {
+            if (isv) plan.push(qu, cta, a.rec, &dead, bound);  // one ahead
+            if (!reader.next(qu, pc, lane, &dead, bound, live)) break;
             const Steps st(pc, pl, a.tokens);
             const int head = pc.head;
             int next_row = 0;

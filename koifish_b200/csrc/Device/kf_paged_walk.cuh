@@ -139,56 +139,62 @@ struct PagedQueue {  // shared memory
         for (int i = 0; i < kPieceSlots; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], readers);
     }
 };
-// The planning warp.  From 33 sequences on all warps of the CTA have been here with plan false, behind which they meet.  rec (or NULL): the piece that later runs go on
-// with, per run, last 0 where there is none (for the kernel that merges them).
+// Works the pieces of run `index` out.  From 33 sequences on all warps of the CTA count first, and meet behind it.
 template <int TILE>
-__device__ __noinline__ void paged_plan(bool plan, PagedQueue& qu, const KfPaged& pg, const PagedPlan& pl, int index, int warp, int warps, int lane, PagedPiece* rec, volatile int* dead,
-                                        const KfBound& bound) {
-    PagedWalk<TILE> walk(pg, pl, lane);
-    if (!plan) {
+struct PagedPlanner {
+    PagedWalk<TILE> walk;
+    int u = 0, u0 = 0, u1 = 0, run = 1;
+    uint32_t i = 0;
+    bool more = true;
+    PagedPiece pc;
+    __device__ __forceinline__ PagedPlanner(const KfPaged& pg, const PagedPlan& pl, int lane) : walk(pg, pl, lane) {}
+    static __device__ __noinline__ void count(const KfPaged& pg, const PagedPlan& pl, int* s_sum, int warp, int warps, int lane) {
+        PagedWalk<TILE> walk(pg, pl, lane);
 #pragma unroll 1
         for (int w = warp; w < (pg.n_seq + 31) / 32; w += warps) {
             walk.load(w * 32);
-            if (lane == 31) qu.s_sum[w] = walk.inc;
+            if (lane == 31) s_sum[w] = walk.inc;
         }
-        return;
     }
-    int W = 0, u = 0, u1 = 0, run = 1;
-    bool ready = false;
-    if (pg.n_seq <= 32) {
-        walk.load(0);
-        W = walk.total(), ready = true;
-    } else {
-        for (int w = lane; w < (pg.n_seq + 31) / 32; w += 32) W += qu.s_sum[w];
-        W = __reduce_add_sync(0xffffffffu, W);
+    __device__ __forceinline__ void start(const PagedQueue& qu, int index) {
+        int W = 0;
+        if (walk.pg.n_seq <= 32) {
+            walk.load(0);
+            W = walk.total();
+        } else {
+            for (int w = walk.lane; w < (walk.pg.n_seq + 31) / 32; w += 32) W += qu.s_sum[w];
+            W = __reduce_add_sync(0xffffffffu, W);
+        }
+        run = max(walk.pl.min_run, (W + walk.pl.runs - 1) / walk.pl.runs);
+        u = u0 = (int)min((long long)W, (long long)index * run), u1 = min(W, u + run);
+        if (u < u1 && walk.pg.n_seq > 32) walk.seek(qu.s_sum, u);
+        pc.last = 0;
     }
-    run = max(pl.min_run, (W + pl.runs - 1) / pl.runs);
-    u = (int)min((long long)W, (long long)index * run), u1 = min(W, u + run);
-    if (u < u1 && !ready) walk.seek(qu.s_sum, u);
-    const int u0 = u;
-    PagedPiece pc;
-    pc.last = 0;
-    for (uint32_t i = 0;; i++) {
-        const bool more = u < u1;
+    // the next piece to the readers; false: there was none, which they have been told.  rec (or NULL): behind the last, the piece that later runs go on with, last 0
+    // where there is none (for the kernel that merges them)
+    __device__ __forceinline__ bool push(PagedQueue& qu, int index, PagedPiece* rec, volatile int* dead, const KfBound& bound) {
+        if (!more) return false;
+        more = u < u1;
         if (more) {
             pc = walk.at(u, u1, run);
             u += pc.t1 - pc.t0;
         } else {
-            if (rec && lane == 0) {
+            if (rec && walk.lane == 0) {
                 if (u0 == u1 || pc.whole || pc.first != index || pc.last == index) pc.last = 0;
                 rec[index] = pc;
             }
             pc.t0 = -1;
         }
         const uint32_t slot = i % kPieceSlots;
-        if (!mbar_wait_warp(smem_u32(&qu.empty[slot]), ((i / kPieceSlots) & 1) ^ 1, dead, bound)) return;
-        if (lane == 0) {
+        if (!mbar_wait_warp(smem_u32(&qu.empty[slot]), ((i / kPieceSlots) & 1) ^ 1, dead, bound)) return more = false;
+        if (walk.lane == 0) {
             qu.piece[slot] = pc;
             mbar_arrive(&qu.full[slot]);
         }
-        if (!more) return;
+        i++;
+        return more;
     }
-}
+};
 // a reader's way through the pieces: false behind the last, or when a wait has run out (live)
 struct PagedReader {
     uint32_t i = 0;

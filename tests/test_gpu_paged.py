@@ -83,9 +83,10 @@ class Step:
         return pool[idx].reshape(-1, self.kv, self.hd)[:n].double(), ok
 
     def expect(self, scale, window, q=None):
-        """(result, bound) of attention.  The bound counts: the result's rounding; the rounding of a weight to bf16 before the product with V (the sum of the weights is not
-        rounded), together at most half a step of the weighted mean of |v|; fp32 errors of a score, hd + 2 roundings of sums whose terms add up to |q|.|k|, which change a
-        weight by as much, and 2^-20 for exponentials and sums; each of them in numerator and denominator."""
+        """(result, bound) of attention.  The bound counts: the result's rounding, at most half a step of it; the rounding of a weight to bf16, (1 + e) with |e| <= half a step
+        -- where the sum of the weights is not rounded with them it changes the result by at most that much of the weighted mean of |v|, where it is, by sum w e (v - r), at most
+        that much of mean |v| + |r|; fp32 errors of a score, hd + 2 roundings of sums whose terms add up to |q|.|k|, which change a weight by as much, and 2^-20 for
+        exponentials and sums; each of them in numerator and denominator."""
         q = self.q if q is None else q
         out = torch.full((self.rows, self.heads * self.hd), float("nan"), device="cuda", dtype=torch.float64)
         tol = torch.zeros_like(out)
@@ -115,7 +116,7 @@ class Step:
                 mean = w @ vh.abs()
                 delta = (hd + 2) * 2.0 ** -24 * (torch.where(sees, size, torch.zeros_like(size)).amax(1, keepdim=True) if e else 0) + 2.0 ** -20
                 out[a:a + n, h * hd:(h + 1) * hd] = r
-                tol[a:a + n, h * hd:(h + 1) * hd] = 1.01 * (HALF16 * r.abs() + (HALF16 + 2 * delta) * mean) + 1e-30
+                tol[a:a + n, h * hd:(h + 1) * hd] = 1.01 * (2 * HALF16 * r.abs() + (HALF16 + 2 * delta) * mean) + 1e-30
         return out, tol
 
     def attend(self, ctx, scale, window=0, max_q=None, q=None, ldq=0, ldo=0, out=None):
