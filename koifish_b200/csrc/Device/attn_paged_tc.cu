@@ -5,8 +5,9 @@
 // scores into weights, the tensor cores work for the other.  The chains are the block's two row tiles, which share every tile of K and V -- or, where the block has one
 // row tile only, its even and odd tiles of positions, whose sums meet in shared memory at the end.
 //   warps 0-3 / 4-7  softmax of chain 0 / 1, thread = row: scores from tensor memory, running maximum, weights as bf16 back over the scores of the second half
-//   warp 8 / 9       matrix instructions of chain 0 / 1: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory, V as it lies: MN-major)
-//   warp 10 / 11     Q and K / V: page look-up and TMA, a box per page (or part of 8 .. 128 positions of it), each asked for by a lane of its own; warp 11 plans the pieces
+//   warp 8           matrix instructions of both chains in turn: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory, V as it lies: MN-major)
+//   warp 9 / 10      Q and K / V: page look-up and TMA, a box per page (or part of 8 .. 128 positions of it), each asked for by a lane of its own
+//   warp 11          the pieces
 // The tiles of all blocks and kv heads are cut into equal runs, one CTA each (PagedWalk).  Blocks that several CTAs share leave their sums in the workspace; a second
 // kernel, launched behind, merges them in order.
 // The output is rescaled whenever a maximum of the warp's rows grows, so the largest weight of a row is 1 and has no rounding error; the denominator adds the unrounded
@@ -18,7 +19,7 @@
 
 namespace {
 constexpr float kSlack = 8.f;
-constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 10, kLoadV = 11, kThreads = 12 * 32, kMasks = 8, kParts4 = 4 /* parts of a tile's weights */;
+constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kPlanW = 11, kThreads = 12 * 32, kMasks = 8, kParts4 = 2 /* parts of a tile's weights */;
 template <int HD>
 struct Cfg {
     static constexpr int kParts = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStages = HD == 128 ? 2 : 4;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sk = sq + 2 * kTile;
     uint8_t* sv = sk + kStages * kTile;
-    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts4], o_done[2], x_full, x_free, x_done, done_bar[2];
+    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts4], o_done[2], x_full, x_free, x_done, done_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ volatile int dead;
     __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
@@ -117,13 +118,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ float s_m[kQ], s_l[kQ];  // chain 1's maximum and denominator, where the chains share a row tile
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&q_full, 1), mbar_init(&q_empty, 2), mbar_init(&v_land, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 8);
-        for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 2), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 2);
+        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 8);
+        for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
         for (int t = 0; t < 2; t++) {
-            mbar_init(&s_full[t], 2), mbar_init(&o_done[t], 1), mbar_init(&done_bar[t], 1);
+            mbar_init(&s_full[t], 2), mbar_init(&o_done[t], 1);
             for (int k = 0; k < kParts4; k++) mbar_init(&p_full[t][k], 4);
         }
-        qu.init(12);
+        qu.init(11);
         dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&tm_q), tma_prefetch_map(&tm_k), tma_prefetch_map(&tm_v);
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float base = finite_or_0(m);
                 const unsigned long long sc22 = pack2(sc2, sc2), nm2 = pack2(-base, -base);
 #pragma unroll
-                for (int c = 0; c < kParts4; c++) {  // a part's O += P V runs while the next one's weights are formed
+                for (int c = 0; c < 4; c++) {  // a part's O += P V runs while the next one's weights are formed
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -220,10 +221,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         l2   = add2(l2, pack2(bf16lo(p[i]), bf16hi(p[i])));  // the weights as they are used: a rounding that numerator and denominator share
                     }
                     tmem_st16(s_row + 16 * c, p);  // over scores, which are in registers
-                    wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_a(pfull + 8 * c);
+                    if ((c + 1) % (4 / kParts4) == 0) {
+                        wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_a(pfull + 8 * (c / (4 / kParts4)));
+                    }
                 }
                 cnt++;
             }
@@ -305,78 +308,65 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             tile0 += st.n;
         }
-    } else if (warp < kLoadK) {
-        const int t = warp - kMmaW;
+    } else if (warp == kMmaW) {
         constexpr uint32_t id_s = make_idesc_bf16(128), id_o = make_idesc_bf16(HD) | (1u << 16);  // bit 16: B is MN-major
-        const uint32_t s_t = tmem + t * 128, o_t = tmem + 256 + t * HD, sfull = smem_u32(&s_full[t]), odone = smem_u32(&o_done[t]), pfull = smem_u32(&p_full[t][0]);
         const uint32_t q_addr = smem_u32(sq), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
-        uint32_t pos = 0, qn = 0, cnt = 0;     // tiles of the CTA before the piece, pieces, steps of the chain
-        uint32_t seen[2] = {0, 0};             // tiles of K and V passed or taken
-        // To tile i of K or V.  Those before it are the other chain's: every tile is seen, and given back, by both, so that no stage gets a phase ahead of a warp's wait.
-        auto come = [&](int v, uint32_t i, bool take) {
-            while (live && seen[v] < i + take) {
-                const uint32_t x = seen[v]++, stage = x % kStages;
-                live = mbar_wait_warp(smem_u32(v ? &v_full[stage] : &k_full[stage]), (x / kStages) & 1, &dead, bound);
-                if (x < i && lane == 0) mbar_arrive(v ? &v_empty[stage] : &k_empty[stage]);
-            }
-            return live;
-        };
+        uint32_t pos = 0, qn = 0, kseen = 0, vseen = 0, cnt[2] = {0, 0};  // tiles of the CTA before the piece, pieces, tiles that have landed, steps of the chains
         while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
-            const int steps = st.of(t);
-            const uint32_t q_t = q_addr + (st.pair ? t * kTile : 0);
             if (!(live = mbar_wait_warp(smem_u32(&q_full), qn & 1, &dead, bound))) break;
-            if (steps == 0 && lane == 0) mbar_arrive(&q_empty);
-            for (int j = -1; j < steps; j++) {  // the sums of step j, the scores of step j + 1
-                const uint32_t iv = pos + st.tile(t, max(j, 0)), ik = pos + st.tile(t, j + 1), sv_ = iv % kStages, sk_ = ik % kStages;
-                // what the loaders bring is waited for first: the weights come last
-                if (j + 1 < steps && !come(0, ik, true)) break;
-                if (j >= 0) {
-                    if (!come(1, iv, true)) break;
-                    const uint64_t vd = make_desc_kv<HD>(v_addr + sv_ * kTile);
+            for (int j = -1; live && j < st.of(0); j++)  // the sums of step j, the scores of step j + 1
 #pragma unroll
-                    for (int k = 0; k < kParts4; k++) {  // O_t += P_t V, 32 positions at a time
-                        live = live && mbar_wait_warp(pfull + 8 * k, cnt & 1, &dead, bound);
-                        tc_fence_after();
-                        if (live) umma_sums_x2<kGroup>(o_t, s_t + k * 16, vd + k * (4 * kGroup / 16), id_o, j > 0 || k > 0);
+                for (int t = 0; t < 2; t++) {
+                    const bool sums = live && j >= 0 && j < st.of(t), scores = live && j + 1 < st.of(t);
+                    const uint32_t iv = pos + st.tile(t, j), ik = pos + st.tile(t, j + 1), vs = iv % kStages, ks = ik % kStages;
+                    // what the loaders bring is waited for first: the weights come last
+                    if (scores && kseen <= ik) live = mbar_wait_warp(smem_u32(&k_full[ks]), (ik / kStages) & 1, &dead, bound), kseen = ik + 1;
+                    if (live && sums) {
+                        if (vseen <= iv) live = mbar_wait_warp(smem_u32(&v_full[vs]), (iv / kStages) & 1, &dead, bound), vseen = iv + 1;
+                        const uint64_t vd = make_desc_kv<HD>(v_addr + vs * kTile);
+#pragma unroll
+                        for (int k = 0; k < kParts4; k++) {  // O_t += P_t V
+                            live = live && mbar_wait_warp(smem_u32(&p_full[t][k]), cnt[t] & 1, &dead, bound);
+                            tc_fence_after();
+                            if (live)
+#pragma unroll
+                                for (int i = 0; i < 4 / kParts4; i++)
+                                    umma_sums_x2<kGroup>(tmem + 256 + t * HD, tmem + t * 128 + k * (64 / kParts4) + i * 16, vd + (k * (4 / kParts4) + i) * (4 * kGroup / 16), id_o, j > 0 || k + i > 0);
+                        }
+                        if (live) umma_commit_a(smem_u32(&o_done[t]));
+                        cnt[t]++;
                     }
-                    if (!live) break;
-                    umma_commit_a(odone);
-                    umma_commit_a(smem_u32(&v_empty[sv_]));
-                    cnt++;
-                }
-                if (j + 1 < steps) {  // S_t = Q K^T, behind the O above, which reads the weights from the same columns
-                    tc_fence_after();
-                    const uint32_t kd = k_addr + sk_ * kTile;
+                    if (live && scores) {  // S_t = Q K^T, behind the O above, which reads the weights from the same columns
+                        tc_fence_after();
+                        const uint32_t qd = q_addr + (st.pair ? t * kTile : 0), kd = k_addr + ks * kTile;
 #pragma unroll
-                    for (int k = 0; k < kParts; k++) umma_scores_x4(s_t, make_desc_sw128(q_t + k * kHalf), make_desc_kv<HD>(kd + k * 1024), id_s, k > 0);
-                    umma_commit_a(sfull);
-                    if (lane == 0) mbar_arrive_a(sfull);  // for what the loader wrote beside the tile
-                    umma_commit_a(smem_u32(&k_empty[sk_]));
-                    if (j + 2 == steps) umma_commit_a(smem_u32(&q_empty));
+                        for (int k = 0; k < kParts; k++) umma_scores_x4(tmem + t * 128, make_desc_sw128(qd + k * kHalf), make_desc_kv<HD>(kd + k * 1024), id_s, k > 0);
+                        umma_commit_a(smem_u32(&s_full[t]));
+                        if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
+                    }
+                    // tiles go back behind the last chain that reads them
+                    if (live && sums && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&v_empty[vs]));
+                    if (live && scores && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&k_empty[ks]));
+                    if (live && t == 1 && j + 2 == st.of(0)) umma_commit_a(smem_u32(&q_empty));
                 }
-            }
             pos += st.n, qn++;
-            come(0, pos, false), come(1, pos, false);
         }
         if (!live) {
-            umma_commit_a(smem_u32(&done_bar[t]));
-            mbar_drain(smem_u32(&done_bar[t]), 0, bound);
+            umma_commit_a(smem_u32(&done_bar));
+            mbar_drain(smem_u32(&done_bar), 0, bound);
         }
+    } else if (warp == kPlanW) {
+        PagedPlanner<kKV> plan(pg, pl, lane);
+        plan.start(qu, cta);
+        while (plan.push(qu, cta, a.rec, &dead, bound)) {}
     } else if (bound.drop != cta + 1) {
         // Q and K, or V
         const bool isv = warp == kLoadV;
         const int n_box = kKV / a.box, bx = lane;  // a lane per box; bx >= n_box: none
         uint32_t pos = 0, landed = 0, qn = 0, xn = 0;  // tiles, ragged tiles, pieces, pieces with an exchange
         bool met = false;
-        PagedPlanner<kKV> plan(pg, pl, lane);
-        if (isv) {
-            plan.start(qu, cta);
-            plan.push(qu, cta, a.rec, &dead, bound);
-        }
-        while (live) {
-            if (isv) plan.push(qu, cta, a.rec, &dead, bound);  // one ahead
-            if (!reader.next(qu, pc, lane, &dead, bound, live)) break;
+        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
             const int head = pc.head;
             int next_row = 0;
