@@ -237,7 +237,7 @@ int kf_sample(kf_ctx* ctx, int32_t* out_tokens_dev, const void* logits_bf16_dev,
  *      read on the device, so a captured step serves other lengths, tables and mixtures of the same panel.
  *      A table entry outside 0 .. n_pages - 1 is a page that is not there (given back behind a window, say): nothing is written to it, and no query sees its
  *      positions.  Entries behind a sequence's last position are not read.  Pages may be shared by sequences as long as no new token falls into them.
- *      Rows outside q_start[0] .. q_start[n_seq] - 1 are padding: not read, and left as they are in every output. ---- */
+ *      Rows outside q_start[0] .. q_start[n_seq] - 1 are padding: what they hold does not matter, and they are left as they are in every output. ---- */
 typedef struct kf_paged_kv {
     void* k_dev;            /* bf16 [n_pages][page_size][n_kv][head_dim], 16-byte aligned */
     void* v_dev;

@@ -3,23 +3,28 @@
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w (per head; optional),  pair j: (a, b) -> amp * (a cos t - b sin t, b cos t + a sin t),  t = pos[axis[j]][row] * inv_freq[j]
 //
-// Every element is read once and written once, so HBM bounds the large calls and latency the small ones.  A block takes one token, whose rotation is worked out once for
-// all its heads: t / pi in 64 bits, reduced to [-1, 1] there (a far position turns many times; its remainder in 32 bits would be off by more than the result's rounding),
-// then sine and cosine in 32 bits.  A head's row is spread over 8, 16 or 32 lanes with eight entries each; the lane that holds a pair's other half is found by a shuffle,
-// and a thread keeps its eight pairs' sines and cosines in registers for all the rows it takes.  The first rows are asked for before the position is known: finding the
-// sequence of a token, its page and its position are three dependent reads.  Few tokens are spread over blocks by heads.
+// Every element is read once and written once, so HBM bounds the large calls and latency the small ones.  A block takes up to four tokens, whose rotations are worked out once
+// for all their heads: t / pi in 64 bits, reduced to [-1, 1] there (a far position turns many times; its remainder in 32 bits would be off by more than the result's
+// rounding), then sine and cosine in 32 bits.  A head's row is spread over 4, 8 or 16 lanes; a lane holds eight pairs, so both of a pair's entries are its own: 16 bytes of
+// either half of the rotated part, or 32 bytes in a row where pairs lie side by side.  (With 16 bytes a lane and the other half from another lane by shuffles, one token a
+// block: 8192 tokens of 64 + 8 + 8 heads with their norm 148 us, 16001 tokens of 40 heads 165 us; here 76 and 57, 4.4 and 5.8 TB/s.)  What bounds it is how many bytes are on
+// their way: four blocks per SM, a lane's next rows asked for before it works on its own (with registers for two more rows of the norm's form three blocks fit: 78 us; without
+// the norm one row ahead is 61 us, three 69).  The first rows are asked for before the positions are known: finding the sequence of a token, its page and its position are
+// three dependent reads.  Few tokens are spread over blocks by heads.
 #include <algorithm>
+#include <type_traits>
 
 #include "kf_paged.cuh"
+#include "kf_tc.cuh"
 
 namespace {
-constexpr int kThreads = 256, kRows = 4;  // rows of a lane in flight
+constexpr int kThreads = 256, kTokens = 4;  // of a block at most
 
 struct RowsParams {
     const void *q, *k, *v;
     long long ldq, ldk, ldv, ldo;
     void* out;
-    int nq, nkv /* 0: no cache */, hd, M, rows_per_block;
+    int nq, nkv /* 0: no cache */, hd, M, tokens, rows_per_block;  // tokens of a block and rows of each
     const double* freq;
     const int32_t *axis, *pos;
     long long pos_stride;
@@ -49,158 +54,185 @@ __device__ __forceinline__ float load1(const uint16_t* p) { return bf16_bits_to_
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ void store1(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-// eight entries as they lie in memory
+// eight entries as they lie in memory, and as four pairs of floats
+typedef unsigned long long f32x2;
 template <typename X>
 struct Raw;
 template <>
 struct Raw<uint16_t> {
     uint4 a;
     __device__ __forceinline__ void load(const uint16_t* p) { a = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        f[0] = bf16lo(a.x), f[1] = bf16hi(a.x), f[2] = bf16lo(a.y), f[3] = bf16hi(a.y), f[4] = bf16lo(a.z), f[5] = bf16hi(a.z), f[6] = bf16lo(a.w), f[7] = bf16hi(a.w);
-    }
+    __device__ __forceinline__ void get(f32x2 (&f)[4]) const { f[0] = pack2(bf16lo(a.x), bf16hi(a.x)), f[1] = pack2(bf16lo(a.y), bf16hi(a.y)), f[2] = pack2(bf16lo(a.z), bf16hi(a.z)), f[3] = pack2(bf16lo(a.w), bf16hi(a.w)); }
 };
 template <>
 struct Raw<float> {
     float4 a, b;
     __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
-    __device__ __forceinline__ void get(float (&f)[8]) const { f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w; }
+    __device__ __forceinline__ void get(f32x2 (&f)[4]) const { f[0] = pack2(a.x, a.y), f[1] = pack2(a.z, a.w), f[2] = pack2(b.x, b.y), f[3] = pack2(b.z, b.w); }
 };
-__device__ __forceinline__ void store8(uint16_t* p, const float (&f)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+__device__ __forceinline__ void store8(uint16_t* p, const f32x2 (&f)[4]) {
+    const float2 a = unpack2(f[0]), b = unpack2(f[1]), c = unpack2(f[2]), d = unpack2(f[3]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y), pack_bf16x2(c.x, c.y), pack_bf16x2(d.x, d.y));
 }
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]), reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void store8(float* p, const f32x2 (&f)[4]) {
+    const float2 a = unpack2(f[0]), b = unpack2(f[1]), c = unpack2(f[2]), d = unpack2(f[3]);
+    reinterpret_cast<float4*>(p)[0] = make_float4(a.x, a.y, b.x, b.y), reinterpret_cast<float4*>(p)[1] = make_float4(c.x, c.y, d.x, d.y);
 }
 
-// LPR: lanes to a row, eight entries each; 0: rows at any element, or pairs that do not fall on whole lanes -- a warp per row, an entry or a pair per lane
-template <typename X, typename Y, int LPR>
-__global__ void __launch_bounds__(kThreads) kf_rows_kernel(const __grid_constant__ RowsParams p) {
-    constexpr int kL = LPR ? LPR : 32, kGroups = kThreads / kL;
-    __shared__ float2 s_cs[128];
-    const int tid = threadIdx.x, lane = tid & 31, grp = tid / kL, v = tid % kL, m = blockIdx.x;
+// LPR: lanes to a row, eight pairs each; 0: rows at any element, or pairs that do not fall on whole lanes -- a warp per row, an entry or a pair per lane
+template <typename X, typename Y, int LPR, bool NORM>
+__global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : 4) kf_rows_kernel(const __grid_constant__ RowsParams p) {
+    constexpr int kL = LPR ? LPR : 32, kGroups = kThreads / kL, kAhead = sizeof(X) == 4 || NORM ? 1 : 2;  // rows of a lane on their way beside those in its hands
+    __shared__ alignas(16) float s_cos[kTokens][128], s_sin[kTokens][128];
+    __shared__ long long s_row[kTokens];  // a token's row in the pools, -1: none
+    __shared__ int s_at[kTokens];         // its position in the sequence
+    __shared__ bool s_ours[kTokens];      // it belongs to a sequence
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid / kL, v = tid % kL, m0 = blockIdx.x * p.tokens, nt = min(p.tokens, p.M - m0);
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();  // the panel, positions, lengths and tables come from the kernels before us
-    const X *q = behind_wait((const X*)p.q) + m * p.ldq, *k = behind_wait((const X*)p.k) + m * p.ldk, *vv = behind_wait((const X*)p.v) + m * p.ldv;
+    const X *q = behind_wait((const X*)p.q), *k = behind_wait((const X*)p.k), *vv = behind_wait((const X*)p.v);
     const KfPaged pg = behind_wait(p.pg);
-    const int all = p.nq + 2 * p.nkv, r0 = blockIdx.y * p.rows_per_block, r1 = min(all, r0 + p.rows_per_block);
-    auto src = [&](int r) -> const X* { return r < p.nq ? q + (long long)r * p.hd : r < p.nq + p.nkv ? k + (long long)(r - p.nq) * p.hd : vv + (long long)(r - p.nq - p.nkv) * p.hd; };
-    Raw<X> raw[kRows];
-    auto fetch = [&](int rb) {
-#pragma unroll
-        for (int u = 0; u < kRows; u++)
-            if (rb + u * kGroups < r1 && v * 8 < p.hd) raw[u].load(src(rb + u * kGroups) + v * 8);
+    const int all = p.nq + 2 * p.nkv, r0 = blockIdx.y * p.rows_per_block, r1 = min(all, r0 + p.rows_per_block), half = p.rot / 2;
+    auto src = [&](int t, int r) -> const X* {
+        const long long m = m0 + t;
+        return r < p.nq ? q + m * p.ldq + r * p.hd : r < p.nq + p.nkv ? k + m * p.ldk + (r - p.nq) * p.hd : vv + m * p.ldv + (r - p.nq - p.nkv) * p.hd;
     };
-    if (LPR) fetch(r0 + grp);
-
-    int at = 0;            // position in the sequence
-    long long row = -1;    // the token's row in the pools
+    // a lane's two runs of eight entries: the pairs' first and second entries, entries side by side, or behind the rotated part
+    const int ea = p.layout && 8 * v < half ? 8 * v : p.layout ? p.rot + 16 * (v - half / 8) : 16 * v, eb = p.layout && 8 * v < half ? half + 8 * v : ea + 8;
+    const bool lives = LPR && 16 * v < p.hd;
+    Raw<X> ra[kAhead], rb[kAhead];
+    auto fetch = [&](int t, int rb0) {  // rows rb0 + grp, kGroups further on, ... of token t
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int r = rb0 + grp + u * kGroups;
+            if (lives && r < r1) {
+                const X* from = src(t, r);
+                ra[u].load(from + ea), rb[u].load(from + eb);
+            }
+        }
+    };
+    if (LPR) fetch(0, r0);
     if (p.nkv) {
-        const int s = find_seq(pg, m, lane);
-        if (s < 0) return;  // padding
-        int q0, n, len;
-        paged_seq(pg, s, q0, n, len);
-        at = len - n + (m - q0);
-        int in         = 0;
-        const int page = at >= 0 ? paged_page(pg, s, at, in) : -1;
-        if (page >= 0) row = page * p.page_stride + (long long)in * p.nkv * p.hd;
+        if (warp < nt) {
+            const int s = find_seq(pg, m0 + warp, lane);
+            long long row = -1;
+            int at = 0;
+            if (s >= 0) {
+                int q0, n, len, in = 0;
+                paged_seq(pg, s, q0, n, len);
+                at             = len - n + (m0 + warp - q0);
+                const int page = at >= 0 ? paged_page(pg, s, at, in) : -1;
+                if (page >= 0) row = page * p.page_stride + (long long)in * p.nkv * p.hd;
+            }
+            if (lane == 0) s_row[warp] = row, s_at[warp] = at, s_ours[warp] = s >= 0;
+        }
+        __syncthreads();
     }
-    for (int j = tid; j < p.rot / 2; j += kThreads) {
-        const int ax = p.axis ? p.axis[j] : 0;
+    for (int i = tid; i < nt * half; i += kThreads) {
+        const int t = i / half, j = i - t * half, ax = p.axis ? p.axis[j] : 0;
         float sn = 0.f, cs = 1.f;
         if (ax >= 0 && ax < p.n_axes) {
-            const double t = (double)(p.pos ? p.pos[ax * p.pos_stride + m] : at) * p.freq[j] * 0.31830988618379067154;
-            sincospif((float)(t - 2.0 * rint(0.5 * t)), &sn, &cs);
+            const double a = (double)(p.pos ? p.pos[ax * p.pos_stride + m0 + t] : s_at[t]) * p.freq[j] * 0.31830988618379067154;
+            sincospif((float)(a - 2.0 * rint(0.5 * a)), &sn, &cs);
             cs *= p.amp, sn *= p.amp;
         }
-        s_cs[j] = make_float2(cs, sn);
+        s_cos[t][j] = cs, s_sin[t][j] = sn;
     }
     __syncthreads();
-    const int half = p.rot / 2;
-    Y* out         = (Y*)p.out + m * p.ldo;
     if constexpr (LPR != 0) {
-        // this lane's pairs: entry i turns with cs[i] (layout 1), entries 2i and 2i + 1 with cs[i] (layout 0)
-        float2 cs[8];
-        const bool lower = 8 * v < half, turns = 8 * v < p.rot;
+        const bool turns = lives && 8 * v < half;
+        Raw<uint16_t> wq[2], wk[2];
+        if (NORM && lives && p.qw) wq[0].load(p.qw + ea), wq[1].load(p.qw + eb);
+        if (NORM && lives && p.kw) wk[0].load(p.kw + ea), wk[1].load(p.kw + eb);
+        for (int t = 0, rb0 = r0; t < nt;) {
+            Raw<X> ca[kAhead], cb[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int j = p.layout ? (lower ? 8 * v + i : 8 * v - half + i) : 4 * v + i;
-            cs[i]       = turns && j < half && (p.layout || i < 4) ? s_cs[j] : make_float2(1.f, 0.f);
-        }
-        const int mate = (lane & ~(LPR - 1)) | (p.layout && turns ? (lower ? v + half / 8 : v - half / 8) : v);
-        uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
-        if (p.qw && v * 8 < p.hd) wq = *reinterpret_cast<const uint4*>(p.qw + v * 8);
-        if (p.kw && v * 8 < p.hd) wk = *reinterpret_cast<const uint4*>(p.kw + v * 8);
-        for (int rb = r0 + grp; rb < r1 + grp; rb += kRows * kGroups) {  // the same number of turns for all lanes of a warp
-            if (rb != r0 + grp) fetch(rb);
+            for (int u = 0; u < kAhead; u++) ca[u] = ra[u], cb[u] = rb[u];
+            int tn = t, rn = rb0 + kAhead * kGroups;
+            if (rn >= r1) tn++, rn = r0;
+            if (tn < nt) fetch(tn, rn);  // the next rows are on their way meanwhile
+            const bool ours  = !p.nkv || s_ours[t];
+            const long long row = p.nkv ? s_row[t] : -1;
+            Y* out           = (Y*)p.out + (m0 + t) * p.ldo;
 #pragma unroll
-            for (int u = 0; u < kRows; u++) {
-                const int r = rb + u * kGroups;
-                if (__all_sync(0xffffffffu, r >= r1)) break;
-                const bool is_q = r < p.nq, is_v = r >= p.nq + p.nkv, live = r < r1 && v * 8 < p.hd;
-                float f[8];
-                raw[u].get(f);
-                const uint16_t* w = is_q ? p.qw : p.kw;
-                if (p.qw || p.kw) {
-                    float ss = 0.f;
+            for (int u = 0; u < kAhead; u++) {
+                const int r = rb0 + grp + u * kGroups;
+                if (!ours || __all_sync(0xffffffffu, r >= r1)) break;
+                const bool is_q = r < p.nq, is_v = r >= p.nq + p.nkv, live = lives && r < r1;
+                f32x2 a[4], b[4];
+                ca[u].get(a), cb[u].get(b);
+                if (NORM) {
+                    f32x2 s2 = 0ull;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) ss = live ? fmaf(f[i], f[i], ss) : 0.f;
+                    for (int i = 0; i < 4; i++) s2 = fma2(a[i], a[i], fma2(b[i], b[i], s2));
+                    const float2 s = unpack2(s2);
+                    float ss       = live ? s.x + s.y : 0.f;
 #pragma unroll
                     for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                    if (w && !is_v) {
+                    if ((is_q ? p.qw : p.kw) && !is_v) {
                         const float inv = rsqrtf(ss / (float)p.hd + p.eps);
-                        Raw<uint16_t> ww;
-                        ww.a = is_q ? wq : wk;
-                        float g[8];
-                        ww.get(g);
+                        const f32x2 iv  = pack2(inv, inv);
+                        f32x2 g[4], h[4];
+                        if (is_q) wq[0].get(g), wq[1].get(h);
+                        else wk[0].get(g), wk[1].get(h);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) f[i] = f[i] * inv * g[i];
-                    }
-                }
-                float y[8];
-                if (p.layout) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float other = __shfl_sync(0xffffffffu, f[i], mate);
-                        y[i]              = !turns || is_v ? f[i] : lower ? f[i] * cs[i].x - other * cs[i].y : f[i] * cs[i].x + other * cs[i].y;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const bool t = !is_v && 8 * v + 2 * i < p.rot;
-                        y[2 * i]     = t ? f[2 * i] * cs[i].x - f[2 * i + 1] * cs[i].y : f[2 * i];
-                        y[2 * i + 1] = t ? f[2 * i + 1] * cs[i].x + f[2 * i] * cs[i].y : f[2 * i + 1];
+                        for (int i = 0; i < 4; i++) a[i] = mul2(mul2(a[i], iv), g[i]), b[i] = mul2(mul2(b[i], iv), h[i]);
                     }
                 }
                 if (!live) continue;
-                if (is_q) store8(out + (long long)r * p.hd + v * 8, y);
-                else if (row >= 0) store8((is_v ? p.vc + row + (long long)(r - p.nq - p.nkv) * p.hd : p.kc + row + (long long)(r - p.nq) * p.hd) + v * 8, y);
+                if (turns && !is_v) {
+                    if (p.layout) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float2 cc = *reinterpret_cast<const float2*>(&s_cos[t][8 * v + 2 * i]), sn = *reinterpret_cast<const float2*>(&s_sin[t][8 * v + 2 * i]);
+                            const f32x2 c2 = pack2(cc.x, cc.y), e = a[i];
+                            a[i] = fma2(b[i], pack2(-sn.x, -sn.y), mul2(e, c2)), b[i] = fma2(e, pack2(sn.x, sn.y), mul2(b[i], c2));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float2 e = unpack2(a[i]), f = unpack2(b[i]);
+                            const float c0 = s_cos[t][8 * v + i], n0 = s_sin[t][8 * v + i], c1 = s_cos[t][8 * v + 4 + i], n1 = s_sin[t][8 * v + 4 + i];
+                            if (8 * v + i < half) a[i] = pack2(e.x * c0 - e.y * n0, e.y * c0 + e.x * n0);
+                            if (8 * v + 4 + i < half) b[i] = pack2(f.x * c1 - f.y * n1, f.y * c1 + f.x * n1);
+                        }
+                    }
+                }
+                if (is_q) {
+                    Y* to = out + r * p.hd;
+                    store8(to + ea, a), store8(to + eb, b);
+                } else if (row >= 0) {
+                    uint16_t* to = is_v ? p.vc + row + (r - p.nq - p.nkv) * p.hd : p.kc + row + (r - p.nq) * p.hd;
+                    store8(to + ea, a), store8(to + eb, b);
+                }
             }
+            t = tn, rb0 = rn;
         }
     } else {
-        for (int r = r0 + grp; r < r1; r += kGroups) {  // a warp per row
+        for (int x = grp; x < nt * (r1 - r0); x += kGroups) {  // a warp per row
+            const int t = x / (r1 - r0), r = r0 + x % (r1 - r0);
             const bool is_q = r < p.nq, is_v = r >= p.nq + p.nkv;
-            const X* x = src(r);
-            if (!is_q && row < 0) continue;
+            if (p.nkv && (!s_ours[t] || (!is_q && s_row[t] < 0))) continue;
+            const X* in_row   = src(t, r);
             const uint16_t* w = is_v ? nullptr : is_q ? p.qw : p.kw;
             float inv = 1.f;
             if (w) {
                 float ss = 0.f;
-                for (int i = lane; i < p.hd; i += 32) ss = fmaf(load1(x + i), load1(x + i), ss);
+                for (int i = lane; i < p.hd; i += 32) ss = fmaf(load1(in_row + i), load1(in_row + i), ss);
                 inv = rsqrtf(warp_sum(ss) / (float)p.hd + p.eps);
             }
-            auto in  = [&](int i) { return w ? load1(x + i) * inv * bf16_bits_to_f32(w[i]) : load1(x + i); };
-            uint16_t* c = is_q ? nullptr : is_v ? p.vc + row + (long long)(r - p.nq - p.nkv) * p.hd : p.kc + row + (long long)(r - p.nq) * p.hd;
-            auto put = [&](int i, float y) {
-                if (is_q) store1(out + (long long)r * p.hd + i, y);
+            auto in     = [&](int i) { return w ? load1(in_row + i) * inv * bf16_bits_to_f32(w[i]) : load1(in_row + i); };
+            Y* to       = (Y*)p.out + (m0 + t) * p.ldo + r * p.hd;
+            uint16_t* c = is_q ? nullptr : is_v ? p.vc + s_row[t] + (r - p.nq - p.nkv) * p.hd : p.kc + s_row[t] + (r - p.nq) * p.hd;
+            auto put    = [&](int i, float y) {
+                if (is_q) store1(to + i, y);
                 else store1(c + i, y);
             };
             const int pairs = is_v ? 0 : half;
             for (int j = lane; j < pairs; j += 32) {
                 const int ia = p.layout ? j : 2 * j, ib = p.layout ? j + half : 2 * j + 1;
-                const float a = in(ia), b = in(ib);
-                const float2 t = s_cs[j];
-                put(ia, a * t.x - b * t.y), put(ib, b * t.x + a * t.y);
+                const float a = in(ia), b = in(ib), cs = s_cos[t][j], sn = s_sin[t][j];
+                put(ia, a * cs - b * sn), put(ib, b * cs + a * sn);
             }
             for (int i = 2 * pairs + lane; i < p.hd; i += 32) put(i, in(i));
         }
@@ -209,12 +241,17 @@ __global__ void __launch_bounds__(kThreads) kf_rows_kernel(const __grid_constant
 
 template <typename X, typename Y>
 int launch_rows(kf_ctx* ctx, RowsParams& p, bool wide) {
-    const int lpr = !wide ? 0 : p.hd <= 64 ? 8 : p.hd <= 128 ? 16 : 32, groups = kThreads / (lpr ? lpr : 32), all = p.nq + 2 * p.nkv;
-    // few tokens: their heads over several blocks, up to four blocks per SM
+    const int lpr = !wide ? 0 : p.hd <= 64 ? 4 : p.hd <= 128 ? 8 : 16, groups = kThreads / (lpr ? lpr : 32), all = p.nq + 2 * p.nkv;
+    // many tokens: four to a block; few: their heads over several blocks, up to four blocks per SM
+    p.tokens        = p.M >= 4 * kTokens * ctx->sm_count ? kTokens : 1;
     const int parts = std::max(1, std::min((all + groups - 1) / groups, 4 * ctx->sm_count / p.M));
     p.rows_per_block = ((all + parts - 1) / parts + groups - 1) / groups * groups;
-    const dim3 grid(p.M, (all + p.rows_per_block - 1) / p.rows_per_block);
-    auto kern = lpr == 0 ? kf_rows_kernel<X, Y, 0> : lpr == 8 ? kf_rows_kernel<X, Y, 8> : lpr == 16 ? kf_rows_kernel<X, Y, 16> : kf_rows_kernel<X, Y, 32>;
+    const dim3 grid((p.M + p.tokens - 1) / p.tokens, (all + p.rows_per_block - 1) / p.rows_per_block);
+    auto pick = [&](auto normed) {
+        constexpr bool N = decltype(normed)::value;
+        return lpr == 0 ? kf_rows_kernel<X, Y, 0, N> : lpr == 4 ? kf_rows_kernel<X, Y, 4, N> : lpr == 8 ? kf_rows_kernel<X, Y, 8, N> : kf_rows_kernel<X, Y, 16, N>;
+    };
+    auto kern = p.qw || p.kw ? pick(std::true_type()) : pick(std::false_type());
     KF_CUDA(ctx, kf_launch_pdl(ctx, kern, grid, dim3(kThreads), 0, p));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
@@ -230,7 +267,7 @@ int rotation(kf_ctx* ctx, const kf_rotation* rot, int hd, int M, RowsParams* p) 
     p->rot = rot->rot_dims, p->layout = rot->layout, p->n_axes = rot->n_axes, p->amp = rot->amp;
     return KF_OK;
 }
-bool whole_lanes(const RowsParams& p) { return p.hd % 8 == 0 && (p.layout == 0 || p.rot % 16 == 0); }
+bool whole_lanes(const RowsParams& p) { return p.hd % 16 == 0 && (p.layout == 0 || p.rot % 16 == 0); }
 }  // namespace
 
 int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out) {
