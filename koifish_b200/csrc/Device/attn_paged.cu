@@ -1,5 +1,5 @@
-// attn_paged.cu -- attention of a step's rows over a cache in pages (kf_paged_attention): the kernel for sequences with up to 16 rows (new tokens x heads of a kv group),
-// and the choice between it and the one for more (attn_paged_tc.cu).
+// attn_paged.cu -- attention of a step's rows over a cache in pages (kf_paged_attention): the kernel for steps whose sequences have up to 16 rows a kv head (new tokens x heads
+// of its group), and the choice between it and the one for more (attn_paged_tc.cu).
 //
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = 2^(c q.k_j - m),  c = scale * log2(e),  m the largest c q.k_j so far, over the positions j that the row sees
 //
@@ -10,7 +10,11 @@
 //   * One warp looks the pages up and loads tiles of K and V by TMA into a ring of stages; a tile is as many boxes as pages (or parts of 8, 16, 32 or 64 positions of
 //     them) meet in it, each asked for by a lane of its own.  Boxes of pages that are not there are out of the tensor map's range and arrive as zeros.
 //   * Four computing warps take a tile, 16 positions each; scores and P V on mma.sync with the block's rows as the 16 rows of the A operand.
-//   * The piece that arrives last at its block merges all of them in order.
+//   * The piece that arrives last at its block merges all of them in order, a row to a warp with eight pieces on their way (sums by slices of the threads, maxima looked up
+//     first: 17 us of 85 for one sequence at 100000 positions, 10 less here).
+//   * Two CTAs of four warps per SM: one's merge runs beside the other's tiles.  (One CTA of eight: 166 against 111 us for 64 sequences, 89 against 76 for one.)
+// Measured: 64 sequences of 400 .. 4000 positions, 8 kv heads (624 MB) 111 us, 5.6 TB/s; one of 100000 positions (410 MB) 76 us, 5.4 TB/s; one of 1300 10.2 us, most of
+// it the way from the lengths over the table to the first tile and the merge.
 // Values behind a block's last position or before its window need not be numbers: their rows of V are zeroed in shared memory.
 #include <algorithm>
 
@@ -24,30 +28,21 @@ __device__ __forceinline__ void put4(uint16_t* p, float4 v, bool vec) {
     else p[0] = f32_to_bf16_bits(v.x), p[1] = f32_to_bf16_bits(v.y), p[2] = f32_to_bf16_bits(v.z), p[3] = f32_to_bf16_bits(v.w);
 }
 
-// Shared memory: a ring of stages (K and V tiles in turn) and the computing warps' sums.  SETS 1: two CTAs per SM.  A stage always comes back to the same warps, which
-// wait for each of its uses; with SETS 2, whose tiles alternate, that needs a number of stages that is a multiple of 4 (a wait tells a phase of a barrier from the one
-// before by one bit), and pieces begin behind a meeting of all warps.
-constexpr int rows_area(int hd, int sets, int rb) { return 4 * sets * rb * hd * 4; }
-constexpr int ring_stages(int hd, int sets, int rb) {
-    const int fit = ((sets == 1 ? 108 : 216) * 1024 - rows_area(hd, sets, rb)) / (kTok * hd * 2), most = fit < 10 * sets ? fit : 10 * sets;
-    return sets == 1 ? most & ~1 : most & ~3;
+// Shared memory of one of two CTAs on an SM: a ring of stages (K and V tiles in turn) and the computing warps' sums.
+constexpr int kWarps = 4, kComp = kWarps * 32, kMaxStages = 10, kSmemKB = 108;
+constexpr int rows_area(int hd, int rb) { return kWarps * rb * hd * 4; }
+constexpr int ring_stages(int hd, int rb) {
+    const int fit = (kSmemKB * 1024 - rows_area(hd, rb)) / (kTok * hd * 2);
+    return (fit < kMaxStages ? fit : kMaxStages) & ~1;
 }
-constexpr bool rings_fit() {
-    for (int hd = 64; hd <= 128; hd += 64)
-        for (int sets = 1; sets <= 2; sets++)
-            for (int rb = 1; rb <= 16; rb++)
-                if (ring_stages(hd, sets, rb) < 4 * sets) return false;
-    return true;
-}
-static_assert(rings_fit(), "two tiles of every set in flight");
+static_assert(ring_stages(128, 16) >= 4, "two tiles in flight");
 
-template <int HD, int SETS>
-__global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
+template <int HD>
+__global__ void __launch_bounds__((kWarps + 2) * 32, 2)
     kf_attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, uint16_t* out, float* ws, float2* ws_ml, unsigned* cnt, const uint16_t* q,
                          const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, long long ldo, long long ldq, int n_kv, int box /* positions */, int stages,
                          float sc2 /* scale * log2(e) */, const __grid_constant__ KfBound bound) {
     constexpr int PARTS = HD / 64, TILE = kTok * HD * 2, GROUP8 = PARTS * 1024;  // a tile lies as groups of 8 rows, each in parts of 64 dims (kf_tmap_pages)
-    constexpr int kWarps = 4 * SETS, kComp = kWarps * 32, kMaxStages = 20;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float* s_o    = reinterpret_cast<float*>(ring + (size_t)stages * TILE);  // [kWarps][rb][HD]
@@ -55,7 +50,7 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
     __shared__ volatile int dead;
     __shared__ int s_there[kMaxStages], s_last;  // bit i: positions 8 i .. 8 i + 7 of the stage's K tile are there
     __shared__ PagedQueue qu;
-    __shared__ float s_m[kWarps][16], s_l[kWarps][16], s_M[16], s_i[16];
+    __shared__ float s_m[kWarps][16], s_l[kWarps][16];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     if (tid == 0) {
         for (int s = 0; s < stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 4);
@@ -120,7 +115,7 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
             for (uint32_t k = asked > (uint32_t)stages ? asked - stages : 0; k < asked; k++) mbar_drain(smem_u32(&full[k % stages]), (k / stages) & 1, bound);
         return;
     }
-    const int set = warp >> 2, w4 = warp & 3, group = pl.group, rb = pl.tb * group;
+    const int group = pl.group, rb = pl.tb * group;
     const bool vec = ((uintptr_t)out & 7) == 0 && ldo % 4 == 0;
     uint32_t mph = 0, done = 0;  // done: tiles of this CTA before the current piece
     auto meet = [&]() {  // all computing warps; bounded like every wait
@@ -154,13 +149,13 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
 #pragma unroll
         for (int j = 0; j < HD / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
-        for (int kt = set; kt < ntiles; kt += SETS) {
+        for (int kt = 0; kt < ntiles; kt++) {
             const uint32_t n = 2 * (done + kt);
             const uint32_t sk = n % stages, pk = (n / stages) & 1, sv = (n + 1) % stages, pv = ((n + 1) / stages) & 1;
             if (!(live = mbar_wait_warp(smem_u32(&full[sk]), pk, &dead, bound))) break;
             const uint32_t kb = smem_u32(ring + (size_t)sk * TILE), vb = smem_u32(ring + (size_t)sv * TILE);
-            const int tok0 = (pc.t0 + kt) * kTok + w4 * 16;  // this warp's 16 positions
-            const unsigned there = ((unsigned)*(volatile int*)&s_there[sk] >> (w4 * 2)) & 3u;
+            const int tok0 = (pc.t0 + kt) * kTok + warp * 16;  // this warp's 16 positions
+            const unsigned there = ((unsigned)*(volatile int*)&s_there[sk] >> (warp * 2)) & 3u;
             const bool mine = tok0 < pc.hi && tok0 + 16 > pc.lo && there;
             float sc[2][4];
 #pragma unroll
@@ -169,7 +164,7 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
 #pragma unroll
                 for (int kc = 0; kc < HD / 16; kc++) {
                     uint32_t b[4];
-                    ldsm4(b, at(kb, w4 * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
+                    ldsm4(b, at(kb, warp * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
                     mma16816(sc[0], qa[kc], b[0], b[1]);
                     mma16816(sc[1], qa[kc], b[2], b[3]);
                 }
@@ -190,7 +185,7 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
                 }
                 if (tok0 + 16 > pc.hi || tok0 < pc.lo) {  // positions that no row sees: no value that might not be a number
                     for (int c = lane; c < 16 * (HD / 8); c += 32) {
-                        const int r = c / (HD / 8), ch = c % (HD / 8), row = w4 * 16 + r;
+                        const int r = c / (HD / 8), ch = c % (HD / 8), row = warp * 16 + r;
                         if (tok0 + r >= pc.hi || tok0 + r < pc.lo)
                             *reinterpret_cast<uint4*>(ring + (size_t)sv * TILE + (row >> 3) * GROUP8 + (ch >> 3) * 1024 + (row & 7) * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
@@ -223,7 +218,7 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
 #pragma unroll
                 for (int jp = 0; jp < HD / 16; jp++) {
                     uint32_t b[4];
-                    ldsm4_t(b, at(vb, w4 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, jp * 2 + (lane >> 4)));
+                    ldsm4_t(b, at(vb, warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, jp * 2 + (lane >> 4)));
                     mma16816(o[2 * jp], pa, b[0], b[1]);
                     mma16816(o[2 * jp + 1], pa, b[2], b[3]);
                 }
@@ -287,49 +282,49 @@ __global__ void __launch_bounds__((4 * SETS + 2) * 32, 3 - SETS)
             meet();
             if (live && s_last) {
                 __threadfence();
+                // a row to a warp (HD 64: the halves of the warp take every second piece), its pieces in order, kAt at a time and as many more on their way
+                constexpr int VEC = HD / 4, LANES = 32 / VEC, kAt = 8;
+                const int half = lane / VEC, c = lane % VEC * 4;
                 for (int r = warp; r < rows; r += kWarps) {
                     float M_ = -INFINITY, L_ = 0.f;
-                    for (int i = lane; i < pieces; i += 32) M_ = fmaxf(M_, __ldcg(ws_ml + slot_of(i) * rb + r).x);
-                    M_ = warp_max(M_);
-                    if (M_ != -INFINITY)
-                        for (int i = lane; i < pieces; i += 32) {
-                            const float2 ml = __ldcg(ws_ml + slot_of(i) * rb + r);
-                            L_ += ml.y * exp2f(ml.x - M_);
-                        }
-                    L_ = warp_sum(L_);
-                    if (lane == 0) s_M[r] = M_, s_i[r] = L_ == 0.f ? 0.f : 1.f / L_;
-                }
-                meet();
-                // a slice of HD / 4 threads adds every kSlices-th piece of a row, then the slices are added
-                constexpr int VEC = HD / 4, kSlices = kComp / VEC;
-                static_assert(kSlices <= 2 * kWarps, "slices fit the warps' area for half the rows at a time");
-                const int slice = tid / VEC, c = tid % VEC * 4, per = HD == 128 ? rb : (rb + 1) / 2;  // rows at a time
-                for (int r0 = 0; live && r0 < rows; r0 += per) {
-                    for (int r = r0; r < min(rows, r0 + per); r++) {
-                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                        const float M_ = s_M[r];
-#pragma unroll 8
-                        for (int i = slice; i < pieces; i += kSlices) {
-                            const size_t row = slot_of(i) * rb + r;
-                            const float4 v   = __ldcg(reinterpret_cast<const float4*>(ws + row * HD + c));
-                            const float m    = __ldcg(ws_ml + row).x, f = m == -INFINITY ? 0.f : exp2f(m - M_);
-                            a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
-                        }
-                        *reinterpret_cast<float4*>(s_o + ((size_t)slice * per + (r - r0)) * HD + c) = a;
-                    }
-                    meet();
-                    for (int idx = tid; live && idx < min(per, rows - r0) * VEC; idx += kComp) {
-                        const int r = idx / VEC, d = idx % VEC * 4;
-                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), v[kAt];
+                    float2 ml[kAt];
+                    auto ask = [&](int i0) {
 #pragma unroll
-                        for (int sl = 0; sl < kSlices; sl++) {
-                            const float4 v = *reinterpret_cast<const float4*>(s_o + ((size_t)sl * per + r) * HD + d);
-                            a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+                        for (int i = 0; i < kAt; i++) {
+                            const int at    = i0 + i * LANES + half;
+                            const size_t at_row = slot_of(min(at, pieces - 1)) * rb + r;
+                            v[i]  = __ldcg(reinterpret_cast<const float4*>(ws + at_row * HD + c));
+                            ml[i] = __ldcg(ws_ml + at_row);
+                            if (at >= pieces) ml[i].x = -INFINITY;  // asked for twice, weighs nothing
                         }
-                        const float i = s_i[r0 + r];
-                        put4(out_row(r0 + r) + d, make_float4(a.x * i, a.y * i, a.z * i, a.w * i), vec);
+                    };
+                    ask(0);
+                    for (int i0 = 0; i0 < pieces; i0 += kAt * LANES) {
+                        float4 w[kAt];
+                        float2 wl[kAt];
+                        float n = M_;
+#pragma unroll
+                        for (int i = 0; i < kAt; i++) w[i] = v[i], wl[i] = ml[i], n = fmaxf(n, ml[i].x);
+                        if (i0 + kAt * LANES < pieces) ask(i0 + kAt * LANES);
+                        const float base = n == -INFINITY ? 0.f : n, f0 = exp2f(M_ - base);
+                        M_ = n, L_ *= f0, a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0;
+#pragma unroll
+                        for (int i = 0; i < kAt; i++) {
+                            const float f = exp2f(wl[i].x - base);
+                            L_ = fmaf(wl[i].y, f, L_);
+                            a.x = fmaf(w[i].x, f, a.x), a.y = fmaf(w[i].y, f, a.y), a.z = fmaf(w[i].z, f, a.z), a.w = fmaf(w[i].w, f, a.w);
+                        }
                     }
-                    meet();
+                    if (LANES == 2) {  // the two halves' sums
+                        const float Mo = __shfl_xor_sync(0xffffffffu, M_, 16), n = fmaxf(M_, Mo), base = n == -INFINITY ? 0.f : n, f = exp2f(M_ - base);
+                        L_ *= f, a.x *= f, a.y *= f, a.z *= f, a.w *= f;
+                        L_ += __shfl_xor_sync(0xffffffffu, L_, 16);
+                        a.x += __shfl_xor_sync(0xffffffffu, a.x, 16), a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
+                        a.z += __shfl_xor_sync(0xffffffffu, a.z, 16), a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
+                    }
+                    const float i = L_ == 0.f ? 0.f : 1.f / L_;
+                    if (half == 0) put4(out_row(r) + c, make_float4(a.x * i, a.y * i, a.z * i, a.w * i), vec);
                 }
             }
         }
@@ -344,11 +339,11 @@ int box_of(int page, int most) {
     return b;
 }
 
-template <int HD, int SETS>
+template <int HD>
 int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, PagedPlan pl, void* out, long long ldo, const void* q, long long ldq, float scale) {
-    const int n_kv = kv->n_kv, teams = std::max(1, (3 - SETS) * ctx->sm_count / n_kv), grid = teams * n_kv, box = box_of(kv->page_size, kTok), rb = pl.tb * pl.group;
+    const int n_kv = kv->n_kv, teams = std::max(1, 2 * ctx->sm_count / n_kv), grid = teams * n_kv, box = box_of(kv->page_size, kTok), rb = pl.tb * pl.group;
     const size_t rows = (size_t)grid * 2 * rb;
-    pl.runs = teams, pl.min_run = 2;
+    pl.runs = teams;
     KF_REQUIRE(ctx, paged_most(kTok, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
     int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
     if (!rc) rc = kf_ensure_attn_cnt(ctx, grid);
@@ -358,15 +353,15 @@ int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, PagedPlan 
     rc = kf_tmap_pages(ctx, &tk, kv->k_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
     if (!rc) rc = kf_tmap_pages(ctx, &tv, kv->v_dev, (uint64_t)n_kv * HD, (uint64_t)kv->page_size, (uint64_t)kv->n_pages, stride, HD / 64, box);
     if (rc) return rc;
-    const int stages  = ring_stages(HD, SETS, rb);
-    const size_t smem = (size_t)stages * kTok * HD * 2 + rows_area(HD, SETS, rb) + 1024;
-    auto kern         = kf_attn_paged_kernel<HD, SETS>;
+    const int stages  = ring_stages(HD, rb);
+    const size_t smem = (size_t)stages * kTok * HD * 2 + rows_area(HD, rb) + 1024;
+    auto kern         = kf_attn_paged_kernel<HD>;
     static bool set[kf_ctx::kMaxDevices] = {};  // function attributes are per device
     if (!set[ctx->device]) {
-        KF_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (SETS == 1 ? 109 : 217) * 1024));
+        KF_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSmemKB + 1) * 1024));
         set[ctx->device] = true;
     }
-    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((4 * SETS + 2) * 32), smem, tk, tv, (uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD),
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((kWarps + 2) * 32), smem, tk, tv, (uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD),
                                ctx->attn_cnt, (const uint16_t*)q, pg, pl, ldo, ldq, n_kv, box, stages, scale * 1.4426950408889634f,
                                KfBound{ctx->wait_flags + 1, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
@@ -392,14 +387,13 @@ extern "C" int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out,
     if (!rc) rc = kf_wait_status(ctx);
     if (rc || M == 0) return rc;
     const int group = n_head / kv->n_kv;
-    // sequences with up to 16 rows a kv head here, the others on tcgen05
-    const int few = 16 / group, tokens = std::max(1, max_q);
-    if (few > 0) {
-        const PagedPlan pl{std::min(few, tokens), group, window, 0, tokens > few ? few : 0x7fffffff, 1, 0, 0};
-        rc = kv->head_dim == 128 ? launch_few<128, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<64, 1>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
-    }
-    if (!rc && tokens > few) rc = kf_attn_paged_tc(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, few);
-    return rc;
+    // steps whose sequences have up to 16 rows a kv head (new tokens x heads of the group) here, others as a whole on tcgen05: a second launch for their single tokens costs
+    // more than the few rows of their row tiles (24 sequences, three of them with chunks, 64 dims: 55 against 60 us; 16 x 5 drafted tokens, launched for nothing: 67 against
+    // 71).  Single tokens alone are faster here: 64 ragged sequences 111 against 193 us, one at 1300 positions 10 against 20.  16 rows in tokens of two: 50 against 65.
+    const int tokens = std::max(1, max_q), few = 16 / group;
+    if (tokens > few) return kf_attn_paged_tc(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window);
+    const PagedPlan pl{tokens, group, window, 1, 0};
+    return kv->head_dim == 128 ? launch_few<128>(ctx, kv, pg, pl, out, ldo, q, ldq, scale) : launch_few<64>(ctx, kv, pg, pl, out, ldo, q, ldq, scale);
 }
 // The checks and the blocks' arithmetic for tests on a host without a device
 extern "C" int kf_paged_attention_args(const kf_paged_kv* kv, const void* out, int ldo, const void* q, int ldq, int M, int n_head, float scale, int max_q) {

@@ -19,7 +19,7 @@
 
 namespace {
 constexpr float kSlack = 8.f;
-constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kPlanW = 11, kThreads = 12 * 32, kMasks = 8, kParts4 = 2 /* parts of a tile's weights */;
+constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kPlanW = 11, kThreads = 12 * 32, kMasks = 8, kParts2 = 2 /* parts of a tile's weights */;
 template <int HD>
 struct Cfg {
     static constexpr int kParts = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStages = HD == 128 ? 2 : 4;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sk = sq + 2 * kTile;
     uint8_t* sv = sk + kStages * kTile;
-    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts4], o_done[2], x_full, x_free, x_done, done_bar;
+    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts2], o_done[2], x_full, x_free, x_done, done_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ volatile int dead;
     __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 2), mbar_init(&o_done[t], 1);
-            for (int k = 0; k < kParts4; k++) mbar_init(&p_full[t][k], 4);
+            for (int k = 0; k < kParts2; k++) mbar_init(&p_full[t][k], 4);
         }
         qu.init(11);
         dead = 0;
@@ -221,11 +221,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         l2   = add2(l2, pack2(bf16lo(p[i]), bf16hi(p[i])));  // the weights as they are used: a rounding that numerator and denominator share
                     }
                     tmem_st16(s_row + 16 * c, p);  // over scores, which are in registers
-                    if ((c + 1) % (4 / kParts4) == 0) {
+                    if ((c + 1) % (4 / kParts2) == 0) {
                         wait_st();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_a(pfull + 8 * (c / (4 / kParts4)));
+                        if (lane == 0) mbar_arrive_a(pfull + 8 * (c / (4 / kParts2)));
                     }
                 }
                 cnt++;
@@ -326,13 +326,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (vseen <= iv) live = mbar_wait_warp(smem_u32(&v_full[vs]), (iv / kStages) & 1, &dead, bound), vseen = iv + 1;
                         const uint64_t vd = make_desc_kv<HD>(v_addr + vs * kTile);
 #pragma unroll
-                        for (int k = 0; k < kParts4; k++) {  // O_t += P_t V
+                        for (int k = 0; k < kParts2; k++) {  // O_t += P_t V
                             live = live && mbar_wait_warp(smem_u32(&p_full[t][k]), cnt[t] & 1, &dead, bound);
                             tc_fence_after();
                             if (live)
 #pragma unroll
-                                for (int i = 0; i < 4 / kParts4; i++)
-                                    umma_sums_x2<kGroup>(tmem + 256 + t * HD, tmem + t * 128 + k * (64 / kParts4) + i * 16, vd + (k * (4 / kParts4) + i) * (4 * kGroup / 16), id_o, j > 0 || k + i > 0);
+                                for (int i = 0; i < 4 / kParts2; i++)
+                                    umma_sums_x2<kGroup>(tmem + 256 + t * HD, tmem + t * 128 + k * (64 / kParts2) + i * 16, vd + (k * (4 / kParts2) + i) * (4 * kGroup / 16), id_o, j > 0 || k + i > 0);
                         }
                         if (live) umma_commit_a(smem_u32(&o_done[t]));
                         cnt[t]++;
@@ -485,11 +485,11 @@ __global__ void __launch_bounds__(256) kf_attn_paged_merge_kernel(const __grid_c
 }
 
 template <int HD>
-int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_n) {
+int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window) {
     const int n_kv = kv->n_kv, group = n_head / n_kv, tokens = kQ / group, grid = ctx->sm_count;
     int box = 8;
     while (box < kKV && kv->page_size % (2 * box) == 0) box *= 2;
-    const PagedPlan pl{2 * tokens, group, window, min_n, 0x7fffffff, n_kv, grid, 4};
+    const PagedPlan pl{2 * tokens, group, window, n_kv, grid};
     const size_t rows = (size_t)grid * 2 * 256;
     KF_REQUIRE(ctx, paged_most(kKV, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
     int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float) + grid * sizeof(PagedPiece));
@@ -515,7 +515,7 @@ int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, 
 }
 }  // namespace
 
-int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_n) {
-    return kv->head_dim == 128 ? launch_tc<128>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_n)
-                               : launch_tc<64>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, min_n);
+int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window) {
+    return kv->head_dim == 128 ? launch_tc<128>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window)
+                               : launch_tc<64>(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window);
 }

@@ -8,8 +8,8 @@ struct KfPaged {  // kernel parameter
     uint32_t page_mul;  // p / page = umulhi(p, page_mul) >> page_shift for 0 <= p < 2^31
     int page_shift;
 };
-// attn_paged_tc.cu: sequences with more than min_n new tokens on tcgen05
-int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int min_n);
+// attn_paged_tc.cu: on tcgen05
+int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window);
 int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out);  // paged_append.cu: arguments that all of them share
 static inline size_t kf_paged_stride(const kf_paged_kv* kv) { return kv->page_stride ? kv->page_stride : (size_t)kv->page_size * kv->n_kv * kv->head_dim; }
 

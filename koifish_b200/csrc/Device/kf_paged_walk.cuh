@@ -8,9 +8,9 @@
 #include "kf_tc.cuh"
 
 struct PagedPlan {  // kernel parameter
-    int tb, group, window, min_n, max_n;  // tokens of a block; sequences with min_n < new tokens <= max_n are taken
-    int heads;                            // kv heads that lie one after the other in the order of tiles (1: every CTA of a team has its own)
-    int runs, min_run;                    // runs at most, and their tiles at least
+    int tb, group, window;  // tokens of a block; heads of a kv group; positions that a row sees at most (<= 0: all)
+    int heads;              // kv heads that lie one after the other in the order of tiles (1: every CTA of a team has its own)
+    int runs;               // runs at most
 };
 // the positions [lo, hi) that a row of block b may see, their first tile and how many tiles they touch
 static inline __host__ __device__ int paged_block(int tile, int cap, int tb, int window, int n, int len, int b, int& lo, int& hi, int& kt0) {
@@ -60,7 +60,7 @@ struct PagedWalk {
         base = base_, n = 0, nb = 0, units = 0;
         if (base + lane < pg.n_seq) {
             paged_seq(pg, base + lane, q0, n, len);
-            if (n > pl.min_n && n <= pl.max_n) nb = n <= pl.tb ? 1 : (n + pl.tb - 1) / pl.tb, units = tiles(n, len, 0);
+            if (n > 0) nb = n <= pl.tb ? 1 : (n + pl.tb - 1) / pl.tb, units = tiles(n, len, 0);
         }
         for (unsigned many = __ballot_sync(0xffffffffu, nb > 1); many; many &= many - 1) {  // the blocks of a sequence over the lanes
             const int l = __ffs(many) - 1, n_ = __shfl_sync(0xffffffffu, n, l), len_ = __shfl_sync(0xffffffffu, len, l), nb_ = __shfl_sync(0xffffffffu, nb, l);
@@ -165,7 +165,7 @@ struct PagedPlanner {
             for (int w = walk.lane; w < (walk.pg.n_seq + 31) / 32; w += 32) W += qu.s_sum[w];
             W = __reduce_add_sync(0xffffffffu, W);
         }
-        run = max(walk.pl.min_run, (W + walk.pl.runs - 1) / walk.pl.runs);
+        run = max(1, (W + walk.pl.runs - 1) / walk.pl.runs);
         u = u0 = (int)min((long long)W, (long long)index * run), u1 = min(W, u + run);
         if (u < u1 && walk.pg.n_seq > 32) walk.seek(qu.s_sum, u);
         pc.last = 0;
