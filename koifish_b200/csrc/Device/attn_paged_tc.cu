@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sk = sq + 2 * kTile;
     uint8_t* sv = sk + kStages * kTile;
-    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts2], o_done[2], x_full, x_free, x_done, done_bar;
+    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts2], o_done[2], x_full, x_free, done_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ volatile int dead;
     __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ float s_m[kQ], s_l[kQ];  // chain 1's maximum and denominator, where the chains share a row tile
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 8);
+        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4);
         for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 2), mbar_init(&o_done[t], 1);
@@ -238,14 +238,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool whole = pc.whole, meet = !st.pair && st.n > 1;
             const size_t slot = ((size_t)cta * 2 + (pc.first == cta)) * 256 + (st.pair ? t * kQ : 0) + row;
             uint16_t* op = a.out + (pc.q0 + tok) * a.ldo + (long long)(pc.head * pl.group + row % pl.group) * HD;
-            if (meet && t == 1) s_m[row] = m2, s_l[row] = l;
-            float f0 = 1.f, f1 = 0.f;
+                        float f0 = 1.f, f1 = 0.f;
             constexpr int kCols = HD / 2;  // columns of an exchange: as many as the second Q tile, which such a block does not have, holds of 128 rows
             float4* xb = reinterpret_cast<float4*>(sq + kTile);
             for (int c0 = 0; live && c0 < HD; c0 += kCols) {
                 if (meet && t == 1) {
-                    if (c0 > 0 && !(live = mbar_wait_warp(smem_u32(&x_free), xph & 1, &dead, bound))) break;
-                    if (c0 > 0) xph++;
+                    if (!(live = mbar_wait_warp(smem_u32(&x_free), (xph & 1) ^ 1, &dead, bound))) break;  // what was there has been read
+                    xph++;
+                    if (c0 == 0) s_m[row] = m2, s_l[row] = l;
 #pragma unroll 1
                     for (int c = 0; c < kCols; c += 32) {
                         uint32_t o[32];
@@ -293,18 +293,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     if (mine && !whole && c0 == 0) __stcg(a.ws_ml + slot, make_float2(m2, l));
-                    if (meet && c0 + kCols < HD) {
+                    if (meet) {
+                        if (c0 + kCols >= HD) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the second Q tile may be the loader's next
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&x_free);
                     }
                 }
             }
             if (!live) break;
-            if (meet) {  // the second Q tile is the loader's again
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&x_done);
-            }
             tc_fence_before();
             tile0 += st.n;
         }
@@ -364,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Q and K, or V
         const bool isv = warp == kLoadV;
         const int n_box = kKV / a.box, bx = lane;  // a lane per box; bx >= n_box: none
-        uint32_t pos = 0, landed = 0, qn = 0, xn = 0;  // tiles, ragged tiles, pieces, pieces with an exchange
+        uint32_t pos = 0, landed = 0, qn = 0;  // tiles, ragged tiles, pieces
         bool met = false;
         while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
@@ -377,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             int next = page_of(pc.t0);
             if (!isv) {
                 if (qn > 0) live = mbar_wait_warp(smem_u32(&q_empty), (qn - 1) & 1, &dead, bound);
-                if (live && met) live = mbar_wait_warp(smem_u32(&x_done), xn++ & 1, &dead, bound);
+                if (live && met && st.pair) live = mbar_wait_warp(smem_u32(&x_free), 1, &dead, bound);  // the second of two rounds
                 if (!live) break;
                 met = !st.pair && st.n > 1;
                 if (lane == 0) {
@@ -438,49 +434,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Blocks that several CTAs share: block (c, s) takes rows 32 s .. 32 s + 31 of the one that begins in run c and goes on behind it, if there is one.
+// Blocks that several CTAs share: block (c, s) takes rows 32 s .. 32 s + 31 of the one that begins in run c and goes on behind it, if there is one.  A thread takes four entries
+// of several rows, the pieces in order, the next one's on their way.
 constexpr int kMergeRows = 32;
 template <int HD>
 __global__ void __launch_bounds__(256) kf_attn_paged_merge_kernel(const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a) {
+    constexpr int kStep = 256 / (HD / 4), kOwn = kMergeRows / kStep;  // rows side by side, rows of a thread
     const int tid = threadIdx.x, cta = blockIdx.x;
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();
     const PagedPiece pc = *behind_wait(a.rec + cta);
-    if (pc.last == 0) return;
-    const bool pair  = pc.n - pc.b * pl.tb > a.tokens;
-    const int pieces = pc.last - cta + 1, c = tid % (HD / 4) * 4;
-    const bool vec   = ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0;
-#pragma unroll 1
-    for (int rr = tid / (HD / 4); rr < kMergeRows; rr += 256 / (HD / 4)) {
-        const int r = blockIdx.y * kMergeRows + rr, t = r / kQ, row = r % kQ, tok = pc.b * pl.tb + t * a.tokens + row / pl.group;
-        if ((t > 0 && !pair) || row >= a.tokens * pl.group || tok >= pc.n) continue;
-        float m = -INFINITY, l = 0.f;
-        auto at = [&](int i) { return ((size_t)(cta + i) * 2 + (i == 0)) * 256 + r; };
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        // in order, four at a time: what they hold is asked for at once
-#pragma unroll 1
-        for (int i0 = 0; i0 < pieces; i0 += 4) {
-            float2 ml[4];
-            float4 v[4];
+    const bool pair     = pc.n - pc.b * pl.tb > a.tokens;
+    const int r0        = blockIdx.y * kMergeRows;
+    if (pc.last == 0 || (r0 >= kQ && !pair)) return;
+    const int pieces = pc.last - cta + 1, c = tid % (HD / 4) * 4, rr = tid / (HD / 4);
+    float m[kOwn], l[kOwn];
+    float4 o[kOwn], v[kOwn];
+    float2 ml[kOwn];
+    auto ask = [&](int i) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool in = i0 + i < pieces;
-                ml[i] = in ? __ldcg(a.ws_ml + at(i0 + i)) : make_float2(-INFINITY, 0.f);
-                v[i]  = in ? __ldcg(reinterpret_cast<const float4*>(a.ws + at(i0 + i) * HD + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            const float n = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m), f = ex2(m - finite_or_0(n));
-            m = n, l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float g = ex2(ml[i].x - finite_or_0(m));
-                l = fmaf(ml[i].y, g, l);
-                o.x = fmaf(v[i].x, g, o.x), o.y = fmaf(v[i].y, g, o.y), o.z = fmaf(v[i].z, g, o.z), o.w = fmaf(v[i].w, g, o.w);
-            }
+        for (int u = 0; u < kOwn; u++) {
+            const size_t row = ((size_t)(cta + i) * 2 + (i == 0)) * 256 + r0 + rr + u * kStep;
+            ml[u] = __ldcg(a.ws_ml + row), v[u] = __ldcg(reinterpret_cast<const float4*>(a.ws + row * HD + c));
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+    };
+    ask(0);
+#pragma unroll
+    for (int u = 0; u < kOwn; u++) m[u] = -INFINITY, l[u] = 0.f, o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i = 0; i < pieces; i++) {
+        float4 w[kOwn];
+        float2 wl[kOwn];
+#pragma unroll
+        for (int u = 0; u < kOwn; u++) w[u] = v[u], wl[u] = ml[u];
+        if (i + 1 < pieces) ask(i + 1);
+#pragma unroll
+        for (int u = 0; u < kOwn; u++) {
+            const float n = fmaxf(m[u], wl[u].x), f = ex2(m[u] - finite_or_0(n)), g = ex2(wl[u].x - finite_or_0(n));
+            m[u] = n, l[u] = fmaf(l[u], f, wl[u].y * g);
+            o[u].x = fmaf(o[u].x, f, w[u].x * g), o[u].y = fmaf(o[u].y, f, w[u].y * g), o[u].z = fmaf(o[u].z, f, w[u].z * g), o[u].w = fmaf(o[u].w, f, w[u].w * g);
+        }
+    }
+    const bool vec = ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0;
+#pragma unroll
+    for (int u = 0; u < kOwn; u++) {
+        const int r = r0 + rr + u * kStep, row = r % kQ, tok = pc.b * pl.tb + r / kQ * a.tokens + row / pl.group;
+        if (row >= a.tokens * pl.group || tok >= pc.n) continue;  // its sums are whatever lay there
+        const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
         uint16_t* op    = a.out + (pc.q0 + tok) * a.ldo + (long long)(pc.head * pl.group + row % pl.group) * HD + c;
-        if (vec) *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-        else op[0] = f32_to_bf16_bits(o.x * inv), op[1] = f32_to_bf16_bits(o.y * inv), op[2] = f32_to_bf16_bits(o.z * inv), op[3] = f32_to_bf16_bits(o.w * inv);
+        const uint32_t lo = pack_bf16x2(o[u].x * inv, o[u].y * inv), hi = pack_bf16x2(o[u].z * inv, o[u].w * inv);
+        if (vec) *reinterpret_cast<uint2*>(op) = make_uint2(lo, hi);
+        else op[0] = lo & 0xffff, op[1] = lo >> 16, op[2] = hi & 0xffff, op[3] = hi >> 16;
     }
 }
 
