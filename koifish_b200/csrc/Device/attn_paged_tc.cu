@@ -22,9 +22,9 @@ constexpr float kSlack = 8.f;
 constexpr int kQ = 128, kKV = 128, kMmaW = 8, kLoadK = 9, kLoadV = 10, kPlanW = 11, kThreads = 12 * 32, kMasks = 8, kParts2 = 2 /* parts of a tile's weights */;
 template <int HD>
 struct Cfg {
-    static constexpr int kParts = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStages = HD == 128 ? 2 : 4;
+    static constexpr int kParts = HD / 64, kTile = kKV * HD * 2, kHalf = kKV * 128, kStagesK = HD == 128 ? 2 : 4, kStagesV = HD == 128 ? 3 : 6;
     static constexpr int kGroup = kParts * 1024;  // tiles of K and V lie as groups of 8 rows, each in parts of 64 dims (kf_tmap_pages); of Q as halves of 64 dims
-    static constexpr size_t kSmem = (2 + 2 * kStages) * (size_t)kTile + 1024;
+    static constexpr size_t kSmem = (2 + kStagesK + kStagesV) * (size_t)kTile + 1024;
 };
 struct TcArgs {  // kernel parameter
     uint16_t* out;
@@ -105,21 +105,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     kf_attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                             const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ TcArgs a, const __grid_constant__ KfBound bound) {
     using C = Cfg<HD>;
-    constexpr int kTile = C::kTile, kHalf = C::kHalf, kParts = C::kParts, kGroup = C::kGroup, kStages = C::kStages;
+    constexpr int kTile = C::kTile, kHalf = C::kHalf, kParts = C::kParts, kGroup = C::kGroup, kStagesK = C::kStagesK, kStagesV = C::kStagesV;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sk = sq + 2 * kTile;
-    uint8_t* sv = sk + kStages * kTile;
-    __shared__ uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_land, s_full[2], p_full[2][kParts2], o_done[2], x_full, x_free, done_bar;
+    uint8_t* sv = sk + kStagesK * kTile;
+    __shared__ uint64_t q_full, q_empty, k_full[kStagesK], k_empty[kStagesK], v_full[kStagesV], v_empty[kStagesV], v_land, s_full[2], p_full[2][kParts2], o_done[2], x_full, x_free, done_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ volatile int dead;
     __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
     __shared__ PagedQueue qu;
-    __shared__ float s_m[kQ], s_l[kQ];  // chain 1's maximum and denominator, where the chains share a row tile
+    // chain 1's maximum and denominator, where the chains share a row tile: over the sequences' tiles, which are not looked at once the first piece is known
+    float *s_m = reinterpret_cast<float*>(qu.s_sum), *s_l = s_m + kQ;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4);
-        for (int s = 0; s < kStages; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
+        for (int s = 0; s < kStagesK; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
+        for (int s = 0; s < kStagesV; s++) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 2), mbar_init(&o_done[t], 1);
             for (int k = 0; k < kParts2; k++) mbar_init(&p_full[t][k], 4);
@@ -315,11 +317,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     const bool sums = live && j >= 0 && j < st.of(t), scores = live && j + 1 < st.of(t);
-                    const uint32_t iv = pos + st.tile(t, j), ik = pos + st.tile(t, j + 1), vs = iv % kStages, ks = ik % kStages;
+                    const uint32_t iv = pos + st.tile(t, j), ik = pos + st.tile(t, j + 1), vs = iv % kStagesV, ks = ik % kStagesK;
                     // what the loaders bring is waited for first: the weights come last
-                    if (scores && kseen <= ik) live = mbar_wait_warp(smem_u32(&k_full[ks]), (ik / kStages) & 1, &dead, bound), kseen = ik + 1;
+                    if (scores && kseen <= ik) live = mbar_wait_warp(smem_u32(&k_full[ks]), (ik / kStagesK) & 1, &dead, bound), kseen = ik + 1;
                     if (live && sums) {
-                        if (vseen <= iv) live = mbar_wait_warp(smem_u32(&v_full[vs]), (iv / kStages) & 1, &dead, bound), vseen = iv + 1;
+                        if (vseen <= iv) live = mbar_wait_warp(smem_u32(&v_full[vs]), (iv / kStagesV) & 1, &dead, bound), vseen = iv + 1;
                         const uint64_t vd = make_desc_kv<HD>(v_addr + vs * kTile);
 #pragma unroll
                         for (int k = 0; k < kParts2; k++) {  // O_t += P_t V
@@ -359,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (bound.drop != cta + 1) {
         // Q and K, or V
         const bool isv = warp == kLoadV;
+        const uint32_t stages = isv ? kStagesV : kStagesK;
         const int n_box = kKV / a.box, bx = lane;  // a lane per box; bx >= n_box: none
         uint32_t pos = 0, landed = 0, qn = 0;  // tiles, ragged tiles, pieces
         bool met = false;
@@ -388,11 +391,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 qn++;
             }
             for (int t = pc.t0; t < pc.t1; t++) {
-                const uint32_t stage = pos % kStages;
+                const uint32_t stage = pos % stages;
                 const int page = next, row = next_row;
                 next = page_of(t + 1);  // a tile ahead: the look-up takes its time
                 const unsigned lanes = __ballot_sync(0xffffffffu, page >= 0);
-                if (!(live = mbar_wait_warp(smem_u32(isv ? &v_empty[stage] : &k_empty[stage]), ((pos / kStages) & 1) ^ 1, &dead, bound))) break;
+                if (!(live = mbar_wait_warp(smem_u32(isv ? &v_empty[stage] : &k_empty[stage]), ((pos / stages) & 1) ^ 1, &dead, bound))) break;
                 const bool ragged = isv && (t * kKV < pc.lo || (t + 1) * kKV > pc.hi);
                 uint64_t* bar = !isv ? &k_full[stage] : ragged ? &v_land : &v_full[stage];
                 uint8_t* dst  = (isv ? sv : sk) + stage * kTile;
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!live) {  // copies in flight write shared memory: wait for what was asked for
             if (!isv && qn > 0) mbar_drain(smem_u32(&q_full), (qn - 1) & 1, bound);
-            for (uint32_t k = pos > (uint32_t)kStages ? pos - kStages : 0; k < pos; k++) mbar_drain(smem_u32(isv ? &v_full[k % kStages] : &k_full[k % kStages]), (k / kStages) & 1, bound);
+            for (uint32_t k = pos > stages ? pos - stages : 0; k < pos; k++) mbar_drain(smem_u32(isv ? &v_full[k % stages] : &k_full[k % stages]), (k / stages) & 1, bound);
             if (isv && landed > 0) mbar_drain(smem_u32(&v_land), (landed - 1) & 1, bound);
         }
     }
