@@ -236,7 +236,7 @@ int kf_sample(kf_ctx* ctx, int32_t* out_tokens_dev, const void* logits_bf16_dev,
  *      positions; its last row is position len[s] - 1.  Position p lies in row p % page_size of page table[s][p / page_size].  Everything per sequence is
  *      read on the device, so a captured step serves other lengths, tables and mixtures of the same panel.
  *      A table entry outside 0 .. n_pages - 1 is a page that is not there (given back behind a window, say): nothing is written to it, and no query sees its
- *      positions.  Entries behind a sequence's last position are not read.  Pages may be shared by sequences as long as no new token falls into them.
+ *      positions.  Entries behind a sequence's last position are not read.  Pages may be shared by sequences, or stand in a table twice, as long as no new token falls into them.
  *      Rows outside q_start[0] .. q_start[n_seq] - 1 are padding: what they hold does not matter, and they are left as they are in every output. ---- */
 typedef struct kf_paged_kv {
     void* k_dev;            /* bf16 [n_pages][page_size][n_kv][head_dim], 16-byte aligned */
@@ -268,8 +268,9 @@ typedef struct kf_rotation {
 int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, void* q_out_dev, int ldqo, const void* q_dev, int ldq, const void* k_dev, int ldk,
                     const void* v_dev, int ldv, int src_f32, int M, int n_head, const void* qnorm_w_dev, const void* knorm_w_dev, float eps);
 /* Causal attention of the panel's rows over the pages: a row at position p sees the positions j <= p of its sequence, with window > 0 only j > p - window.
- * out [M][ldo], q [M][ldq] bf16, n_head * head_dim entries a row; softmax(scale * q . k) in fp32.  A row that sees nothing gets zeros.  n_head / n_kv at most 64;
- * q 16-byte aligned, ldq a multiple of 8.  max_q: the largest number of new tokens of a sequence, as a hint: it chooses the kernels, results do not depend on it. */
+ * out [M][ldo], q [M][ldq] bf16, n_head * head_dim entries a row; softmax(scale * q . k) in fp32.  A row that sees nothing, or nothing but scores of -inf,
+ * gets zeros.  Keys that a row does not see may hold anything; so may values that no row of the call's sequence sees, but a value that is not a number reaches the rows
+ * of the same panel in front of it too.  n_head / n_kv at most 64; q 16-byte aligned, ldq a multiple of 8; out must not lie over q.  max_q: the largest number of new tokens of a sequence, as a hint: it chooses the kernels, results do not depend on it. */
 int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int max_q);
 /* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x. */
 int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out_dev, int ldo, const void* x_dev, int ldx, int f32, int M, int n_head, int head_dim);

@@ -377,6 +377,7 @@ static int check_args(kf_ctx* ctx, const kf_paged_kv* kv, const void* out, int l
     KF_REQUIRE(ctx, (long long)n_head * kv->head_dim <= ldq && (long long)n_head * kv->head_dim <= ldo, "rows as long as their heads");
     KF_REQUIRE(ctx, ((uintptr_t)q & 15) == 0 && ldq % 8 == 0, "q at 16 bytes, ldq a multiple of 8");
     KF_REQUIRE(ctx, (long long)M * (n_head / kv->n_kv) < 0x7fffff00, "rows");
+    KF_REQUIRE(ctx, out != q, "the result over the queries");
     KF_REQUIRE(ctx, scale > 0.f && scale < INFINITY && max_q >= 0, "scale above 0, max_q not negative");
     return KF_OK;
 }

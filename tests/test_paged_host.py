@@ -55,7 +55,7 @@ def test_caches_that_are_refused(lib, bad):
 
 
 @pytest.mark.parametrize("bad", [dict(out=None), dict(q=None), dict(ldq=1016), dict(ldo=1023), dict(q=8200), dict(ldq=1028), dict(M=-1), dict(n_head=0), dict(n_head=7), dict(n_head=130),
-                                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(max_q=-1)])
+                                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(max_q=-1), dict(out=8192), dict(M=2 ** 30)])
 def test_attention_refusals(lib, bad):
     assert attention(lib, cache(), **bad) == BAD
 
