@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sk = sq + 2 * kTile;
     uint8_t* sv = sk + kStagesK * kTile;
-    __shared__ uint64_t q_full, q_empty, k_full[kStagesK], k_empty[kStagesK], v_full[kStagesV], v_empty[kStagesV], v_land, s_full[2], p_full[2][kParts2], o_done[2], x_full, x_free, done_bar;
+    __shared__ uint64_t q_full, q_empty, k_full[kStagesK], k_empty[kStagesK], v_full[kStagesV], v_empty[kStagesV], v_land, s_full[2], p_full[2][kParts2], o_done[2], x_full, x_free, x_done, done_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ volatile int dead;
     __shared__ volatile int s_there[kMasks];  // bit i: positions 8 i .. 8 i + 7 of a tile are there; by tile
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *s_m = reinterpret_cast<float*>(qu.s_sum), *s_l = s_m + kQ;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4);
+        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&v_land, 1), mbar_init(&done_bar, 1), mbar_init(&x_full, 4), mbar_init(&x_free, 4), mbar_init(&x_done, 4);
         for (int s = 0; s < kStagesK; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
         for (int s = 0; s < kStagesV; s++) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
         for (int t = 0; t < 2; t++) {
@@ -312,9 +312,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (mine && !whole && c0 == 0) __stcg(a.ws_ml + slot, make_float2(m2, l));
                     if (meet) {
-                        if (c0 + kCols >= HD) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the second Q tile may be the loader's next
+                        const bool over = c0 + kCols >= HD;
+                        if (over) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the second Q tile may be the loader's next
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&x_free);
+                        if (over && lane == 0) mbar_arrive(&x_done);
                     }
                 }
             }
@@ -379,8 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool isv = warp == kLoadV;
         const uint32_t stages = isv ? kStagesV : kStagesK;
         const int n_box = kKV / a.box, bx = lane;  // a lane per box; bx >= n_box: none
-        uint32_t pos = 0, landed = 0, qn = 0;  // tiles, ragged tiles, pieces
-        bool met = false;
+        uint32_t pos = 0, landed = 0, qn = 0, xn = 0;  // tiles, ragged tiles, pieces, meetings that are over
+        bool met = false;  // the chains meet over the piece before this one, and that has not been waited for
         while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
             const Steps st(pc, pl, a.tokens);
             const int head = pc.head;
@@ -392,9 +394,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             int next = page_of(pc.t0);
             if (!isv) {
                 if (qn > 0) live = mbar_wait_warp(smem_u32(&q_empty), (qn - 1) & 1, &dead, bound);
-                if (live && met && st.pair) live = mbar_wait_warp(smem_u32(&x_free), 1, &dead, bound);  // the second of two rounds
+                // the chains may still be meeting over the piece before, in the second Q tile
+                if (live && met && st.pair) live = mbar_wait_warp(smem_u32(&x_done), xn++ & 1, &dead, bound), met = false;
                 if (!live) break;
-                met = !st.pair && st.n > 1;
                 if (lane == 0) {
                     const int tiles = st.pair ? 2 : 1;
                     mbar_arrive_expect_tx(&q_full, (uint32_t)(tiles * kParts * a.tokens * pl.group * 128));
@@ -411,6 +413,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int page = next, row = next_row;
                 next = page_of(t + 1);  // a tile ahead: the look-up takes its time
                 const unsigned lanes = __ballot_sync(0xffffffffu, page >= 0);
+                // ... which this warp has to have seen before the next meeting can be over (a wait tells a phase from the one before by one bit), for which a tile is missing yet
+                if (met && t + 1 == pc.t1) {
+                    if (!(live = mbar_wait_warp(smem_u32(&x_done), xn++ & 1, &dead, bound))) break;
+                    met = false;
+                }
                 if (!(live = mbar_wait_warp(smem_u32(isv ? &v_empty[stage] : &k_empty[stage]), ((pos / stages) & 1) ^ 1, &dead, bound))) break;
                 const bool ragged = isv && (t * kKV < pc.lo || (t + 1) * kKV > pc.hi);
                 uint64_t* bar = !isv ? &k_full[stage] : ragged ? &v_land : &v_full[stage];
@@ -438,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) mbar_arrive(&v_full[stage]);
                 }
             }
+            met = !isv && !st.pair && st.n > 1;
         }
         if (!live) {  // copies in flight write shared memory: wait for what was asked for
             if (!isv && qn > 0) mbar_drain(smem_u32(&q_full), (qn - 1) & 1, bound);

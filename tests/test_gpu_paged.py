@@ -238,6 +238,17 @@ def test_chunks_window(ctx, hd, window):
     Step(new, length, 8, 2, hd, 8, seed=window, drop=drop, beside=True).check(ctx, window=window)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group,kv,window", [(7, 4, 0), (7, 4, 300), (4, 2, 0)])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_mixed_runs(ctx, hd, group, kv, window, seed):
+    """Steps with several blocks in a run: blocks of one row tile and of two, of one tile of positions and of many, in every order."""
+    r = np.random.RandomState(seed)
+    new = [1, 1, 1, 90, 1, 0, 30, 1, 40, 1] + [int(r.choice([1, 1, 2, 20, 75])) for _ in range(50)]
+    length = [n + int(r.choice([0, 60, 200, r.randint(0, 900)])) for n in new]
+    Step(new, length, group * kv, kv, hd, 16, seed=seed).check(ctx, window=window)
+
+
 def test_chunks_before_the_first_position(ctx):
     """More new tokens than positions: the first rows stand before position 0 and see nothing."""
     s = Step([20, 40], [8, 33], 4, 1, 128, 8, seed=4)
