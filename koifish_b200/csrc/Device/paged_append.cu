@@ -7,9 +7,9 @@
 // for all their heads: t / pi in 64 bits, reduced to [-1, 1] there (a far position turns many times; its remainder in 32 bits would be off by more than the result's
 // rounding), then sine and cosine in 32 bits.  A head's row is spread over 4, 8 or 16 lanes; a lane holds eight pairs, so both of a pair's entries are its own: 16 bytes of
 // either half of the rotated part, or 32 bytes in a row where pairs lie side by side.  (With 16 bytes a lane and the other half from another lane by shuffles, one token a
-// block: 8192 tokens of 64 + 8 + 8 heads with their norm 148 us, 16001 tokens of 40 heads 165 us; here 76 and 57, 4.4 and 5.8 TB/s.)  What bounds it is how many bytes are on
-// their way: four blocks per SM, a lane's next rows asked for before it works on its own (with registers for two more rows of the norm's form three blocks fit: 78 us; without
-// the norm one row ahead is 61 us, three 69).  The first rows are asked for before the positions are known: finding the sequence of a token, its page and its position are
+// block: 8192 tokens of 64 + 8 + 8 heads with their norm 148 us, 16001 tokens of 40 heads 165 us; here 64 and 57, 5.2 and 5.8 TB/s.)  What bounds it is how many bytes are on
+// their way: four or five blocks per SM, a lane's next rows asked for before it works on its own.  With the norm: one row ahead and the weights in shared memory, five blocks (two rows, four blocks:
+// 67 us; weights in registers, which spill: 76); without, two rows ahead (one: 61, three: 69).  The first rows are asked for before the positions are known: finding the sequence of a token, its page and its position are
 // three dependent reads.  Few tokens are spread over blocks by heads.
 #include <algorithm>
 #include <type_traits>
@@ -81,12 +81,13 @@ __device__ __forceinline__ void store8(float* p, const f32x2 (&f)[4]) {
 
 // LPR: lanes to a row, eight pairs each; 0: rows at any element, or pairs that do not fall on whole lanes -- a warp per row, an entry or a pair per lane
 template <typename X, typename Y, int LPR, bool NORM>
-__global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : 4) kf_rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 2 ? 5 : 4) kf_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int kL = LPR ? LPR : 32, kGroups = kThreads / kL, kAhead = sizeof(X) == 4 || NORM ? 1 : 2;  // rows of a lane on their way beside those in its hands
     __shared__ alignas(16) float s_cos[kTokens][128], s_sin[kTokens][128];
     __shared__ long long s_row[kTokens];  // a token's row in the pools, -1: none
     __shared__ int s_at[kTokens];         // its position in the sequence
     __shared__ bool s_ours[kTokens];      // it belongs to a sequence
+    __shared__ alignas(16) uint16_t s_w[NORM ? 2 : 1][256];  // norm weights of q and k
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid / kL, v = tid % kL, m0 = blockIdx.x * p.tokens, nt = min(p.tokens, p.M - m0);
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();  // the panel, positions, lengths and tables come from the kernels before us
@@ -128,6 +129,11 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : 4) kf_rows_kernel(con
         }
         __syncthreads();
     }
+    if (NORM && LPR)
+        for (int i = tid; i < 2 * p.hd; i += kThreads) {
+            const uint16_t* w = i < p.hd ? p.qw : p.kw;
+            if (w) s_w[i >= p.hd][i < p.hd ? i : i - p.hd] = w[i < p.hd ? i : i - p.hd];
+        }
     for (int i = tid; i < nt * half; i += kThreads) {
         const int t = i / half, j = i - t * half, ax = p.axis ? p.axis[j] : 0;
         float sn = 0.f, cs = 1.f;
@@ -141,9 +147,6 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : 4) kf_rows_kernel(con
     __syncthreads();
     if constexpr (LPR != 0) {
         const bool turns = lives && 8 * v < half;
-        Raw<uint16_t> wq[2], wk[2];
-        if (NORM && lives && p.qw) wq[0].load(p.qw + ea), wq[1].load(p.qw + eb);
-        if (NORM && lives && p.kw) wk[0].load(p.kw + ea), wk[1].load(p.kw + eb);
         for (int t = 0, rb0 = r0; t < nt;) {
             Raw<X> ca[kAhead], cb[kAhead];
 #pragma unroll
@@ -173,8 +176,9 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : 4) kf_rows_kernel(con
                         const float inv = rsqrtf(ss / (float)p.hd + p.eps);
                         const f32x2 iv  = pack2(inv, inv);
                         f32x2 g[4], h[4];
-                        if (is_q) wq[0].get(g), wq[1].get(h);
-                        else wk[0].get(g), wk[1].get(h);
+                        Raw<uint16_t> w[2];  // from shared memory: in registers they cost a block per SM
+                        w[0].load(s_w[!is_q] + ea), w[1].load(s_w[!is_q] + eb);
+                        w[0].get(g), w[1].get(h);
 #pragma unroll
                         for (int i = 0; i < 4; i++) a[i] = mul2(mul2(a[i], iv), g[i]), b[i] = mul2(mul2(b[i], iv), h[i]);
                     }
