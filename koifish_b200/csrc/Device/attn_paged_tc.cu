@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < kKV; i += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
-                const float mn = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sc2;
+                const float mn = mine ? max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sc2 : -INFINITY;  // nobody's rows hold what lay there: they have no say in a rescaling
                 if (j == 0) {
                     m = mn;
                 } else if (__any_sync(0xffffffffu, mn > m + kSlack)) {

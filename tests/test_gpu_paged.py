@@ -530,6 +530,21 @@ def test_same_bits(ctx):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
+@pytest.mark.parametrize("group,kv", [(5, 8), (7, 4), (12, 3), (17, 3)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_same_bits_whatever_ran_before(ctx, group, kv, hd):
+    """Rows of a row tile that are nobody's hold what the call before left in shared memory, here queries fifty times as large: no result depends on them."""
+    s = Step([138, 1, 77], [2231, 900, 1500], group * kv, kv, hd, 16, seed=group)
+    other = Step([130] * 20, [400] * 20, 64, 1, hd, 16, seed=3)
+    loud = other.q * 50
+    a = s.attend(ctx, hd ** -0.5)
+    for _ in range(6):
+        other.attend(ctx, hd ** -0.5, q=loud)
+        b = s.attend(ctx, hd ** -0.5)
+        ctx.sync()
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
 def test_against_the_contiguous_cache(ctx):
     """One page per sequence is a contiguous cache: the same step through kf_attn_decode_gqa.  Both are within their bound of the 64-bit result, so within twice of each other."""
     s = Step([1] * 4, [512, 100, 33, 400], 16, 4, 128, 512, seed=40)
