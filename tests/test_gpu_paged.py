@@ -318,16 +318,8 @@ def normed(x, w, eps):
 TURN, NORM = 2.0 ** -21, 2.0 ** -20
 
 
-@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("hd,heads,kv,rot,layout,axes,norm", [
-    (128, 8, 2, 128, 1, 1, True), (128, 5, 5, 64, 1, 3, False), (128, 32, 8, 128, 0, 3, True), (64, 7, 1, 64, 1, 1, True), (64, 4, 2, 6, 0, 2, False),
-    (128, 3, 1, 40, 1, 2, True), (64, 16, 4, 0, 1, 1, True)])
-@pytest.mark.parametrize("off", [0, 1])
-def test_append(ctx, src, hd, heads, kv, rot, layout, axes, norm, off):
-    """Every layout and type, rows at 16 bytes and at any element (off), tokens on page ends, a sequence without new tokens, padding on both sides; every row of the pools
-    that belongs to no new token stays as it was."""
+def append_and_check(ctx, src, hd, heads, kv, rot, layout, axes, norm, off, new, length):
     g = gen(hd + rot + axes)
-    new, length = [1, 40, 0, 7, 1], [1, 100, 30, 24, 300]
     s = Step(new, length, heads, kv, hd, 24, seed=1, extra=1, pad=2, beside=off == 1)
     wide = (heads + 2 * kv) * hd + 8 + off
     panel = torch.randn(s.rows, wide, generator=g, device="cuda").to(src)
@@ -364,6 +356,25 @@ def test_append(ctx, src, hd, heads, kv, rot, layout, axes, norm, off):
     assert torch.equal(k0.contiguous().view(torch.int16), s.k.contiguous().view(torch.int16)) and torch.equal(v0.contiguous().view(torch.int16), s.v.contiguous().view(torch.int16))
 
 
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,heads,kv,rot,layout,axes,norm", [
+    (128, 8, 2, 128, 1, 1, True), (128, 5, 5, 64, 1, 3, False), (128, 32, 8, 128, 0, 3, True), (64, 7, 1, 64, 1, 1, True), (64, 4, 2, 6, 0, 2, False),
+    (128, 3, 1, 40, 1, 2, True), (64, 16, 4, 0, 1, 1, True)])
+@pytest.mark.parametrize("off", [0, 1])
+def test_append(ctx, src, hd, heads, kv, rot, layout, axes, norm, off):
+    """Every layout and type, rows at 16 bytes and at any element (off), tokens on page ends, a sequence without new tokens, padding on both sides; every row of the pools
+    that belongs to no new token stays as it was."""
+    append_and_check(ctx, src, hd, heads, kv, rot, layout, axes, norm, off, [1, 40, 0, 7, 1], [1, 100, 30, 24, 300])
+
+
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,heads,kv,rot,layout,axes,norm", [(128, 3, 1, 128, 1, 3, True), (64, 20, 5, 32, 0, 1, False), (128, 65, 8, 128, 0, 1, True), (64, 2, 2, 64, 1, 2, False)])
+@pytest.mark.parametrize("off", [0, 1])
+def test_append_panels(ctx, src, hd, heads, kv, rot, layout, axes, norm, off):
+    """Panels of so many tokens that a block takes four: sequences that end inside one, padding on both sides, heads that take one turn of a block and several."""
+    append_and_check(ctx, src, hd, heads, kv, rot, layout, axes, norm, off, [1501, 1, 0, 1202, 3, 1], [1501, 700, 5, 1300, 24, 1])
+
+
 def test_append_many_sequences(ctx):
     """Finding a token's sequence among up to 8192, most of them without new tokens."""
     r = np.random.RandomState(0)
@@ -398,7 +409,8 @@ def test_append_missing_pages(ctx):
 
 @pytest.mark.parametrize("t", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("M,heads,hd,rot,layout,axes", [(1, 1, 2, 2, 0, 1), (259, 16, 64, 64, 0, 2), (5, 3, 80, 80, 1, 3), (70, 2, 72, 36, 1, 2), (33, 4, 256, 256, 1, 3), (1000, 8, 128, 96, 1, 1),
-                                                        (3, 200, 32, 32, 0, 2), (2, 5, 7, 4, 1, 1)])
+                                                        (3, 200, 32, 32, 0, 2), (2, 5, 7, 4, 1, 1),
+                                                        (2371, 3, 128, 128, 1, 3), (2500, 1, 64, 48, 0, 2), (4001, 35, 96, 96, 1, 2), (2369, 2, 72, 36, 1, 1)])
 @pytest.mark.parametrize("inplace", [False, True])
 def test_rope_axes(ctx, t, M, heads, hd, rot, layout, axes, inplace):
     g = gen(M + hd)
