@@ -269,8 +269,8 @@ int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, 
                     const void* v_dev, int ldv, int src_f32, int M, int n_head, const void* qnorm_w_dev, const void* knorm_w_dev, float eps);
 /* Causal attention of the panel's rows over the pages: a row at position p sees the positions j <= p of its sequence, with window > 0 only j > p - window.
  * out [M][ldo], q [M][ldq] bf16, n_head * head_dim entries a row; softmax(scale * q . k) in fp32.  A row that sees nothing, or nothing but scores of -inf,
- * gets zeros.  Keys that a row does not see may hold anything; so may values that no row of the call's sequence sees, but a value that is not a number reaches the rows
- * of the same panel in front of it too.  n_head / n_kv at most 64; q 16-byte aligned, ldq a multiple of 8; out must not lie over q.  max_q: the largest number of new tokens of a sequence, as a hint: it chooses the kernels, results do not depend on it. */
+ * gets zeros.  Keys that a row does not see may hold anything, and so may values behind the sequence's last position or before every row's window; a value of one of
+ * the panel's own tokens that is not finite may reach rows of its sequence in front of it as well (its weight there is 0, and 0 times it is not a number).  n_head / n_kv at most 64; q 16-byte aligned, ldq a multiple of 8; out must not lie over q.  max_q: the largest number of new tokens of a sequence, as a hint: it chooses the kernels, results do not depend on it. */
 int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int max_q);
 /* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x. */
 int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out_dev, int ldo, const void* x_dev, int ldx, int f32, int M, int n_head, int head_dim);

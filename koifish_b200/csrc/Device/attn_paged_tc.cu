@@ -4,20 +4,20 @@
 // is two row tiles.  Its visible positions go by in tiles of 128, and the two chains of scores -> weights -> sums fill each other's gaps: while the softmax warps of one turn
 // scores into weights, the tensor cores work for the other.  The chains are the block's two row tiles, which share every tile of K and V -- or, where the block has one
 // row tile only, its even and odd tiles of positions, whose sums meet in shared memory at the end.
-//   warps 0-3 / 4-7  softmax of chain 0 / 1, thread = row: scores from tensor memory, running maximum, weights as bf16 back over the scores of the second half
+//   warps 0-3 / 4-7  softmax of chain 0 / 1, thread = row: scores from tensor memory into registers, running maximum, weights as bf16 back over the first half of the scores
 //   warp 8           matrix instructions of both chains in turn: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory, V as it lies: MN-major)
 //   warp 9 / 10      Q and K / V: page look-up and TMA, a box per page (or part of 8 .. 128 positions of it), each asked for by a lane of its own
 //   warp 11          the pieces
 // The tiles of all blocks and kv heads are cut into equal runs, one CTA each (PagedWalk).  Blocks that several CTAs share leave their sums in the workspace; a second
 // kernel, launched behind, merges them in order.
 // Sums are rescaled when a row's maximum has grown by more than 2^8 over the one they refer to: until about 32 tiles have gone by nearly every tile brings one of a warp's rows a
-// new maximum, and the rescaling stands in a chain's way (2048 tokens behind 8192, 32 heads: 362 us rescaling whenever a maximum grows, 301 so).  Weights up to 2^8 are
+// new maximum, and the rescaling stands in a chain's way (2048 tokens behind 8192, 32 heads: 362 us rescaling whenever a maximum grows, 301 with the slack).  Weights up to 2^8 are
 // rounded to bf16 like the others, and the denominator adds them as they are rounded: the error of a row that one weight carries cancels.  Relative to 64 bits, 512 tokens:
 // 2.3e-3 flat and 1.8e-3 sharp (scores four times as large), 2.1e-3 and 1.7e-3 rescaling always, 2.3e-3 and 2.0e-3 with the unrounded weights in the denominator; the
 // result's own rounding is 1.7e-3.
 // What bounds it: a chain's way.  A tile takes it about 3600 clocks -- scores 512, from them to the first half of the weights 1500, to the second 900, sums behind these 256, the
 // rest hand-overs -- while the tensor cores are busy for 2048 of both chains' clocks and the special-function units for as many.  Forming a quarter of the exponentials on the
-// multiply-add units made it 5 % slower, an issuing warp for each chain 16 % (they fall into step).  Measured: 301 us, 1026 TFLOP/s; 16 sequences of 500 .. 5000 positions with five
+// multiply-add units made it 5 % slower, an issuing warp for each chain 16 % (they fall into step).  Measured, with warps without rows passing: 290 us, 1070 TFLOP/s; 16 sequences of 500 .. 5000 positions with five
 // drafted tokens of 40 heads 55 us, 3.3 TB/s, where the way of a tile of V through three stages adds to it.
 // Rows of V that no row of the block sees are zeroed in shared memory, since they need not hold numbers; boxes of pages that are not there arrive as zeros.
 // Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool whole = pc.whole, meet = !st.pair && st.n > 1;
             const size_t slot = ((size_t)cta * 2 + (pc.first == cta)) * 256 + (st.pair ? t * kQ : 0) + row;
             uint16_t* op = a.out + (pc.q0 + tok) * a.ldo + (long long)(pc.head * pl.group + row % pl.group) * HD;
-                        float f0 = 1.f, f1 = 0.f;
+            float f0 = 1.f, f1 = 0.f;
             constexpr int kCols = HD / 2;  // columns of an exchange: as many as the second Q tile, which such a block does not have, holds of 128 rows
             float4* xb = reinterpret_cast<float4*>(sq + kTile);
             for (int c0 = 0; live && c0 < HD; c0 += kCols) {
