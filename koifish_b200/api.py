@@ -339,8 +339,10 @@ def paged_append(ctx, kv, rot, q, k, v, M, n_head, q_norm=None, k_norm=None, eps
     wide, kvw = n_head * kv.head_dim, kv.n_kv * kv.head_dim
     if out is None:
         out = ctx.empty(M * (ldo or wide) * 2)
-    ctx.check(ctx.lib.kf_paged_append(ctx.h, kv.ref, rot.ref if rot is not None else None, out.ptr, ldo or wide, q.ptr, ldq or wide, k.ptr, ldk or kvw, v.ptr, ldv or kvw,
-                                      int(src_f32), M, n_head, q_norm.ptr if q_norm is not None else None, k_norm.ptr if k_norm is not None else None, eps), "kf_paged_append")
+    st = ctx.lib.kf_paged_append(ctx.h, kv.ref, rot.ref if rot is not None else None, out.ptr, ldo or wide, q.ptr, ldq or wide, k.ptr, ldk or kvw, v.ptr, ldv or kvw,
+                                 int(src_f32), M, n_head, q_norm.ptr if q_norm is not None else None, k_norm.ptr if k_norm is not None else None, eps)
+    if st:
+        ctx.check(st, "kf_paged_append")
     return out
 
 
@@ -349,8 +351,9 @@ def paged_attention(ctx, kv, q, M, n_head, max_q, scale=None, window=0, ldq=0, o
     wide = n_head * kv.head_dim
     if out is None:
         out = ctx.empty(M * (ldo or wide) * 2)
-    ctx.check(ctx.lib.kf_paged_attention(ctx.h, kv.ref, out.ptr, ldo or wide, q.ptr, ldq or wide, M, n_head, kv.head_dim ** -0.5 if scale is None else scale, window, max_q),
-              "kf_paged_attention")
+    st = ctx.lib.kf_paged_attention(ctx.h, kv.ref, out.ptr, ldo or wide, q.ptr, ldq or wide, M, n_head, kv.head_dim ** -0.5 if scale is None else scale, window, max_q)
+    if st:
+        ctx.check(st, "kf_paged_attention")
     return out
 
 
@@ -359,7 +362,9 @@ def rope_axes(ctx, rot, x, M, n_head, head_dim, ldx=0, out=None, ldo=0, f32=Fals
     wide = n_head * head_dim
     if out is None:
         out = ctx.empty(M * (ldo or wide) * (4 if f32 else 2))
-    ctx.check(ctx.lib.kf_rope_axes(ctx.h, rot.ref, out.ptr, ldo or (ldx if out is x and ldx else wide), x.ptr, ldx or wide, int(f32), M, n_head, head_dim), "kf_rope_axes")
+    st = ctx.lib.kf_rope_axes(ctx.h, rot.ref, out.ptr, ldo or (ldx if out is x and ldx else wide), x.ptr, ldx or wide, int(f32), M, n_head, head_dim)
+    if st:
+        ctx.check(st, "kf_rope_axes")
     return out
 
 
