@@ -532,6 +532,43 @@ def test_serving_captured():
     c.close()
 
 
+def test_two_captured_steps():
+    """Two captured steps of one context, which share its workspace, replayed in turn and twice each; a context without a workspace refuses the capture and works afterwards."""
+    c = kf.Context(0)
+    a, b = Step([1, 1], [3000, 800], 8, 2, 128, 16, seed=60), Step([90, 1, 7], [700, 2000, 300], 8, 2, 64, 16, seed=61)
+    outs = [torch.full((s.rows, s.heads * s.hd), 7.0, device="cuda", dtype=torch.bfloat16) for s in (a, b)]
+    torch.cuda.synchronize()
+    ctx_call = lambda s, o: kf.paged_attention(c, s.desc, At(s.q), s.rows, s.heads, max_q=max(s.new), scale=0.1, out=At(o))  # noqa: E731
+    h = C.c_void_p()
+    c.check(c.lib.kf_graph_begin(c.h), "begin")
+    with pytest.raises(kf.KoifishError, match="before graph capture"):
+        ctx_call(a, outs[0])
+    c.check(c.lib.kf_graph_end(c.h, C.byref(h)), "end")
+    c.check(c.lib.kf_graph_destroy(h), "destroy")
+    for s, o in zip((b, a), reversed(outs)):
+        ctx_call(s, o)
+    graphs = []
+    for s, o in zip((a, b), outs):
+        h = C.c_void_p()
+        c.check(c.lib.kf_graph_begin(c.h), "begin")
+        ctx_call(s, o)
+        c.check(c.lib.kf_graph_end(c.h, C.byref(h)), "end")
+        graphs.append(h)
+    c.sync()
+    for o in outs:
+        o.fill_(7.0)
+    torch.cuda.synchronize()
+    for h in graphs * 2 + graphs[::-1]:
+        c.check(c.lib.kf_graph_launch(c.h, h), "launch")
+    c.sync()
+    for s, o in zip((a, b), outs):
+        ref, tol = s.expect(0.1, 0)
+        assert torch.all((o.double() - ref).abs() <= tol)
+    for h in graphs:
+        c.check(c.lib.kf_graph_destroy(h), "destroy")
+    c.close()
+
+
 def test_same_bits(ctx):
     """Pieces are merged in order: the same call gives the same bits."""
     s = Step([1, 1, 60, 5], [3000, 700, 900, 5000], 8, 2, 128, 16, seed=31)
