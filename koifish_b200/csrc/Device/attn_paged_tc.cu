@@ -374,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == kPlanW) {
         PagedPlanner<kKV> plan(pg, pl, lane);
+        if (lane == 0) a.rec[cta].last = 0;  // nothing to merge, should a wait run out before the end of the run is known
         plan.start(qu, cta);
         while (plan.push(qu, cta, a.rec, &dead, bound)) {}
     } else if (bound.drop != cta + 1) {
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(256) kf_attn_paged_merge_kernel(const __grid_c
     const PagedPiece pc = *behind_wait(a.rec + cta);
     const bool pair     = pc.n - pc.b * pl.tb > a.tokens;
     const int r0        = blockIdx.y * kMergeRows;
-    if (pc.last == 0 || (r0 >= kQ && !pair)) return;
+    if (pc.last <= cta || pc.last >= (int)gridDim.x || (r0 >= kQ && !pair)) return;  // last 0: nothing that goes on
     const int pieces = pc.last - cta + 1, c = tid % (HD / 4) * 4, rr = tid / (HD / 4);
     float m[kOwn], l[kOwn];
     float4 o[kOwn], v[kOwn];

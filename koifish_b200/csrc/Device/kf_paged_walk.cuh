@@ -171,7 +171,7 @@ struct PagedPlanner {
         pc.last = 0;
     }
     // the next piece to the readers; false: there was none, which they have been told.  rec (or NULL): behind the last, the piece that later runs go on with, last 0
-    // where there is none (for the kernel that merges them)
+    // where there is none (for the kernel that merges them).  It stays unwritten when a wait runs out before
     __device__ __forceinline__ bool push(PagedQueue& qu, int index, PagedPiece* rec, volatile int* dead, const KfBound& bound) {
         if (!more) return false;
         more = u < u1;

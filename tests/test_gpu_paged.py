@@ -639,3 +639,35 @@ def test_wait_that_runs_out_is_reported():
         c.sync()
         s.check(c)
         c.close()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cta", [0, 70])
+@pytest.mark.parametrize("fresh", [False, True])
+def test_wait_that_runs_out_among_many_pieces(hd, cta, fresh):
+    """A thread block that loads nothing and whose run is longer than the queue of pieces, so that it never comes to the run's end: what the merge reads of it says so, whatever the
+    workspace held -- nothing yet, or sums of the other head size over the records.  The error is told, rows of nobody stay as they are, and the next call is right."""
+    c = kf.Context(0, stream=torch.cuda.current_stream().cuda_stream or 1)
+    r = np.random.RandomState(hd)
+    length = r.randint(20, 121, 200).tolist() + [400]
+    s = Step([1] * 200 + [256], length, 32, 8, hd, 16, seed=hd, extra=2, pad=3)
+    other = Step([130] * 20, [400] * 20, 64, 1, 192 - hd, 16, seed=3)
+    # tiles: one for each of the 200 and kv head; the chunk's are fewer than 200 more a head, so a run of the first 70 thread blocks and more is pieces of one tile
+    run = -(-8 * 200 // c.lib.kf_ctx_sm_count(c.h))
+    assert run >= 6 and (cta + 1) * run < 8 * 200
+    if not fresh:
+        other.attend(c, 0.1)
+        s.check(c)
+        other.attend(c, 0.1, q=other.q * 50)
+    c.sync()
+    out = torch.full((s.rows, 32 * hd), 7.0, device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    c.set_int("attn_wait_us", 20000), c.set_int("attn_drop", cta + 1)
+    s.attend(c, 0.1, out=out)
+    with pytest.raises(kf.KoifishError, match="wait ran out"):
+        c.sync()
+    c.set_int("attn_drop", 0), c.set_int("attn_wait_us", 0)
+    assert torch.all(out[:2] == 7) and torch.all(out[-3:] == 7)
+    c.sync()
+    s.check(c)
+    c.close()
