@@ -16,7 +16,7 @@ static inline size_t kf_paged_stride(const kf_paged_kv* kv) { return kv->page_st
 // With l bits in page - 1: page_mul = ceil(2^(31 + l) / page) exceeds the quotient by less than page, so p * page_mul / 2^(31 + l) exceeds p / page by less than p / 2^(31 + l) < 1 / page
 static inline void kf_paged_divisor(KfPaged* pg) {
     int l = 0;
-    while ((1 << l) < pg->page) l++;
+    while ((1ll << l) < pg->page) l++;  // up to 31
     pg->page_mul = (uint32_t)(((1ull << (31 + l)) + pg->page - 1) / pg->page), pg->page_shift = l - 1;
 }
 #ifdef __CUDACC__

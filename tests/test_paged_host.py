@@ -128,3 +128,12 @@ def test_page_of_a_position(lib):
         for p in near + r.randint(0, 2 ** 31 - 1, 200).tolist():
             if 0 <= p < 2 ** 31:
                 assert lib.kf_paged_page_of(page, p) == p // page
+
+
+@pytest.mark.parametrize("page", [(1 << 30) + 8, (1 << 30) + (1 << 29), 2 ** 31 - 264])
+def test_largest_pages(lib, page):
+    """Pages of more than 2^30 positions: accepted as one column of a table, and divided by."""
+    assert attention(lib, cache(page_size=page, table_cols=1, n_kv=1), n_head=8) == 0 and append(lib, cache(page_size=page, table_cols=1), None) == 0
+    assert attention(lib, cache(page_size=page, table_cols=2)) == BAD
+    for p in [0, 1, 7, page // 2, page - 1, page, page + 1, 2 ** 31 - 1]:
+        assert lib.kf_paged_page_of(page, p) == p // page
