@@ -103,10 +103,10 @@ uint64_t kf_scratch_generation(kf_ctx* ctx);
  * kernel; default 1024), "tc_min_m" (token count from which kf_linear* use the tcgen05 GEMM: -1 = measured per-type crossover, 0 = never, n = from n),
  * "tc_bn" (token tile of the tcgen05 GEMM: 16, 32, 64, 128 or 256; 0 = by modelled time), "attn_tc_min_m" (panel size from which
  * kf_attn_prefill takes the tcgen05 kernel, at least 65 tokens; 0 = where it is the faster one), "attn_wait_us" (how long a wait inside kf_attn_prefill /
- * kf_attn_decode_gqa may take, default 4 s; when one runs out the kernel ends and kf_ctx_sync -- or the next of these calls -- returns KF_ERR_CUDA, once, and the
+ * kf_attn_decode_gqa / kf_paged_attention may take, default 4 s; when one runs out the kernel ends and kf_ctx_sync -- or the next of these calls -- returns KF_ERR_CUDA, once, and the
  * context is usable again), "attn_drop" (n > 0: the n-th thread block of these kernels loads nothing, so that its waits run out; for tests) */
 int kf_ctx_set_int(kf_ctx* ctx, const char* key, int value);
-int kf_ctx_get_int(kf_ctx* ctx, const char* key, int* value_out); /* gqa_min_ctx, tc_min_m, pdl, attn_split; attn_tc_error, attn_gqa_error (waits for the stream): not 0 when a bounded wait of these kernels ran out and has not been reported yet; tmap_weights: tensor maps of weights held; gemv_last_s, gemv_last_kernel: k-parts and file (0 gemv.cu, 1 gemv_tma.cu, 2 gemv_i8.cu) of the last skinny matmul; tc_last_bn, tc_last_split, tc_last_cluster: token tile, k-parts and whether these met in clusters, of the last tcgen05 GEMM */
+int kf_ctx_get_int(kf_ctx* ctx, const char* key, int* value_out); /* gqa_min_ctx, tc_min_m, pdl, attn_split; attn_tc_error (kf_attn_prefill), attn_gqa_error (kf_attn_decode_gqa), attn_paged_error (kf_paged_attention) (wait for the stream): not 0 when a bounded wait of these kernels ran out and has not been reported yet; tmap_weights: tensor maps of weights held; gemv_last_s, gemv_last_kernel: k-parts and file (0 gemv.cu, 1 gemv_tma.cu, 2 gemv_i8.cu) of the last skinny matmul; tc_last_bn, tc_last_split, tc_last_cluster: token tile, k-parts and whether these met in clusters, of the last tcgen05 GEMM */
 
 /* ---- device memory (huTensor::Alloc_1, src/Device/CUDA/huTensor.cu:70-103) ---- */
 int kf_malloc(kf_ctx* ctx, size_t bytes, void** dev_out);

@@ -395,7 +395,7 @@ int gqa_launch(kf_ctx* ctx, void* out, const void* q, const void* kc, const void
     const long long items = (long long)M * runs * n_kv, slots = (long long)(3 - SETS) * ctx->sm_count;
     KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3((unsigned)std::min(items, slots)), dim3((4 * SETS + 1) * 32), smem, tk, tv, (uint16_t*)out, ws,
                                reinterpret_cast<float2*>(ws ? ws + rows * HD : nullptr), ctx->attn_cnt, (const uint16_t*)q, pos_dev, M, n_head, n_kv, max_seq, chunk, runs, stages,
-                               1.4426950408889634f / sqrtf((float)HD), KfBound{ctx->wait_flags + 1, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+                               1.4426950408889634f / sqrtf((float)HD), KfBound{ctx->wait_flags + kWaitDecode, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
 }

@@ -363,7 +363,7 @@ int launch_few(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, PagedPlan 
     }
     KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((kWarps + 2) * 32), smem, tk, tv, (uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD),
                                ctx->attn_cnt, (const uint16_t*)q, pg, pl, ldo, ldq, n_kv, box, stages, scale * 1.4426950408889634f,
-                               KfBound{ctx->wait_flags + 1, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+                               KfBound{ctx->wait_flags + kWaitPaged, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
 }

@@ -539,7 +539,7 @@ int launch_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, 
     }
     const TcArgs a{(uint16_t*)out, ctx->attn_ws, reinterpret_cast<float2*>(ctx->attn_ws + rows * HD), reinterpret_cast<PagedPiece*>(ctx->attn_ws + rows * (HD + 2)), ldo, tokens, box,
                    scale * 1.4426950408889634f};
-    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, tq, tk, tv, pg, pl, a, KfBound{ctx->wait_flags, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, tq, tk, tv, pg, pl, a, KfBound{ctx->wait_flags + kWaitPaged, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
     KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_paged_merge_kernel<HD>, dim3(grid, 256 / kMergeRows), dim3(256), 0, pl, a));
     KF_LAUNCH_CHECK(ctx);

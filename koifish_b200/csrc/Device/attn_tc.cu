@@ -282,7 +282,7 @@ int kf_attn_prefill_tc(kf_ctx* ctx, void* out, const void* q, const void* kc, co
         set[ctx->device] = true;
     }
     KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_prefill_tc_kernel, dim3((M + kQ - 1) / kQ, n_head / 2), dim3(kThreads), kSmem, tq, tk, tv, (uint16_t*)out, pos_dev, M, n_head, n_kv,
-                               max_seq, 1.4426950408889634f / sqrtf((float)kHD), KfBound{ctx->wait_flags, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+                               max_seq, 1.4426950408889634f / sqrtf((float)kHD), KfBound{ctx->wait_flags + kWaitPrefill, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
 }

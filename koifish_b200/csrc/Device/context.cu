@@ -63,13 +63,13 @@ extern "C" int kf_ctx_create(int device, void* cuda_stream, kf_ctx** out) {
         }
         ctx->own_stream = true;
     }
-    if (cudaHostAlloc((void**)&ctx->wait_flags, 2 * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {  // one address for host and device
+    if (cudaHostAlloc((void**)&ctx->wait_flags, kWaitFlags * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {  // one address for host and device
         (void)cudaGetLastError();
         if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
         delete ctx;
         return KF_ERR_OOM;
     }
-    ctx->wait_flags[0] = ctx->wait_flags[1] = 0;
+    for (int i = 0; i < kWaitFlags; i++) ctx->wait_flags[i] = 0;
     *out = ctx;
     return KF_OK;
 }
@@ -130,15 +130,19 @@ extern "C" int kf_ctx_sync(kf_ctx* ctx) {
 }
 int kf_wait_status(kf_ctx* ctx) {
     volatile int* flag = ctx->wait_flags;
-    if (!flag[0] && !flag[1]) return KF_OK;
-    ctx->last_error = std::string("a bounded wait ran out in the ") + (flag[0] ? "prefill" : "grouped decode") + " attention kernel: results since the last synchronisation are not valid";
+    static const char* const names[kWaitFlags] = {"prefill", "grouped decode", "paged"};
+    std::string ran_out;
+    for (int i = 0; i < kWaitFlags; i++)
+        if (flag[i]) ran_out += (ran_out.empty() ? "" : ", ") + std::string(names[i]);
+    if (ran_out.empty()) return KF_OK;
+    ctx->last_error = "a bounded wait ran out in the " + ran_out + " attention kernel: results since the last synchronisation are not valid";
     if (ctx->capturing) return KF_ERR_CUDA;  // nothing can be cleared here: told again by the next call
     KF_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
     if (ctx->attn_cnt) {  // runs that arrived before the kernel gave up are still counted
         KF_CUDA(ctx, cudaMemsetAsync(ctx->attn_cnt, 0, sizeof(unsigned) * ctx->attn_cnt_n, ctx->stream));
         KF_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
     }
-    flag[0] = flag[1] = 0;
+    for (int i = 0; i < kWaitFlags; i++) flag[i] = 0;
     return KF_ERR_CUDA;
 }
 extern "C" void* kf_ctx_stream(kf_ctx* ctx) { return ctx ? (void*)ctx->stream : nullptr; }
@@ -178,9 +182,9 @@ extern "C" int kf_ctx_get_int(kf_ctx* ctx, const char* key, int* value_out) {
         *value_out = ctx->gemv_xg_min_m;
     else if (!strcmp(key, "tmap_weights"))
         *value_out = kf_tmap_count(ctx, true);
-    else if (!strcmp(key, "attn_tc_error") || !strcmp(key, "attn_gqa_error")) {
+    else if (!strcmp(key, "attn_tc_error") || !strcmp(key, "attn_gqa_error") || !strcmp(key, "attn_paged_error")) {
         if (!ctx->capturing) KF_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-        *value_out = ((volatile int*)ctx->wait_flags)[key[5] == 'g'];
+        *value_out = ((volatile int*)ctx->wait_flags)[key[5] == 't' ? kWaitPrefill : key[5] == 'g' ? kWaitDecode : kWaitPaged];
     } else
         return KF_ERR_BAD_ARG;
     return KF_OK;

@@ -62,7 +62,7 @@ struct kf_ctx {
     int deq_fma      = 1;
     int attn_split   = 0;
     int gqa_min_ctx  = 1024;  // single-sequence decode: contexts beyond this use the kv-group tensor-core attention (Transformer layer reads it)
-    // bounded waits of the attention kernels that run on copies and barriers: a kernel that gives up sets its flag ([0] prefill, [1] grouped decode; host memory)
+    // bounded waits of the attention kernels that run on copies and barriers: a kernel that gives up sets its flag (KfWaitFlag; host memory)
     int* wait_flags  = nullptr;
     int attn_tc_min_m = 0;       // panels from which the tcgen05 prefill attention is taken (from 65 queries); 0 = where it gains (attn_tc.cu)
     int attn_wait_us = 4000000;  // how long a wait may take
@@ -182,6 +182,7 @@ int kf_attn_prefill_tc_ok(const kf_ctx* ctx, const void* out, const void* q, con
 int kf_attn_prefill_tc(kf_ctx* ctx, void* out, const void* q, const void* kc, const void* vc, const int32_t* pos_dev, int M, int n_head, int n_kv, int max_seq);
 int kf_gemm_tc_multi(kf_ctx* ctx, int n, void* const* y, const kf_tensor_desc* w, const void* xp, int M, int epilogue, const void* residual);
 
+enum KfWaitFlag { kWaitPrefill, kWaitDecode, kWaitPaged, kWaitFlags };  // attn_tc.cu, attn_gqa.cu, attn_paged.cu and attn_paged_tc.cu
 struct KfBound {  // kernel parameter: see wait_flags
     int* flag;
     unsigned us;

@@ -671,3 +671,22 @@ def test_wait_that_runs_out_among_many_pieces(hd, cta, fresh):
     c.sync()
     s.check(c)
     c.close()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [70, 1]])
+def test_wait_that_runs_out_is_reported_as_this_kernel_s(new):
+    """Named in the message and asked for by its own key, not by those of the other attention kernels."""
+    c = kf.Context(0, stream=torch.cuda.current_stream().cuda_stream or 1)
+    s = Step(new, [400, 300], 8, 2, 128, 16, seed=51)
+    keys = ("attn_tc_error", "attn_gqa_error", "attn_paged_error")
+    for told_by in ("sync", "call"):
+        c.set_int("attn_wait_us", 20000), c.set_int("attn_drop", 1)
+        s.attend(c, 0.1)
+        c.set_int("attn_drop", 0), c.set_int("attn_wait_us", 0)
+        assert [c.get_int(k) for k in keys] == [0, 0, 1]
+        with pytest.raises(kf.KoifishError, match="wait ran out in the paged attention kernel"):
+            c.sync() if told_by == "sync" else s.attend(c, 0.1)
+        assert [c.get_int(k) for k in keys] == [0, 0, 0]
+        c.sync()
+        s.check(c)
+    c.close()
