@@ -262,7 +262,8 @@ typedef struct kf_rotation {
     size_t pos_stride;          /* 0: as many as the panel has rows */
 } kf_rotation;
 /* New tokens into their pages: q and k get an RMS norm per head (weights bf16 [head_dim], NULL: none) and the rotation (rot NULL: none; rot->pos_dev NULL: the
- * position in the sequence on every axis), k and v go to the sequence's pages as bf16, the finished q to q_out (bf16 [M][ldqo]; q itself when the panel is bf16).
+ * position in the sequence on every axis), k and v go to the sequence's pages as bf16, the finished q to q_out (bf16 [M][ldqo]; q itself when the panel is bf16,
+ * otherwise over no row of q, k or v).
  * All in fp32 with one rounding at the end.  q [M][n_head * head_dim], k and v [M][n_kv * head_dim], bf16 or (src_f32) float, rows ldq / ldk / ldv elements apart.
  * A token whose page is not there or whose position is outside the table keeps its finished q only. */
 int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, void* q_out_dev, int ldqo, const void* q_dev, int ldq, const void* k_dev, int ldk,
@@ -272,7 +273,7 @@ int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, 
  * gets zeros.  Keys that a row does not see may hold anything, and so may values behind the sequence's last position or before every row's window; a value of one of
  * the panel's own tokens that is not finite may reach rows of its sequence in front of it as well (its weight there is 0, and 0 times it is not a number).  n_head / n_kv at most 64; q 16-byte aligned, ldq a multiple of 8; out must not lie over q.  max_q: the largest number of new tokens of a sequence, as a hint: it chooses the kernels, results do not depend on it. */
 int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int max_q);
-/* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x. */
+/* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x, otherwise it must not lie over a row of x. */
 int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out_dev, int ldo, const void* x_dev, int ldx, int f32, int M, int n_head, int head_dim);
 
 /* ---- tensor parallel: no reference equivalent (multi_gpu.cuh is dead code).  One process per GPU;

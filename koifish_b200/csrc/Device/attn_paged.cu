@@ -385,7 +385,10 @@ extern "C" int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out,
     if (!ctx) return KF_ERR_BAD_ARG;
     KfPaged pg;
     int rc = check_args(ctx, kv, out, ldo, q, ldq, M, n_head, scale, max_q, &pg);
-    if (!rc) rc = kf_wait_status(ctx);
+    if (rc) return rc;
+    const size_t wide = (size_t)n_head * kv->head_dim * 2;
+    KF_REQUIRE(ctx, !kf_rows_overlap(out, (size_t)ldo * 2, wide, q, (size_t)ldq * 2, wide, M), "the result over a part of the queries");
+    rc = kf_wait_status(ctx);
     if (rc || M == 0) return rc;
     const int group = n_head / kv->n_kv;
     // steps whose sequences have up to 16 rows a kv head (new tokens x heads of the group) here, others as a whole on tcgen05: a second launch for their single tokens costs

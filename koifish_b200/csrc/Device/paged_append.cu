@@ -287,6 +287,17 @@ int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out) {
     return KF_OK;
 }
 
+extern "C" int kf_rows_overlap(const void* a, size_t a_pitch, size_t a_wide, const void* b, size_t b_pitch, size_t b_wide, int M) {
+    const long long d = (long long)((uintptr_t)b - (uintptr_t)a), ap = (long long)a_pitch, bp = (long long)b_pitch, aw = (long long)a_wide, bw = (long long)b_wide;
+    if (M <= 0 || d >= (M - 1) * ap + aw || d + (M - 1) * bp + bw <= 0) return 0;
+    // rows side by side in one panel have one pitch: then only the distance of two rows matters, and the first and the last row of a meet every distance there is
+    for (long long i = 0; i < M; i += ap == bp && M > 1 ? M - 1 : 1) {
+        const long long before = i * ap - d - bw, j = before < 0 ? 0 : before / bp + 1;  // the first row of b that ends behind the start of row i of a
+        if (j < M && d + j * bp < i * ap + aw) return 1;
+    }
+    return 0;
+}
+
 static int append_args(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, const void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
                        int src_f32, int M, int n_head, RowsParams* p) {
     if (!kv || !q_out || !q || !k || !v) return KF_ERR_BAD_ARG;
@@ -308,6 +319,9 @@ extern "C" int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rota
     if (rc) return rc;
     const int hd = kv->head_dim;
     if (M == 0) return KF_OK;
+    const size_t per_in = src_f32 ? 4 : 2, q_wide = (size_t)n_head * hd, kv_wide = (size_t)kv->n_kv * hd;
+    auto over = [&](const void* x, int ldx, size_t wide) { return kf_rows_overlap(q_out, (size_t)ldqo * 2, q_wide * 2, x, ldx * per_in, wide * per_in, M); };
+    KF_REQUIRE(ctx, (q_out == q || !over(q, ldq, q_wide)) && !over(k, ldk, kv_wide) && !over(v, ldv, kv_wide), "the finished queries over a part of the panel");
     p.q = q, p.k = k, p.v = v, p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.out = q_out, p.ldo = ldqo, p.nq = n_head, p.nkv = kv->n_kv, p.hd = hd, p.M = M;
     p.qw = (const uint16_t*)qnorm_w, p.kw = (const uint16_t*)knorm_w, p.eps = eps;
     p.kc = (uint16_t*)kv->k_dev, p.vc = (uint16_t*)kv->v_dev, p.page_stride = (long long)kf_paged_stride(kv);
@@ -332,6 +346,8 @@ extern "C" int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out, int 
     const int rc = rope_args(ctx, rot, out, ldo, x, ldx, f32, M, n_head, hd, &p);
     if (rc) return rc;
     if (M == 0) return KF_OK;
+    const size_t size = f32 ? 4 : 2, wide_bytes = (size_t)n_head * hd * size;
+    KF_REQUIRE(ctx, out == x || !kf_rows_overlap(out, ldo * size, wide_bytes, x, ldx * size, wide_bytes, M), "the result over a part of the panel");
     p.q = p.k = p.v = x, p.ldq = ldx, p.out = out, p.ldo = ldo, p.nq = n_head, p.hd = hd, p.M = M;
     const int per = f32 ? 4 : 8;
     const bool wide = whole_lanes(p) && (((uintptr_t)x | (uintptr_t)out) & 15) == 0 && ldx % per == 0 && ldo % per == 0;

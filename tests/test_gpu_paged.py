@@ -690,3 +690,38 @@ def test_wait_that_runs_out_is_reported_as_this_kernel_s(new):
         c.sync()
         s.check(c)
     c.close()
+
+
+def test_results_over_their_sources(ctx):
+    """A result that lies over a part of what it is made of is refused; beside it in the same rows, or where the documentation has it in place, it is taken."""
+    s = Step([1, 3, 1], [30, 20, 9], 4, 2, 64, 16, seed=70)
+    wide, n = 4 * 64, s.rows
+    buf = torch.zeros(n + 4, 3 * wide, device="cuda", dtype=torch.bfloat16)
+    buf[1:n + 1, :wide] = s.q
+    q, rows = buf[1:n + 1], buf.stride(0)
+    bad = [(q, rows), (buf[2:], rows), (buf[0:], rows), (buf[1:n + 1, 8:], rows), (buf.flatten()[rows - wide + 8:], rows), (q, wide)]
+    for o, ld in bad:
+        with pytest.raises(kf.KoifishError, match="over"):
+            s.attend(ctx, 0.1, q=q, ldq=rows, out=o, ldo=ld)
+    ref, tol = s.expect(0.1, 0)
+    s.attend(ctx, 0.1, q=q, ldq=rows, out=buf[1:n + 1, wide:], ldo=rows)
+    torch.cuda.synchronize()
+    assert torch.all((buf[1:n + 1, wide:2 * wide].double() - ref).abs() <= tol) and torch.equal(buf[1:n + 1, :wide], s.q)
+    r = kf.Rotation(At(torch.ones(32, device="cuda", dtype=torch.float64)), 64, pos=At(i32([0] * n)))
+    for o, ld in bad[1:]:
+        with pytest.raises(kf.KoifishError, match="over|in place"):
+            kf.rope_axes(ctx, r, At(q), n, 4, 64, ldx=rows, out=At(o), ldo=ld)
+        with pytest.raises(kf.KoifishError, match="over|in place"):
+            kf.paged_append(ctx, s.desc, None, At(q), At(q[:, wide:]), At(q[:, wide + 128:]), n, 4, ldq=rows, ldk=rows, ldv=rows, out=At(o), ldo=ld)
+    for o in (q[:, wide:], q[:, wide + 200:]):  # over the keys, over the values
+        with pytest.raises(kf.KoifishError, match="over"):
+            kf.paged_append(ctx, s.desc, None, At(q), At(q[:, wide:]), At(q[:, wide + 128:]), n, 4, ldq=rows, ldk=rows, ldv=rows, out=At(o), ldo=rows)
+    panel = torch.zeros(n, 3 * wide, device="cuda")
+    with pytest.raises(kf.KoifishError, match="over"):  # bf16 queries over a float panel's
+        kf.paged_append(ctx, s.desc, None, At(panel), At(panel[:, wide:]), At(panel[:, wide + 128:]), n, 4, ldq=3 * wide, ldk=3 * wide, ldv=3 * wide, out=At(panel[:, 8:]), ldo=6 * wide,
+                        src_f32=True)
+    for o in (q, q[:, 2 * wide:]):
+        kf.rope_axes(ctx, r, At(q), n, 4, 64, ldx=rows, out=At(o), ldo=rows)
+        kf.paged_append(ctx, s.desc, None, At(q), At(q[:, wide:]), At(q[:, wide + 128:]), n, 4, ldq=rows, ldk=rows, ldv=rows, out=At(o), ldo=rows)
+    torch.cuda.synchronize()
+    assert torch.equal(q[:, :wide], s.q) and torch.equal(q[:, 2 * wide:], s.q)

@@ -137,3 +137,22 @@ def test_largest_pages(lib, page):
     assert attention(lib, cache(page_size=page, table_cols=2)) == BAD
     for p in [0, 1, 7, page // 2, page - 1, page, page + 1, 2 ** 31 - 1]:
         assert lib.kf_paged_page_of(page, p) == p // page
+
+
+def test_rows_that_overlap(lib):
+    """Panels in one buffer, side by side, interleaved and shifted, against a count of every byte."""
+    lib.kf_rows_overlap.argtypes = [C.c_void_p, C.c_size_t, C.c_size_t] * 2 + [C.c_int]
+    r = np.random.RandomState(2)
+    base, seen = 1 << 20, [0, 0]
+    for _ in range(6000):
+        M, aw, bw = int(r.randint(1, 7)), int(r.randint(1, 9)), int(r.randint(1, 9))
+        ap = aw + int(r.choice([0, 1, 5, 20]))
+        bp = ap if r.rand() < 0.6 and bw <= ap else bw + int(r.choice([0, 2, 17]))
+        d = int(r.randint(-60, 61))
+        a, b = ({x for i in range(M) for x in range(at + i * p, at + i * p + w)} for at, p, w in ((0, ap, aw), (d, bp, bw)))
+        assert lib.kf_rows_overlap(base, ap, aw, base + d, bp, bw, M) == int(bool(a & b)), (M, ap, aw, d, bp, bw)
+        seen[bool(a & b)] += 1
+    assert min(seen) > 1000
+    assert lib.kf_rows_overlap(base, 8, 8, base, 8, 8, 0) == 0
+    far = 1 << 40  # offsets of more than 32 bits
+    assert lib.kf_rows_overlap(far, 1 << 20, 64, far + (1 << 34) + 32, 1 << 20, 64, 20000) == 1 and lib.kf_rows_overlap(far, 1 << 20, 64, far + (1 << 34) + 64, 1 << 20, 64, 20000) == 0
