@@ -335,12 +335,12 @@ class Rotation:
 
 
 def paged_append(ctx, kv, rot, q, k, v, M, n_head, q_norm=None, k_norm=None, eps=1e-6, ldq=0, ldk=0, ldv=0, out=None, ldo=0, src_f32=False):
-    """a step's keys and values into the pages of their sequences, norm and rotation on the way; returns the finished queries"""
+    """a step's keys and values into the pages of their sequences, norm and rotation on the way; returns the finished queries (out may be q, in its rows)"""
     wide, kvw = n_head * kv.head_dim, kv.n_kv * kv.head_dim
     if out is None:
         out = ctx.empty(M * (ldo or wide) * 2)
-    st = ctx.lib.kf_paged_append(ctx.h, kv.ref, rot.ref if rot is not None else None, out.ptr, ldo or wide, q.ptr, ldq or wide, k.ptr, ldk or kvw, v.ptr, ldv or kvw,
-                                 int(src_f32), M, n_head, q_norm.ptr if q_norm is not None else None, k_norm.ptr if k_norm is not None else None, eps)
+    st = ctx.lib.kf_paged_append(ctx.h, kv.ref, rot.ref if rot is not None else None, out.ptr, ldo or (ldq if out.ptr == q.ptr and ldq else wide), q.ptr, ldq or wide,
+                                 k.ptr, ldk or kvw, v.ptr, ldv or kvw, int(src_f32), M, n_head, q_norm.ptr if q_norm is not None else None, k_norm.ptr if k_norm is not None else None, eps)
     if st:
         ctx.check(st, "kf_paged_append")
     return out
@@ -362,7 +362,7 @@ def rope_axes(ctx, rot, x, M, n_head, head_dim, ldx=0, out=None, ldo=0, f32=Fals
     wide = n_head * head_dim
     if out is None:
         out = ctx.empty(M * (ldo or wide) * (4 if f32 else 2))
-    st = ctx.lib.kf_rope_axes(ctx.h, rot.ref, out.ptr, ldo or (ldx if out is x and ldx else wide), x.ptr, ldx or wide, int(f32), M, n_head, head_dim)
+    st = ctx.lib.kf_rope_axes(ctx.h, rot.ref, out.ptr, ldo or (ldx if out.ptr == x.ptr and ldx else wide), x.ptr, ldx or wide, int(f32), M, n_head, head_dim)
     if st:
         ctx.check(st, "kf_rope_axes")
     return out

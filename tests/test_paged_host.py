@@ -156,3 +156,33 @@ def test_rows_that_overlap(lib):
     assert lib.kf_rows_overlap(base, 8, 8, base, 8, 8, 0) == 0
     far = 1 << 40  # offsets of more than 32 bits
     assert lib.kf_rows_overlap(far, 1 << 20, 64, far + (1 << 34) + 32, 1 << 20, 64, 20000) == 1 and lib.kf_rows_overlap(far, 1 << 20, 64, far + (1 << 34) + 64, 1 << 20, 64, 20000) == 0
+
+
+class Recorder:
+    """Stands in for a context: remembers the arguments of the library's calls."""
+
+    def __init__(self):
+        self.h, self.lib, self.calls = None, self, []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append((name, a)) or 0
+
+
+class Buf:
+    def __init__(self, ptr):
+        self.ptr = ptr
+
+
+@pytest.mark.parametrize("same", [True, False])  # the panel's own object, or another one at its address
+def test_in_place_rows_from_python(same):
+    """In place, the rows of the result are those of the panel unless they are given."""
+    c, q, b = Recorder(), Buf(4096), Buf(64)
+    o = q if same else Buf(4096)
+    kv = kf.PagedKV(b, b, 4, 16, 2, 128, b, 4, 1, b, b)
+    rot = kf.Rotation(b, 128, pos=b)
+    kf.paged_append(c, kv, rot, q, Buf(8192), Buf(9216), 3, 8, ldq=1536, ldk=1536, ldv=1536, out=o)
+    kf.paged_append(c, kv, rot, q, Buf(8192), Buf(9216), 3, 8, ldq=1536, ldk=1536, ldv=1536, out=Buf(1 << 20))
+    kf.paged_append(c, kv, rot, q, Buf(8192), Buf(9216), 3, 8, out=o)
+    kf.rope_axes(c, rot, q, 3, 8, 128, ldx=1536, out=o)
+    kf.rope_axes(c, rot, q, 3, 8, 128, ldx=1536, out=Buf(1 << 20))
+    assert [a[4 if name == "kf_paged_append" else 3] for name, a in c.calls] == [1536, 1024, 1024, 1536, 1024]
