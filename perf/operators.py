@@ -168,16 +168,16 @@ class _At:
         self.ptr = t.data_ptr()
 
 
-_CTX = []
+_CTX = {}  # by device and stream: a context's kernels go to the stream it was made for
 
 
-def _handles(s):
+def _handles(s, device, stream):
     """What a program keeps between its calls: the context, the descriptions of the cache and of the rotation, the addresses."""
     import koifish_b200 as kf
-    if not _CTX:
-        _CTX.append(kf.Context(0, stream=torch.cuda.current_stream().cuda_stream or 1))  # 1: the handle of torch's default stream
+    if (device, stream) not in _CTX:
+        _CTX[device, stream] = kf.Context(device, stream=stream or 1)  # 1: the handle of torch's default stream
     at = {n: _At(t) for n, t in s.items() if isinstance(t, torch.Tensor)}
-    h = dict(kf=kf, ctx=_CTX[0], at=at)
+    h = dict(kf=kf, ctx=_CTX[device, stream], at=at, stream=stream)
     if s["op"] != "attention":
         h["rot"] = kf.Rotation(at["freq"], s["rot"], layout=s["layout"], n_axes=s["axes"], pair_axis=at["axis"] if s["axes"] > 1 else None, pos=at.get("pos"))
     if s["op"] != "rope":
@@ -187,9 +187,10 @@ def _handles(s):
 
 
 def _own(s):
-    h = s.get("handles")
-    if h is None:
-        h = s["handles"] = _handles(s)
+    h, device = s.get("handles"), s["out"].get_device()
+    stream = torch._C._cuda_getCurrentRawStream(device)  # 0.1 us; torch.cuda.current_stream() makes an object, 3 us, as long as the whole call
+    if h is None or h["stream"] != stream:
+        h = s["handles"] = _handles(s, device, stream)
     kf, ctx, at = h["kf"], h["ctx"], h["at"]
     if s["op"] == "rope":
         kf.rope_axes(ctx, h["rot"], at["x"], s["M"], s["heads"], s["hd"], ldx=s["x"].stride(0), out=at["out"], f32=s["f32"])
