@@ -725,3 +725,27 @@ def test_results_over_their_sources(ctx):
         kf.paged_append(ctx, s.desc, None, At(q), At(q[:, wide:]), At(q[:, wide + 128:]), n, 4, ldq=rows, ldk=rows, ldv=rows, out=At(o), ldo=rows)
     torch.cuda.synchronize()
     assert torch.equal(q[:, :wide], s.q) and torch.equal(q[:, 2 * wide:], s.q)
+
+
+def test_timed_calls_on_another_stream():
+    """The calls of perf/operators.py go to the stream that is current, for a state of another stream as well, and give the same bits there."""
+    import importlib.util
+    import os
+    spec = importlib.util.spec_from_file_location("timed_operators", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf", "operators.py"))
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    ops.own = True
+    case = [c for c in ops.listed() if c["name"] == "append_decode"][0]
+    first, side = ops.prepare(case, 1), torch.cuda.Stream()
+    want = [t.clone() for t in ops.run(first)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for s in (first, ops.prepare(case, 1)):
+            got = ops.run(s)
+            c = s["handles"]["ctx"]
+            assert c.lib.kf_ctx_stream(c.h) == side.cuda_stream
+            side.synchronize()
+            assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(want, got))
+    ops.run(first)
+    assert first["handles"]["ctx"].lib.kf_ctx_stream(first["handles"]["ctx"].h) == 1
+    torch.cuda.synchronize()
