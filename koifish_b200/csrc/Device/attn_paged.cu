@@ -111,8 +111,8 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, 2)
                 }
             }
         }
-        if (!live)  // copies in flight write shared memory
-            for (uint32_t k = asked > (uint32_t)stages ? asked - stages : 0; k < asked; k++) mbar_drain(smem_u32(&full[k % stages]), (k / stages) & 1, bound);
+        // copies in flight write shared memory, which is another's once the CTA has ended, and where a wait has run out nobody else may have waited for them
+        for (uint32_t k = asked > (uint32_t)stages ? asked - stages : 0; k < asked; k++) mbar_drain(smem_u32(&full[k % stages]), (k / stages) & 1, bound);
         return;
     }
     const int group = pl.group, rb = pl.tb * group;

@@ -368,10 +368,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             pos += st.n, qn++;
         }
-        if (!live) {
-            umma_commit_a(smem_u32(&done_bar));
-            mbar_drain(smem_u32(&done_bar), 0, bound);
-        }
+        // instructions in flight write tensor memory: waited for here, since where a wait has run out nobody else may have
+        umma_commit_a(smem_u32(&done_bar));
+        mbar_drain(smem_u32(&done_bar), 0, bound);
     } else if (warp == kPlanW) {
         PagedPlanner<kKV> plan(pg, pl, lane);
         if (lane == 0) a.rec[cta].last = 0;  // nothing to merge, should a wait run out before the end of the run is known
@@ -448,11 +447,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             met = !isv && !st.pair && st.n > 1;
         }
-        if (!live) {  // copies in flight write shared memory: wait for what was asked for
-            if (!isv && qn > 0) mbar_drain(smem_u32(&q_full), (qn - 1) & 1, bound);
-            for (uint32_t k = pos > stages ? pos - stages : 0; k < pos; k++) mbar_drain(smem_u32(isv ? &v_full[k % stages] : &k_full[k % stages]), (k / stages) & 1, bound);
-            if (isv && landed > 0) mbar_drain(smem_u32(&v_land), (landed - 1) & 1, bound);
-        }
+        // copies in flight write shared memory, which is another's once the CTA has ended: the same
+        if (!isv && qn > 0) mbar_drain(smem_u32(&q_full), (qn - 1) & 1, bound);
+        for (uint32_t k = pos > stages ? pos - stages : 0; k < pos; k++) mbar_drain(smem_u32(isv ? &v_full[k % stages] : &k_full[k % stages]), (k / stages) & 1, bound);
+        if (isv && landed > 0) mbar_drain(smem_u32(&v_land), (landed - 1) & 1, bound);
     }
     tc_fence_before();
     __syncthreads();
