@@ -749,3 +749,55 @@ def test_timed_calls_on_another_stream():
     ops.run(first)
     assert first["handles"]["ctx"].lib.kf_ctx_stream(first["handles"]["ctx"].h) == 1
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_seq,chunk", [(1100, 0), (1100, 90), (2500, 3), (8192, 40)])
+def test_attention_of_many_sequences(ctx, hd, n_seq, chunk):
+    """More than 1024 sequences, most of them idle or with one token, in both kernels: a run begins behind many that it has no part in."""
+    r = np.random.RandomState(n_seq + chunk)
+    new = (r.rand(n_seq) < min(1.0, 400 / n_seq)).astype(int)
+    length = new + r.randint(0, 30, n_seq)
+    new[0], length[0], new[-1], length[-1] = 1, 200, 1, 333
+    if chunk:
+        for i in (5, n_seq // 2, n_seq - 2):
+            new[i], length[i] = chunk, chunk + 100
+    Step(new, length, 4, 2, hd, 16, seed=chunk, pad=1).check(ctx)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("page", [8, 16, 64])
+@pytest.mark.parametrize("window", [5, 70, 300])
+def test_chunks_hidden_values(ctx, hd, page, window):
+    """Infinities and NaN in keys and values before the first row's window, in pages that are still there, and behind the last position."""
+    new, length = [3, 150, 1, 60], [500, 640, 777, 64]
+    s = Step(new, length, 8, 2, hd, page, seed=window + page)
+    for i, n in enumerate(length):
+        for j in range(max(0, n - new[i] + 1 - window)):
+            e, m = int(s.table[i, j // page]), j % page
+            s.k[e, m], s.v[e, m] = float("inf") if j % 2 else float("nan"), float("nan") if j % 3 else float("-inf")
+    s.check(ctx, window=window)
+    s.check(ctx, window=window, max_q=2)
+
+
+def test_append_far_pages(ctx):
+    """Rows that lie more than 2^32 elements into the pool."""
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 20 GB")
+    kv, hd, page, n_pages = 2, 64, 16, 40
+    stride = (1 << 27) + 8
+    pool = torch.zeros(n_pages * stride, device="cuda", dtype=torch.bfloat16)
+    s = Step([1, 30], [300, 200], 4, kv, hd, page, seed=16)
+    s.table[s.table == s.n_pages - 1], s.table[0, 18] = s.table[0, 18], s.n_pages - 1  # the page that the first sequence's token falls into is the last
+    s.d[0].copy_(i32(np.where(s.table > 2 ** 31 - 1, 0, s.table)))
+    assert (s.n_pages - 1) * stride > 1 << 32
+    far = [pool[off:off + (s.n_pages - 1) * stride + page * kv * hd].as_strided((s.n_pages, page, kv, hd), (stride, kv * hd, hd, 1)) for off in (0, page * kv * hd)]
+    desc = kf.PagedKV(At(far[0]), At(far[1]), s.n_pages, page, kv, hd, At(s.d[0]), s.cols, 2, At(s.d[1]), At(s.d[2]), page_stride=stride)
+    k, v = (torch.randn(s.rows, kv * hd, device="cuda").bfloat16() for _ in "kv")
+    kf.paged_append(ctx, desc, None, At(s.q), At(k), At(v), s.rows, 4, out=At(s.q))
+    torch.cuda.synchronize()
+    for i, n in enumerate(s.new):
+        for j in range(n):
+            t = s.length[i] - n + j
+            e, m = int(s.table[i, t // page]), t % page
+            assert torch.equal(far[0][e, m].flatten(), k[s.start[i] + j]) and torch.equal(far[1][e, m].flatten(), v[s.start[i] + j])
