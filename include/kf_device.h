@@ -270,8 +270,12 @@ int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, 
                     const void* v_dev, int ldv, int src_f32, int M, int n_head, const void* qnorm_w_dev, const void* knorm_w_dev, float eps);
 /* Causal attention of the panel's rows over the pages: a row at position p sees the positions j <= p of its sequence, with window > 0 only j > p - window.
  * out [M][ldo], q [M][ldq] bf16, n_head * head_dim entries a row; softmax(scale * q . k) in fp32.  A row that sees nothing, or nothing but scores of -inf,
- * gets zeros.  Keys that a row does not see may hold anything, and so may values behind the sequence's last position or before every row's window; a value of one of
- * the panel's own tokens that is not finite may reach rows of its sequence in front of it as well (its weight there is 0, and 0 times it is not a number).  n_head / n_kv at most 64; q 16-byte aligned, ldq a multiple of 8; out must not lie over q.  max_q: the largest number of new tokens of a sequence, as a hint: it chooses the kernels, results do not depend on it. */
+ * gets zeros.  Keys that a row does not see may hold anything, and so may values behind the sequence's last position or before every row's window.  A value that is not
+ * finite and that some row sees may reach other rows of the panel of the same sequence as well (its weight there is 0, and 0 times it is not a number): one of the panel's
+ * own tokens the rows in front of it, with a window a cached one the rows whose window has gone past it.
+ * n_head / n_kv at most 64; q 16-byte aligned, ldq a multiple of 8; out must not lie over a row of q.  max_q: the largest number of new tokens of a sequence, as a hint.  It
+ * chooses one of two kernels for the whole step, whatever it says is right: results agree within their rounding, not in the last bits, and times differ (single tokens alone
+ * take up to 1.5 times as long in the kernel for many rows).  A captured step keeps the kernel it was captured with. */
 int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int max_q);
 /* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x, otherwise it must not lie over a row of x. */
 int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out_dev, int ldo, const void* x_dev, int ldx, int f32, int M, int n_head, int head_dim);

@@ -13,8 +13,8 @@
 //   * The piece that arrives last at its block merges all of them in order, a row to a warp with eight pieces on their way (sums by slices of the threads, maxima looked up
 //     first: 17 us of 85 for one sequence at 100000 positions, 10 less here).
 //   * Two CTAs of four warps per SM: one's merge runs beside the other's tiles.  (One CTA of eight: 166 against 111 us for 64 sequences, 89 against 76 for one.)
-// Measured: 64 sequences of 400 .. 4000 positions, 8 kv heads (624 MB) 111 us, 5.6 TB/s; one of 100000 positions (410 MB) 76 us, 5.4 TB/s; one of 1300 10.2 us, most of
-// it the way from the lengths over the table to the first tile and the merge.
+// Measured in a steady run (in brackets: a few dozen passes): 64 sequences of 400 .. 4000 positions, 8 kv heads (624 MB) 117 us, 5.3 TB/s (111 us, 5.6 TB/s); one of 100000
+// positions (410 MB) 77 us, 5.3 TB/s (76 us); one of 1300 10.3 us, most of it the way from the lengths over the table to the first tile and the merge.
 // Values behind a block's last position or before its window need not be numbers: their rows of V are zeroed in shared memory.
 #include <algorithm>
 
@@ -391,9 +391,11 @@ extern "C" int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out,
     rc = kf_wait_status(ctx);
     if (rc || M == 0) return rc;
     const int group = n_head / kv->n_kv;
-    // steps whose sequences have up to 16 rows a kv head (new tokens x heads of the group) here, others as a whole on tcgen05: a second launch for their single tokens costs
-    // more than the few rows of their row tiles (24 sequences, three of them with chunks, 64 dims: 55 against 60 us; 16 x 5 drafted tokens, launched for nothing: 67 against
-    // 71).  Single tokens alone are faster here: 64 ragged sequences 111 against 193 us, one at 1300 positions 10 against 20.  16 rows in tokens of two: 50 against 65.
+    // steps whose sequences have up to 16 rows a kv head (new tokens x heads of the group) here, others as a whole on tcgen05.  Single tokens alone, here / there: 64 ragged
+    // sequences 112 / 158 us, one at 1300 positions 10.5 / 15.9; 16 sequences with two tokens of 8 heads 49 / 54.  For the single tokens of a step with chunks a second launch
+    // was measured where their rows have few positions, and costs more than their row tiles (24 sequences, three of them with chunks, 64 dims, a window of 1000: 60 against 55
+    // us; 16 x 5 drafted tokens, launched for nothing: 71 against 67).  Where they have many it would gain: the 64 sequences and a chunk of 512 behind 2000 positions
+    // take 228 us, the two apart 112 + 67.
     const int tokens = std::max(1, max_q), few = 16 / group;
     if (tokens > few) return kf_attn_paged_tc(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window);
     const PagedPlan pl{tokens, group, window, 1, 0};

@@ -10,15 +10,17 @@
 //   warp 11          the pieces
 // The tiles of all blocks and kv heads are cut into equal runs, one CTA each (PagedWalk).  Blocks that several CTAs share leave their sums in the workspace; a second
 // kernel, launched behind, merges them in order.
-// Sums are rescaled when a row's maximum has grown by more than 2^8 over the one they refer to: until about 32 tiles have gone by nearly every tile brings one of a warp's rows a
-// new maximum, and the rescaling stands in a chain's way (2048 tokens behind 8192, 32 heads: 362 us rescaling whenever a maximum grows, 301 with the slack).  Weights up to 2^8 are
-// rounded to bf16 like the others, and the denominator adds them as they are rounded: the error of a row that one weight carries cancels.  Relative to 64 bits, 512 tokens:
+// Sums are rescaled when a row's maximum has grown by more than 2^8 over the one they refer to (deferring it so is a published method of attention on this generation of tensor
+// cores): until about 32 tiles have gone by nearly every tile brings one of a warp's rows a new maximum, and the rescaling stands in a chain's way (2048 tokens behind 8192, 32
+// heads: 362 us rescaling whenever a maximum grows, 301 with the slack).  Weights up to 2^8 are rounded to bf16 like the others, and the denominator adds them as they are rounded: the error of a row that one weight carries cancels.  Relative to 64 bits, 512 tokens:
 // 2.3e-3 flat and 1.8e-3 sharp (scores four times as large), 2.1e-3 and 1.7e-3 rescaling always, 2.3e-3 and 2.0e-3 with the unrounded weights in the denominator; the
 // result's own rounding is 1.7e-3.
 // What bounds it: a chain's way.  A tile takes it about 3600 clocks -- scores 512, from them to the first half of the weights 1500, to the second 900, sums behind these 256, the
 // rest hand-overs -- while the tensor cores are busy for 2048 of both chains' clocks and the special-function units for as many.  Forming a quarter of the exponentials on the
-// multiply-add units made it 5 % slower, an issuing warp for each chain 16 % (they fall into step).  Measured, with warps without rows passing: 290 us, 1070 TFLOP/s; 16 sequences of 500 .. 5000 positions with five
-// drafted tokens of 40 heads 55 us, 3.3 TB/s, where the way of a tile of V through three stages adds to it.
+// multiply-add units made it 5 % slower, an issuing warp for each chain 16 % (they fall into step).  Measured: that chunk 330 us in a steady run, 935 TFLOP/s
+// under the power cap (290 us, 1070 TFLOP/s in a few dozen passes); 16 sequences of 500 .. 5000 positions with five drafted tokens of 40 heads 56 us, 3.2 TB/s, where the
+// way of a tile of V through three stages adds to it.  Runs are equal in tiles, not in time: a tile of a block with two row tiles takes both chains a step, of another
+// block half of one, so in steps that mix chunks and single tokens the CTAs end at different times.
 // Rows of V that no row of the block sees are zeroed in shared memory, since they need not hold numbers; boxes of pages that are not there arrive as zeros.
 // Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
 #include <algorithm>

@@ -7,10 +7,12 @@
 // for all their heads: t / pi in 64 bits, reduced to [-1, 1] there (a far position turns many times; its remainder in 32 bits would be off by more than the result's
 // rounding), then sine and cosine in 32 bits.  A head's row is spread over 4, 8 or 16 lanes; a lane holds eight pairs, so both of a pair's entries are its own: 16 bytes of
 // either half of the rotated part, or 32 bytes in a row where pairs lie side by side.  (With 16 bytes a lane and the other half from another lane by shuffles, one token a
-// block: 8192 tokens of 64 + 8 + 8 heads with their norm 148 us, 16001 tokens of 40 heads 165 us; here 64 and 57, 5.2 and 5.8 TB/s.)  What bounds it is how many bytes are on
-// their way: four or five blocks per SM, a lane's next rows asked for before it works on its own.  With the norm: one row ahead and the weights in shared memory, five blocks (two rows, four blocks:
-// 67 us; weights in registers, which spill: 76); without, two rows ahead (one: 61, three: 69).  The first rows are asked for before the positions are known: finding the sequence of a token, its page and its position are
-// three dependent reads.  Few tokens are spread over blocks by heads.
+// block: 8192 tokens of 64 + 8 + 8 heads with their norm 148 us, 16001 tokens of 40 heads 165 us; here 64 and 57, in a steady run 68 and 59, 4.9 and 5.5
+// TB/s.)  What bounds it is how many bytes are on their way: four or five blocks per SM, a lane's next rows asked for before it works on its own.  With the norm: one row ahead
+// and the weights in shared memory, five blocks (two rows, four blocks: 67 us; weights in registers, which spill: 76); without, two rows ahead (one: 61, three: 69).  The first
+// rows are asked for before the positions are known: finding the sequence of a token, its page and its position are three dependent reads.  Few tokens are spread over blocks by
+// heads.  Rows at any element, heads that are no multiple of 16 and, with pairs apart, rotated parts that are none go entry by entry: 16000 tokens of 16 heads of 72 83 us, 0.9 TB/s
+// (of 80, whole lanes: 33 us, 2.5 TB/s); with 24 of 64 entries rotated 91 us.
 #include <algorithm>
 #include <type_traits>
 
