@@ -277,6 +277,40 @@ int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, 
  * chooses one of two kernels for the whole step, whatever it says is right: results agree within their rounding, not in the last bits, and times differ (single tokens alone
  * take up to 1.5 times as long in the kernel for many rows).  A captured step keeps the kernel it was captured with. */
 int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int max_q);
+/* ---- the same cache in 4 bits (paged_append.cu, paged_read_q4.cu, attn_paged_q4.cu): steps, tables and padding as above, rows of K and V as codes.  Every 32 entries of a head's
+ *      row are a group with a step and a zero in bf16; a code c of 0 .. 15 stands for step * (c - zero):
+ *        step = max((max - min) / 15, max |x| / 2048), rounded up to bf16; zero = -min / step, rounded to bf16 (0 where step is 0);
+ *        c = x / step + zero, rounded to the nearest whole number (ties to even) and kept to 0 .. 15; all in fp32.
+ *      So x comes back within step * (1/2 + |zero| / 256).  A group with an entry that is not finite comes back as NaN.  Meant for values below 2^50.
+ *      0.625 bytes an entry, against 2 in bf16.
+ *      A page holds for every kv head page_size / 8 units, one behind the other; a unit is 8 positions (10 * head_dim bytes, G = head_dim / 32):
+ *        K codes [8][head_dim / 2] bytes | K steps [8][G] | K zeros [8][G] | V codes [8][4][2][head_dim / 16] bytes | V steps [8][G] | V zeros [G][8]   (bf16)
+ *      K: word (t, j) of [4][G] words of a position holds entries 32 j + 8 t .. + 7, from the lowest 4 bits up.  V: word w of (g, p / 2, p % 2) holds position p's entries
+ *      64 w + 4 g .. + 3, then 64 w + 32 + 4 g .. + 3. ---- */
+typedef struct kf_paged_q4 {
+    void* pool_dev;         /* pages, 16-byte aligned */
+    size_t page_stride;     /* bytes from one page to the next, a multiple of 16 (0: pages are dense, kf_paged_q4_page_bytes) */
+    int n_pages, page_size; /* page_size: a multiple of 8 */
+    int n_kv, head_dim;     /* head_dim 64 or 128 */
+    const int32_t* table_dev; /* [n_seq][table_cols] */
+    int table_cols;
+    int n_seq;              /* up to 8192 */
+    const int32_t* q_start_dev; /* [n_seq + 1], not decreasing */
+    const int32_t* len_dev; /* [n_seq], at most table_cols * page_size (more is cut) */
+} kf_paged_q4;
+size_t kf_paged_q4_page_bytes(int page_size, int n_kv, int head_dim); /* 0: not a page */
+/* kf_paged_append into such a cache: k and v are quantised as they are written, k behind its norm and rotation, from 32 bits. */
+int kf_paged_append_q4(kf_ctx* ctx, const kf_paged_q4* kv, const kf_rotation* rot, void* q_out_dev, int ldqo, const void* q_dev, int ldq, const void* k_dev, int ldk,
+                       const void* v_dev, int ldv, int src_f32, int M, int n_head, const void* qnorm_w_dev, const void* knorm_w_dev, float eps);
+/* What the cache holds of the step's positions -- of whole sequences, with q_start running over their lengths -- as rows of n_kv * head_dim entries, bf16 or (out_f32) float,
+ * ldk / ldv elements apart; k_out and v_out may lie side by side in one panel, not over one another; one of them may be NULL.  Rows of positions whose page is not there or that
+ * are outside the table become zeros. */
+int kf_paged_read_q4(kf_ctx* ctx, const kf_paged_q4* kv, void* k_out_dev, int ldk, void* v_out_dev, int ldv, int out_f32, int M);
+/* kf_paged_attention over such a cache.  With window > 0 a row at position p sees the positions p - window < j <= p and, of those before, j < first.
+ * What it says of rows that see nothing, of values that are not finite, of alignment and of max_q holds here too; scale at most 2^20.  The codes' arithmetic is exact; weights
+ * times steps are rounded to bf16 for the product with V (in the kernel for many rows keys and values as well). */
+int kf_paged_attention_q4(kf_ctx* ctx, const kf_paged_q4* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int first,
+                          int max_q);
 /* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x, otherwise it must not lie over a row of x. */
 int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out_dev, int ldo, const void* x_dev, int ldx, int f32, int M, int n_head, int head_dim);
 

@@ -46,6 +46,11 @@ class PagedKVDesc(C.Structure):
                 ("head_dim", C.c_int), ("table_dev", C.c_void_p), ("table_cols", C.c_int), ("n_seq", C.c_int), ("q_start_dev", C.c_void_p), ("len_dev", C.c_void_p)]
 
 
+class PagedQ4Desc(C.Structure):
+    _fields_ = [("pool_dev", C.c_void_p), ("page_stride", C.c_size_t), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv", C.c_int), ("head_dim", C.c_int),
+                ("table_dev", C.c_void_p), ("table_cols", C.c_int), ("n_seq", C.c_int), ("q_start_dev", C.c_void_p), ("len_dev", C.c_void_p)]
+
+
 class RotationDesc(C.Structure):
     _fields_ = [("inv_freq_dev", C.c_void_p), ("rot_dims", C.c_int), ("layout", C.c_int), ("amp", C.c_float), ("n_axes", C.c_int), ("axis_dev", C.c_void_p),
                 ("pos_dev", C.c_void_p), ("pos_stride", C.c_size_t)]
@@ -179,6 +184,10 @@ SIGNATURES = {
     "kf_qk_heads_prepare_ex": (_I, [_P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _F, _I, _P, _F, _I, _P, _I, _P, _P, _I, _SZ, _I, _I, _I, _P, _P, _P, _I]),
     "kf_paged_append": (_I, [_P, C.POINTER(PagedKVDesc), C.POINTER(RotationDesc), _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _F]),
     "kf_paged_attention": (_I, [_P, C.POINTER(PagedKVDesc), _P, _I, _P, _I, _I, _I, _F, _I, _I]),
+    "kf_paged_q4_page_bytes": (_SZ, [_I, _I, _I]),
+    "kf_paged_append_q4": (_I, [_P, C.POINTER(PagedQ4Desc), C.POINTER(RotationDesc), _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _F]),
+    "kf_paged_read_q4": (_I, [_P, C.POINTER(PagedQ4Desc), _P, _I, _P, _I, _I, _I]),
+    "kf_paged_attention_q4": (_I, [_P, C.POINTER(PagedQ4Desc), _P, _I, _P, _I, _I, _I, _F, _I, _I, _I]),
     "kf_rope_axes": (_I, [_P, C.POINTER(RotationDesc), _P, _I, _P, _I, _I, _I, _I, _I]),
     "kf_nccl_unique_id": (_I, [_P]),
     "kf_ctx_init_nccl": (_I, [_P, _P, _I, _I]),

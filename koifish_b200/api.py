@@ -324,6 +324,21 @@ class PagedKV:
         self.ref = C.byref(self.desc)
 
 
+class PagedQ4:
+    """A layer's keys and values in pages of 4-bit codes and the step over them (kf_paged_q4); keeps what it was given alive.  page_stride in bytes."""
+
+    def __init__(self, pool, n_pages, page_size, n_kv, head_dim, table, table_cols, n_seq, q_start, lens, page_stride=0):
+        self.keep = (pool, table, q_start, lens)
+        self.n_kv, self.head_dim = n_kv, head_dim
+        self.desc = L.PagedQ4Desc(pool.ptr, page_stride, n_pages, page_size, n_kv, head_dim, table.ptr, table_cols, n_seq, q_start.ptr, lens.ptr)
+        self.ref = C.byref(self.desc)
+
+    @staticmethod
+    def page_bytes(page_size, n_kv, head_dim):
+        """bytes of a page, 0 where there is no such page"""
+        return L.load().kf_paged_q4_page_bytes(page_size, n_kv, head_dim)
+
+
 class Rotation:
     """Frequencies, axes and positions of a rotation (kf_rotation)."""
 
@@ -336,13 +351,22 @@ class Rotation:
 
 def paged_append(ctx, kv, rot, q, k, v, M, n_head, q_norm=None, k_norm=None, eps=1e-6, ldq=0, ldk=0, ldv=0, out=None, ldo=0, src_f32=False):
     """a step's keys and values into the pages of their sequences, norm and rotation on the way; returns the finished queries (out may be q, in its rows)"""
+    return _paged_append(ctx, "kf_paged_append", kv, rot, q, k, v, M, n_head, q_norm, k_norm, eps, ldq, ldk, ldv, out, ldo, src_f32)
+
+
+def paged_append_q4(ctx, kv, rot, q, k, v, M, n_head, q_norm=None, k_norm=None, eps=1e-6, ldq=0, ldk=0, ldv=0, out=None, ldo=0, src_f32=False):
+    """paged_append into a cache of 4-bit codes: k and v are quantised as they are written"""
+    return _paged_append(ctx, "kf_paged_append_q4", kv, rot, q, k, v, M, n_head, q_norm, k_norm, eps, ldq, ldk, ldv, out, ldo, src_f32)
+
+
+def _paged_append(ctx, name, kv, rot, q, k, v, M, n_head, q_norm, k_norm, eps, ldq, ldk, ldv, out, ldo, src_f32):
     wide, kvw = n_head * kv.head_dim, kv.n_kv * kv.head_dim
     if out is None:
         out = ctx.empty(M * (ldo or wide) * 2)
-    st = ctx.lib.kf_paged_append(ctx.h, kv.ref, rot.ref if rot is not None else None, out.ptr, ldo or (ldq if out.ptr == q.ptr and ldq else wide), q.ptr, ldq or wide,
+    st = getattr(ctx.lib, name)(ctx.h, kv.ref, rot.ref if rot is not None else None, out.ptr, ldo or (ldq if out.ptr == q.ptr and ldq else wide), q.ptr, ldq or wide,
                                  k.ptr, ldk or kvw, v.ptr, ldv or kvw, int(src_f32), M, n_head, q_norm.ptr if q_norm is not None else None, k_norm.ptr if k_norm is not None else None, eps)
     if st:
-        ctx.check(st, "kf_paged_append")
+        ctx.check(st, name)
     return out
 
 
@@ -354,6 +378,28 @@ def paged_attention(ctx, kv, q, M, n_head, max_q, scale=None, window=0, ldq=0, o
     st = ctx.lib.kf_paged_attention(ctx.h, kv.ref, out.ptr, ldo or wide, q.ptr, ldq or wide, M, n_head, kv.head_dim ** -0.5 if scale is None else scale, window, max_q)
     if st:
         ctx.check(st, "kf_paged_attention")
+    return out
+
+
+def paged_read_q4(ctx, kv, M, k_out=None, v_out=None, ldk=0, ldv=0, out_f32=False):
+    """what a cache of 4-bit codes holds of a step's positions, as rows of K and V; both are made where neither is given, otherwise only what is given is written"""
+    wide = kv.n_kv * kv.head_dim
+    if k_out is None and v_out is None:
+        k_out, v_out = (ctx.empty(M * (ld or wide) * (4 if out_f32 else 2)) for ld in (ldk, ldv))
+    st = ctx.lib.kf_paged_read_q4(ctx.h, kv.ref, k_out.ptr if k_out is not None else None, ldk or wide, v_out.ptr if v_out is not None else None, ldv or wide, int(out_f32), M)
+    if st:
+        ctx.check(st, "kf_paged_read_q4")
+    return k_out, v_out
+
+
+def paged_attention_q4(ctx, kv, q, M, n_head, max_q, scale=None, window=0, first=0, ldq=0, out=None, ldo=0):
+    """paged_attention over a cache of 4-bit codes; with a window the `first` positions stay visible"""
+    wide = n_head * kv.head_dim
+    if out is None:
+        out = ctx.empty(M * (ldo or wide) * 2)
+    st = ctx.lib.kf_paged_attention_q4(ctx.h, kv.ref, out.ptr, ldo or wide, q.ptr, ldq or wide, M, n_head, kv.head_dim ** -0.5 if scale is None else scale, window, first, max_q)
+    if st:
+        ctx.check(st, "kf_paged_attention_q4")
     return out
 
 

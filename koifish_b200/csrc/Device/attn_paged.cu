@@ -407,7 +407,11 @@ extern "C" int kf_paged_attention_args(const kf_paged_kv* kv, const void* out, i
     return check_args(nullptr, kv, out, ldo, q, ldq, M, n_head, scale, max_q, &pg);
 }
 extern "C" int kf_paged_attention_block(int tile, int cap, int tb, int window, int n, int len, int b, int* lo_hi_first) {
-    return paged_block(tile, cap, tb, window, n, len, b, lo_hi_first[0], lo_hi_first[1], lo_hi_first[2]);
+    int ns;
+    return paged_block(tile, cap, tb, window, 0, n, len, b, lo_hi_first[0], lo_hi_first[1], lo_hi_first[2], ns);
+}
+extern "C" int kf_paged_attention_block_first(int tile, int cap, int tb, int window, int first, int n, int len, int b, int* lo_hi_first_ns) {
+    return paged_block(tile, cap, tb, window, first, n, len, b, lo_hi_first_ns[0], lo_hi_first_ns[1], lo_hi_first_ns[2], lo_hi_first_ns[3]);
 }
 extern "C" int kf_paged_page_of(int page, int p) {
     KfPaged pg = {};

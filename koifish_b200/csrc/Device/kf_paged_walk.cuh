@@ -1,4 +1,4 @@
-// kf_paged_walk.cuh -- how the attention kernels share a step over a cache in pages among their CTAs (attn_paged.cu, attn_paged_tc.cu).
+// kf_paged_walk.cuh -- how the attention kernels share a step over a cache in pages among their CTAs (attn_paged.cu, attn_paged_tc.cu, attn_paged_q4.cu).
 //
 // The new tokens of a sequence are cut into blocks of `tb`, a block's visible positions into tiles; the tiles of all blocks (and of plan.heads kv heads of each), one after the
 // other, are cut into equal runs, so that every CTA has the same number of them whatever the lengths are.  A block that two or more runs share is a piece in each and is merged
@@ -11,18 +11,27 @@ struct PagedPlan {  // kernel parameter
     int tb, group, window;  // tokens of a block; heads of a kv group; positions that a row sees at most (<= 0: all)
     int heads;              // kv heads that lie one after the other in the order of tiles (1: every CTA of a team has its own)
     int runs;               // runs at most
+    int first;              // with a window, positions from 0 on that stay visible
 };
-// the positions [lo, hi) that a row of block b may see, their first tile and how many tiles they touch
-static inline __host__ __device__ int paged_block(int tile, int cap, int tb, int window, int n, int len, int b, int& lo, int& hi, int& kt0) {
-    const int first = len - n + b * tb, last = len - n + (n < (b + 1) * tb ? n : (b + 1) * tb);  // positions of the block's rows: first .. last - 1
-    hi  = last < cap ? last : cap;
-    lo  = window > 0 && first >= window ? first - window + 1 : 0;
+// The positions [lo, hi) that a row of block b may see, and with a window and first positions that lie apart from it [0, first) too; the first tile of [lo, hi), how many tiles
+// of the first positions lie in front of it (ns), and how many tiles there are.
+static inline __host__ __device__ int paged_block(int tile, int cap, int tb, int window, int first, int n, int len, int b, int& lo, int& hi, int& kt0, int& ns) {
+    const int p0 = len - n + b * tb, p1 = len - n + (n < (b + 1) * tb ? n : (b + 1) * tb);  // positions of the block's rows: p0 .. p1 - 1
+    hi = p1 < cap ? p1 : cap, ns = 0;
+    lo = window > 0 && p0 >= window ? p0 - window + 1 : 0;
+    if (window > 0) {
+        const int f = first < hi ? first : hi;
+        if (lo <= f) lo = 0;  // side by side
+        else if (f > 0 && hi <= lo) lo = 0, hi = f;  // the window lies behind the table
+        else if (f > 0) ns = (f + tile - 1) / tile;
+    }
     kt0 = lo / tile;
     if (hi <= lo) {  // nothing to see: a tile without positions, so that the rows are written
         kt0 = 0, lo = hi = 0;
         return 1;
     }
-    return (hi + tile - 1) / tile - kt0;
+    if (ns > kt0) ns = kt0;  // they end in the tile in which the window begins
+    return (hi + tile - 1) / tile - kt0 + ns;
 }
 // tiles that a step can have at most
 static inline long long paged_most(int tile, const KfPaged& pg, const PagedPlan& pl) {
@@ -31,9 +40,13 @@ static inline long long paged_most(int tile, const KfPaged& pg, const PagedPlan&
 #ifdef __CUDACC__
 struct alignas(16) PagedPiece {
     int s, q0, n, len;          // sequence, its rows in the panel, its positions
-    int t0, t1, lo, hi;         // tiles of this piece (t0 < 0: no more pieces); positions that a row of the block may see
+    int t0, t1, lo, hi;         // tiles of this piece (t0 < 0: no more pieces), see tile(); positions that a row of the block may see
     int b, head, whole, first;  // block; head of plan.heads; 1: all tiles of the block; run in which the block begins
-    int last, pad[3];           // run in which it ends
+    int last;                   // run in which it ends
+    int kt0, ns;                // first tile of [lo, hi); tiles of the first positions, which come before it
+    int pad;
+    // the tile of positions that index t stands for: those of the first positions have the ns indices in front of kt0
+    __device__ __forceinline__ int tile(int t) const { return t < kt0 ? t - kt0 + ns : t; }
 };
 // One warp's way through the sequences, 32 at a time: every lane holds one.
 template <int TILE>
@@ -53,8 +66,8 @@ struct PagedWalk {
         return v;
     }
     __device__ __forceinline__ int tiles(int n_, int len_, int b) const {
-        int lo, hi, kt0;
-        return paged_block(TILE, pg.cap, pl.tb, pl.window, n_, len_, b, lo, hi, kt0);
+        int lo, hi, kt0, ns;
+        return paged_block(TILE, pg.cap, pl.tb, pl.window, pl.first, n_, len_, b, lo, hi, kt0, ns);
     }
     __device__ __forceinline__ void load(int base_) {
         base = base_, n = 0, nb = 0, units = 0;
@@ -117,11 +130,10 @@ struct PagedWalk {
                 off -= __shfl_sync(0xffffffffu, c, 31);
             }
         }
-        int kt0;
-        const int all = paged_block(TILE, pg.cap, pl.tb, pl.window, p.n, p.len, p.b, p.lo, p.hi, kt0);
+        const int all = paged_block(TILE, pg.cap, pl.tb, pl.window, pl.first, p.n, p.len, p.b, p.lo, p.hi, p.kt0, p.ns);
         if (off >= all) p.head = off / all, off -= p.head * all;
         const int n_tiles = min(all - off, end - u);
-        p.t0 = kt0 + off, p.t1 = p.t0 + n_tiles;
+        p.t0 = p.kt0 - p.ns + off, p.t1 = p.t0 + n_tiles;
         p.whole = n_tiles == all;
         p.first = p.last = 0;
         if (!p.whole) p.first = (u - off) / run, p.last = (u - off + all - 1) / run;

@@ -35,22 +35,10 @@ struct RowsParams {
     const uint16_t *qw, *kw;
     float eps;
     uint16_t *kc, *vc;
-    long long page_stride;
+    uint8_t* pool;          // the 4-bit cache's pages, instead
+    long long page_stride;  // elements; of the 4-bit cache bytes
     KfPaged pg;
 };
-
-// the sequence that row m of the panel belongs to, -1: none.  One warp, 32 candidates at a time
-__device__ __forceinline__ int find_seq(const KfPaged& pg, int m, int lane) {
-    int lo = 0, size = pg.n_seq + 1;  // the number of starts at or before m is looked for
-    while (true) {
-        const int step = (size + 31) / 32, at = lo + lane * step;
-        const int c = __popc(__ballot_sync(0xffffffffu, at < lo + size && pg.q_start[min(at, pg.n_seq)] <= m));
-        if (c == 0) return -1;
-        const int first = lo + (c - 1) * step;
-        if (step == 1) return first < pg.n_seq ? first : -1;
-        size = min(step, lo + size - first), lo = first;
-    }
-}
 
 __device__ __forceinline__ float load1(const uint16_t* p) { return bf16_bits_to_f32(*p); }
 __device__ __forceinline__ float load1(const float* p) { return *p; }
@@ -81,15 +69,66 @@ __device__ __forceinline__ void store8(float* p, const f32x2 (&f)[4]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(a.x, a.y, b.x, b.y), reinterpret_cast<float4*>(p)[1] = make_float4(c.x, c.y, d.x, d.y);
 }
 
+__device__ __forceinline__ uint16_t bf16_bits_up(float f) { return (uint16_t)((__float_as_uint(f) + 0xffffu) >> 16); }  // f >= 0
+// A finished row of K or V into its unit of the 4-bit cache.  HD / 16 lanes side by side hold 16 entries each in `x`, entries 16 u .. 16 u + 15 in lane u; two lanes are a group.
+// All lanes of the warp call it; `to` (NULL: nothing is written) is the unit, p the position in it.  The division is the rounded one, so that a tie is a tie.
+template <int HD>
+__device__ __forceinline__ void store_q4(uint8_t* to, int p, bool is_v, int u, const float (&x)[16]) {
+    constexpr Q4Unit un(HD);
+    constexpr int G = un.groups;
+    float lo = x[0], hi = x[0];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]), most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1)), most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    const bool fine   = most < 0x7f800000u;
+    const uint32_t sb = fine ? bf16_bits_up(fmaxf(__fdiv_rn(hi - lo, 15.f), __uint_as_float(most) * (1.f / 2048.f))) : 0x7fffu;
+    const float step  = fine && sb ? bf16_bits_to_f32(sb) : 1.f;
+    const uint32_t zb = fine && sb ? f32_to_bf16_bits(__fdiv_rn(-lo, step)) : 0u;
+    const float zero  = bf16_bits_to_f32(zb);
+    uint32_t c[2] = {0u, 0u};  // entries 8 e .. 8 e + 7
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const float y = fminf(fmaxf(rintf(__fdiv_rn(x[i], step) + zero), 0.f), 15.f);  // NaN: 0
+        c[i >> 3] |= (fine ? (uint32_t)y : 0u) << (4 * (i & 7));
+    }
+    const int j = u >> 1;
+    // Values: entries 4 g .. 4 g + 3 of two groups are a word.  The lanes that hold the same entries of the two (u and u ^ 2) exchange halves, so that each has two whole words, of the
+    // first two of their four g in the lane of the even group, of the others in that of the odd one; with four groups (HD 128) the words of both halves of the row meet likewise.
+    const bool odd      = j & 1;
+    const uint32_t got  = __shfl_xor_sync(0xffffffffu, odd ? c[0] : c[1], 2), keep = odd ? c[1] : c[0];
+    const uint32_t even = odd ? got : keep, other = odd ? keep : got;
+    const uint32_t w0 = (even & 0xffffu) | other << 16, w1 = even >> 16 | (other & 0xffff0000u);
+    const bool far      = u >> 2;
+    const uint32_t give = HD == 128 ? __shfl_xor_sync(0xffffffffu, far ? w0 : w1, 4) : 0u, mine = far ? w1 : w0;
+    if (!to) return;
+    uint16_t *step_at, *zero_at;
+    if (is_v) {
+        const int g = (u & 1) * 4 + odd * 2;
+        uint8_t* at = to + un.v_code() + (p >> 1) * (HD / 8) + (p & 1) * (HD / 16);
+        if (HD == 128) *reinterpret_cast<uint2*>(at + (g + far) * (HD / 2)) = make_uint2(far ? give : mine, far ? mine : give);
+        else *reinterpret_cast<uint32_t*>(at + g * (HD / 2)) = w0, *reinterpret_cast<uint32_t*>(at + (g + 1) * (HD / 2)) = w1;
+        step_at = reinterpret_cast<uint16_t*>(to + un.v_step()) + p * G + j, zero_at = reinterpret_cast<uint16_t*>(to + un.v_zero()) + j * 8 + p;
+    } else {
+        uint32_t* w = reinterpret_cast<uint32_t*>(to + p * (HD / 2));
+        w[(u & 1) * 2 * G + j] = c[0], w[((u & 1) * 2 + 1) * G + j] = c[1];
+        step_at = reinterpret_cast<uint16_t*>(to + un.k_step()) + p * G + j, zero_at = reinterpret_cast<uint16_t*>(to + un.k_zero()) + p * G + j;
+    }
+    if (!(u & 1)) *step_at = (uint16_t)sb, *zero_at = (uint16_t)zb;
+}
+
 // LPR: lanes to a row, eight pairs each; 0: rows at any element, or pairs that do not fall on whole lanes -- a warp per row, an entry or a pair per lane
-template <typename X, typename Y, int LPR, bool NORM>
-__global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 2 ? 5 : 4) kf_rows_kernel(const __grid_constant__ RowsParams p) {
+// Q4: the cache is the 4-bit one, head_dim Q4 (0: bf16).  A finished row of K or V goes through shared memory there, so that a lane gets 16 entries side by side
+template <typename X, typename Y, int LPR, bool NORM, int Q4 = 0>
+__global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : Q4 ? 3 : NORM && sizeof(X) == 2 ? 5 : 4) kf_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int kL = LPR ? LPR : 32, kGroups = kThreads / kL, kAhead = sizeof(X) == 4 || NORM ? 1 : 2;  // rows of a lane on their way beside those in its hands
     __shared__ alignas(16) float s_cos[kTokens][128], s_sin[kTokens][128];
     __shared__ long long s_row[kTokens];  // a token's row in the pools, -1: none
     __shared__ int s_at[kTokens];         // its position in the sequence
     __shared__ bool s_ours[kTokens];      // it belongs to a sequence
     __shared__ alignas(16) uint16_t s_w[NORM ? 2 : 1][256];  // norm weights of q and k
+    __shared__ alignas(16) float s_cache[Q4 ? kThreads / kL : 1][Q4 ? Q4 + 4 : 1];
+    __shared__ int s_in[kTokens];  // Q4: the position's row in its page
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid / kL, v = tid % kL, m0 = blockIdx.x * p.tokens, nt = min(p.tokens, p.M - m0);
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();  // the panel, positions, lengths and tables come from the kernels before us
@@ -117,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 
     if (LPR) fetch(0, r0);
     if (p.nkv) {
         if (warp < nt) {
-            const int s = find_seq(pg, m0 + warp, lane);
+            const int s = paged_find_seq(pg, m0 + warp, lane);
             long long row = -1;
             int at = 0;
             if (s >= 0) {
@@ -125,7 +164,8 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 
                 paged_seq(pg, s, q0, n, len);
                 at             = len - n + (m0 + warp - q0);
                 const int page = at >= 0 ? paged_page(pg, s, at, in) : -1;
-                if (page >= 0) row = page * p.page_stride + (long long)in * p.nkv * p.hd;
+                if (page >= 0) row = page * p.page_stride + (Q4 ? in / 8 * (long long)Q4Unit(Q4).bytes : (long long)in * p.nkv * p.hd);
+                if (Q4 && lane == 0) s_in[warp] = in;
             }
             if (lane == 0) s_row[warp] = row, s_at[warp] = at, s_ours[warp] = s >= 0;
         }
@@ -185,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 
                         for (int i = 0; i < 4; i++) a[i] = mul2(mul2(a[i], iv), g[i]), b[i] = mul2(mul2(b[i], iv), h[i]);
                     }
                 }
-                if (!live) continue;
+                if (!Q4 && !live) continue;
                 if (turns && !is_v) {
                     if (p.layout) {
 #pragma unroll
@@ -204,7 +244,22 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 
                         }
                     }
                 }
-                if (is_q) {
+                if (Q4) {
+                    if (is_q && live) {
+                        Y* to = out + r * p.hd;
+                        store8(to + ea, a), store8(to + eb, b);
+                    }
+                    if (!__any_sync(0xffffffffu, live && !is_q)) continue;
+                    float* st = s_cache[grp];
+                    store8(st + ea, a), store8(st + eb, b);
+                    __syncwarp();
+                    float x[16];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) *reinterpret_cast<float4*>(&x[4 * i]) = *reinterpret_cast<const float4*>(st + 16 * v + 4 * i);
+                    const int head = is_v ? r - p.nq - p.nkv : r - p.nq;
+                    store_q4<Q4 ? Q4 : 128>(live && !is_q && row >= 0 ? p.pool + row + (long long)head * (pg.page / 8) * Q4Unit(Q4).bytes : nullptr, s_in[t] & 7, is_v, v, x);
+                    __syncwarp();
+                } else if (is_q) {
                     Y* to = out + r * p.hd;
                     store8(to + ea, a), store8(to + eb, b);
                 } else if (row >= 0) {
@@ -229,9 +284,10 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 
             }
             auto in     = [&](int i) { return w ? load1(in_row + i) * inv * bf16_bits_to_f32(w[i]) : load1(in_row + i); };
             Y* to       = (Y*)p.out + (m0 + t) * p.ldo + r * p.hd;
-            uint16_t* c = is_q ? nullptr : is_v ? p.vc + s_row[t] + (r - p.nq - p.nkv) * p.hd : p.kc + s_row[t] + (r - p.nq) * p.hd;
+            uint16_t* c = is_q || Q4 ? nullptr : is_v ? p.vc + s_row[t] + (r - p.nq - p.nkv) * p.hd : p.kc + s_row[t] + (r - p.nq) * p.hd;
             auto put    = [&](int i, float y) {
                 if (is_q) store1(to + i, y);
+                else if (Q4) s_cache[grp][i] = y;
                 else store1(c + i, y);
             };
             const int pairs = is_v ? 0 : half;
@@ -241,6 +297,14 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : NORM && sizeof(X) == 
                 put(ia, a * cs - b * sn), put(ib, b * cs + a * sn);
             }
             for (int i = 2 * pairs + lane; i < p.hd; i += 32) put(i, in(i));
+            if (Q4 && !is_q) {
+                __syncwarp();
+                const int u = min(lane, Q4 / 16 - 1), head = is_v ? r - p.nq - p.nkv : r - p.nq;
+                float e[16];
+                for (int i = 0; i < 16; i++) e[i] = s_cache[grp][16 * u + i];
+                store_q4<Q4 ? Q4 : 128>(lane < Q4 / 16 ? p.pool + s_row[t] + (long long)head * (pg.page / 8) * Q4Unit(Q4).bytes : nullptr, s_in[t] & 7, is_v, lane & (Q4 / 16 - 1), e);
+                __syncwarp();
+            }
         }
     }
 }
@@ -255,6 +319,11 @@ int launch_rows(kf_ctx* ctx, RowsParams& p, bool wide) {
     const dim3 grid((p.M + p.tokens - 1) / p.tokens, (all + p.rows_per_block - 1) / p.rows_per_block);
     auto pick = [&](auto normed) {
         constexpr bool N = decltype(normed)::value;
+        if constexpr (std::is_same_v<Y, uint16_t>)  // finished queries are bf16
+            if (p.pool) {
+                if (p.hd == 64) return lpr ? kf_rows_kernel<X, Y, 4, N, 64> : kf_rows_kernel<X, Y, 0, N, 64>;
+                return lpr ? kf_rows_kernel<X, Y, 8, N, 128> : kf_rows_kernel<X, Y, 0, N, 128>;
+            }
         return lpr == 0 ? kf_rows_kernel<X, Y, 0, N> : lpr == 4 ? kf_rows_kernel<X, Y, 4, N> : lpr == 8 ? kf_rows_kernel<X, Y, 8, N> : kf_rows_kernel<X, Y, 16, N>;
     };
     auto kern = p.qw || p.kw ? pick(std::true_type()) : pick(std::false_type());
@@ -276,16 +345,37 @@ int rotation(kf_ctx* ctx, const kf_rotation* rot, int hd, int M, RowsParams* p) 
 bool whole_lanes(const RowsParams& p) { return p.hd % 16 == 0 && (p.layout == 0 || p.rot % 16 == 0); }
 }  // namespace
 
-int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out) {
-    KF_REQUIRE(ctx, kv->k_dev && kv->v_dev && kv->table_dev && kv->q_start_dev && kv->len_dev, "cache, table, starts and lengths");
+// what the caches in bf16 and in 4 bits have in common
+template <typename KV>
+static int check_step(kf_ctx* ctx, const KV* kv, int M, KfPaged* out) {
+    KF_REQUIRE(ctx, kv->table_dev && kv->q_start_dev && kv->len_dev, "table, starts and lengths");
     KF_REQUIRE(ctx, kv->head_dim == 64 || kv->head_dim == 128, "head_dim 64 or 128");
     KF_REQUIRE(ctx, kv->n_kv >= 1 && kv->n_kv <= 1024 && kv->n_pages >= 1 && kv->page_size >= 8 && kv->page_size % 8 == 0, "n_kv 1 .. 1024, page_size a multiple of 8");
     KF_REQUIRE(ctx, kv->table_cols >= 1 && (long long)kv->table_cols * kv->page_size <= 0x7fffffff - 256, "table_cols");
     KF_REQUIRE(ctx, kv->n_seq >= 1 && kv->n_seq <= 8192 && M >= 0, "n_seq 1 .. 8192");
-    KF_REQUIRE(ctx, kv->page_stride == 0 || (kv->page_stride % 8 == 0 && kv->page_stride >= (size_t)kv->page_size * kv->n_kv * kv->head_dim), "page_stride: a multiple of 8, at least a page");
-    KF_REQUIRE(ctx, (((uintptr_t)kv->k_dev | (uintptr_t)kv->v_dev) & 15) == 0, "pages at 16 bytes");
     *out = KfPaged{kv->table_dev, kv->q_start_dev, kv->len_dev, kv->table_cols, kv->n_seq, kv->n_pages, kv->page_size, kv->table_cols * kv->page_size, M, 0, 0};
     kf_paged_divisor(out);
+    return KF_OK;
+}
+int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out) {
+    KF_REQUIRE(ctx, kv->k_dev && kv->v_dev, "cache");
+    const int rc = check_step(ctx, kv, M, out);
+    if (rc) return rc;
+    KF_REQUIRE(ctx, kv->page_stride == 0 || (kv->page_stride % 8 == 0 && kv->page_stride >= (size_t)kv->page_size * kv->n_kv * kv->head_dim), "page_stride: a multiple of 8, at least a page");
+    KF_REQUIRE(ctx, (((uintptr_t)kv->k_dev | (uintptr_t)kv->v_dev) & 15) == 0, "pages at 16 bytes");
+    return KF_OK;
+}
+extern "C" size_t kf_paged_q4_page_bytes(int page_size, int n_kv, int head_dim) {
+    return page_size >= 8 && page_size % 8 == 0 && n_kv >= 1 && (head_dim == 64 || head_dim == 128) ? (size_t)(page_size / 8) * n_kv * Q4Unit(head_dim).bytes : 0;
+}
+int kf_paged_q4_check(kf_ctx* ctx, const kf_paged_q4* kv, int M, KfPaged* out) {
+    KF_REQUIRE(ctx, kv->pool_dev, "cache");
+    const int rc = check_step(ctx, kv, M, out);
+    if (rc) return rc;
+    KF_REQUIRE(ctx, kv->page_stride == 0 || (kv->page_stride % 16 == 0 && kv->page_stride >= kf_paged_q4_page_bytes(kv->page_size, kv->n_kv, kv->head_dim)),
+               "page_stride: a multiple of 16, at least a page");
+    KF_REQUIRE(ctx, kv->page_stride < (1ull << 62), "page_stride");
+    KF_REQUIRE(ctx, ((uintptr_t)kv->pool_dev & 15) == 0, "pages at 16 bytes");
     return KF_OK;
 }
 
@@ -300,10 +390,13 @@ extern "C" int kf_rows_overlap(const void* a, size_t a_pitch, size_t a_wide, con
     return 0;
 }
 
-static int append_args(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, const void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
+static int check_cache(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out) { return kf_paged_check(ctx, kv, M, out); }
+static int check_cache(kf_ctx* ctx, const kf_paged_q4* kv, int M, KfPaged* out) { return kf_paged_q4_check(ctx, kv, M, out); }
+template <typename KV>
+static int append_args(kf_ctx* ctx, const KV* kv, const kf_rotation* rot, const void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
                        int src_f32, int M, int n_head, RowsParams* p) {
     if (!kv || !q_out || !q || !k || !v) return KF_ERR_BAD_ARG;
-    int rc = kf_paged_check(ctx, kv, M, &p->pg);
+    int rc = check_cache(ctx, kv, M, &p->pg);
     if (!rc) rc = rotation(ctx, rot, kv->head_dim, M, p);
     if (rc) return rc;
     const int hd = kv->head_dim;
@@ -313,10 +406,10 @@ static int append_args(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* ro
     KF_REQUIRE(ctx, q_out != q || ldqo == ldq, "in place: rows where they were");
     return KF_OK;
 }
-extern "C" int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
-                               int src_f32, int M, int n_head, const void* qnorm_w, const void* knorm_w, float eps) {
-    if (!ctx) return KF_ERR_BAD_ARG;
-    RowsParams p = {};
+// the cache's own addresses are in p already
+template <typename KV>
+static int append(kf_ctx* ctx, RowsParams& p, const KV* kv, const kf_rotation* rot, void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int src_f32,
+                  int M, int n_head, const void* qnorm_w, const void* knorm_w, float eps) {
     const int rc = append_args(ctx, kv, rot, q_out, ldqo, q, ldq, k, ldk, v, ldv, src_f32, M, n_head, &p);
     if (rc) return rc;
     const int hd = kv->head_dim;
@@ -326,11 +419,24 @@ extern "C" int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rota
     KF_REQUIRE(ctx, (q_out == q || !over(q, ldq, q_wide)) && !over(k, ldk, kv_wide) && !over(v, ldv, kv_wide), "the finished queries over a part of the panel");
     p.q = q, p.k = k, p.v = v, p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.out = q_out, p.ldo = ldqo, p.nq = n_head, p.nkv = kv->n_kv, p.hd = hd, p.M = M;
     p.qw = (const uint16_t*)qnorm_w, p.kw = (const uint16_t*)knorm_w, p.eps = eps;
-    p.kc = (uint16_t*)kv->k_dev, p.vc = (uint16_t*)kv->v_dev, p.page_stride = (long long)kf_paged_stride(kv);
     const int per = src_f32 ? 4 : 8;  // elements in 16 bytes
     const bool wide = whole_lanes(p) && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)qnorm_w | (uintptr_t)knorm_w) & 15) == 0 && ldq % per == 0 &&
                       ldk % per == 0 && ldv % per == 0 && ldqo % 8 == 0;
     return src_f32 ? launch_rows<float, uint16_t>(ctx, p, wide) : launch_rows<uint16_t, uint16_t>(ctx, p, wide);
+}
+extern "C" int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
+                               int src_f32, int M, int n_head, const void* qnorm_w, const void* knorm_w, float eps) {
+    if (!ctx || !kv) return KF_ERR_BAD_ARG;
+    RowsParams p = {};
+    p.kc = (uint16_t*)kv->k_dev, p.vc = (uint16_t*)kv->v_dev, p.page_stride = (long long)kf_paged_stride(kv);
+    return append(ctx, p, kv, rot, q_out, ldqo, q, ldq, k, ldk, v, ldv, src_f32, M, n_head, qnorm_w, knorm_w, eps);
+}
+extern "C" int kf_paged_append_q4(kf_ctx* ctx, const kf_paged_q4* kv, const kf_rotation* rot, void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
+                                  int src_f32, int M, int n_head, const void* qnorm_w, const void* knorm_w, float eps) {
+    if (!ctx || !kv) return KF_ERR_BAD_ARG;
+    RowsParams p = {};
+    p.pool = (uint8_t*)kv->pool_dev, p.page_stride = (long long)kf_paged_q4_stride(kv);
+    return append(ctx, p, kv, rot, q_out, ldqo, q, ldq, k, ldk, v, ldv, src_f32, M, n_head, qnorm_w, knorm_w, eps);
 }
 
 static int rope_args(kf_ctx* ctx, const kf_rotation* rot, const void* out, int ldo, const void* x, int ldx, int f32, int M, int n_head, int hd, RowsParams* p) {
@@ -358,6 +464,11 @@ extern "C" int kf_rope_axes(kf_ctx* ctx, const kf_rotation* rot, void* out, int 
 // The checks for tests on a host without a device
 extern "C" int kf_paged_append_args(const kf_paged_kv* kv, const kf_rotation* rot, const void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
                                     int src_f32, int M, int n_head) {
+    RowsParams p = {};
+    return append_args(nullptr, kv, rot, q_out, ldqo, q, ldq, k, ldk, v, ldv, src_f32, M, n_head, &p);
+}
+extern "C" int kf_paged_append_q4_args(const kf_paged_q4* kv, const kf_rotation* rot, const void* q_out, int ldqo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
+                                       int src_f32, int M, int n_head) {
     RowsParams p = {};
     return append_args(nullptr, kv, rot, q_out, ldqo, q, ldq, k, ldk, v, ldv, src_f32, M, n_head, &p);
 }
