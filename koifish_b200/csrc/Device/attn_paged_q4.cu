@@ -15,10 +15,15 @@
 //   * A warp takes 16 positions (two units) of a tile of 64; a unit is contiguous (Q4Unit), so a tile is a bulk copy per page (or part of 8, 16, 32 or 64 positions of it).
 #include <algorithm>
 
-#include "kf_paged_finish.cuh"
+#include "kf_paged_walk.cuh"
 
 namespace {
-constexpr int kTok = 64, kWarps = 4, kMaxStages = 12;
+#ifndef Q4_WARPS
+#define Q4_WARPS 4
+#define Q4_SUB 2
+#define Q4_OCC 2
+#endif
+constexpr int kWarps = Q4_WARPS, kSub = Q4_SUB, kTok = 16 * kSub * kWarps, kMaxStages = 12;  // computing warps; groups of 16 positions that a warp takes of a tile; positions of a tile
 constexpr float kSlack = 8.f;  // growth of a maximum, log2, that sums are not rescaled for
 
 // bytes from global into shared memory, both at 16 bytes, a multiple of 16
@@ -27,8 +32,30 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+// products of 16 rows, 16 steps and 8 columns: c + a b, and a b.  Not volatile, nor are the loads around them: the scheduler is to mix what is independent
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// N words of shared memory, aligned to as many (up to four)
+template <int N>
+__device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 // pairs of codes out of a word: nibbles (0, 4), (1, 5), (2, 6), (3, 7); the second and the fourth stand for 16 times their codes
 __device__ __forceinline__ void codes(uint32_t w, uint32_t (&c)[4]) { c[0] = w & 0x000f000fu, c[1] = w & 0x00f000f0u, c[2] = (w >> 8) & 0x000f000fu, c[3] = (w >> 8) & 0x00f000f0u; }
@@ -38,9 +65,9 @@ struct Q4Args {  // kernel parameter
     long long page_stride;
     uint16_t* out;
     const uint16_t* q;
-    float* ws;
+    float* ws;        // [CTA][2][rb][HD] sums, then as many (maximum, denominator) pairs, then what begins in a run and goes on behind it, per CTA
     float2* ws_ml;
-    unsigned* cnt;
+    PagedPiece* rec;
     long long ldo, ldq;
     int n_kv, parts, heads;  // a kv head's group in `parts` of up to `heads` heads, a CTA of the team each
     int box, stages;         // positions of a copy
@@ -49,8 +76,18 @@ struct Q4Args {  // kernel parameter
 __host__ __device__ constexpr int stage_bytes(int hd) { return kTok / 8 * Q4Unit(hd).bytes; }
 constexpr int rows_area(int hd, int rb) { return kWarps * rb * hd * 4; }
 
+__device__ __forceinline__ uint16_t* out_row(const Q4Args& a, const PagedPlan& pl, const PagedPiece& pc, int kvh, int h0, int heads, int r, int hd) {
+    return a.out + (pc.q0 + pc.b * pl.tb + r / heads) * a.ldo + (long long)(kvh * pl.group + h0 + r % heads) * hd;
+}
+__device__ __forceinline__ void put_row(uint16_t* p, float4 v, float l, bool vec) {
+    const float f      = l == 0.f ? 0.f : 1.f / l;
+    const uint32_t lo = pack_bf16x2(v.x * f, v.y * f), hi = pack_bf16x2(v.z * f, v.w * f);
+    if (vec) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+    else p[0] = lo & 0xffff, p[1] = lo >> 16, p[2] = hi & 0xffff, p[3] = hi >> 16;
+}
+
 template <int HD, int NT, int OCC>
-__global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
+__global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     kf_attn_paged_q4_kernel(const __grid_constant__ Q4Args a, const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ KfBound bound) {
     constexpr Q4Unit un(HD);
     constexpr int G = un.groups, UNIT = un.bytes, STAGE = stage_bytes(HD);
@@ -58,14 +95,14 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
     float* s_o = reinterpret_cast<float*>(ring + (size_t)a.stages * STAGE);  // [kWarps][rb][HD]
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], meet_bar;
     __shared__ volatile int dead;
-    __shared__ int s_there[kMaxStages], s_last;  // bit i: positions 8 i .. 8 i + 7 of the tile are there
+    __shared__ int s_there[kMaxStages];  // bit i: positions 8 i .. 8 i + 7 of the tile are there
     __shared__ PagedQueue qu;
     __shared__ float s_m[kWarps][16], s_l[kWarps][16];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     if (tid == 0) {
         for (int s = 0; s < a.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], kWarps);
         mbar_init(&meet_bar, kWarps);
-        qu.init(kWarps + 1);
+        qu.init(kWarps);
         dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -75,49 +112,56 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
     const KfPaged pg    = behind_wait(pg_);
     const uint16_t* q   = behind_wait(a.q);
     const int mates = a.n_kv * a.parts, team = (int)blockIdx.x / mates, mate = (int)blockIdx.x % mates, kvh = mate / a.parts, h0 = mate % a.parts * a.heads;
+    const int rec = mate * ((int)gridDim.x / mates) + team;
     if (pg.n_seq > 32) {
-        PagedPlanner<kTok>::count(pg, pl, qu.s_sum, warp, kWarps + 2, lane);
+        PagedPlanner<kTok>::count(pg, pl, qu.s_sum, warp, kWarps + 1, lane);
         __syncthreads();
-    }
-    if (warp == kWarps + 1) {
-        PagedPlanner<kTok> plan(pg, pl, lane);
-        plan.start(qu, team);
-        while (plan.push(qu, team, nullptr, &dead, bound)) {}
-        return;
     }
     PagedReader reader;
     PagedPiece pc;
     bool live = true;
     if (warp == kWarps) {
-        if (bound.drop == (int)blockIdx.x + 1) return;
+        // One warp works the pieces out and loads their tiles, up to a ring ahead of the others
+        PagedPlanner<kTok> plan(pg, pl, lane);
+        if (lane == 0) a.rec[rec].last = 0;  // nothing to merge, should a wait run out before the end of the run is known
+        plan.start(qu, team);
+        if (bound.drop == (int)blockIdx.x + 1) {
+            while (plan.push(qu, team, a.rec + rec - team, &dead, bound)) {}
+            return;
+        }
         uint32_t st = 0, ph = 0, asked = 0;
-        const int n_box = kTok / a.box, bx = lane;  // a lane per box; bx >= n_box: none
-        const uint32_t bytes = (uint32_t)(a.box / 8 * UNIT);
-        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
+        // A lane per box (page, or part of one) of several tiles: the pages of the next 32 boxes are looked up while those before are copied.  A look-up takes about as long as
+        // two tiles (one tile ahead, as where tiles are four times as large: 78 us for the 64 sequences below)
+        const int n_box = kTok / a.box, units = a.box / 8, ahead = 32 / n_box, bx = lane % n_box, mine = lane < ahead * n_box ? lane / n_box : 1 << 24;
+        const uint32_t bytes = (uint32_t)(units * UNIT);
+        uint8_t* dst         = ring + bx * units * UNIT;
+        while (live && plan.push(qu, team, a.rec + rec - team, &dead, bound)) {
+            pc           = plan.pc;
             const int fs = pc.lo > 0 ? pl.first : 0;
             int next_row = 0;
-            auto page_of = [&](int t) {  // the page of this lane's box of tile t
+            auto page_of = [&](int t) {
                 const int p = pc.tile(t) * kTok + bx * a.box;
-                return t < pc.t1 && bx < n_box && p < pc.hi && (p + a.box > pc.lo || p < fs) ? paged_page(pg, pc.s, p, next_row) : -1;
+                return t < pc.t1 && p < pc.hi && (p + a.box > pc.lo || p < fs) ? paged_page(pg, pc.s, p, next_row) : -1;
             };
-            int next = page_of(pc.t0);
-            for (int t = pc.t0; live && t < pc.t1; t++) {
-                const int page = next, row = next_row;
-                next = page_of(t + 1);  // a tile ahead: the look-up takes as long as a tile
-                const unsigned lanes = __ballot_sync(0xffffffffu, page >= 0);
-                if (!(live = mbar_wait_warp(smem_u32(&empty[st]), ph ^ 1, &dead, bound))) break;
-                if (lane == 0) {
-                    unsigned there = 0;
-                    for (int i = 0; i < kTok / 8; i++) there |= (lanes >> (i * 8 / a.box) & 1) << i;
-                    s_there[st] = (int)there;
-                    mbar_arrive_expect_tx(&full[st], (uint32_t)__popc(lanes) * bytes);
+            int next = page_of(pc.t0 + mine);
+            for (int t0 = pc.t0; live && t0 < pc.t1; t0 += ahead) {
+                const int page = next, row = next_row, n = min(ahead, pc.t1 - t0);
+                next = page_of(t0 + ahead + mine);
+                const uint8_t* src   = a.pool + page * a.page_stride + ((long long)kvh * (pg.page / 8) + row / 8) * UNIT;
+                const unsigned has = page >= 0 ? ((1u << units) - 1u) << (bx * units) : 0u;  // units of its tile that the lane brings
+                for (int i = 0; i < n; i++) {
+                    const unsigned there = __reduce_or_sync(0xffffffffu, mine == i ? has : 0u);
+                    if (!(live = mbar_wait_warp(smem_u32(&empty[st]), ph ^ 1, &dead, bound))) break;
+                    if (lane == 0) {
+                        s_there[st] = (int)there;
+                        mbar_arrive_expect_tx(&full[st], (uint32_t)__popc(there) * UNIT);
+                    }
+                    __syncwarp();
+                    if (mine == i && page >= 0) bulk_load(dst + st * STAGE, src, bytes, &full[st]);
+                    __syncwarp();
+                    asked++;
+                    if (++st == (uint32_t)a.stages) st = 0, ph ^= 1;
                 }
-                __syncwarp();
-                if (page >= 0)
-                    bulk_load(ring + (size_t)st * STAGE + bx * a.box / 8 * UNIT, a.pool + page * a.page_stride + ((long long)kvh * (pg.page / 8) + row / 8) * UNIT, bytes, &full[st]);
-                __syncwarp();
-                asked++;
-                if (++st == (uint32_t)a.stages) st = 0, ph ^= 1;
             }
         }
         // copies in flight write shared memory, which is another's once the CTA has ended, and where a wait has run out nobody else may have waited for them
@@ -136,7 +180,7 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
     while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
         const int rows = min(pl.tb, pc.n - pc.b * pl.tb) * heads, fs = pc.lo > 0 ? pl.first : 0;
         // The block's queries as B operands.  Slot pairs of a lane's words: entries (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of its 8 of every group, times 2^60; rows past the end: zero
-        uint32_t qb[NT][G][4], qz[NT][2];  // qz: minus the sum of q over group t4, times 2^-73, as three numbers
+        uint32_t qb[NT][G][4], qz[NT][G][2];  // qz: minus the sum of q over a group, times 2^-73, as three numbers in the lanes of the group's slot
         int lim[NT][2], low[NT][2];        // what the lane's columns see: positions above `low`, or of the first, up to `lim`
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -160,7 +204,8 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
             }
             mine *= -0x1p-73f;
             const float hi = __bfloat162float(__float2bfloat16_rn(mine)), mid = __bfloat162float(__float2bfloat16_rn(mine - hi));
-            qz[n][0] = t4 < G ? pack_bf16x2(hi, mid) : 0u, qz[n][1] = t4 < G ? pack_bf16x2(mine - hi - mid, 0.f) : 0u;
+#pragma unroll
+            for (int j = 0; j < G; j++) qz[n][j][0] = t4 == j ? pack_bf16x2(hi, mid) : 0u, qz[n][j][1] = t4 == j ? pack_bf16x2(mine - hi - mid, 0.f) : 0u;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const int tc = pc.b * pl.tb + (n * 8 + 2 * t4 + e) / heads;
@@ -182,28 +227,21 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
         }
         for (int t = pc.t0; t < pc.t1; t++) {
             if (!(live = mbar_wait_warp(smem_u32(&full[st]), ph, &dead, bound))) break;
-            const int tok0 = pc.tile(t) * kTok + warp * 16;  // this warp's 16 positions
-            const unsigned there = ((unsigned)*(volatile int*)&s_there[st] >> (warp * 2)) & 3u;
-            if (there && tok0 < pc.hi && (tok0 + 16 > pc.lo || tok0 < fs)) {
-                const uint32_t u0 = smem_u32(ring + (size_t)st * STAGE + warp * 2 * UNIT);  // the two units
-                const bool ragged = there != 3u || tok0 + 16 > sure_hi || (tok0 < sure_lo && tok0 + 16 > fw);
-                // ---- scores, transposed: rows are positions g of both units, columns the block's rows ----
-                float sc[NT][4];
+            const int tok0 = pc.tile(t) * kTok + warp * 16 * kSub;  // this warp's positions
+            const unsigned there = ((unsigned)*(volatile int*)&s_there[st] >> (warp * 2 * kSub)) & ((1u << (2 * kSub)) - 1u);
+            if (there && tok0 < pc.hi && (tok0 + 16 * kSub > pc.lo || tok0 < fs)) {
+                const uint8_t* u0 = ring + st * STAGE + warp * 2 * kSub * UNIT;  // their units
+                const bool ragged = there != (1u << (2 * kSub)) - 1u || tok0 + 16 * kSub > sure_hi || (tok0 < sure_lo && tok0 + 16 * kSub > fw);
+                // ---- scores, transposed: rows are positions g of two units, columns the block's rows ----
+                float sc[kSub][NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-                {
+                for (int b = 0; b < kSub; b++) {
                     uint32_t kw[2][G], kz[2], ks[2][G / 2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const uint32_t u = u0 + e * UNIT;
-                        if constexpr (G == 4) lds128(u + lane * 16, kw[e]), lds64(u + un.k_step() + g * 8, ks[e]);
-                        else {
-                            lds64(u + lane * 8, kw[e]);
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(ks[e][0]) : "r"(u + un.k_step() + g * 4) : "memory");
-                        }
-                        uint16_t z;
-                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(z) : "r"(u + un.k_zero() + (g * G + t4 % G) * 2) : "memory");
-                        kz[e] = z | (uint32_t)z << 16;
+                        const uint8_t* u = u0 + (2 * b + e) * UNIT;
+                        words(u + lane * 4 * G, kw[e]), words(u + un.k_step() + g * 2 * G, ks[e]);
+                        kz[e] = *reinterpret_cast<const uint16_t*>(u + un.k_zero() + (g * G + t4 % G) * 2) * 0x10001u;
                     }
                     const uint32_t az[4] = {kz[0], kz[1], kz[0], kz[1]};
 #pragma unroll
@@ -214,102 +252,112 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
                         const float s0 = j & 1 ? bf16hi(ks[0][j / 2]) : bf16lo(ks[0][j / 2]), s1 = j & 1 ? bf16hi(ks[1][j / 2]) : bf16lo(ks[1][j / 2]);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma16816(acc, az, t4 == j ? qz[n][0] : 0u, t4 == j ? qz[n][1] : 0u);
-                            mma16816(acc, a0, qb[n][j][0], qb[n][j][1]);
-                            mma16816(acc, a1, qb[n][j][2], qb[n][j][3]);
-                            sc[n][0] = fmaf(s0, acc[0], sc[n][0]), sc[n][1] = fmaf(s0, acc[1], sc[n][1]);
-                            sc[n][2] = fmaf(s1, acc[2], sc[n][2]), sc[n][3] = fmaf(s1, acc[3], sc[n][3]);
+                            float acc[4];
+                            mma_new(acc, az, qz[n][j][0], qz[n][j][1]);
+                            mma(acc, a0, qb[n][j][0], qb[n][j][1]);
+                            mma(acc, a1, qb[n][j][2], qb[n][j][3]);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) sc[b][n][i] = j == 0 ? (i < 2 ? s0 : s1) * acc[i] : fmaf(i < 2 ? s0 : s1, acc[i], sc[b][n][i]);
                         }
                     }
                 }
                 // ---- weights, times 2^60 ----
-                bool ok[2] = {true, true};  // somebody may see the lane's positions, and they are there
+                unsigned ok = ~0u;  // bit 2 b + e: somebody may see the lane's position, and it is there
                 if (ragged) {
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
+                    for (int e = 0; e < 2 * kSub; e++) {
                         const int p = tok0 + 8 * e + g;
-                        ok[e] = p < pc.hi && (p >= pc.lo || p < fs) && (there >> e & 1);
+                        if (!(p < pc.hi && (p >= pc.lo || p < fs) && (there >> e & 1))) ok &= ~(1u << e);
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
                             for (int i = 0; i < 2; i++)
-                                if (!ok[e] || p > lim[n][i] || (p <= low[n][i] && p >= fw)) sc[n][2 * e + i] = -INFINITY;
+                                if (!(ok >> e & 1) || p > lim[n][i] || (p <= low[n][i] && p >= fw)) sc[e / 2][n][2 * (e & 1) + i] = -INFINITY;
                     }
                 }
+                float mx[NT][2];
                 bool grown = false;
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) grown |= fmaxf(sc[n][i], sc[n][2 + i]) * a.sc2 > m[n][i] + kSlack;
+                    for (int i = 0; i < 2; i++) {
+                        mx[n][i] = fmaxf(sc[0][n][i], sc[0][n][2 + i]);
+#pragma unroll
+                        for (int b = 1; b < kSub; b++) mx[n][i] = fmaxf(mx[n][i], fmaxf(sc[b][n][i], sc[b][n][2 + i]));
+                        mx[n][i] *= a.sc2;
+                        grown |= mx[n][i] > m[n][i] + kSlack;
+                    }
                 if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            float mx = fmaxf(sc[n][i], sc[n][2 + i]) * a.sc2;
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4)), mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8)), mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                            mx = fmaxf(mx, m[n][i]);
-                            const float f = ex2(m[n][i] - finite_or_0(mx));
-                            m[n][i] = mx, l[n][i] *= f, oz[n][i] *= f, oz[n][2 + i] *= f;
+                            float x = mx[n][i];
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4)), x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8)), x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            x = fmaxf(x, m[n][i]);
+                            const float f = ex2(m[n][i] - finite_or_0(x));
+                            m[n][i] = x, l[n][i] *= f, oz[n][i] *= f, oz[n][2 + i] *= f;
 #pragma unroll
                             for (int j = 0; j < G; j++) o[n][j][0][i] *= f, o[n][j][0][2 + i] *= f, o[n][j][1][i] *= f, o[n][j][1][2 + i] *= f;
                         }
                 }
-                float p[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const float base = finite_or_0(m[n][i]) - 60.f;
-                        p[n][i] = ex2(fmaf(sc[n][i], a.sc2, -base)), p[n][2 + i] = ex2(fmaf(sc[n][2 + i], a.sc2, -base));
-                        l[n][i] += p[n][i] + p[n][2 + i];
+                        const float base = 60.f - finite_or_0(m[n][i]);
+#pragma unroll
+                        for (int b = 0; b < kSub; b++) {
+                            float(&p)[4] = sc[b][n];
+                            p[i] = ex2(fmaf(p[i], a.sc2, base)), p[2 + i] = ex2(fmaf(p[2 + i], a.sc2, base));
+                            l[n][i] += p[i] + p[2 + i];
+                        }
                     }
                 // ---- sums, transposed: rows are dims ----
-                uint32_t vs[2][G / 2], vw[2][G], vz[2];
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t u = u0 + e * UNIT;
-                    if constexpr (G == 4) lds128(u + un.v_code() + lane * 16, vw[e]), lds64(u + un.v_step() + g * 8, vs[e]);
-                    else {
-                        lds64(u + un.v_code() + lane * 8, vw[e]);
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vs[e][0]) : "r"(u + un.v_step() + g * 4) : "memory");
-                    }
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vz[e]) : "r"(u + un.v_zero() + (g % G) * 16 + t4 * 4) : "memory");  // positions 2 t4, 2 t4 + 1 of group g
-                }
-                if (ragged) {  // what no row sees need not be numbers
+                for (int b = 0; b < kSub; b++) {
+                    uint32_t vs[2][G / 2], vw[2][G], vz[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        if (!ok[e]) {
+                        const uint8_t* u = u0 + (2 * b + e) * UNIT;
+                        words(u + un.v_code() + lane * 4 * G, vw[e]), words(u + un.v_step() + g * 2 * G, vs[e]);
+                        vz[e] = *reinterpret_cast<const uint32_t*>(u + un.v_zero() + (g % G) * 16 + t4 * 4);  // positions 2 t4, 2 t4 + 1 of group g
+                    }
+                    if (ragged) {  // what no row sees need not be numbers
 #pragma unroll
-                            for (int j = 0; j < G / 2; j++) vs[e][j] = 0u;
-                        }
+                        for (int e = 0; e < 2; e++) {
+                            if (!(ok >> (2 * b + e) & 1)) {
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const int pp = tok0 + 8 * e + 2 * t4 + i;
-                            if (!(pp < pc.hi && (pp >= pc.lo || pp < fs) && (there >> e & 1))) vz[e] &= i ? 0x0000ffffu : 0xffff0000u;
+                                for (int j = 0; j < G / 2; j++) vs[e][j] = 0u;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const int pp = tok0 + 8 * (2 * b + e) + 2 * t4 + i;
+                                if (!(pp < pc.hi && (pp >= pc.lo || pp < fs) && (there >> (2 * b + e) & 1))) vz[e] &= i ? 0x0000ffffu : 0xffff0000u;
+                            }
                         }
                     }
+#pragma unroll
+                    for (int w = 0; w < G / 2; w++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {  // group 2 w + h
+                            const int j = 2 * w + h;
+                            uint32_t c0[4], c1[4];
+                            codes(__byte_perm(vw[0][w], vw[0][G / 2 + w], h ? 0x7632 : 0x5410), c0);
+                            codes(__byte_perm(vw[1][w], vw[1][G / 2 + w], h ? 0x7632 : 0x5410), c1);
+                            const uint32_t a0[4] = {c0[0], c0[1], c1[0], c1[1]}, a1[4] = {c0[2], c0[3], c1[2], c1[3]};
+                            const uint32_t az[4] = {g == j ? vz[0] : 0u, 0u, g == j ? vz[1] : 0u, 0u};
+                            const float s0 = h ? bf16hi(vs[0][w]) : bf16lo(vs[0][w]), s1 = h ? bf16hi(vs[1][w]) : bf16lo(vs[1][w]);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                const float(&p)[4] = sc[b][n];
+                                const uint32_t b0 = transpose8x8(pack_bf16x2(p[0] * s0, p[1] * s0)), b1 = transpose8x8(pack_bf16x2(p[2] * s1, p[3] * s1));
+                                mma(o[n][j][0], a0, b0, b1);
+                                mma(o[n][j][1], a1, b0, b1);
+                                mma(oz[n], az, b0, b1);
+                            }
+                        }
                 }
-#pragma unroll
-                for (int w = 0; w < G / 2; w++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {  // group 2 w + h
-                        const int j = 2 * w + h;
-                        uint32_t c0[4], c1[4];
-                        codes(__byte_perm(vw[0][w], vw[0][G / 2 + w], h ? 0x7632 : 0x5410), c0);
-                        codes(__byte_perm(vw[1][w], vw[1][G / 2 + w], h ? 0x7632 : 0x5410), c1);
-                        const uint32_t a0[4] = {c0[0], c0[1], c1[0], c1[1]}, a1[4] = {c0[2], c0[3], c1[2], c1[3]};
-                        const uint32_t az[4] = {g == j ? vz[0] : 0u, 0u, g == j ? vz[1] : 0u, 0u};
-                        const float s0 = h ? bf16hi(vs[0][w]) : bf16lo(vs[0][w]), s1 = h ? bf16hi(vs[1][w]) : bf16lo(vs[1][w]);
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            const uint32_t b0 = transpose8x8(pack_bf16x2(p[n][0] * s0, p[n][1] * s0)), b1 = transpose8x8(pack_bf16x2(p[n][2] * s1, p[n][3] * s1));
-                            mma16816(o[n][j][0], a0, b0, b1);
-                            mma16816(o[n][j][1], a1, b0, b1);
-                            mma16816(oz[n], az, b0, b1);
-                        }
-                    }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
@@ -335,12 +383,88 @@ __global__ void __launch_bounds__((kWarps + 2) * 32, OCC)
             }
         meet();
         if (!live) break;
-        auto out_row = [&](int r) {
-            return a.out + (pc.q0 + pc.b * pl.tb + r / heads) * a.ldo + (long long)(kvh * group + h0 + r % heads) * HD;
-        };
-        paged_finish<HD, kWarps>(pc, PagedSums{team, mate, mates, a.ws, a.ws_ml, a.cnt}, rows, rb, s_o, s_m, s_l, &s_last, vec, live, out_row, meet);
+        // the warps' sums as one, in order: the result, or what is left for the merge -- a CTA has at most one piece that others have begun (slot 0) and one that others go on with (slot 1)
+        const size_t slot = (size_t)blockIdx.x * 2 + (pc.first == team);
+        for (int idx = tid; idx < rows * (HD / 4); idx += kWarps * 32) {
+            const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w][r]);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float f  = ex2(s_m[w][r] - finite_or_0(top));
+                const float4 x = *reinterpret_cast<const float4*>(s_o + ((size_t)w * rb + r) * HD + c);
+                sum = fmaf(s_l[w][r], f, sum);
+                v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
+            }
+            if (pc.whole) put_row(out_row(a, pl, pc, kvh, h0, heads, r, HD) + c, v, sum, vec);
+            else {
+                __stcg(reinterpret_cast<float4*>(a.ws + (slot * rb + r) * HD + c), v);
+                if (c == 0) __stcg(a.ws_ml + slot * rb + r, make_float2(top, sum));
+            }
+        }
         meet();  // the area belongs to the next piece
     }
+}
+
+// Blocks that several CTAs share: a thread block takes the one that begins in its number's run and goes on behind it, if there is one.  Its rows are spread over the warps, and a row's pieces
+// over as many warps as there are for it, kAt on their way for each; these meet in order.
+constexpr int kMergeWarps = 16;
+template <int HD>
+__global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kernel(const __grid_constant__ PagedPlan pl, const __grid_constant__ Q4Args a) {
+    constexpr int VEC = HD / 4, LANES = 32 / VEC, kAt = 8;  // HD 64: half a warp to a row
+    __shared__ float4 s_v[kMergeWarps * LANES][VEC];
+    __shared__ float2 s_ml[kMergeWarps * LANES];
+    kf_grid_launch_dependents();
+    kf_grid_dependency_wait();
+    const int mates = a.n_kv * a.parts, team = (int)blockIdx.x / mates, mate = (int)blockIdx.x % mates, kvh = mate / a.parts, h0 = mate % a.parts * a.heads, teams = (int)gridDim.x / mates;
+    const PagedPiece pc = *behind_wait(a.rec + mate * teams + team);
+    if (pc.last <= team || pc.last >= teams) return;  // last 0: nothing that goes on
+    const int heads = min(a.heads, pl.group - h0), rb = pl.tb * a.heads, rows = min(pl.tb, pc.n - pc.b * pl.tb) * heads, pieces = pc.last - team + 1;
+    const int tid = threadIdx.x, slot = tid / VEC, c = tid % VEC * 4, slots = kMergeWarps * LANES, spread = slots / rows, r = slot / spread, part = slot % spread;
+    if (r < rows) {
+        float top = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = part; i0 < pieces; i0 += kAt * spread) {
+            float4 w[kAt];
+            float2 ml[kAt];
+#pragma unroll
+            for (int k = 0; k < kAt; k++) {
+                const int i = i0 + k * spread;
+                if (i < pieces) {
+                    const size_t row = (((size_t)(team + i) * mates + mate) * 2 + (i == 0)) * rb + r;
+                    w[k] = __ldcg(reinterpret_cast<const float4*>(a.ws + row * HD + c)), ml[k] = __ldcg(a.ws_ml + row);
+                } else w[k] = make_float4(0.f, 0.f, 0.f, 0.f), ml[k] = make_float2(-INFINITY, 0.f);
+            }
+            float n = top;
+#pragma unroll
+            for (int k = 0; k < kAt; k++) n = fmaxf(n, ml[k].x);
+            const float base = finite_or_0(n), f0 = ex2(top - base);
+            top = n, sum *= f0, v.x *= f0, v.y *= f0, v.z *= f0, v.w *= f0;
+#pragma unroll
+            for (int k = 0; k < kAt; k++) {
+                const float f = ex2(ml[k].x - base);
+                sum = fmaf(ml[k].y, f, sum);
+                v.x = fmaf(w[k].x, f, v.x), v.y = fmaf(w[k].y, f, v.y), v.z = fmaf(w[k].z, f, v.z), v.w = fmaf(w[k].w, f, v.w);
+            }
+        }
+        s_v[slot][c / 4] = v;
+        if (c == 0) s_ml[slot] = make_float2(top, sum);
+    }
+    __syncthreads();
+    if (r >= rows || part != 0) return;
+    const int n = min(spread, pieces);
+    float top = -INFINITY, sum = 0.f;
+    for (int k = 0; k < n; k++) top = fmaxf(top, s_ml[slot + k].x);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < n; k++) {
+        const float f  = ex2(s_ml[slot + k].x - finite_or_0(top));
+        const float4 x = s_v[slot + k][c / 4];
+        sum = fmaf(s_ml[slot + k].y, f, sum);
+        v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
+    }
+    put_row(out_row(a, pl, pc, kvh, h0, heads, r, HD) + c, v, sum, ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0);
 }
 
 template <int HD, int NT, int OCC>
@@ -349,15 +473,14 @@ int launch_q4(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, PagedPlan p
     const size_t rows = (size_t)grid * 2 * rb;
     pl.runs = teams;
     KF_REQUIRE(ctx, paged_most(kTok, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
-    int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float));
-    if (!rc) rc = kf_ensure_attn_cnt(ctx, grid);
+    const int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float) + 16 + grid * sizeof(PagedPiece));
     if (rc) return rc;
     a.box = 8;
-    while (a.box < kTok && kv->page_size % (2 * a.box) == 0) a.box *= 2;
+    while (kTok % (2 * a.box) == 0 && kv->page_size % (2 * a.box) == 0) a.box *= 2;
     constexpr int kBytes = (224 / OCC - 4) * 1024;  // of shared memory for a CTA, its fixed part aside
     a.stages             = std::min(kMaxStages, (kBytes - rows_area(HD, rb)) / stage_bytes(HD));
     const size_t smem    = (size_t)a.stages * stage_bytes(HD) + rows_area(HD, rb);
-    a.ws = ctx->attn_ws, a.ws_ml = reinterpret_cast<float2*>(ctx->attn_ws + rows * HD), a.cnt = ctx->attn_cnt;
+    a.ws = ctx->attn_ws, a.ws_ml = reinterpret_cast<float2*>(ctx->attn_ws + rows * HD), a.rec = reinterpret_cast<PagedPiece*>(ctx->attn_ws + (rows * (HD + 2) + 3) / 4 * 4);
     a.sc2     = scale * 1.4426950408889634f * 0x1p73f;
     auto kern = kf_attn_paged_q4_kernel<HD, NT, OCC>;
     static bool set[kf_ctx::kMaxDevices] = {};  // function attributes are per device
@@ -365,7 +488,9 @@ int launch_q4(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, PagedPlan p
         KF_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
         set[ctx->device] = true;
     }
-    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((kWarps + 2) * 32), smem, a, pg, pl, KfBound{ctx->wait_flags + kWaitPaged, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((kWarps + 1) * 32), smem, a, pg, pl, KfBound{ctx->wait_flags + kWaitPaged, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
+    KF_LAUNCH_CHECK(ctx);
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_paged_q4_merge_kernel<HD>, dim3(grid), dim3(kMergeWarps * 32), 0, pl, a));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
 }
@@ -397,7 +522,7 @@ extern "C" int kf_paged_attention_q4(kf_ctx* ctx, const kf_paged_q4* kv, void* o
     a.parts = (group + 15) / 16, a.heads = (group + a.parts - 1) / a.parts;
     const int tokens = std::max(1, std::min(std::max(1, max_q), 16 / a.heads));
     const PagedPlan pl{tokens, group, window, 1, 0, first};
-    if (kv->head_dim == 128) return tokens * a.heads <= 8 ? launch_q4<128, 1, 2>(ctx, kv, pg, pl, a, scale) : launch_q4<128, 2, 2>(ctx, kv, pg, pl, a, scale);
+    if (kv->head_dim == 128) return tokens * a.heads <= 8 ? launch_q4<128, 1, Q4_OCC>(ctx, kv, pg, pl, a, scale) : launch_q4<128, 2, 2>(ctx, kv, pg, pl, a, scale);
     return tokens * a.heads <= 8 ? launch_q4<64, 1, 3>(ctx, kv, pg, pl, a, scale) : launch_q4<64, 2, 2>(ctx, kv, pg, pl, a, scale);
 }
 // The checks for tests on a host without a device
