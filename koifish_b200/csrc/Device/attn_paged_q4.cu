@@ -69,15 +69,15 @@ struct Q4Args {  // kernel parameter
     float2* ws_ml;
     PagedPiece* rec;
     long long ldo, ldq;
-    int n_kv, parts, heads;  // a kv head's group in `parts` of up to `heads` heads, a CTA of the team each
+    int n_kv;
     int box, stages;         // positions of a copy
     float sc2;               // scale * log2(e) * 2^73
 };
 __host__ __device__ constexpr int stage_bytes(int hd) { return kTok / 8 * Q4Unit(hd).bytes; }
 constexpr int rows_area(int hd, int rb) { return kWarps * rb * hd * 4; }
 
-__device__ __forceinline__ uint16_t* out_row(const Q4Args& a, const PagedPlan& pl, const PagedPiece& pc, int kvh, int h0, int heads, int r, int hd) {
-    return a.out + (pc.q0 + pc.b * pl.tb + r / heads) * a.ldo + (long long)(kvh * pl.group + h0 + r % heads) * hd;
+__device__ __forceinline__ uint16_t* out_row(const Q4Args& a, const PagedPlan& pl, const PagedPiece& pc, int kvh, int r, int hd) {
+    return a.out + (pc.q0 + pc.b * pl.tb + r / pl.group) * a.ldo + (long long)(kvh * pl.group + r % pl.group) * hd;
 }
 __device__ __forceinline__ void put_row(uint16_t* p, float4 v, float l, bool vec) {
     const float f      = l == 0.f ? 0.f : 1.f / l;
@@ -111,8 +111,8 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     kf_grid_dependency_wait();  // queries, the new positions' codes, lengths and tables, workspace
     const KfPaged pg    = behind_wait(pg_);
     const uint16_t* q   = behind_wait(a.q);
-    const int mates = a.n_kv * a.parts, team = (int)blockIdx.x / mates, mate = (int)blockIdx.x % mates, kvh = mate / a.parts, h0 = mate % a.parts * a.heads;
-    const int rec = mate * ((int)gridDim.x / mates) + team;
+    const int team = (int)blockIdx.x / a.n_kv, kvh = (int)blockIdx.x % a.n_kv;
+    PagedPiece* rec = a.rec + kvh * ((int)gridDim.x / a.n_kv);  // by team
     if (pg.n_seq > 32) {
         PagedPlanner<kTok>::count(pg, pl, qu.s_sum, warp, kWarps + 1, lane);
         __syncthreads();
@@ -123,10 +123,10 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     if (warp == kWarps) {
         // One warp works the pieces out and loads their tiles, up to a ring ahead of the others
         PagedPlanner<kTok> plan(pg, pl, lane);
-        if (lane == 0) a.rec[rec].last = 0;  // nothing to merge, should a wait run out before the end of the run is known
+        if (lane == 0) rec[team].last = 0;  // nothing to merge, should a wait run out before the end of the run is known
         plan.start(qu, team);
         if (bound.drop == (int)blockIdx.x + 1) {
-            while (plan.push(qu, team, a.rec + rec - team, &dead, bound)) {}
+            while (plan.push(qu, team, rec, &dead, bound)) {}
             return;
         }
         uint32_t st = 0, ph = 0, asked = 0;
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
         const int n_box = kTok / a.box, units = a.box / 8, ahead = 32 / n_box, bx = lane % n_box, mine = lane < ahead * n_box ? lane / n_box : 1 << 24;
         const uint32_t bytes = (uint32_t)(units * UNIT);
         uint8_t* dst         = ring + bx * units * UNIT;
-        while (live && plan.push(qu, team, a.rec + rec - team, &dead, bound)) {
+        while (live && plan.push(qu, team, rec, &dead, bound)) {
             pc           = plan.pc;
             const int fs = pc.lo > 0 ? pl.first : 0;
             int next_row = 0;
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
         for (uint32_t k = asked > (uint32_t)a.stages ? asked - a.stages : 0; k < asked; k++) mbar_drain(smem_u32(&full[k % a.stages]), (k / a.stages) & 1, bound);
         return;
     }
-    const int group = pl.group, rb = pl.tb * a.heads, heads = min(a.heads, group - h0);
+    const int group = pl.group, rb = pl.tb * group;
     const bool vec = ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0;
     uint32_t mph = 0, st = 0, ph = 0;
     auto meet = [&]() {  // all computing warps; bounded like every wait
@@ -178,14 +178,14 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
         mph ^= 1;
     };
     while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
-        const int rows = min(pl.tb, pc.n - pc.b * pl.tb) * heads, fs = pc.lo > 0 ? pl.first : 0;
+        const int rows = min(pl.tb, pc.n - pc.b * pl.tb) * group, fs = pc.lo > 0 ? pl.first : 0;
         // The block's queries as B operands.  Slot pairs of a lane's words: entries (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of its 8 of every group, times 2^60; rows past the end: zero
         uint32_t qb[NT][G][4], qz[NT][G][2];  // qz: minus the sum of q over a group, times 2^-73, as three numbers in the lanes of the group's slot
         int lim[NT][2], low[NT][2];        // what the lane's columns see: positions above `low`, or of the first, up to `lim`
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int r = n * 8 + g, tok = pc.b * pl.tb + r / heads;
-            const uint16_t* qp = q + (pc.q0 + tok) * a.ldq + (long long)(kvh * group + h0 + r % heads) * HD;
+            const int r = n * 8 + g, tok = pc.b * pl.tb + r / group;
+            const uint16_t* qp = q + (pc.q0 + tok) * a.ldq + (long long)(kvh * group + r % group) * HD;
             float mine = 0.f;
 #pragma unroll
             for (int j = 0; j < G; j++) {
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
             for (int j = 0; j < G; j++) qz[n][j][0] = t4 == j ? pack_bf16x2(hi, mid) : 0u, qz[n][j][1] = t4 == j ? pack_bf16x2(mine - hi - mid, 0.f) : 0u;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const int tc = pc.b * pl.tb + (n * 8 + 2 * t4 + e) / heads;
+                const int tc = pc.b * pl.tb + (n * 8 + 2 * t4 + e) / group;
                 lim[n][e] = min(pc.len - pc.n + tc, pg.cap - 1), low[n][e] = pl.window > 0 ? pc.len - pc.n + tc - pl.window : -1;
             }
         }
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
                 sum = fmaf(s_l[w][r], f, sum);
                 v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
             }
-            if (pc.whole) put_row(out_row(a, pl, pc, kvh, h0, heads, r, HD) + c, v, sum, vec);
+            if (pc.whole) put_row(out_row(a, pl, pc, kvh, r, HD) + c, v, sum, vec);
             else {
                 __stcg(reinterpret_cast<float4*>(a.ws + (slot * rb + r) * HD + c), v);
                 if (c == 0) __stcg(a.ws_ml + slot * rb + r, make_float2(top, sum));
@@ -418,10 +418,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kerne
     __shared__ float2 s_ml[kMergeWarps * LANES];
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();
-    const int mates = a.n_kv * a.parts, team = (int)blockIdx.x / mates, mate = (int)blockIdx.x % mates, kvh = mate / a.parts, h0 = mate % a.parts * a.heads, teams = (int)gridDim.x / mates;
-    const PagedPiece pc = *behind_wait(a.rec + mate * teams + team);
+    const int team = (int)blockIdx.x / a.n_kv, kvh = (int)blockIdx.x % a.n_kv, teams = (int)gridDim.x / a.n_kv;
+    const PagedPiece pc = *behind_wait(a.rec + kvh * teams + team);
     if (pc.last <= team || pc.last >= teams) return;  // last 0: nothing that goes on
-    const int heads = min(a.heads, pl.group - h0), rb = pl.tb * a.heads, rows = min(pl.tb, pc.n - pc.b * pl.tb) * heads, pieces = pc.last - team + 1;
+    const int rb = pl.tb * pl.group, rows = min(pl.tb, pc.n - pc.b * pl.tb) * pl.group, pieces = pc.last - team + 1;
     const int tid = threadIdx.x, slot = tid / VEC, c = tid % VEC * 4, slots = kMergeWarps * LANES, spread = slots / rows, r = slot / spread, part = slot % spread;
     if (r < rows) {
         float top = -INFINITY, sum = 0.f;
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kerne
             for (int k = 0; k < kAt; k++) {
                 const int i = i0 + k * spread;
                 if (i < pieces) {
-                    const size_t row = (((size_t)(team + i) * mates + mate) * 2 + (i == 0)) * rb + r;
+                    const size_t row = (((size_t)(team + i) * a.n_kv + kvh) * 2 + (i == 0)) * rb + r;
                     w[k] = __ldcg(reinterpret_cast<const float4*>(a.ws + row * HD + c)), ml[k] = __ldcg(a.ws_ml + row);
                 } else w[k] = make_float4(0.f, 0.f, 0.f, 0.f), ml[k] = make_float2(-INFINITY, 0.f);
             }
@@ -464,12 +464,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kerne
         sum = fmaf(s_ml[slot + k].y, f, sum);
         v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
     }
-    put_row(out_row(a, pl, pc, kvh, h0, heads, r, HD) + c, v, sum, ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0);
+    put_row(out_row(a, pl, pc, kvh, r, HD) + c, v, sum, ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0);
 }
 
 template <int HD, int NT, int OCC>
 int launch_q4(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, PagedPlan pl, Q4Args a, float scale) {
-    const int mates = a.n_kv * a.parts, teams = std::max(1, OCC * ctx->sm_count / mates), grid = teams * mates, rb = pl.tb * a.heads;
+    const int teams = std::max(1, OCC * ctx->sm_count / a.n_kv), grid = teams * a.n_kv, rb = pl.tb * pl.group;
     const size_t rows = (size_t)grid * 2 * rb;
     pl.runs = teams;
     KF_REQUIRE(ctx, paged_most(kTok, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
@@ -516,14 +516,13 @@ extern "C" int kf_paged_attention_q4(kf_ctx* ctx, const kf_paged_q4* kv, void* o
     int rc = check_args(ctx, kv, out, ldo, q, ldq, M, n_head, scale, first, max_q, &pg);
     if (!rc) rc = kf_wait_status(ctx);
     if (rc || M == 0) return rc;
-    const int group = n_head / kv->n_kv;
+    const int group = n_head / kv->n_kv, tokens = std::max(1, max_q);
+    if (tokens * (long long)group > 16) return kf_attn_paged_q4_tc(ctx, kv, pg, out, ldo, q, ldq, n_head, scale, window, first);
     Q4Args a = {};
     a.pool = (const uint8_t*)kv->pool_dev, a.page_stride = (long long)kf_paged_q4_stride(kv), a.out = (uint16_t*)out, a.q = (const uint16_t*)q, a.ldo = ldo, a.ldq = ldq, a.n_kv = kv->n_kv;
-    a.parts = (group + 15) / 16, a.heads = (group + a.parts - 1) / a.parts;
-    const int tokens = std::max(1, std::min(std::max(1, max_q), 16 / a.heads));
     const PagedPlan pl{tokens, group, window, 1, 0, first};
-    if (kv->head_dim == 128) return tokens * a.heads <= 8 ? launch_q4<128, 1, Q4_OCC>(ctx, kv, pg, pl, a, scale) : launch_q4<128, 2, 2>(ctx, kv, pg, pl, a, scale);
-    return tokens * a.heads <= 8 ? launch_q4<64, 1, 3>(ctx, kv, pg, pl, a, scale) : launch_q4<64, 2, 2>(ctx, kv, pg, pl, a, scale);
+    if (kv->head_dim == 128) return tokens * group <= 8 ? launch_q4<128, 1, Q4_OCC>(ctx, kv, pg, pl, a, scale) : launch_q4<128, 2, 2>(ctx, kv, pg, pl, a, scale);
+    return tokens * group <= 8 ? launch_q4<64, 1, 3>(ctx, kv, pg, pl, a, scale) : launch_q4<64, 2, 2>(ctx, kv, pg, pl, a, scale);
 }
 // The checks for tests on a host without a device
 extern "C" int kf_paged_attention_q4_args(const kf_paged_q4* kv, const void* out, int ldo, const void* q, int ldq, int M, int n_head, float scale, int first, int max_q) {

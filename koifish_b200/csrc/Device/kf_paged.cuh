@@ -10,6 +10,8 @@ struct KfPaged {  // kernel parameter
 };
 // attn_paged_tc.cu: on tcgen05
 int kf_attn_paged_tc(kf_ctx* ctx, const kf_paged_kv* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window);
+// attn_paged_q4_tc.cu: the same over the 4-bit cache
+int kf_attn_paged_q4_tc(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, void* out, long long ldo, const void* q, long long ldq, int n_head, float scale, int window, int first);
 // whether M rows of a_wide bytes from a on, a_pitch bytes apart, and M rows of b_wide bytes from b on have a byte in common (paged_append.cu)
 extern "C" int kf_rows_overlap(const void* a, size_t a_pitch, size_t a_wide, const void* b, size_t b_pitch, size_t b_wide, int M);
 int kf_paged_check(kf_ctx* ctx, const kf_paged_kv* kv, int M, KfPaged* out);  // paged_append.cu: arguments that all of them share
