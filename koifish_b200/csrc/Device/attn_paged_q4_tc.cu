@@ -45,57 +45,61 @@ __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
     } else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 __device__ __forceinline__ float half_of(uint32_t w, int h) { return h ? bf16hi(w) : bf16lo(w); }
-// four codes of a word (its lower or upper half) as entries times 2^-60
-struct Group {
-    unsigned long long a, b;  // step * (2^73, 2^69), and minus step * zero * 2^-60 twice
-    __device__ __forceinline__ Group(float step, float zero) {
-        const float off = step * zero * -0x1p-60f;
-        a = pack2(step * 0x1p73f, step * 0x1p69f), b = pack2(off, off);
-    }
-    __device__ __forceinline__ uint2 four(uint32_t w, int upper) const {
-        const uint32_t x = upper ? w : w << 16, y = upper ? w >> 8 : w << 8;
-        const float2 p = unpack2(fma2(pack2(__uint_as_float(x & 0x000f0000u), __uint_as_float(x & 0x00f00000u)), a, b));
-        const float2 q = unpack2(fma2(pack2(__uint_as_float(y & 0x000f0000u), __uint_as_float(y & 0x00f00000u)), a, b));
-        return make_uint2(pack_bf16x2(p.x, p.y), pack_bf16x2(q.x, q.y));
-    }
-};
-// the keys of a unit into eight rows of a tile
-template <int HD>
-__device__ __forceinline__ void expand_k(uint8_t* rows, const uint8_t* u, int lane) {
-    constexpr Q4Unit un(HD);
-    constexpr int G = un.groups;
-    const int g = lane >> 2, t4 = lane & 3;
-    uint32_t w[G], s[G / 2], z[G / 2];
-    words(u + lane * 4 * G, w), words(u + un.k_step() + g * 2 * G, s), words(u + un.k_zero() + g * 2 * G, z);
+// Keys or values of a unit and eight rows of a tile.  A lane takes the codes of one row that stand for eight dims of every group, as one word each: K dims 32 j + 8 t .. + 7, which it stores as
+// 16 bytes, V dims 32 j + 4 t .. + 3 and 32 j + 16 + 4 t .. + 3, half words of two words in the unit, stored as 8 bytes each.  Lanes of four are rows 0, 4, 2, 6, 1, 5, 3, 7: those that store
+// together meet all 32 banks.  The code is small, and one for both, for a reason: with two units of K and two of V unrolled beside one another, instructions had to be fetched again and again
+// (2048 tokens behind 8192: 478 us against 405 one at a time).
+template <int HD, bool is_v>
+struct Eight {
+    static constexpr int G = HD / 32;
+    uint32_t w[G], s[G / 2];
+    float z[G];
+    static __device__ __forceinline__ int row(int lane) { return (lane & 4) | (lane >> 2 & 2) | lane >> 4; }
+    __device__ __forceinline__ void load(const uint8_t* u, int lane) {
+        constexpr Q4Unit un(HD);
+        const int r = row(lane), t = lane & 3;
+        if constexpr (is_v) {
+            uint32_t x[G / 2], y[G / 2];
+            const uint8_t* at = u + un.v_code() + t * (HD / 2) + (r >> 1) * (HD / 8) + (r & 1) * (HD / 16);
+            words(at, x), words(at + 2 * HD, y), words(u + un.v_step() + r * 2 * G, s);
 #pragma unroll
-    for (int j = 0; j < G; j++) {
-        const Group gr(half_of(s[j / 2], j & 1), half_of(z[j / 2], j & 1));
-        const uint2 lo = gr.four(w[j], 0), hi = gr.four(w[j], 1);
-        *reinterpret_cast<uint4*>(rows + (j >> 1) * 1024 + g * 128 + (((4 * (j & 1) + t4) ^ g) << 4)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
-}
-// the values; ok: bit r, row r counts
-template <int HD>
-__device__ __forceinline__ void expand_v(uint8_t* rows, const uint8_t* u, int lane, unsigned ok) {
-    constexpr Q4Unit un(HD);
-    constexpr int G = un.groups;
-    const int g = lane >> 2, t4 = lane & 3;
-    uint32_t w[G], s[G], z[G];
-    words(u + un.v_code() + lane * 4 * G, w), words(u + un.v_step() + t4 * 4 * G, s);
+            for (int j = 0; j < G; j++) {
+                w[j] = __byte_perm(x[j / 2], y[j / 2], j & 1 ? 0x7632 : 0x5410);
+                z[j] = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(u + un.v_zero() + j * 16 + r * 2));
+            }
+        } else {
+            uint32_t x[G / 2];
+            words(u + r * (HD / 2) + t * 4 * G, w), words(u + un.k_step() + r * 2 * G, s), words(u + un.k_zero() + r * 2 * G, x);
 #pragma unroll
-    for (int j = 0; j < G; j++) z[j] = *reinterpret_cast<const uint32_t*>(u + un.v_zero() + j * 16 + t4 * 4);
-#pragma unroll
-    for (int e = 0; e < 2; e++) {  // rows 2 t4, 2 t4 + 1
-        const int r    = 2 * t4 + e;
-        const bool has = ok >> r & 1;
-#pragma unroll
-        for (int j = 0; j < G; j++) {
-            const Group gr(half_of(s[(e * G + j) / 2], j & 1), half_of(z[j], e));
-            const uint2 x = gr.four(w[e * (G / 2) + j / 2], j & 1);
-            *reinterpret_cast<uint2*>(rows + (j >> 1) * 1024 + r * 128 + (((4 * (j & 1) + (g >> 1)) ^ r) << 4) + (g & 1) * 8) = has ? x : make_uint2(0u, 0u);
+            for (int j = 0; j < G; j++) z[j] = half_of(x[j / 2], j & 1);
         }
     }
-}
+    __device__ __forceinline__ void hide() {  // rows that nobody sees become zeros, whatever their steps and zeros are
+#pragma unroll
+        for (int j = 0; j < G; j++) s[j / 2] = 0u, z[j] = 0.f;
+    }
+    __device__ __forceinline__ void store(uint8_t* rows, int lane) const {
+        const int r = row(lane), t = lane & 3;
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            // step * (2^73, 2^69) and minus step * zero * 2^-60 twice
+            const float step = half_of(s[j / 2], j & 1), off = step * -0x1p-60f * z[j];
+            const unsigned long long fa = pack2(step * 0x1p73f, step * 0x1p69f), fb = pack2(off, off);
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t x = i == 0 ? w[j] << 16 : i == 1 ? w[j] << 8 : i == 2 ? w[j] : w[j] >> 8;
+                const float2 e   = unpack2(fma2(pack2(__uint_as_float(x & 0x000f0000u), __uint_as_float(x & 0x00f00000u)), fa, fb));
+                v[i]             = pack_bf16x2(e.x, e.y);
+            }
+            uint8_t* at = rows + (j >> 1) * 1024 + r * 128;
+            if (is_v) {
+                *reinterpret_cast<uint2*>(at + (((4 * (j & 1) + (t >> 1)) ^ r) << 4) + (t & 1) * 8)     = make_uint2(v[0], v[1]);
+                *reinterpret_cast<uint2*>(at + (((4 * (j & 1) + 2 + (t >> 1)) ^ r) << 4) + (t & 1) * 8) = make_uint2(v[2], v[3]);
+            } else *reinterpret_cast<uint4*>(at + (((4 * (j & 1) + t) ^ r) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
+};
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -106,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int UNIT = Q4Unit(HD).bytes;
     const TcArgs& a = qa.t;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sq = smem_raw + (-smem_u32(smem_raw) & 1023u);  // still an address in shared memory for the compiler
     uint8_t* sk = sq + 2 * kTile;
     uint8_t* sv = sk + kStagesK * kTile;
     uint8_t* sr = sv + kStagesV * kTile;
@@ -453,25 +457,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int fs = pc.lo > 0 ? pl.first : 0;
             for (int t = pc.t0; live && t < pc.t1; t++, pos++) {
                 const uint32_t sr_ = pos % kStagesR, sk_ = pos % kStagesK, sv_ = pos % kStagesV;
-                const int p0 = pc.tile(t) * kKV;
+                const int p0        = pc.tile(t) * kKV;
                 if (!(live = mbar_wait_warp(smem_u32(&r_full[sr_]), (pos / kStagesR) & 1, &dead, bound))) break;
-                if (!(live = mbar_wait_warp(smem_u32(&k_empty[sk_]), ((pos / kStagesK) & 1) ^ 1, &dead, bound))) break;
                 const unsigned there = (unsigned)s_there[pos % kMasks];
                 const uint8_t* raw   = sr + sr_ * kRaw;
-#pragma unroll 2
-                for (int u = warp - kExpW; u < kKV / 8; u += kExps) expand_k<HD>(sk + sk_ * kTile + u * kGroup, raw + u * UNIT, lane);
+                if (!(live = mbar_wait_warp(smem_u32(&k_empty[sk_]), ((pos / kStagesK) & 1) ^ 1, &dead, bound))) break;
+#pragma unroll 1
+                for (int u = warp - kExpW; u < kKV / 8; u += kExps) {
+                    Eight<HD, false> x;
+                    x.load(raw + u * UNIT, lane);
+                    x.store(sk + sk_ * kTile + u * kGroup, lane);
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the matrix instructions
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[sk_]);
                 if (!(live = mbar_wait_warp(smem_u32(&v_empty[sv_]), ((pos / kStagesV) & 1) ^ 1, &dead, bound))) break;
-#pragma unroll 2
+#pragma unroll 1
                 for (int u = warp - kExpW; u < kKV / 8; u += kExps) {
-                    unsigned ok = there >> u & 1 ? 0xffu : 0u;
+                    Eight<HD, true> x;
+                    x.load(raw + u * UNIT, lane);
                     const int p = p0 + 8 * u;
-                    if (p + 8 > pc.hi || p < pc.lo)
-                        for (int r = 0; r < 8; r++)
-                            if (!(p + r < pc.hi && (p + r >= pc.lo || p + r < fs))) ok &= ~(1u << r);
-                    expand_v<HD>(sv + sv_ * kTile + u * kGroup, raw + u * UNIT, lane, ok);
+                    if (!(there >> u & 1) || p + 8 > pc.hi || p < pc.lo) {
+                        const int at = p + x.row(lane);
+                        if (!(there >> u & 1) || at >= pc.hi || (at < pc.lo && at >= fs)) x.hide();
+                    }
+                    x.store(sv + sv_ * kTile + u * kGroup, lane);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
