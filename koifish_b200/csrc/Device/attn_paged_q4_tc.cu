@@ -5,8 +5,8 @@
 // four warps expand them, step * code - step * zero in fp32 with one rounding to bf16, into the swizzled tiles that the bf16 kernel gets by TMA.  A code at bits 16 .. 19 of a word is the fp32
 // number code * 2^-133, at bits 20 .. 23 code * 2^-129 (subnormal numbers and the first normal ones are one ladder), so a shift and an AND make the operand and one f32x2 multiply-add two
 // entries; steps carry 2^73, so what is stored is 2^-60 of the entry, and the scale and the final division undo it.
-//   warps 0-3 / 4-7  softmax of chain 0 / 1, thread = row.  128 registers a thread (15 warps) do not hold a row's 128 scores, so they are read twice: for the maximum, of which the second half
-//                    stays, and the first half again for its weights, which come second
+//   warps 0-3 / 4-7  softmax of chain 0 / 1, thread = row.  128 registers a thread (15 warps) do not hold a row's 128 scores, so the first half is read twice: for the maximum, behind which the
+//                    second half stays for its weights, and for its own weights, which come second
 //   warp 8           matrix instructions of both chains in turn
 //   warp 9           Q by TMA, raw tiles by bulk copies
 //   warp 10          the pieces
@@ -204,16 +204,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
                 };
-                uint32_t x[32], y[32], z[32];
-                ld32_async(s_row, x), ld32_async(s_row + 64, y), ld32_async(s_row + 96, z);
+                uint32_t x[32], y[32];
+                ld32_async(s_row, x), ld32_async(s_row + 32, y);
                 wait_ld();
-                if (ragged) hide(x, 0), hide(y, 2), hide(z, 3);
+                if (ragged) hide(x, 0), hide(y, 1);
                 most(x);
-                ld32_async(s_row + 32, x);
-                most(y), most(z);
+                ld32_async(s_row + 96, x);
+                most(y);
                 wait_ld();
-                if (ragged) hide(x, 1);
+                if (ragged) hide(x, 3);
+                ld32_async(s_row + 64, y);
                 most(x);
+                wait_ld();
+                if (ragged) hide(y, 2);
+                most(y);
                 const float mn = mine ? max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sc2 : -INFINITY;  // nobody's rows hold what lay there: they have no say in a rescaling
                 if (j == 0) {
                     m = mn;
@@ -239,8 +243,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         const float2 e = unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc22, nm2));
-                        p[i] = pack_bf16x2(ex2(e.x), ex2(e.y));
-                        l2   = add2(l2, pack2(bf16lo(p[i]), bf16hi(p[i])));  // the weights as they are used: a rounding that numerator and denominator share
+                        const float w0 = ex2(e.x), w1 = ex2(e.y);
+                        p[i] = pack_bf16x2(w0, w1);
+                        l2   = add2(l2, pack2(w0, w1));
                     }
                     tmem_st16(at, p);
                 };
@@ -253,10 +258,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the second half first, over its own scores; a part's O += P V runs while the next one's weights are formed
                 weigh(y, s_row + 64);
                 ld32_async(s_row, y);
-                weigh(z, s_row + 80);
+                weigh(x, s_row + 80);
+                ld32_async(s_row + 32, x);
                 part_done(1);
                 wait_ld();
-                if (ragged) hide(y, 0);
+                if (ragged) hide(y, 0), hide(x, 1);
                 weigh(y, s_row);
                 weigh(x, s_row + 16);
                 part_done(0);
