@@ -70,28 +70,55 @@ __device__ __forceinline__ void store8(float* p, const f32x2 (&f)[4]) {
 }
 
 __device__ __forceinline__ uint16_t bf16_bits_up(float f) { return (uint16_t)((__float_as_uint(f) + 0xffffu) >> 16); }  // f >= 0
+// the smallest and the largest of three; NaN if one of them is
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(a) : "f"(a), "f"(b), "f"(c));
+    return a;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(a) : "f"(a), "f"(b), "f"(c));
+    return a;
+}
 // A finished row of K or V into its unit of the 4-bit cache.  HD / 16 lanes side by side hold 16 entries each in `x`, entries 16 u .. 16 u + 15 in lane u; two lanes are a group.
-// All lanes of the warp call it; `to` (NULL: nothing is written) is the unit, p the position in it.  The division is the rounded one, so that a tie is a tie.
+// All lanes of the warp call it; `to` (NULL: nothing is written) is the unit, p the position in it.
 template <int HD>
 __device__ __forceinline__ void store_q4(uint8_t* to, int p, bool is_v, int u, const float (&x)[16]) {
     constexpr Q4Unit un(HD);
     constexpr int G = un.groups;
     float lo = x[0], hi = x[0];
-    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 16; i++) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]), most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1)), most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    const bool fine   = most < 0x7f800000u;
-    const uint32_t sb = fine ? bf16_bits_up(fmaxf(__fdiv_rn(hi - lo, 15.f), __uint_as_float(most) * (1.f / 2048.f))) : 0x7fffu;
+    for (int i = 1; i < 15; i += 2) lo = min3_nan(lo, x[i], x[i + 1]), hi = max3_nan(hi, x[i], x[i + 1]);
+    lo = min3_nan(lo, x[15], __shfl_xor_sync(0xffffffffu, min3_nan(lo, x[15], x[15]), 1)), hi = max3_nan(hi, x[15], __shfl_xor_sync(0xffffffffu, max3_nan(hi, x[15], x[15]), 1));
+    const float most  = max3_nan(hi, -lo, 0.f);
+    const bool fine   = most < INFINITY;  // not NaN either
+    const uint32_t sb = fine ? bf16_bits_up(fmaxf(__fdiv_rn(hi - lo, 15.f), most * (1.f / 2048.f))) : 0x7fffu;
     const float step  = fine && sb ? bf16_bits_to_f32(sb) : 1.f;
     const uint32_t zb = fine && sb ? f32_to_bf16_bits(__fdiv_rn(-lo, step)) : 0u;
     const float zero  = bf16_bits_to_f32(zb);
+    // x / step, correctly rounded, so that a tie is a tie: with y = 1 / step correctly rounded and q = x y, q + (x - q step) y is (Markstein's theorem), away from the ends of the range
+    f32x2 q[8];
+    const bool mid = step > 0x1p-90f && step < 0x1p90f;
+    if (__all_sync(0xffffffffu, mid)) {
+        const float y   = __frcp_rn(step);
+        const f32x2 y2  = pack2(y, y), s2 = pack2(-step, -step);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const f32x2 a = pack2(x[2 * i], x[2 * i + 1]), b = mul2(a, y2);
+            q[i] = fma2(fma2(b, s2, a), y2, b);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[i] = pack2(__fdiv_rn(x[2 * i], step), __fdiv_rn(x[2 * i + 1], step));
+    }
     uint32_t c[2] = {0u, 0u};  // entries 8 e .. 8 e + 7
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const float y = fminf(fmaxf(rintf(__fdiv_rn(x[i], step) + zero), 0.f), 15.f);  // NaN: 0
-        c[i >> 3] |= (fine ? (uint32_t)y : 0u) << (4 * (i & 7));
+    for (int i = 7; i >= 0; i--) {
+        const float2 t = unpack2(add2(q[i], pack2(zero, zero)));
+        // kept to 0 .. 15 (NaN: 0); in front of 1.5 * 2^23 the nearest whole number, ties to even, is what is left in the lowest bits
+        const float2 r = unpack2(add2(pack2(fminf(fmaxf(t.x, 0.f), 15.f), fminf(fmaxf(t.y, 0.f), 15.f)), pack2(12582912.f, 12582912.f)));
+        c[i >> 2]      = c[i >> 2] << 8 | (__float_as_uint(r.y) & 15u) << 4 | (__float_as_uint(r.x) & 15u);
     }
+    if (!fine) c[0] = c[1] = 0u;
     const int j = u >> 1;
     // Values: entries 4 g .. 4 g + 3 of two groups are a word.  The lanes that hold the same entries of the two (u and u ^ 2) exchange halves, so that each has two whole words, of the
     // first two of their four g in the lane of the even group, of the others in that of the odd one; with four groups (HD 128) the words of both halves of the row meet likewise.
@@ -143,10 +170,12 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : Q4 ? 3 : NORM && size
     const int ea = p.layout && 8 * v < half ? 8 * v : p.layout ? p.rot + 16 * (v - half / 8) : 16 * v, eb = p.layout && 8 * v < half ? half + 8 * v : ea + 8;
     const bool lives = LPR && 16 * v < p.hd;
     Raw<X> ra[kAhead], rb[kAhead];
-    auto fetch = [&](int t, int rb0) {  // rows rb0 + grp, kGroups further on, ... of token t
+    // rows rb0 + grp, kGroups further on, ... of token t.  Q4: half a turn further in every other token, since rows of K and V, the last ones, take longer
+    auto row_at = [&](int t, int rb0, int u) { return rb0 + (Q4 ? (grp + (t & 1) * (kGroups / 2)) % kGroups : grp) + u * kGroups; };
+    auto fetch  = [&](int t, int rb0) {
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
-            const int r = rb0 + grp + u * kGroups;
+            const int r = row_at(t, rb0, u);
             if (lives && r < r1) {
                 const X* from = src(t, r);
                 ra[u].load(from + ea), rb[u].load(from + eb);
@@ -201,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : Q4 ? 3 : NORM && size
             Y* out           = (Y*)p.out + (m0 + t) * p.ldo;
 #pragma unroll
             for (int u = 0; u < kAhead; u++) {
-                const int r = rb0 + grp + u * kGroups;
+                const int r = row_at(t, rb0, u);
                 if (!ours || __all_sync(0xffffffffu, r >= r1)) break;
                 const bool is_q = r < p.nq, is_v = r >= p.nq + p.nkv, live = lives && r < r1;
                 f32x2 a[4], b[4];

@@ -2,11 +2,14 @@
 //
 //   x = step * (code - zero), in fp32, rounded once
 //
-// Every byte is read once and every entry written once, so HBM bounds it.  A warp takes four positions that lie side by side in the panel and one of K and V of one head at a time: eight (or four)
-// lanes a row, eight bytes of codes each, so that four positions of one unit meet in whole sectors of V's codes, which lie by pairs of positions.
+// Every byte is read once and every entry written once, so HBM bounds it, and instructions are not far.  A warp takes eight positions that lie side by side in the panel, four lanes a row, and one of
+// K and V of one head at a time: a unit, where the positions are one, in whole.  A lane has one word of eight codes for every group.  A code at bits 16 .. 19 of a word is the fp32 number
+// code * 2^-133, at bits 20 .. 23 code * 2^-129 (subnormal numbers and the first normal ones are one ladder): a shift and an AND take the place of a conversion, and the multiply-add that brings
+// it back to size takes the zero off with the rounding of code - zero.
 #include <algorithm>
 
 #include "kf_paged.cuh"
+#include "kf_tc.cuh"
 
 namespace {
 constexpr int kThreads = 256, kTokens = 16;  // of a block
@@ -19,24 +22,32 @@ struct ReadParams {
     int n_kv, rows_per_block;
     KfPaged pg;
 };
-__device__ __forceinline__ void put(uint16_t* p, const float (&x)[8], int n) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 4)
-        if (i < n) *reinterpret_cast<uint2*>(p + i) = make_uint2(pack_bf16x2(x[i], x[i + 1]), pack_bf16x2(x[i + 2], x[i + 3]));
+template <bool VEC>
+__device__ __forceinline__ void put4(uint16_t* p, float2 a, float2 b) {
+    if (VEC) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y));
+    else p[0] = f32_to_bf16_bits(a.x), p[1] = f32_to_bf16_bits(a.y), p[2] = f32_to_bf16_bits(b.x), p[3] = f32_to_bf16_bits(b.y);
 }
-__device__ __forceinline__ void put(float* p, const float (&x)[8], int n) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 4)
-        if (i < n) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+template <bool VEC>
+__device__ __forceinline__ void put4(float* p, float2 a, float2 b) {
+    if (VEC) *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
+    else p[0] = a.x, p[1] = a.y, p[2] = b.x, p[3] = b.y;
 }
-__device__ __forceinline__ void put1(uint16_t* p, float x) { *p = f32_to_bf16_bits(x); }
-__device__ __forceinline__ void put1(float* p, float x) { *p = x; }
+template <int N>
+__device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else w[0] = *reinterpret_cast<const uint32_t*>(p);
+}
 
 // VEC: rows of the results are aligned to four entries
 template <int HD, typename Y, bool VEC>
 __global__ void __launch_bounds__(kThreads) kf_paged_read_q4_kernel(const __grid_constant__ ReadParams p) {
     constexpr Q4Unit un(HD);
-    constexpr int G = un.groups, LPR = 8, RPW = 32 / LPR, kWarps = kThreads / 32;  // lanes of a row: one for each g of V's codes
+    constexpr int G = un.groups, kWarps = kThreads / 32;
     __shared__ long long s_row[kTokens];  // a token's unit in the pool, -1: none
     __shared__ int s_in[kTokens];         // position in the unit; -1: the token belongs to no sequence
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, m0 = blockIdx.x * kTokens, nt = min(kTokens, p.pg.M - m0);
@@ -57,41 +68,47 @@ __global__ void __launch_bounds__(kThreads) kf_paged_read_q4_kernel(const __grid
         if (lane == 0) s_row[t] = row, s_in[t] = s >= 0 ? in & 7 : -1;
     }
     __syncthreads();
-    const int r0 = blockIdx.y * p.rows_per_block, r1 = min(2 * p.n_kv, r0 + p.rows_per_block), quads = (nt + RPW - 1) / RPW, u = lane % LPR;
-    for (int x = warp; x < quads * (r1 - r0); x += kWarps) {
-        const int t = x / (r1 - r0) * RPW + lane / LPR, r = r0 + x % (r1 - r0), head = r >> 1;
+    const int r0 = blockIdx.y * p.rows_per_block, r1 = min(2 * p.n_kv, r0 + p.rows_per_block), l = lane & 3, t = warp % 2 * 8 + (lane >> 2);
+    if (t >= nt || s_in[t] < 0) return;
+    const long long row = s_row[t], head_bytes = (long long)(pg.page / 8) * un.bytes;
+    const int in        = s_in[t];
+    for (int r = r0 + warp / 2; r < r1; r += kWarps / 2) {
+        const int head  = r >> 1;
         const bool is_v = r & 1;
-        if (t >= nt || s_in[t] < 0 || !(is_v ? p.v : p.k)) continue;
+        if (!(is_v ? p.v : p.k)) continue;
         Y* to = is_v ? (Y*)p.v + (m0 + t) * p.ldv + head * HD : (Y*)p.k + (m0 + t) * p.ldk + head * HD;
-        const long long row = s_row[t];
-        const int in        = s_in[t];
-        const uint8_t* at   = pool + max(row, 0ll) + (long long)head * (pg.page / 8) * un.bytes;
-        const uint16_t *steps = reinterpret_cast<const uint16_t*>(at + (is_v ? un.v_step() : un.k_step())) + in * G;
-        const uint16_t *zeros = reinterpret_cast<const uint16_t*>(at + (is_v ? un.v_zero() : un.k_zero()));
+        const uint8_t* at = pool + row + head * head_bytes;
+        uint32_t w[G], s[G / 2], z[G];
+        if (row < 0) {
 #pragma unroll
-        for (int w = 0; w < G / 2; w++) {  // a word a time
-            // K: word w of the lane's G / 2 is entries 32 j + 8 t .. + 7, j = (u * G / 2 + w) % G, t = (u * G / 2 + w) / G; V: 4 entries of groups 2 w and 2 w + 1
-            uint32_t c = 0;
-            if (row >= 0) c = is_v ? *reinterpret_cast<const uint32_t*>(at + un.v_code() + u * (HD / 2) + (in >> 1) * (HD / 8) + (in & 1) * (HD / 16) + w * 4)
-                                   : *reinterpret_cast<const uint32_t*>(at + in * (HD / 2) + (u * (G / 2) + w) * 4);
-            const int ka = (u * (G / 2) + w) % G, kt = (u * (G / 2) + w) / G;
-            float e[8];
+            for (int j = 0; j < G; j++) w[j] = z[j] = s[j / 2] = 0u;
+        } else if (is_v) {  // dims 32 j + 4 l .. + 3 and 32 j + 16 + 4 l .. + 3
+            uint32_t x[G / 2], y[G / 2];
+            const uint8_t* c = at + un.v_code() + l * (HD / 2) + (in >> 1) * (HD / 8) + (in & 1) * (HD / 16);
+            words(c, x), words(c + 2 * HD, y), words(at + un.v_step() + in * 2 * G, s);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int j      = is_v ? 2 * w + h : ka;
-                const float step = row >= 0 ? bf16_bits_to_f32(steps[j]) : 0.f, zero = row >= 0 ? bf16_bits_to_f32(is_v ? zeros[j * 8 + in] : zeros[in * G + j]) : 0.f;
+            for (int j = 0; j < G; j++) z[j] = *reinterpret_cast<const uint16_t*>(at + un.v_zero() + j * 16 + in * 2);
 #pragma unroll
-                for (int i = 0; i < 4; i++) e[4 * h + i] = step * ((float)((c >> (16 * h + 4 * i)) & 15u) - zero);
+            for (int j = 0; j < G; j++) w[j] = __byte_perm(x[j / 2], y[j / 2], j & 1 ? 0x7632 : 0x5410);
+        } else {  // dims 32 j + 8 l .. + 7
+            uint32_t x[G / 2];
+            words(at + in * (HD / 2) + l * 4 * G, w), words(at + un.k_step() + in * 2 * G, s), words(at + un.k_zero() + in * 2 * G, x);
+#pragma unroll
+            for (int j = 0; j < G; j++) z[j] = j & 1 ? x[j / 2] >> 16 : x[j / 2] & 0xffffu;
+        }
+        const int d0 = is_v ? 4 * l : 8 * l, d1 = is_v ? d0 + 16 : d0 + 4;
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            const float step = j & 1 ? bf16hi(s[j / 2]) : bf16lo(s[j / 2]), zero = __uint_as_float(z[j] << 16);
+            const unsigned long long up = pack2(0x1p127f, 0x1p123f), off = pack2(zero * -0x1p-6f, zero * -0x1p-6f), back = pack2(step, step), by = pack2(0x1p6f, 0x1p6f);
+            float2 e[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t x = i == 0 ? w[j] << 16 : i == 1 ? w[j] << 8 : i == 2 ? w[j] : w[j] >> 8;
+                // (code - zero) / 64, times 64, which is exact, times the step
+                e[i] = unpack2(mul2(mul2(fma2(pack2(__uint_as_float(x & 0x000f0000u), __uint_as_float(x & 0x00f00000u)), up, off), by), back));
             }
-            const int d0 = is_v ? 64 * w + 4 * u : 32 * ka + 8 * kt, d1 = is_v ? d0 + 32 : d0 + 4;
-            if (VEC) {
-                put(to + d0, e, 4);
-                const float f[8] = {e[4], e[5], e[6], e[7]};
-                put(to + d1, f, 4);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) put1(to + d0 + i, e[i]), put1(to + d1 + i, e[4 + i]);
-            }
+            put4<VEC>(to + 32 * j + d0, e[0], e[1]), put4<VEC>(to + 32 * j + d1, e[2], e[3]);
         }
     }
 }
@@ -99,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) kf_paged_read_q4_kernel(const __grid
 template <int HD, typename Y>
 int launch_read(kf_ctx* ctx, ReadParams& p, bool vec) {
     const int blocks = (p.pg.M + kTokens - 1) / kTokens, all = 2 * p.n_kv;
-    const int parts  = std::max(1, std::min(all, 4 * ctx->sm_count / blocks));  // few tokens: their heads over several blocks
+    const int parts  = std::max(1, std::min((all + 3) / 4, 4 * ctx->sm_count / blocks));  // few tokens: their heads over several blocks
     p.rows_per_block = (all + parts - 1) / parts;
     const dim3 grid(blocks, (all + p.rows_per_block - 1) / p.rows_per_block);
     KF_CUDA(ctx, kf_launch_pdl(ctx, vec ? kf_paged_read_q4_kernel<HD, Y, true> : kf_paged_read_q4_kernel<HD, Y, false>, grid, dim3(kThreads), 0, p));
