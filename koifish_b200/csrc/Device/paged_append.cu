@@ -147,7 +147,7 @@ __device__ __forceinline__ void store_q4(uint8_t* to, int p, bool is_v, int u, c
 // LPR: lanes to a row, eight pairs each; 0: rows at any element, or pairs that do not fall on whole lanes -- a warp per row, an entry or a pair per lane
 // Q4: the cache is the 4-bit one, head_dim Q4 (0: bf16).  A finished row of K or V goes through shared memory there, so that a lane gets 16 entries side by side
 template <typename X, typename Y, int LPR, bool NORM, int Q4 = 0>
-__global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : Q4 ? 3 : NORM && sizeof(X) == 2 ? 5 : 4) kf_rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kThreads, LPR == 0 ? 1 : Q4 ? 4 : NORM && sizeof(X) == 2 ? 5 : 4) kf_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int kL = LPR ? LPR : 32, kGroups = kThreads / kL, kAhead = sizeof(X) == 4 || NORM ? 1 : 2;  // rows of a lane on their way beside those in its hands
     __shared__ alignas(16) float s_cos[kTokens][128], s_sin[kTokens][128];
     __shared__ long long s_row[kTokens];  // a token's row in the pools, -1: none

@@ -12,7 +12,7 @@
 #include "kf_tc.cuh"
 
 namespace {
-constexpr int kThreads = 256, kTokens = 16;  // of a block
+constexpr int kThreads = 256, kTokens = 8;  // of a block: a warp's
 
 struct ReadParams {
     void *k, *v;
@@ -48,6 +48,7 @@ template <int HD, typename Y, bool VEC>
 __global__ void __launch_bounds__(kThreads) kf_paged_read_q4_kernel(const __grid_constant__ ReadParams p) {
     constexpr Q4Unit un(HD);
     constexpr int G = un.groups, kWarps = kThreads / 32;
+    static_assert(kWarps == kTokens, "a warp looks a token up");
     __shared__ long long s_row[kTokens];  // a token's unit in the pool, -1: none
     __shared__ int s_in[kTokens];         // position in the unit; -1: the token belongs to no sequence
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, m0 = blockIdx.x * kTokens, nt = min(kTokens, p.pg.M - m0);
@@ -55,24 +56,24 @@ __global__ void __launch_bounds__(kThreads) kf_paged_read_q4_kernel(const __grid
     kf_grid_dependency_wait();
     const KfPaged pg    = behind_wait(p.pg);
     const uint8_t* pool = behind_wait(p.pool);
-    for (int t = warp; t < nt; t += kWarps) {
-        const int s = paged_find_seq(pg, m0 + t, lane);
+    if (warp < nt) {
+        const int s = paged_find_seq(pg, m0 + warp, lane);
         long long row = -1;
         int in = 0;
         if (s >= 0) {
             int q0, n, len;
             paged_seq(pg, s, q0, n, len);
-            const int at = len - n + (m0 + t - q0), page = at >= 0 ? paged_page(pg, s, at, in) : -1;
+            const int at = len - n + (m0 + warp - q0), page = at >= 0 ? paged_page(pg, s, at, in) : -1;
             if (page >= 0) row = page * p.page_stride + in / 8 * (long long)un.bytes;
         }
-        if (lane == 0) s_row[t] = row, s_in[t] = s >= 0 ? in & 7 : -1;
+        if (lane == 0) s_row[warp] = row, s_in[warp] = s >= 0 ? in & 7 : -1;
     }
     __syncthreads();
-    const int r0 = blockIdx.y * p.rows_per_block, r1 = min(2 * p.n_kv, r0 + p.rows_per_block), l = lane & 3, t = warp % 2 * 8 + (lane >> 2);
+    const int r0 = blockIdx.y * p.rows_per_block, r1 = min(2 * p.n_kv, r0 + p.rows_per_block), l = lane & 3, t = lane >> 2;
     if (t >= nt || s_in[t] < 0) return;
     const long long row = s_row[t], head_bytes = (long long)(pg.page / 8) * un.bytes;
     const int in        = s_in[t];
-    for (int r = r0 + warp / 2; r < r1; r += kWarps / 2) {
+    for (int r = r0 + warp; r < r1; r += kWarps) {
         const int head  = r >> 1;
         const bool is_v = r & 1;
         if (!(is_v ? p.v : p.k)) continue;
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) kf_paged_read_q4_kernel(const __grid
 template <int HD, typename Y>
 int launch_read(kf_ctx* ctx, ReadParams& p, bool vec) {
     const int blocks = (p.pg.M + kTokens - 1) / kTokens, all = 2 * p.n_kv;
-    const int parts  = std::max(1, std::min((all + 3) / 4, 4 * ctx->sm_count / blocks));  // few tokens: their heads over several blocks
+    const int parts  = std::max(1, std::min((all + 7) / 8, 16 * ctx->sm_count / blocks));  // few tokens: their heads over several blocks
     p.rows_per_block = (all + parts - 1) / parts;
     const dim3 grid(blocks, (all + p.rows_per_block - 1) / p.rows_per_block);
     KF_CUDA(ctx, kf_launch_pdl(ctx, vec ? kf_paged_read_q4_kernel<HD, Y, true> : kf_paged_read_q4_kernel<HD, Y, false>, grid, dim3(kThreads), 0, p));
