@@ -12,18 +12,14 @@
 //     The zeros are one more step of 16 per group, in which the sum of the group's q stands as three bf16 numbers.
 //   * O^T = V^T P^T: dims are the rows; P goes from the scores' layout to the operand's by a transposition of 8 x 8 (movmatrix), and the zeros of group j are row j of a
 //     fifth accumulator.
-//   * A warp takes 16 positions (two units) of a tile of 64; a unit is contiguous (Q4Unit), so a tile is a bulk copy per page (or part of 8, 16, 32 or 64 positions of it).
+//   * A warp takes 32 positions (four units) of a tile of 128; a unit is contiguous (Q4Unit), so a tile is a bulk copy per page (or part of 8 .. 128 positions of it).
 #include <algorithm>
 
 #include "kf_paged_walk.cuh"
 
 namespace {
-#ifndef Q4_WARPS
-#define Q4_WARPS 4
-#define Q4_SUB 2
-#define Q4_OCC 2
-#endif
-constexpr int kWarps = Q4_WARPS, kSub = Q4_SUB, kTok = 16 * kSub * kWarps, kMaxStages = 12;  // computing warps; groups of 16 positions that a warp takes of a tile; positions of a tile
+// computing warps; groups of 16 positions that a warp takes of a tile beside one another (one: 77 us for the 64 sequences above, two: 68 at the time); positions of a tile
+constexpr int kWarps = 4, kSub = 2, kTok = 16 * kSub * kWarps, kMaxStages = 12;
 constexpr float kSlack = 8.f;  // growth of a maximum, log2, that sums are not rescaled for
 
 // bytes from global into shared memory, both at 16 bytes, a multiple of 16
@@ -57,6 +53,7 @@ __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
         w[0] = v.x, w[1] = v.y;
     } else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
+__device__ __forceinline__ float half_of(uint32_t w, int h) { return h ? bf16hi(w) : bf16lo(w); }
 // pairs of codes out of a word: nibbles (0, 4), (1, 5), (2, 6), (3, 7); the second and the fourth stand for 16 times their codes
 __device__ __forceinline__ void codes(uint32_t w, uint32_t (&c)[4]) { c[0] = w & 0x000f000fu, c[1] = w & 0x00f000f0u, c[2] = (w >> 8) & 0x000f000fu, c[3] = (w >> 8) & 0x00f000f0u; }
 
@@ -74,8 +71,16 @@ struct Q4Args {  // kernel parameter
     float sc2;               // scale * log2(e) * 2^73
 };
 __host__ __device__ constexpr int stage_bytes(int hd) { return kTok / 8 * Q4Unit(hd).bytes; }
+__host__ __device__ constexpr int q_bytes(int hd, int nt) { return nt * 8 * hd * 2; }  // queries of a block, which there are two of
 constexpr int rows_area(int hd, int rb) { return kWarps * rb * hd * 4; }
 
+// positions that all rows of a block see: below `hi`, the first row's end, and from `lo` on, where the last row's window begins, or below `first`
+struct Sure {
+    int hi, lo, first;
+    __device__ __forceinline__ Sure(const PagedPiece& pc, const PagedPlan& pl, int cap) {
+        hi = min(pc.len - pc.n + pc.b * pl.tb + 1, cap), lo = pl.window > 0 ? pc.len - pc.n + min(pc.n, (pc.b + 1) * pl.tb) - pl.window : 0, first = pl.window > 0 ? pl.first : 0;
+    }
+};
 __device__ __forceinline__ uint16_t* out_row(const Q4Args& a, const PagedPlan& pl, const PagedPiece& pc, int kvh, int r, int hd) {
     return a.out + (pc.q0 + pc.b * pl.tb + r / pl.group) * a.ldo + (long long)(kvh * pl.group + r % pl.group) * hd;
 }
@@ -90,17 +95,21 @@ template <int HD, int NT, int OCC>
 __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     kf_attn_paged_q4_kernel(const __grid_constant__ Q4Args a, const __grid_constant__ KfPaged pg_, const __grid_constant__ PagedPlan pl, const __grid_constant__ KfBound bound) {
     constexpr Q4Unit un(HD);
-    constexpr int G = un.groups, UNIT = un.bytes, STAGE = stage_bytes(HD);
+    constexpr int G = un.groups, UNIT = un.bytes, STAGE = stage_bytes(HD), QB = q_bytes(HD, NT);
     extern __shared__ __align__(128) uint8_t ring[];
-    float* s_o = reinterpret_cast<float*>(ring + (size_t)a.stages * STAGE);  // [kWarps][rb][HD]
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], meet_bar;
+    uint8_t* s_q = ring + (size_t)a.stages * STAGE;              // [2][8 NT][HD] queries
+    float* s_o   = reinterpret_cast<float*>(s_q + 2 * QB);       // [kWarps][rb][HD]
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], q_full[2], q_empty[2], meet_bar;
     __shared__ volatile int dead;
-    __shared__ int s_there[kMaxStages];  // bit i: positions 8 i .. 8 i + 7 of the tile are there
+    __shared__ int s_there[kMaxStages];  // bit i: positions 8 i .. 8 i + 7 of the tile are there; bit 31: all are, and all rows of the block see them
     __shared__ PagedQueue qu;
-    __shared__ float s_m[kWarps][16], s_l[kWarps][16];
+    __shared__ float s_m[kWarps][8 * NT], s_l[kWarps][8 * NT];
+    __shared__ uint4 s_qb[NT == 1 ? 1 : NT * G][32];  // 9 .. 16 rows: the operands of q, which the warps' registers do not hold beside the sums
+
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     if (tid == 0) {
         for (int s = 0; s < a.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], kWarps);
+        for (int s = 0; s < 2; s++) mbar_init(&q_full[s], 1), mbar_init(&q_empty[s], kWarps);
         mbar_init(&meet_bar, kWarps);
         qu.init(kWarps);
         dead = 0;
@@ -113,6 +122,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     const uint16_t* q   = behind_wait(a.q);
     const int team = (int)blockIdx.x / a.n_kv, kvh = (int)blockIdx.x % a.n_kv;
     PagedPiece* rec = a.rec + kvh * ((int)gridDim.x / a.n_kv);  // by team
+    const int group = pl.group, rb = pl.tb * group;
     if (pg.n_seq > 32) {
         PagedPlanner<kTok>::count(pg, pl, qu.s_sum, warp, kWarps + 1, lane);
         __syncthreads();
@@ -129,7 +139,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
             while (plan.push(qu, team, rec, &dead, bound)) {}
             return;
         }
-        uint32_t st = 0, ph = 0, asked = 0;
+        uint32_t st = 0, ph = 0, asked = 0, qn = 0;
         // A lane per box (page, or part of one) of several tiles: the pages of the next 32 boxes are looked up while those before are copied.  A look-up takes about as long as
         // two tiles (one tile ahead, as where tiles are four times as large: 78 us for the 64 sequences below)
         const int n_box = kTok / a.box, units = a.box / 8, ahead = 32 / n_box, bx = lane % n_box, mine = lane < ahead * n_box ? lane / n_box : 1 << 24;
@@ -143,7 +153,16 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
                 const int p = pc.tile(t) * kTok + bx * a.box;
                 return t < pc.t1 && p < pc.hi && (p + a.box > pc.lo || p < fs) ? paged_page(pg, pc.s, p, next_row) : -1;
             };
+            const Sure sure(pc, pl, pg.cap);
             int next = page_of(pc.t0 + mine);
+            // the block's queries, a token to a lane
+            const int tok0 = pc.b * pl.tb, toks = min(pl.tb, pc.n - tok0);
+            if (!(live = mbar_wait_warp(smem_u32(&q_empty[qn & 1]), ((qn >> 1) & 1) ^ 1, &dead, bound))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&q_full[qn & 1], (uint32_t)(toks * group * HD * 2));
+            __syncwarp();
+            if (lane < toks) bulk_load(s_q + (qn & 1) * QB + lane * group * HD * 2, q + (pc.q0 + tok0 + lane) * a.ldq + (long long)kvh * group * HD, (uint32_t)(group * HD * 2), &q_full[qn & 1]);
+            __syncwarp();
+            qn++;
             for (int t0 = pc.t0; live && t0 < pc.t1; t0 += ahead) {
                 const int page = next, row = next_row, n = min(ahead, pc.t1 - t0);
                 next = page_of(t0 + ahead + mine);
@@ -153,7 +172,8 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
                     const unsigned there = __reduce_or_sync(0xffffffffu, mine == i ? has : 0u);
                     if (!(live = mbar_wait_warp(smem_u32(&empty[st]), ph ^ 1, &dead, bound))) break;
                     if (lane == 0) {
-                        s_there[st] = (int)there;
+                        const int p0 = pc.tile(t0 + i) * kTok;
+                        s_there[st]  = (int)(there == (1u << kTok / 8) - 1u && p0 + kTok <= sure.hi && (p0 >= sure.lo || p0 + kTok <= sure.first) ? there | 1u << 31 : there);
                         mbar_arrive_expect_tx(&full[st], (uint32_t)__popc(there) * UNIT);
                     }
                     __syncwarp();
@@ -165,12 +185,12 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
             }
         }
         // copies in flight write shared memory, which is another's once the CTA has ended, and where a wait has run out nobody else may have waited for them
+        for (uint32_t k = qn > 2 ? qn - 2 : 0; k < qn; k++) mbar_drain(smem_u32(&q_full[k & 1]), (k >> 1) & 1, bound);
         for (uint32_t k = asked > (uint32_t)a.stages ? asked - a.stages : 0; k < asked; k++) mbar_drain(smem_u32(&full[k % a.stages]), (k / a.stages) & 1, bound);
         return;
     }
-    const int group = pl.group, rb = pl.tb * group;
     const bool vec = ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0;
-    uint32_t mph = 0, st = 0, ph = 0;
+    uint32_t mph = 0, st = 0, ph = 0, qn = 0;
     auto meet = [&]() {  // all computing warps; bounded like every wait
         __syncwarp();
         if (lane == 0) mbar_arrive(&meet_bar);
@@ -180,41 +200,46 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
         const int rows = min(pl.tb, pc.n - pc.b * pl.tb) * group, fs = pc.lo > 0 ? pl.first : 0;
         // The block's queries as B operands.  Slot pairs of a lane's words: entries (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of its 8 of every group, times 2^60; rows past the end: zero
-        uint32_t qb[NT][G][4], qz[NT][G][2];  // qz: minus the sum of q over a group, times 2^-73, as three numbers in the lanes of the group's slot
-        int lim[NT][2], low[NT][2];        // what the lane's columns see: positions above `low`, or of the first, up to `lim`
+        uint32_t qb[NT == 1 ? G : 1][4], qz[NT][NT == 1 ? G : 1][2];  // qz: minus the sum of q over a group, times 2^-73, as three numbers in the lanes t4 of the group's number
+        uint32_t toks = 0;                 // tokens of the lane's columns, eight bits each
+        if (!(live = mbar_wait_warp(smem_u32(&q_full[qn & 1]), (qn >> 1) & 1, &dead, bound))) break;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int r = n * 8 + g, tok = pc.b * pl.tb + r / group;
-            const uint16_t* qp = q + (pc.q0 + tok) * a.ldq + (long long)(kvh * group + r % group) * HD;
+            const int r = n * 8 + g;
+            const uint8_t* qp = s_q + (qn & 1) * QB + r * HD * 2;
             float mine = 0.f;
 #pragma unroll
             for (int j = 0; j < G; j++) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (r < rows) w = *reinterpret_cast<const uint4*>(qp + 32 * j + 8 * t4);
+                uint4 w = *reinterpret_cast<const uint4*>(qp + (32 * j + 8 * t4) * 2);
+                if (r >= rows) w = make_uint4(0u, 0u, 0u, 0u);
                 const float e[8] = {bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y), bf16lo(w.z), bf16hi(w.z), bf16lo(w.w), bf16hi(w.w)};
                 float sum = 0.f;
+                uint32_t x[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float f = i & 1 ? 0x1p56f : 0x1p60f;
-                    qb[n][j][i] = pack_bf16x2(e[i] * f, e[i + 4] * f);
+                    x[i] = pack_bf16x2(e[i] * f, e[i + 4] * f);
+                    if constexpr (NT == 1) qb[j][i] = x[i];
                     sum += e[i] + e[i + 4];
                 }
+                if (NT > 1 && warp == (n * G + j) % kWarps) s_qb[n * G + j][lane] = make_uint4(x[0], x[1], x[2], x[3]);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1), sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (t4 % G == j) mine = sum;
+                if (t4 == j) mine = sum;
             }
             mine *= -0x1p-73f;
             const float hi = __bfloat162float(__float2bfloat16_rn(mine)), mid = __bfloat162float(__float2bfloat16_rn(mine - hi));
 #pragma unroll
-            for (int j = 0; j < G; j++) qz[n][j][0] = t4 == j ? pack_bf16x2(hi, mid) : 0u, qz[n][j][1] = t4 == j ? pack_bf16x2(mine - hi - mid, 0.f) : 0u;
+            for (int j = 0; j < (NT == 1 ? G : 1); j++)  // registers allow it for 8 rows; otherwise chosen as they are used
+                qz[n][j][0] = NT == 2 || t4 == j ? pack_bf16x2(hi, mid) : 0u, qz[n][j][1] = NT == 2 || t4 == j ? pack_bf16x2(mine - hi - mid, 0.f) : 0u;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int tc = pc.b * pl.tb + (n * 8 + 2 * t4 + e) / group;
-                lim[n][e] = min(pc.len - pc.n + tc, pg.cap - 1), low[n][e] = pl.window > 0 ? pc.len - pc.n + tc - pl.window : -1;
-            }
+            for (int e = 0; e < 2; e++) toks |= (uint32_t)((n * 8 + 2 * t4 + e) / group) << (8 * (2 * n + e));
         }
-        // positions that all rows see: below the first row's, and above the last row's window or of the first
-        const int sure_hi = min(pc.len - pc.n + pc.b * pl.tb + 1, pg.cap), sure_lo = pl.window > 0 ? pc.len - pc.n + min(pc.n, (pc.b + 1) * pl.tb) - pl.window : 0;
-        const int fw = pl.window > 0 ? pl.first : 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[qn & 1]);
+        qn++;
+        if (NT > 1) meet();
+        if (!live) break;
+        const Sure sure(pc, pl, pg.cap);
         float o[NT][G][2][4], oz[NT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -225,13 +250,22 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
             oz[n][0] = oz[n][1] = oz[n][2] = oz[n][3] = 0.f;
             m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
         }
+        const int place = pc.len - pc.n + pc.b * pl.tb;  // position of the block's first token
         for (int t = pc.t0; t < pc.t1; t++) {
             if (!(live = mbar_wait_warp(smem_u32(&full[st]), ph, &dead, bound))) break;
-            const int tok0 = pc.tile(t) * kTok + warp * 16 * kSub;  // this warp's positions
-            const unsigned there = ((unsigned)*(volatile int*)&s_there[st] >> (warp * 2 * kSub)) & ((1u << (2 * kSub)) - 1u);
-            if (there && tok0 < pc.hi && (tok0 + 16 * kSub > pc.lo || tok0 < fs)) {
+            const unsigned there_ = (unsigned)*(volatile int*)&s_there[st];
+            const bool fine       = (int)there_ < 0;
+            int tok0 = 0;  // this warp's positions and which of their units are there, where that is not all
+            unsigned there = 0;
+            bool any = true;
+            if (!fine) {
+                tok0  = pc.tile(t) * kTok + warp * 16 * kSub;
+                there = (there_ >> (warp * 2 * kSub)) & ((1u << (2 * kSub)) - 1u);
+                any   = there && tok0 < pc.hi && (tok0 + 16 * kSub > pc.lo || tok0 < fs);
+            }
+            if (any) {
                 const uint8_t* u0 = ring + st * STAGE + warp * 2 * kSub * UNIT;  // their units
-                const bool ragged = there != (1u << (2 * kSub)) - 1u || tok0 + 16 * kSub > sure_hi || (tok0 < sure_lo && tok0 + 16 * kSub > fw);
+                const bool ragged = !fine && (there != (1u << (2 * kSub)) - 1u || tok0 + 16 * kSub > sure.hi || (tok0 < sure.lo && tok0 + 16 * kSub > sure.first));
                 // ---- scores, transposed: rows are positions g of two units, columns the block's rows ----
                 float sc[kSub][NT][4];
 #pragma unroll
@@ -249,13 +283,18 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
                         uint32_t c0[4], c1[4];
                         codes(kw[0][j], c0), codes(kw[1][j], c1);
                         const uint32_t a0[4] = {c0[0], c1[0], c0[1], c1[1]}, a1[4] = {c0[2], c1[2], c0[3], c1[3]};
-                        const float s0 = j & 1 ? bf16hi(ks[0][j / 2]) : bf16lo(ks[0][j / 2]), s1 = j & 1 ? bf16hi(ks[1][j / 2]) : bf16lo(ks[1][j / 2]);
+                        const float s0 = half_of(ks[0][j / 2], j & 1), s1 = half_of(ks[1][j / 2], j & 1);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
                             float acc[4];
-                            mma_new(acc, az, qz[n][j][0], qz[n][j][1]);
-                            mma(acc, a0, qb[n][j][0], qb[n][j][1]);
-                            mma(acc, a1, qb[n][j][2], qb[n][j][3]);
+                            if constexpr (NT == 1) {
+                                mma_new(acc, az, qz[n][j][0], qz[n][j][1]);
+                                mma(acc, a0, qb[j][0], qb[j][1]), mma(acc, a1, qb[j][2], qb[j][3]);
+                            } else {
+                                const uint4 x = s_qb[n * G + j][lane];
+                                mma_new(acc, az, t4 == j ? qz[n][0][0] : 0u, t4 == j ? qz[n][0][1] : 0u);
+                                mma(acc, a0, x.x, x.y), mma(acc, a1, x.z, x.w);
+                            }
 #pragma unroll
                             for (int i = 0; i < 4; i++) sc[b][n][i] = j == 0 ? (i < 2 ? s0 : s1) * acc[i] : fmaf(i < 2 ? s0 : s1, acc[i], sc[b][n][i]);
                         }
@@ -271,8 +310,10 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
-                            for (int i = 0; i < 2; i++)
-                                if (!(ok >> e & 1) || p > lim[n][i] || (p <= low[n][i] && p >= fw)) sc[e / 2][n][2 * (e & 1) + i] = -INFINITY;
+                            for (int i = 0; i < 2; i++) {
+                                const int at = place + (int)(toks >> (8 * (2 * n + i)) & 255u);  // the column's position
+                                if (!(ok >> e & 1) || p > at || (pl.window > 0 && p <= at - pl.window && p >= pl.first)) sc[e / 2][n][2 * (e & 1) + i] = -INFINITY;
+                            }
                     }
                 }
                 float mx[NT][2];
@@ -338,25 +379,20 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
                         }
                     }
 #pragma unroll
-                    for (int w = 0; w < G / 2; w++)
+                    for (int j = 0; j < G; j++) {
+                        uint32_t c0[4], c1[4];
+                        codes(__byte_perm(vw[0][j / 2], vw[0][G / 2 + j / 2], j & 1 ? 0x7632 : 0x5410), c0);
+                        codes(__byte_perm(vw[1][j / 2], vw[1][G / 2 + j / 2], j & 1 ? 0x7632 : 0x5410), c1);
+                        const uint32_t a0[4] = {c0[0], c0[1], c1[0], c1[1]}, a1[4] = {c0[2], c0[3], c1[2], c1[3]};
+                        const uint32_t az[4] = {g == j ? vz[0] : 0u, 0u, g == j ? vz[1] : 0u, 0u};
+                        const float s0 = half_of(vs[0][j / 2], j & 1), s1 = half_of(vs[1][j / 2], j & 1);
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {  // group 2 w + h
-                            const int j = 2 * w + h;
-                            uint32_t c0[4], c1[4];
-                            codes(__byte_perm(vw[0][w], vw[0][G / 2 + w], h ? 0x7632 : 0x5410), c0);
-                            codes(__byte_perm(vw[1][w], vw[1][G / 2 + w], h ? 0x7632 : 0x5410), c1);
-                            const uint32_t a0[4] = {c0[0], c0[1], c1[0], c1[1]}, a1[4] = {c0[2], c0[3], c1[2], c1[3]};
-                            const uint32_t az[4] = {g == j ? vz[0] : 0u, 0u, g == j ? vz[1] : 0u, 0u};
-                            const float s0 = h ? bf16hi(vs[0][w]) : bf16lo(vs[0][w]), s1 = h ? bf16hi(vs[1][w]) : bf16lo(vs[1][w]);
-#pragma unroll
-                            for (int n = 0; n < NT; n++) {
-                                const float(&p)[4] = sc[b][n];
-                                const uint32_t b0 = transpose8x8(pack_bf16x2(p[0] * s0, p[1] * s0)), b1 = transpose8x8(pack_bf16x2(p[2] * s1, p[3] * s1));
-                                mma(o[n][j][0], a0, b0, b1);
-                                mma(o[n][j][1], a1, b0, b1);
-                                mma(oz[n], az, b0, b1);
-                            }
+                        for (int n = 0; n < NT; n++) {
+                            const float(&p)[4] = sc[b][n];
+                            const uint32_t b0 = transpose8x8(pack_bf16x2(p[0] * s0, p[1] * s0)), b1 = transpose8x8(pack_bf16x2(p[2] * s1, p[3] * s1));
+                            mma(o[n][j][0], a0, b0, b1), mma(o[n][j][1], a1, b0, b1), mma(oz[n], az, b0, b1);
                         }
+                    }
                 }
             }
             __syncwarp();
@@ -408,30 +444,30 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     }
 }
 
-// Blocks that several CTAs share: a thread block takes the one that begins in its number's run and goes on behind it, if there is one.  Its rows are spread over the warps, and a row's pieces
-// over as many warps as there are for it, kAt on their way for each; these meet in order.
-constexpr int kMergeWarps = 16;
+// Blocks that several CTAs share: thread block (n, y) takes rows kMergeRows y .. of the one that begins in run n and goes on behind it, if there is one.  A row's pieces are spread over as many
+// warps as there are for it, kAt on their way for each; these meet in order.
+constexpr int kMergeWarps = 4, kMergeRows = 1;
 template <int HD>
 __global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kernel(const __grid_constant__ PagedPlan pl, const __grid_constant__ Q4Args a) {
-    constexpr int VEC = HD / 4, LANES = 32 / VEC, kAt = 8;  // HD 64: half a warp to a row
-    __shared__ float4 s_v[kMergeWarps * LANES][VEC];
-    __shared__ float2 s_ml[kMergeWarps * LANES];
+    constexpr int VEC = HD / 4, kAt = 8, kSlots = kMergeWarps * 32 / VEC, kSpread = kSlots / kMergeRows;  // HD 64: half a warp to a row
+    __shared__ float4 s_v[kSlots][VEC];
+    __shared__ float2 s_ml[kSlots];
     kf_grid_launch_dependents();
     kf_grid_dependency_wait();
     const int team = (int)blockIdx.x / a.n_kv, kvh = (int)blockIdx.x % a.n_kv, teams = (int)gridDim.x / a.n_kv;
     const PagedPiece pc = *behind_wait(a.rec + kvh * teams + team);
-    if (pc.last <= team || pc.last >= teams) return;  // last 0: nothing that goes on
     const int rb = pl.tb * pl.group, rows = min(pl.tb, pc.n - pc.b * pl.tb) * pl.group, pieces = pc.last - team + 1;
-    const int tid = threadIdx.x, slot = tid / VEC, c = tid % VEC * 4, slots = kMergeWarps * LANES, spread = slots / rows, r = slot / spread, part = slot % spread;
-    if (r < rows) {
+    if (pc.last <= team || pc.last >= teams || (int)blockIdx.y * kMergeRows >= rows) return;  // last 0: nothing that goes on
+    const int tid = threadIdx.x, slot = tid / VEC, c = tid % VEC * 4, r = blockIdx.y * kMergeRows + slot / kSpread, part = slot % kSpread;
+    if (r < rows && part < pieces) {
         float top = -INFINITY, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = part; i0 < pieces; i0 += kAt * spread) {
+        for (int i0 = part; i0 < pieces; i0 += kAt * kSpread) {
             float4 w[kAt];
             float2 ml[kAt];
 #pragma unroll
             for (int k = 0; k < kAt; k++) {
-                const int i = i0 + k * spread;
+                const int i = i0 + k * kSpread;
                 if (i < pieces) {
                     const size_t row = (((size_t)(team + i) * a.n_kv + kvh) * 2 + (i == 0)) * rb + r;
                     w[k] = __ldcg(reinterpret_cast<const float4*>(a.ws + row * HD + c)), ml[k] = __ldcg(a.ws_ml + row);
@@ -454,7 +490,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kerne
     }
     __syncthreads();
     if (r >= rows || part != 0) return;
-    const int n = min(spread, pieces);
+    const int n = min(kSpread, pieces);
     float top = -INFINITY, sum = 0.f;
     for (int k = 0; k < n; k++) top = fmaxf(top, s_ml[slot + k].x);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -469,6 +505,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kerne
 
 template <int HD, int NT, int OCC>
 int launch_q4(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, PagedPlan pl, Q4Args a, float scale) {
+    constexpr int kStage = stage_bytes(HD);
     const int teams = std::max(1, OCC * ctx->sm_count / a.n_kv), grid = teams * a.n_kv, rb = pl.tb * pl.group;
     const size_t rows = (size_t)grid * 2 * rb;
     pl.runs = teams;
@@ -478,8 +515,9 @@ int launch_q4(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, PagedPlan p
     a.box = 8;
     while (kTok % (2 * a.box) == 0 && kv->page_size % (2 * a.box) == 0) a.box *= 2;
     constexpr int kBytes = (224 / OCC - 4) * 1024;  // of shared memory for a CTA, its fixed part aside
-    a.stages             = std::min(kMaxStages, (kBytes - rows_area(HD, rb)) / stage_bytes(HD));
-    const size_t smem    = (size_t)a.stages * stage_bytes(HD) + rows_area(HD, rb);
+    const int other      = 2 * q_bytes(HD, NT) + rows_area(HD, rb);
+    a.stages             = std::min(kMaxStages, (kBytes - other) / kStage);
+    const size_t smem    = (size_t)a.stages * kStage + other;
     a.ws = ctx->attn_ws, a.ws_ml = reinterpret_cast<float2*>(ctx->attn_ws + rows * HD), a.rec = reinterpret_cast<PagedPiece*>(ctx->attn_ws + (rows * (HD + 2) + 3) / 4 * 4);
     a.sc2     = scale * 1.4426950408889634f * 0x1p73f;
     auto kern = kf_attn_paged_q4_kernel<HD, NT, OCC>;
@@ -490,7 +528,7 @@ int launch_q4(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, PagedPlan p
     }
     KF_CUDA(ctx, kf_launch_pdl(ctx, kern, dim3(grid), dim3((kWarps + 1) * 32), smem, a, pg, pl, KfBound{ctx->wait_flags + kWaitPaged, (unsigned)ctx->attn_wait_us, ctx->attn_drop}));
     KF_LAUNCH_CHECK(ctx);
-    KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_paged_q4_merge_kernel<HD>, dim3(grid), dim3(kMergeWarps * 32), 0, pl, a));
+    KF_CUDA(ctx, kf_launch_pdl(ctx, kf_attn_paged_q4_merge_kernel<HD>, dim3(grid, (rb + kMergeRows - 1) / kMergeRows), dim3(kMergeWarps * 32), 0, pl, a));
     KF_LAUNCH_CHECK(ctx);
     return KF_OK;
 }
@@ -521,7 +559,7 @@ extern "C" int kf_paged_attention_q4(kf_ctx* ctx, const kf_paged_q4* kv, void* o
     Q4Args a = {};
     a.pool = (const uint8_t*)kv->pool_dev, a.page_stride = (long long)kf_paged_q4_stride(kv), a.out = (uint16_t*)out, a.q = (const uint16_t*)q, a.ldo = ldo, a.ldq = ldq, a.n_kv = kv->n_kv;
     const PagedPlan pl{tokens, group, window, 1, 0, first};
-    if (kv->head_dim == 128) return tokens * group <= 8 ? launch_q4<128, 1, Q4_OCC>(ctx, kv, pg, pl, a, scale) : launch_q4<128, 2, 2>(ctx, kv, pg, pl, a, scale);
+    if (kv->head_dim == 128) return tokens * group <= 8 ? launch_q4<128, 1, 2>(ctx, kv, pg, pl, a, scale) : launch_q4<128, 2, 2>(ctx, kv, pg, pl, a, scale);
     return tokens * group <= 8 ? launch_q4<64, 1, 3>(ctx, kv, pg, pl, a, scale) : launch_q4<64, 2, 2>(ctx, kv, pg, pl, a, scale);
 }
 // The checks for tests on a host without a device
