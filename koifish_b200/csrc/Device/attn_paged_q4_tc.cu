@@ -371,6 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                          j > 0 || k < kParts2 - 1 || i > 0);
                         }
                         if (live) umma_commit_a(smem_u32(&o_done[t]));
+                        // the tile goes back behind the last chain that reads it, and ahead of the wait for the next one, which the same warps expand
+                        if (live && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&v_empty[vs]));
                         cnt[t]++;
                     }
                     if (live && scores && kseen <= ik) live = mbar_wait_warp(smem_u32(&k_full[ks]), (ik / kStagesK) & 1, &dead, bound), kseen = ik + 1;
@@ -382,8 +384,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         umma_commit_a(smem_u32(&s_full[t]));
                         if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
                     }
-                    // tiles go back behind the last chain that reads them
-                    if (live && sums && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&v_empty[vs]));
                     if (live && scores && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&k_empty[ks]));
                     if (live && t == 1 && j + 2 == st.of(0)) umma_commit_a(smem_u32(&q_empty));
                 }
