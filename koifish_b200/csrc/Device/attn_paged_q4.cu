@@ -117,11 +117,12 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     }
     __syncthreads();
     kf_grid_launch_dependents();
+    int team = (int)blockIdx.x / a.n_kv, kvh = (int)blockIdx.x % a.n_kv, teams = (int)gridDim.x / a.n_kv, n_box = kTok / a.box;
+    asm volatile("" : "+r"(team), "+r"(kvh), "+r"(teams), "+r"(n_box));  // worked out ahead of the wait: divisions
     kf_grid_dependency_wait();  // queries, the new positions' codes, lengths and tables, workspace
     const KfPaged pg    = behind_wait(pg_);
     const uint16_t* q   = behind_wait(a.q);
-    const int team = (int)blockIdx.x / a.n_kv, kvh = (int)blockIdx.x % a.n_kv;
-    PagedPiece* rec = a.rec + kvh * ((int)gridDim.x / a.n_kv);  // by team
+    PagedPiece* rec = a.rec + kvh * teams;  // by team
     const int group = pl.group, rb = pl.tb * group;
     if (pg.n_seq > 32) {
         PagedPlanner<kTok>::count(pg, pl, qu.s_sum, warp, kWarps + 1, lane);
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
         uint32_t st = 0, ph = 0, asked = 0, qn = 0;
         // A lane per box (page, or part of one) of several tiles: the pages of the next 32 boxes are looked up while those before are copied.  A look-up takes about as long as
         // two tiles (one tile ahead, as where tiles are four times as large: 78 us for the 64 sequences below)
-        const int n_box = kTok / a.box, units = a.box / 8, ahead = 32 / n_box, bx = lane % n_box, mine = lane < ahead * n_box ? lane / n_box : 1 << 24;
+        const int units = a.box / 8, ahead = 32 / n_box, bx = lane % n_box, mine = lane < ahead * n_box ? lane / n_box : 1 << 24;
         const uint32_t bytes = (uint32_t)(units * UNIT);
         uint8_t* dst         = ring + bx * units * UNIT;
         while (live && plan.push(qu, team, rec, &dead, bound)) {

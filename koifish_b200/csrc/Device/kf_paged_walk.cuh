@@ -103,8 +103,8 @@ struct PagedWalk {
             before += __shfl_sync(0xffffffffu, c, 31);
         }
     }
-    // the piece that starts at tile u and ends before tile end (u < end <= all tiles, u not before what was asked for last)
-    __device__ __forceinline__ PagedPiece at(int u, int end, int run) {
+    // the piece of run `index` that starts at tile u and ends before tile end (u < end <= all tiles, u not before what was asked for last); runs have `run` tiles
+    __device__ __forceinline__ PagedPiece at(int u, int end, int run, int index) {
         unsigned hit;
 #pragma unroll 1
         while (!(hit = __ballot_sync(0xffffffffu, before + inc > u)) && base + 32 < pg.n_seq) {
@@ -136,7 +136,8 @@ struct PagedWalk {
         p.t0 = p.kt0 - p.ns + off, p.t1 = p.t0 + n_tiles;
         p.whole = n_tiles == all;
         p.first = p.last = 0;
-        if (!p.whole) p.first = (u - off) / run, p.last = (u - off + all - 1) / run;
+        // a division where the block begins or ends in another run
+        if (!p.whole) p.first = off == 0 ? index : (u - off) / run, p.last = off + n_tiles == all ? index : (u - off + all - 1) / run;
         return p;
     }
 };
@@ -188,7 +189,7 @@ struct PagedPlanner {
         if (!more) return false;
         more = u < u1;
         if (more) {
-            pc = walk.at(u, u1, run);
+            pc = walk.at(u, u1, run, index);
             u += pc.t1 - pc.t0;
         } else {
             if (rec && walk.lane == 0) {
