@@ -103,10 +103,10 @@ uint64_t kf_scratch_generation(kf_ctx* ctx);
  * kernel; default 1024), "tc_min_m" (token count from which kf_linear* use the tcgen05 GEMM: -1 = measured per-type crossover, 0 = never, n = from n),
  * "tc_bn" (token tile of the tcgen05 GEMM: 16, 32, 64, 128 or 256; 0 = by modelled time), "attn_tc_min_m" (panel size from which
  * kf_attn_prefill takes the tcgen05 kernel, at least 65 tokens; 0 = where it is the faster one), "attn_wait_us" (how long a wait inside kf_attn_prefill /
- * kf_attn_decode_gqa / kf_paged_attention may take, default 4 s; when one runs out the kernel ends and kf_ctx_sync -- or the next of these calls -- returns KF_ERR_CUDA, once, and the
+ * kf_attn_decode_gqa / kf_paged_attention / kf_paged_attention_q4 may take, default 4 s; when one runs out the kernel ends and kf_ctx_sync -- or the next of these calls -- returns KF_ERR_CUDA, once, and the
  * context is usable again), "attn_drop" (n > 0: the n-th thread block of these kernels loads nothing, so that its waits run out; for tests) */
 int kf_ctx_set_int(kf_ctx* ctx, const char* key, int value);
-int kf_ctx_get_int(kf_ctx* ctx, const char* key, int* value_out); /* gqa_min_ctx, tc_min_m, pdl, attn_split; attn_tc_error (kf_attn_prefill), attn_gqa_error (kf_attn_decode_gqa), attn_paged_error (kf_paged_attention) (wait for the stream): not 0 when a bounded wait of these kernels ran out and has not been reported yet; tmap_weights: tensor maps of weights held; gemv_last_s, gemv_last_kernel: k-parts and file (0 gemv.cu, 1 gemv_tma.cu, 2 gemv_i8.cu) of the last skinny matmul; tc_last_bn, tc_last_split, tc_last_cluster: token tile, k-parts and whether these met in clusters, of the last tcgen05 GEMM */
+int kf_ctx_get_int(kf_ctx* ctx, const char* key, int* value_out); /* gqa_min_ctx, tc_min_m, pdl, attn_split; attn_tc_error (kf_attn_prefill), attn_gqa_error (kf_attn_decode_gqa), attn_paged_error (kf_paged_attention, kf_paged_attention_q4) (wait for the stream): not 0 when a bounded wait of these kernels ran out and has not been reported yet; tmap_weights: tensor maps of weights held; gemv_last_s, gemv_last_kernel: k-parts and file (0 gemv.cu, 1 gemv_tma.cu, 2 gemv_i8.cu) of the last skinny matmul; tc_last_bn, tc_last_split, tc_last_cluster: token tile, k-parts and whether these met in clusters, of the last tcgen05 GEMM */
 
 /* ---- device memory (huTensor::Alloc_1, src/Device/CUDA/huTensor.cu:70-103) ---- */
 int kf_malloc(kf_ctx* ctx, size_t bytes, void** dev_out);
@@ -277,11 +277,12 @@ int kf_paged_append(kf_ctx* ctx, const kf_paged_kv* kv, const kf_rotation* rot, 
  * chooses one of two kernels for the whole step, whatever it says is right: results agree within their rounding, not in the last bits, and times differ (single tokens alone
  * take up to 1.5 times as long in the kernel for many rows).  A captured step keeps the kernel it was captured with. */
 int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int max_q);
-/* ---- the same cache in 4 bits (paged_append.cu, paged_read_q4.cu, attn_paged_q4.cu): steps, tables and padding as above, rows of K and V as codes.  Every 32 entries of a head's
+/* ---- the same cache in 4 bits (paged_append.cu, paged_read_q4.cu, attn_paged_q4.cu, attn_paged_q4_tc.cu): steps, tables and padding as above, rows of K and V as codes.  Every 32 entries of a head's
  *      row are a group with a step and a zero in bf16; a code c of 0 .. 15 stands for step * (c - zero):
  *        step = max((max - min) / 15, max |x| / 2048), rounded up to bf16; zero = -min / step, rounded to bf16 (0 where step is 0);
  *        c = x / step + zero, rounded to the nearest whole number (ties to even) and kept to 0 .. 15; all in fp32.
- *      So x comes back within step * (1/2 + |zero| / 256).  A group with an entry that is not finite comes back as NaN.  Meant for values below 2^50.
+ *      So x comes back within step * (1/2 + |zero| / 256).  A group with an entry that is not finite comes back as NaN.  The attention is meant for keys, values and
+ *      queries below 2^50.
  *      0.625 bytes an entry, against 2 in bf16.
  *      A page holds for every kv head page_size / 8 units, one behind the other; a unit is 8 positions (10 * head_dim bytes, G = head_dim / 32):
  *        K codes [8][head_dim / 2] bytes | K steps [8][G] | K zeros [8][G] | V codes [8][4][2][head_dim / 16] bytes | V steps [8][G] | V zeros [G][8]   (bf16)
@@ -307,8 +308,8 @@ int kf_paged_append_q4(kf_ctx* ctx, const kf_paged_q4* kv, const kf_rotation* ro
  * are outside the table become zeros. */
 int kf_paged_read_q4(kf_ctx* ctx, const kf_paged_q4* kv, void* k_out_dev, int ldk, void* v_out_dev, int ldv, int out_f32, int M);
 /* kf_paged_attention over such a cache.  With window > 0 a row at position p sees the positions p - window < j <= p and, of those before, j < first.
- * What it says of rows that see nothing, of values that are not finite, of alignment and of max_q holds here too; scale at most 2^20.  The codes' arithmetic is exact; weights
- * times steps are rounded to bf16 for the product with V (in the kernel for many rows keys and values as well). */
+ * What it says of rows that see nothing, of values that are not finite, of alignment and of max_q holds here too; scale at most 2^20.  Weights times steps are rounded to bf16 for
+ * the product with the values' codes; in the kernel for many rows (more than 16 of a sequence and kv head, by max_q) keys and values are, and weights. */
 int kf_paged_attention_q4(kf_ctx* ctx, const kf_paged_q4* kv, void* out_dev, int ldo, const void* q_dev, int ldq, int M, int n_head, float scale, int window, int first,
                           int max_q);
 /* The rotation without a cache: out[m] = rotated x[m], n_head heads of head_dim (up to 256) entries, bf16 or (f32) float; out may be x, otherwise it must not lie over a row of x. */

@@ -13,12 +13,20 @@
 //   * O^T = V^T P^T: dims are the rows; P goes from the scores' layout to the operand's by a transposition of 8 x 8 (movmatrix), and the zeros of group j are row j of a
 //     fifth accumulator.
 //   * A warp takes 32 positions (four units) of a tile of 128; a unit is contiguous (Q4Unit), so a tile is a bulk copy per page (or part of 8 .. 128 positions of it).
+//   * A team of n_kv CTAs takes a run of tiles, a kv head each; runs are equal whatever the lengths are (PagedWalk), and a second kernel, launched behind, merges what several share.
+// For up to 16 rows of a sequence and kv head (new tokens x heads of the group); more go to attn_paged_q4_tc.cu, where single rows take longer (64 sequences with 12 heads to a kv head 106
+// us here, 186 there).
+// What bounds it: instructions.  16 positions of 128 dims and 8 rows take a warp 305 of them, 149 on the pipe of logic and shifts, 24 of matrix; beside loads that bring 5.7 TB/s alone
+// (43 us for the 64 sequences of 400 .. 4000 positions, 64 / 8 heads, 196 MB) they run at 3.1 TB/s.  Measured: these 62.6 us in a steady run, one sequence of 100000 positions (128 MB) 38 us, 3.3
+// TB/s, of which 7 are the start, 4 the end and the merge; one of 1300 9.3 us, as long as issuing two launches takes from Python; 40 with a window of 1000 and 4 first positions 28.5.
+// Not kept: three CTAs per SM (62 us, and more pieces to merge: 42 for the one of 100000), one of eight computing warps (80 and 47), the merge by the CTA that arrives last (44 for the one of 100000:
+// a fence, an atomic and rounds of loads one behind the other).
 #include <algorithm>
 
 #include "kf_paged_walk.cuh"
 
 namespace {
-// computing warps; groups of 16 positions that a warp takes of a tile beside one another (one: 77 us for the 64 sequences above, two: 68 at the time); positions of a tile
+// computing warps; groups of 16 positions that a warp takes of a tile beside one another (one: 77 us for the 64 sequences above, two: 68, at the time); positions of a tile
 constexpr int kWarps = 4, kSub = 2, kTok = 16 * kSub * kWarps, kMaxStages = 12;
 constexpr float kSlack = 8.f;  // growth of a maximum, log2, that sums are not rescaled for
 
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
         }
         uint32_t st = 0, ph = 0, asked = 0, qn = 0;
         // A lane per box (page, or part of one) of several tiles: the pages of the next 32 boxes are looked up while those before are copied.  A look-up takes about as long as
-        // two tiles (one tile ahead, as where tiles are four times as large: 78 us for the 64 sequences below)
+        // a tile
         const int units = a.box / 8, ahead = 32 / n_box, bx = lane % n_box, mine = lane < ahead * n_box ? lane / n_box : 1 << 24;
         const uint32_t bytes = (uint32_t)(units * UNIT);
         uint8_t* dst         = ring + bx * units * UNIT;
@@ -445,7 +453,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     }
 }
 
-// Blocks that several CTAs share: thread block (n, y) takes rows kMergeRows y .. of the one that begins in run n and goes on behind it, if there is one.  A row's pieces are spread over as many
+// Blocks that several CTAs share (256 threads for two rows: 39.6 us for the sequence of 100000 positions, 128 for one: 39.3; 512 for all: 40.2): thread block (n, y) takes rows kMergeRows y .. of the one that begins in run n and goes on behind it, if there is one.  A row's pieces are spread over as many
 // warps as there are for it, kAt on their way for each; these meet in order.
 constexpr int kMergeWarps = 4, kMergeRows = 1;
 template <int HD>

@@ -12,6 +12,11 @@
 //   warp 10          the pieces
 //   warps 11-14      expansion: a unit of 8 positions at a time, K of a tile before V of it
 // Rows of V that no row of the block sees, or whose page is not there, are written as zeros.
+// What bounds it: the chains' way, as in attn_paged_tc.cu, and beside it instructions (2048 tokens behind 8192, 32 / 8 heads: 288 us with nothing stored by the expanding warps, 333 in all, 850
+// TFLOP/s in a steady run under the power cap, 363 us; bf16 335); where a tile has few rows, the expanding warps and shared memory (16 sequences of 500 .. 5000 positions with five drafted
+// tokens of 40 / 8 heads 61 us: a tile takes 2700 clocks, of which the matrix operands read 770 and the expansion 880 out of and into shared memory; eight or eleven expanding
+// warps there make no difference, five instead of four beside many rows 360 against 342 us).  A tile of K ahead of the V before it: 434 us.  Denominators add the weights before their
+// rounding (with it, as the bf16 kernel has them: 392 against 342 us for two more instructions a pair): error relative to 64 bits 2.4e-3, of which the result's rounding is 1.7e-3.
 // Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
 #include <algorithm>
 
@@ -47,8 +52,8 @@ __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
 __device__ __forceinline__ float half_of(uint32_t w, int h) { return h ? bf16hi(w) : bf16lo(w); }
 // Keys or values of a unit and eight rows of a tile.  A lane takes the codes of one row that stand for eight dims of every group, as one word each: K dims 32 j + 8 t .. + 7, which it stores as
 // 16 bytes, V dims 32 j + 4 t .. + 3 and 32 j + 16 + 4 t .. + 3, half words of two words in the unit, stored as 8 bytes each.  Lanes of four are rows 0, 4, 2, 6, 1, 5, 3, 7: those that store
-// together meet all 32 banks.  The code is small, and one for both, for a reason: with two units of K and two of V unrolled beside one another, instructions had to be fetched again and again
-// (2048 tokens behind 8192: 478 us against 405 one at a time).
+// together meet all 32 banks.  The code is small for a reason: with two units unrolled beside one another, instructions had to be fetched again and again (2048 tokens behind 8192: 478 us
+// against 405 one at a time).
 template <int HD, bool is_v>
 struct Eight {
     static constexpr int G = HD / 32;

@@ -279,15 +279,25 @@ def test_zeros_far_from_the_codes(ctx):
     s.check(ctx)
 
 
-def test_rows_and_strides(ctx):
+@pytest.mark.parametrize("new,length", [([1, 1, 1], [70, 5, 640]), ([1, 50, 3], [70, 55, 640])])
+def test_rows_and_strides(ctx, new, length):
     """Queries inside wider rows, results in wider rows and at any element, rows in front of the first sequence, pages of more entries than the table says."""
-    s = Step([1, 1, 1], [70, 5, 640], 8, 2, 128, 32, seed=8, extra=2, pad=1, cols=40)
+    s = Step(new, length, 8, 2, 128, 32, seed=8, extra=2, pad=1, cols=40)
     wider = torch.zeros(s.rows, 8 * 128 + 64, device="cuda", dtype=torch.bfloat16)
     wider[:, 64:] = s.q
     buf = torch.full((s.rows * (8 * 128 + 5) + 1,), 7.0, device="cuda", dtype=torch.bfloat16)
     out = buf[1:].view(s.rows, 8 * 128 + 5)
     s.check(ctx, q=wider[:, 64:], ldq=8 * 128 + 64, ldo=8 * 128 + 5, out=out)
     assert buf[0] == 7
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q", [2, 3, 4, 7])
+def test_drafts(ctx, hd, q):
+    """A few tokens each, 10 to 35 rows a kv head: two columns of rows, and the step from one kernel to the other."""
+    r = np.random.RandomState(q)
+    new = [q] * 9 + [1, 0, q - 1]
+    Step(new, [n + int(r.choice([0, 1, 100, 127, 128, 600, 1300])) for n in new], 15, 3, hd, 24, seed=q, pad=1).check(ctx)
 
 
 @pytest.mark.parametrize("max_q", [1, 40])
