@@ -16,7 +16,9 @@
 // TFLOP/s in a steady run under the power cap, 363 us; bf16 335); where a tile has few rows, the expanding warps and shared memory (16 sequences of 500 .. 5000 positions with five drafted
 // tokens of 40 / 8 heads 61 us: a tile takes 2700 clocks, of which the matrix operands read 770 and the expansion 880 out of and into shared memory; eight or eleven expanding
 // warps there make no difference, five instead of four beside many rows 360 against 342 us).  A tile of K ahead of the V before it: 434 us.  Denominators add the weights before their
-// rounding (with it, as the bf16 kernel has them: 392 against 342 us for two more instructions a pair): error relative to 64 bits 2.4e-3, of which the result's rounding is 1.7e-3.
+// rounding (with it, as the bf16 kernel has them: 392 against 342 us for two more instructions a pair).  Keys, values and weights are rounded to bf16 each, the roundings that reading the
+// pages as bf16 and attending the result would have: 4.0e-3 of the result's norm from the formula in 64 bits, of which the result's own rounding is 1.7e-3 (16 rows and fewer, where
+// only weights are rounded, 2.3e-3).  With fp16 operands, tiles and rows of q brought into its range by powers of two that another warp finds: 496 against 366 us, drafts 91 against 61.
 // Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
 #include <algorithm>
 
