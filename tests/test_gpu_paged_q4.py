@@ -451,6 +451,42 @@ def test_same_bits(ctx):
             assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
+@pytest.mark.parametrize("group,kv", [(5, 8), (7, 4), (12, 3), (17, 3)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_same_bits_whatever_ran_before(ctx, group, kv, hd):
+    """Rows of a row tile that are nobody's hold what the call before left in shared memory, here queries fifty times as large: no result depends on them."""
+    for new in ([138, 1, 77], [1, 1, 1]):
+        s = Step(new, [2231, 900, 1500], group * kv, kv, hd, 16, seed=group)
+        other = Step([130] * 20, [400] * 20, 64, 1, hd, 16, seed=3)
+        loud = other.q * 50
+        a = s.attend(ctx, hd ** -0.5)
+        for _ in range(4):
+            other.attend(ctx, hd ** -0.5, q=loud)
+            b = s.attend(ctx, hd ** -0.5)
+            ctx.sync()
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("page", [8, 16, 64])
+@pytest.mark.parametrize("window,first", [(5, 0), (70, 3), (300, 40)])
+@pytest.mark.parametrize("max_q", [150, 2])
+def test_chunks_hidden_values(ctx, hd, page, window, first, max_q):
+    """Steps and zeros that are not finite behind the first positions and before the first row's window, in pages that are still there, and behind the last position."""
+    new, length = [3, 150, 1, 60], [500, 640, 777, 64]
+    s = Step(new, length, 8, 2, hd, page, seed=window + page)
+    for i, n in enumerate(length):
+        t = torch.arange(first, max(first, n - new[i] + 1 - window), device="cuda")
+        if len(t) == 0:
+            continue
+        e, r = torch.from_numpy(s.table[i]).cuda()[t // page], t % page
+        for value in (0, 1):
+            codes, step, zero = read(s.pages, s.kv, s.hd, page, value, e, r)
+            nan = (t % 2 == 0)[:, None, None].expand_as(step)
+            write(s.pages, s.kv, s.hd, page, value, e, r, codes, torch.where(nan, float("nan"), torch.full_like(step, float("inf"))), torch.where(nan, zero, torch.full_like(zero, float("-inf"))))
+    s.check(ctx, window=window, first=first, max_q=max_q)
+
+
 # ---------------------------------------------------------------------------------------------------------------- append and read
 def quantised(x):
     """x [.., hd] fp32 -> codes [.., hd], step, zero [.., groups] by the definition, in fp32 on the CPU (true divisions)."""
@@ -829,6 +865,35 @@ def test_nothing_to_do(ctx):
         s.d[1][:] = 0
     torch.cuda.synchronize()
     assert torch.all(out == 7) and torch.equal(before, s.pool)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cta", [0, 70])
+@pytest.mark.parametrize("chunk,fresh", [(256, False), (256, True), (2, False), (2, True)])
+def test_wait_that_runs_out_among_many_pieces(hd, cta, chunk, fresh):
+    """A thread block that loads nothing and whose run is longer than the queue of pieces: what the merge reads of it says that nothing goes on, whatever the workspace held.  The
+    error is told, rows of nobody stay as they are, and the next call is right."""
+    c = kf.Context(0, stream=torch.cuda.current_stream().cuda_stream or 1)
+    r = np.random.RandomState(hd)
+    length = r.randint(20, 121, 200).tolist() + [400]
+    s = Step([1] * 200 + [chunk], length, 32, 8, hd, 16, seed=hd, extra=2, pad=3)
+    other = Step([130] * 20, [400] * 20, 64, 1, 192 - hd, 16, seed=3)
+    if not fresh:
+        other.attend(c, 0.1)
+        s.check(c)
+        other.attend(c, 0.1, q=other.q * 50)
+    c.sync()
+    out = torch.full((s.rows, 32 * hd), 7.0, device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    c.set_int("attn_wait_us", 20000), c.set_int("attn_drop", cta + 1)
+    s.attend(c, 0.1, out=out)
+    with pytest.raises(kf.KoifishError, match="wait ran out"):
+        c.sync()
+    c.set_int("attn_drop", 0), c.set_int("attn_wait_us", 0)
+    assert torch.all(out[:2] == 7) and torch.all(out[-3:] == 7)
+    c.sync()
+    s.check(c)
+    c.close()
 
 
 @pytest.mark.parametrize("new", [[1, 1], [70, 1]])
