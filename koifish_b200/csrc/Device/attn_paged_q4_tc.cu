@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     xph++;
                     if (c0 == 0) s_m[row] = m2, s_l[row] = l;
 #pragma unroll 1
-                    for (int c = 0; c < kCols; c += 32) {
+                    for (int c = 0; c < kCols && !idle; c += 32) {
                         uint32_t o[32];
                         ld32_async(o_row + c0 + c, o);
                         wait_ld();
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const float inv = l == 0.f ? 0.f : 0x1p60f / l;
 #pragma unroll 1
-                    for (int c = 0; c < kCols; c += 32) {
+                    for (int c = 0; c < kCols && !idle; c += 32) {
                         uint32_t o[32];
                         ld32_async(o_row + c0 + c, o);
                         wait_ld();
