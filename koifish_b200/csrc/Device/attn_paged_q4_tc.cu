@@ -33,6 +33,14 @@ struct Cfg {
     static constexpr int kGroup = kParts * 1024;  // tiles of K and V lie as groups of 8 rows, each in parts of 64 dims; of Q as halves of 64 dims
     static constexpr size_t kSmem = (2 + kStagesK + kStagesV) * (size_t)kTile + kStagesR * (size_t)kRaw + 1024;
 };
+// What the runs are equal in.  A step of a block whose chains share their tiles (2.2 .. 2.7 us) is near two tiles of one whose chains take turns (1.6 .. 1.9 each), and what a block
+// takes beside its tiles, queries, first scores and sums, is about as much (3.7 us): 16 sequences with five drafted tokens 57.3 us, 62.1 with runs equal in tiles, 24 sequences with
+// three chunks and 64 dims 51.3 and 55.1.  A run must then be four units or more, which costs more than it gives where there are few tiles for all CTAs: 300 tokens of one
+// sequence alone 20.3 us, 28.5 by units.
+struct ChainTiles {
+    static constexpr int kMost = 2, kBlock = 2, kFew = 4;
+    static __device__ __forceinline__ int tile(int left, int tb) { return left > tb / 2; }
+};
 struct Q4TcArgs {  // kernel parameter
     TcArgs t;
     const uint8_t* pool;
@@ -157,14 +165,101 @@ __global__ void __launch_bounds__(kThreads, 1)
     kf_grid_dependency_wait();  // queries, codes, lengths and tables, workspace
     const KfPaged pg = behind_wait(pg_);
     if (pg.n_seq > 32) {
-        PagedPlanner<kKV>::count(pg, pl, qu.s_sum, warp, kThreads / 32, lane);
+        PagedPlanner<kKV, ChainTiles>::count(pg, pl, qu.s_sum, warp, kThreads / 32, lane);
         __syncthreads();
     }
     PagedReader reader;
     PagedPiece pc;
     bool live = true;
 
-    if (warp < 8) {
+    // The order of the roles is that of their code: with the same instructions 2048 tokens behind 8192 take 326 us in this order and up to 349 in others, the planning code, which runs
+    // once, in front of or between the loops (it is no function of its own, since the kernel's registers then pay for the call: 385)
+    if (warp >= kExpW) {
+        uint32_t pos = 0;
+        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
+            const int fs = pc.lo > 0 ? pl.first : 0;
+            for (int t = pc.t0; live && t < pc.t1; t++, pos++) {
+                const uint32_t sr_ = pos % kStagesR, sk_ = pos % kStagesK, sv_ = pos % kStagesV;
+                const int p0        = pc.tile(t) * kKV;
+                if (!(live = mbar_wait_warp(smem_u32(&r_full[sr_]), (pos / kStagesR) & 1, &dead, bound))) break;
+                const unsigned there = (unsigned)s_there[pos % kMasks];
+                const uint8_t* raw   = sr + sr_ * kRaw;
+                if (!(live = mbar_wait_warp(smem_u32(&k_empty[sk_]), ((pos / kStagesK) & 1) ^ 1, &dead, bound))) break;
+#pragma unroll 1
+                for (int u = warp - kExpW; u < kKV / 8; u += kExps) {
+                    Eight<HD, false> x;
+                    x.load(raw + u * UNIT, lane);
+                    x.store(sk + sk_ * kTile + u * kGroup, lane);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the matrix instructions
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[sk_]);
+                if (!(live = mbar_wait_warp(smem_u32(&v_empty[sv_]), ((pos / kStagesV) & 1) ^ 1, &dead, bound))) break;
+#pragma unroll 1
+                for (int u = warp - kExpW; u < kKV / 8; u += kExps) {
+                    Eight<HD, true> x;
+                    x.load(raw + u * UNIT, lane);
+                    const int p = p0 + 8 * u;
+                    if (!(there >> u & 1) || p + 8 > pc.hi || p < pc.lo) {
+                        const int at = p + x.row(lane);
+                        if (!(there >> u & 1) || at >= pc.hi || (at < pc.lo && at >= fs)) x.hide();
+                    }
+                    x.store(sv + sv_ * kTile + u * kGroup, lane);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[sv_]), mbar_arrive(&r_empty[sr_]);
+            }
+        }
+    } else if (warp == kMmaW) {
+        constexpr uint32_t id_s = make_idesc_bf16(128), id_o = make_idesc_bf16(HD) | (1u << 16);  // bit 16: B is MN-major
+        const uint32_t q_addr = smem_u32(sq), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
+        uint32_t pos = 0, qn = 0, kseen = 0, vseen = 0, cnt[2] = {0, 0};  // tiles of the CTA before the piece, pieces, tiles that are expanded, steps of the chains
+        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
+            const Steps st(pc, pl, a.tokens);
+            if (!(live = mbar_wait_warp(smem_u32(&q_full), qn & 1, &dead, bound))) break;
+            for (int j = -1; live && j < st.of(0); j++)  // the sums of step j, the scores of step j + 1
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const bool sums = live && j >= 0 && j < st.of(t), scores = live && j + 1 < st.of(t);
+                    const uint32_t iv = pos + st.tile(t, j), ik = pos + st.tile(t, j + 1), vs = iv % kStagesV, ks = ik % kStagesK;
+                    // what is expanded is waited for first: the weights come last
+                    if (live && sums) {
+                        if (vseen <= iv) live = mbar_wait_warp(smem_u32(&v_full[vs]), (iv / kStagesV) & 1, &dead, bound), vseen = iv + 1;
+                        const uint64_t vd = make_desc_kv<HD>(v_addr + vs * kTile);
+#pragma unroll
+                        for (int k = kParts2 - 1; k >= 0; k--) {  // O_t += P_t V, the second part first
+                            live = live && mbar_wait_warp(smem_u32(&p_full[t][k]), cnt[t] & 1, &dead, bound);
+                            tc_fence_after();
+                            if (live)
+#pragma unroll
+                                for (int i = 0; i < 4 / kParts2; i++)
+                                    umma_sums_x2<kGroup>(tmem + 256 + t * HD, tmem + t * 128 + k * 64 + i * 16, vd + (k * (4 / kParts2) + i) * (4 * kGroup / 16), id_o,
+                                                         j > 0 || k < kParts2 - 1 || i > 0);
+                        }
+                        if (live) umma_commit_a(smem_u32(&o_done[t]));
+                        // the tile goes back behind the last chain that reads it, and ahead of the wait for the next one, which the same warps expand
+                        if (live && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&v_empty[vs]));
+                        cnt[t]++;
+                    }
+                    if (live && scores && kseen <= ik) live = mbar_wait_warp(smem_u32(&k_full[ks]), (ik / kStagesK) & 1, &dead, bound), kseen = ik + 1;
+                    if (live && scores) {  // S_t = Q K^T, behind the O above, which reads the weights from the same columns
+                        tc_fence_after();
+                        const uint32_t qd = q_addr + (st.pair ? t * kTile : 0), kd = k_addr + ks * kTile;
+#pragma unroll
+                        for (int k = 0; k < kParts; k++) umma_scores_x4(tmem + t * 128, make_desc_sw128(qd + k * kHalf), make_desc_kv<HD>(kd + k * 1024), id_s, k > 0);
+                        umma_commit_a(smem_u32(&s_full[t]));
+                        if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
+                    }
+                    if (live && scores && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&k_empty[ks]));
+                    if (live && t == 1 && j + 2 == st.of(0)) umma_commit_a(smem_u32(&q_empty));
+                }
+            pos += st.n, qn++;
+        }
+        // instructions in flight write tensor memory: waited for here, since where a wait has run out nobody else may have
+        umma_commit_a(smem_u32(&done_bar));
+        mbar_drain(smem_u32(&done_bar), 0, bound);
+    } else if (warp < 8) {
         const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t s_row = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(t * 128), o_row = tmem + ((uint32_t)(quad * 32) << 16) + 256u + (uint32_t)(t * HD);
         const uint32_t sfull = smem_u32(&s_full[t]), pfull = smem_u32(&p_full[t][0]), odone = smem_u32(&o_done[t]);
@@ -351,59 +446,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             tile0 += st.n;
         }
-    } else if (warp == kMmaW) {
-        constexpr uint32_t id_s = make_idesc_bf16(128), id_o = make_idesc_bf16(HD) | (1u << 16);  // bit 16: B is MN-major
-        const uint32_t q_addr = smem_u32(sq), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
-        uint32_t pos = 0, qn = 0, kseen = 0, vseen = 0, cnt[2] = {0, 0};  // tiles of the CTA before the piece, pieces, tiles that are expanded, steps of the chains
-        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
-            const Steps st(pc, pl, a.tokens);
-            if (!(live = mbar_wait_warp(smem_u32(&q_full), qn & 1, &dead, bound))) break;
-            for (int j = -1; live && j < st.of(0); j++)  // the sums of step j, the scores of step j + 1
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const bool sums = live && j >= 0 && j < st.of(t), scores = live && j + 1 < st.of(t);
-                    const uint32_t iv = pos + st.tile(t, j), ik = pos + st.tile(t, j + 1), vs = iv % kStagesV, ks = ik % kStagesK;
-                    // what is expanded is waited for first: the weights come last
-                    if (live && sums) {
-                        if (vseen <= iv) live = mbar_wait_warp(smem_u32(&v_full[vs]), (iv / kStagesV) & 1, &dead, bound), vseen = iv + 1;
-                        const uint64_t vd = make_desc_kv<HD>(v_addr + vs * kTile);
-#pragma unroll
-                        for (int k = kParts2 - 1; k >= 0; k--) {  // O_t += P_t V, the second part first
-                            live = live && mbar_wait_warp(smem_u32(&p_full[t][k]), cnt[t] & 1, &dead, bound);
-                            tc_fence_after();
-                            if (live)
-#pragma unroll
-                                for (int i = 0; i < 4 / kParts2; i++)
-                                    umma_sums_x2<kGroup>(tmem + 256 + t * HD, tmem + t * 128 + k * 64 + i * 16, vd + (k * (4 / kParts2) + i) * (4 * kGroup / 16), id_o,
-                                                         j > 0 || k < kParts2 - 1 || i > 0);
-                        }
-                        if (live) umma_commit_a(smem_u32(&o_done[t]));
-                        // the tile goes back behind the last chain that reads it, and ahead of the wait for the next one, which the same warps expand
-                        if (live && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&v_empty[vs]));
-                        cnt[t]++;
-                    }
-                    if (live && scores && kseen <= ik) live = mbar_wait_warp(smem_u32(&k_full[ks]), (ik / kStagesK) & 1, &dead, bound), kseen = ik + 1;
-                    if (live && scores) {  // S_t = Q K^T, behind the O above, which reads the weights from the same columns
-                        tc_fence_after();
-                        const uint32_t qd = q_addr + (st.pair ? t * kTile : 0), kd = k_addr + ks * kTile;
-#pragma unroll
-                        for (int k = 0; k < kParts; k++) umma_scores_x4(tmem + t * 128, make_desc_sw128(qd + k * kHalf), make_desc_kv<HD>(kd + k * 1024), id_s, k > 0);
-                        umma_commit_a(smem_u32(&s_full[t]));
-                        if (lane == 0) mbar_arrive(&s_full[t]);  // for what the loader wrote beside the tile
-                    }
-                    if (live && scores && (t == 1 || !st.pair)) umma_commit_a(smem_u32(&k_empty[ks]));
-                    if (live && t == 1 && j + 2 == st.of(0)) umma_commit_a(smem_u32(&q_empty));
-                }
-            pos += st.n, qn++;
-        }
-        // instructions in flight write tensor memory: waited for here, since where a wait has run out nobody else may have
-        umma_commit_a(smem_u32(&done_bar));
-        mbar_drain(smem_u32(&done_bar), 0, bound);
-    } else if (warp == kPlanW) {
-        PagedPlanner<kKV> plan(pg, pl, lane);
-        if (lane == 0) a.rec[cta].last = 0;  // nothing to merge, should a wait run out before the end of the run is known
-        plan.start(qu, cta);
-        while (plan.push(qu, cta, a.rec, &dead, bound)) {}
     } else if (warp == kLoadW) {
         if (bound.drop != cta + 1) {
             // a lane per box (page, or part of one) of one or several tiles: the next 32 boxes are looked up while those before are copied
@@ -465,42 +507,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (uint32_t k = pos > kStagesR ? pos - kStagesR : 0; k < pos; k++) mbar_drain(smem_u32(&r_full[k % kStagesR]), (k / kStagesR) & 1, bound);
         }
     } else {
-        uint32_t pos = 0;
-        while (live && reader.next(qu, pc, lane, &dead, bound, live)) {
-            const int fs = pc.lo > 0 ? pl.first : 0;
-            for (int t = pc.t0; live && t < pc.t1; t++, pos++) {
-                const uint32_t sr_ = pos % kStagesR, sk_ = pos % kStagesK, sv_ = pos % kStagesV;
-                const int p0        = pc.tile(t) * kKV;
-                if (!(live = mbar_wait_warp(smem_u32(&r_full[sr_]), (pos / kStagesR) & 1, &dead, bound))) break;
-                const unsigned there = (unsigned)s_there[pos % kMasks];
-                const uint8_t* raw   = sr + sr_ * kRaw;
-                if (!(live = mbar_wait_warp(smem_u32(&k_empty[sk_]), ((pos / kStagesK) & 1) ^ 1, &dead, bound))) break;
-#pragma unroll 1
-                for (int u = warp - kExpW; u < kKV / 8; u += kExps) {
-                    Eight<HD, false> x;
-                    x.load(raw + u * UNIT, lane);
-                    x.store(sk + sk_ * kTile + u * kGroup, lane);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the matrix instructions
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[sk_]);
-                if (!(live = mbar_wait_warp(smem_u32(&v_empty[sv_]), ((pos / kStagesV) & 1) ^ 1, &dead, bound))) break;
-#pragma unroll 1
-                for (int u = warp - kExpW; u < kKV / 8; u += kExps) {
-                    Eight<HD, true> x;
-                    x.load(raw + u * UNIT, lane);
-                    const int p = p0 + 8 * u;
-                    if (!(there >> u & 1) || p + 8 > pc.hi || p < pc.lo) {
-                        const int at = p + x.row(lane);
-                        if (!(there >> u & 1) || at >= pc.hi || (at < pc.lo && at >= fs)) x.hide();
-                    }
-                    x.store(sv + sv_ * kTile + u * kGroup, lane);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[sv_]), mbar_arrive(&r_empty[sr_]);
-            }
-        }
+        PagedPlanner<kKV, ChainTiles> plan(pg, pl, lane);
+        if (lane == 0) a.rec[cta].last = 0;  // nothing to merge, should a wait run out before the end of the run is known
+        plan.start(qu, cta);
+        while (plan.push(qu, cta, a.rec, &dead, bound)) {}
     }
     tc_fence_before();
     __syncthreads();
@@ -517,7 +527,7 @@ int launch_tc(kf_ctx* ctx, const kf_paged_q4* kv, const KfPaged& pg, void* out, 
     while (box < kKV && kv->page_size % (2 * box) == 0) box *= 2;
     const PagedPlan pl{2 * tokens, group, window, n_kv, grid, first};
     const size_t rows = (size_t)grid * 2 * 256;
-    KF_REQUIRE(ctx, paged_most(kKV, pg, pl) < 0x7fff0000, "as many tiles as M rows over full tables have");
+    KF_REQUIRE(ctx, paged_most(kKV, pg, pl) * ChainTiles::kMost + ((long long)pg.M / pl.tb + pg.n_seq) * n_kv * ChainTiles::kBlock < 0x7fff0000, "as many tiles as M rows over full tables have");
     int rc = kf_ensure_attn_ws(ctx, rows * (HD + 2) * sizeof(float) + grid * sizeof(PagedPiece));
     CUtensorMap tq;
     if (!rc) rc = kf_tmap_heads(ctx, &tq, q, HD, n_head, (uint64_t)pg.M, (uint64_t)ldq * 2, 64, group, tokens);

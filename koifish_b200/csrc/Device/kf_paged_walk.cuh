@@ -1,8 +1,8 @@
 // kf_paged_walk.cuh -- how the attention kernels share a step over a cache in pages among their CTAs (attn_paged.cu, attn_paged_tc.cu, attn_paged_q4.cu).
 //
 // The new tokens of a sequence are cut into blocks of `tb`, a block's visible positions into tiles; the tiles of all blocks (and of plan.heads kv heads of each), one after the
-// other, are cut into equal runs, so that every CTA has the same number of them whatever the lengths are.  A block that two or more runs share is a piece in each and is merged
-// afterwards.
+// other, are cut into equal runs, so that every CTA has the same number of them (or of units that tiles are worth) whatever the lengths are.  A block that two or more runs share is a
+// piece in each and is merged afterwards.
 #pragma once
 #include "kf_paged.cuh"
 #include "kf_tc.cuh"
@@ -48,14 +48,22 @@ struct alignas(16) PagedPiece {
     // the tile of positions that index t stands for: those of the first positions have the ns indices in front of kt0
     __device__ __forceinline__ int tile(int t) const { return t < kt0 ? t - kt0 + ns : t; }
 };
+// What the runs are equal in: units.  A tile of a block that has `left` tokens from its first on is worth 2^tile() of them, a block kBlock beside its tiles.  Up to kFew tiles a run
+// and up to 32 sequences each tile is one and a block none all the same.
+struct EqualTiles {
+    static constexpr int kMost = 1, kBlock = 0, kFew = 0;
+    static __device__ __forceinline__ int tile(int left, int tb) { return 0; }
+};
 // One warp's way through the sequences, 32 at a time: every lane holds one.
-template <int TILE>
+template <int TILE, class Units = EqualTiles>
 struct PagedWalk {
     const KfPaged pg;
     const PagedPlan pl;
     const int lane;
     int base, q0, n, len, nb;
-    int units, inc, before = 0;  // tiles of the lane's sequence, of it and the lanes below, of the sequences before these 32
+    int units, inc, before = 0;  // of the lane's sequence, of it and the lanes below, of the sequences before these 32
+    int took = 0;                // units of what at() found last
+    bool equal = Units::kMost == 1;
     __device__ __forceinline__ PagedWalk(const KfPaged& pg_, const PagedPlan& pl_, int lane_) : pg(pg_), pl(pl_), lane(lane_) {}
     static __device__ __forceinline__ int scan(int v, int lane) {
 #pragma unroll
@@ -65,21 +73,25 @@ struct PagedWalk {
         }
         return v;
     }
-    __device__ __forceinline__ int tiles(int n_, int len_, int b) const {
+    __device__ __forceinline__ int cost(int n_, int len_, int b) const {  // units of a block
         int lo, hi, kt0, ns;
-        return paged_block(TILE, pg.cap, pl.tb, pl.window, pl.first, n_, len_, b, lo, hi, kt0, ns);
+        return (paged_block(TILE, pg.cap, pl.tb, pl.window, pl.first, n_, len_, b, lo, hi, kt0, ns) << worth(n_, b)) + block();
     }
+    __device__ __forceinline__ int worth(int n_, int b) const { return Units::kMost == 1 || equal ? 0 : Units::tile(n_ - b * pl.tb, pl.tb); }
+    __device__ __forceinline__ int block() const { return Units::kMost == 1 || equal ? 0 : Units::kBlock; }
+    // tiles of a block that begin in its first x units: the first one at 0, tile i at block() + (i << w)
+    __device__ __forceinline__ int below(int x, int w) const { return Units::kMost == 1 ? x : x <= 0 ? 0 : 1 + (max(0, x - 1 - block()) >> w); }
     __device__ __forceinline__ void load(int base_) {
         base = base_, n = 0, nb = 0, units = 0;
         if (base + lane < pg.n_seq) {
             paged_seq(pg, base + lane, q0, n, len);
-            if (n > 0) nb = n <= pl.tb ? 1 : (n + pl.tb - 1) / pl.tb, units = tiles(n, len, 0);
+            if (n > 0) nb = n <= pl.tb ? 1 : (n + pl.tb - 1) / pl.tb, units = cost(n, len, 0);
         }
         for (unsigned many = __ballot_sync(0xffffffffu, nb > 1); many; many &= many - 1) {  // the blocks of a sequence over the lanes
             const int l = __ffs(many) - 1, n_ = __shfl_sync(0xffffffffu, n, l), len_ = __shfl_sync(0xffffffffu, len, l), nb_ = __shfl_sync(0xffffffffu, nb, l);
             int sum = 0;
 #pragma unroll 1
-            for (int b = lane; b < nb_; b += 32) sum += tiles(n_, len_, b);
+            for (int b = lane; b < nb_; b += 32) sum += cost(n_, len_, b);
             sum = __reduce_add_sync(0xffffffffu, sum);
             if (lane == l) units = sum;
         }
@@ -87,7 +99,7 @@ struct PagedWalk {
         inc = scan(units, lane);
     }
     __device__ __forceinline__ int total() const { return __shfl_sync(0xffffffffu, inc, 31); }
-    // to the 32 sequences that hold tile u
+    // to the 32 sequences that hold unit u
     __device__ __forceinline__ void seek(const int* s_sum, int u) {
         const int wins = (pg.n_seq + 31) / 32;
 #pragma unroll 1
@@ -103,7 +115,8 @@ struct PagedWalk {
             before += __shfl_sync(0xffffffffu, c, 31);
         }
     }
-    // the piece of run `index` that starts at tile u and ends before tile end (u < end <= all tiles, u not before what was asked for last); runs have `run` tiles
+    // The piece of run `index` of the tiles that begin in units u .. end - 1 (u < end <= all units, u not before what was asked for last), up to the block's end; runs have `run`
+    // units.  Where tiles have several units and the run begins inside one, that may be none (t0 == t1).
     __device__ __forceinline__ PagedPiece at(int u, int end, int run, int index) {
         unsigned hit;
 #pragma unroll 1
@@ -120,7 +133,7 @@ struct PagedWalk {
         if (nb_ > 1) {
 #pragma unroll 1
             for (int b0 = 0; b0 < nb_; b0 += 32) {
-                const int t = b0 + lane < nb_ ? tiles(p.n, p.len, b0 + lane) * pl.heads : 0, c = scan(t, lane);
+                const int t = b0 + lane < nb_ ? cost(p.n, p.len, b0 + lane) * pl.heads : 0, c = scan(t, lane);
                 const unsigned in = __ballot_sync(0xffffffffu, c > off);
                 if (in) {
                     const int f = __ffs(in) - 1;
@@ -131,13 +144,15 @@ struct PagedWalk {
             }
         }
         const int all = paged_block(TILE, pg.cap, pl.tb, pl.window, pl.first, p.n, p.len, p.b, p.lo, p.hi, p.kt0, p.ns);
-        if (off >= all) p.head = off / all, off -= p.head * all;
-        const int n_tiles = min(all - off, end - u);
-        p.t0 = p.kt0 - p.ns + off, p.t1 = p.t0 + n_tiles;
-        p.whole = n_tiles == all;
+        const int w = worth(p.n, p.b), span = (all << w) + block();
+        if (off >= span) p.head = off / span, off -= p.head * span;
+        took = min(span - off, end - u);
+        const int t0 = below(off, w), t1 = below(off + took, w);
+        p.t0 = p.kt0 - p.ns + t0, p.t1 = p.kt0 - p.ns + t1;
+        p.whole = t1 - t0 == all;
         p.first = p.last = 0;
-        // a division where the block begins or ends in another run
-        if (!p.whole) p.first = off == 0 ? index : (u - off) / run, p.last = off + n_tiles == all ? index : (u - off + all - 1) / run;
+        // a division where the block begins or its last tile does in another run
+        if (!p.whole) p.first = off == 0 ? index : (u - off) / run, p.last = t1 == all ? index : (u - off + (all - 1 << w) + (all > 1 ? block() : 0)) / run;
         return p;
     }
 };
@@ -147,22 +162,22 @@ constexpr int kPieceSlots = 4;
 struct PagedQueue {  // shared memory
     PagedPiece piece[kPieceSlots];
     uint64_t full[kPieceSlots], empty[kPieceSlots];
-    int s_sum[256];  // tiles of every 32 sequences, from 33 on
+    int s_sum[256];  // units of every 32 sequences, from 33 on
     __device__ __forceinline__ void init(int readers) {  // one thread
         for (int i = 0; i < kPieceSlots; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], readers);
     }
 };
 // Works the pieces of run `index` out.  From 33 sequences on all warps of the CTA count first, and meet behind it.
-template <int TILE>
+template <int TILE, class Units = EqualTiles>
 struct PagedPlanner {
-    PagedWalk<TILE> walk;
+    PagedWalk<TILE, Units> walk;
     int u = 0, u0 = 0, u1 = 0, run = 1;
     uint32_t i = 0;
     bool more = true;
     PagedPiece pc;
     __device__ __forceinline__ PagedPlanner(const KfPaged& pg, const PagedPlan& pl, int lane) : walk(pg, pl, lane) {}
     static __device__ __noinline__ void count(const KfPaged& pg, const PagedPlan& pl, int* s_sum, int warp, int warps, int lane) {
-        PagedWalk<TILE> walk(pg, pl, lane);
+        PagedWalk<TILE, Units> walk(pg, pl, lane);
 #pragma unroll 1
         for (int w = warp; w < (pg.n_seq + 31) / 32; w += warps) {
             walk.load(w * 32);
@@ -172,13 +187,19 @@ struct PagedPlanner {
     __device__ __forceinline__ void start(const PagedQueue& qu, int index) {
         int W = 0;
         if (walk.pg.n_seq <= 32) {
-            walk.load(0);
-            W = walk.total();
+            walk.equal = true;
+#pragma unroll 1
+            while (true) {
+                walk.load(0);
+                W = walk.total();
+                if (Units::kMost == 1 || !walk.equal || W <= Units::kFew * walk.pl.runs) break;
+                walk.equal = false;
+            }
         } else {
             for (int w = walk.lane; w < (walk.pg.n_seq + 31) / 32; w += 32) W += qu.s_sum[w];
             W = __reduce_add_sync(0xffffffffu, W);
         }
-        run = max(1, (W + walk.pl.runs - 1) / walk.pl.runs);
+        run = max(Units::kMost == 1 || walk.equal ? 1 : Units::kMost + Units::kBlock, (W + walk.pl.runs - 1) / walk.pl.runs);  // a run inside a block has a tile that begins in it
         u = u0 = (int)min((long long)W, (long long)index * run), u1 = min(W, u + run);
         if (u < u1 && walk.pg.n_seq > 32) walk.seek(qu.s_sum, u);
         pc.last = 0;
@@ -189,9 +210,14 @@ struct PagedPlanner {
         if (!more) return false;
         more = u < u1;
         if (more) {
-            pc = walk.at(u, u1, run, index);
-            u += pc.t1 - pc.t0;
-        } else {
+            pc = walk.at(u, u1, run, index), u += walk.took;
+            if (Units::kMost > 1 && pc.t0 == pc.t1) {  // the rest of a tile that began in the run before
+                more = u < u1;
+                if (more) pc = walk.at(u, u1, run, index), u += walk.took;
+                else pc.last = 0;
+            }
+        }
+        if (!more) {
             if (rec && walk.lane == 0) {
                 if (u0 == u1 || pc.whole || pc.first != index || pc.last == index) pc.last = 0;
                 rec[index] = pc;

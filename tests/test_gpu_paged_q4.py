@@ -364,6 +364,19 @@ def test_mixed_runs(ctx, hd, group, kv, window, first, seed):
     Step(new, length, group * kv, kv, hd, 16, seed=seed).check(ctx, window=window, first=first)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window,first", [(0, 0), (700, 5)])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_long_mixed_runs(ctx, hd, window, first, seed):
+    """Many tiles a thread block: blocks with one and with two row tiles and single tokens, whose tiles are worth one or two units, so that runs begin and end inside tiles."""
+    r = np.random.RandomState(100 * hd + seed)
+    new = [int(x) for x in r.choice([1, 1, 2, 5, 20, 33, 70, 150], 14)] + [0, 1]
+    length = [n + int(r.randint(0, 7000)) for n in new]
+    s = Step(new, length, 8 * (4 if seed else 7), 8, hd, 64, seed=seed, pad=1)
+    assert sum(-(-n // 128) for n in length) * 8 > 4 * 148 and 8 * 4 * 2 > 16
+    s.check(ctx, window=window, first=first, max_q=150)
+
+
 def test_chunks_before_the_first_position(ctx):
     """More new tokens than positions: the first rows stand before position 0 and see nothing."""
     s = Step([20, 40], [8, 33], 4, 1, 128, 8, seed=4)
