@@ -12,10 +12,10 @@
 //   warp 10          the pieces
 //   warps 11-14      expansion: a unit of 8 positions at a time, K of a tile before V of it
 // Rows of V that no row of the block sees, or whose page is not there, are written as zeros.
-// What bounds it: the chains' way, as in attn_paged_tc.cu, and beside it instructions (2048 tokens behind 8192, 32 / 8 heads: 288 us with nothing stored by the expanding warps, 333 in all, 850
-// TFLOP/s in a steady run under the power cap, 363 us; bf16 335); where a tile has few rows, the expanding warps and shared memory (16 sequences of 500 .. 5000 positions with five drafted
-// tokens of 40 / 8 heads 61 us: a tile takes 2700 clocks, of which the matrix operands read 770 and the expansion 880 out of and into shared memory; eight or eleven expanding
-// warps there make no difference, five instead of four beside many rows 360 against 342 us).  A tile of K ahead of the V before it: 434 us.  Denominators add the weights before their
+// What bounds it: the chains' way, as in attn_paged_tc.cu, and beside it instructions (2048 tokens behind 8192, 32 / 8 heads: 288 us with nothing stored by the expanding warps where 333 were taken in all, 326 now; 860
+// TFLOP/s in a steady run under the power cap, 359 us; bf16 335); where a tile has few rows, the expanding warps and shared memory (16 sequences of 500 .. 5000 positions with five drafted
+// tokens of 40 / 8 heads 57 us: a tile takes 1.85 us, K 0.64 of them, V 0.70 and where the softmax runs on the same scheduler 0.90; the matrix operands read 770 clocks' worth of shared
+// memory, the expansion 880; five, eight or eleven expanding warps make no difference there, five beside many rows 360 against 342 us).  A tile of K ahead of the V before it: 434 us.  Denominators add the weights before their
 // rounding (with it, as the bf16 kernel has them: 392 against 342 us for two more instructions a pair).  Keys, values and weights are rounded to bf16 each, the roundings that reading the
 // pages as bf16 and attending the result would have: 4.0e-3 of the result's norm from the formula in 64 bits, of which the result's own rounding is 1.7e-3 (16 rows and fewer, where
 // only weights are rounded, 2.3e-3).  With fp16 operands, tiles and rows of q brought into its range by powers of two that another warp finds: 496 against 366 us, drafts 91 against 61.
