@@ -18,7 +18,8 @@
 // memory, the expansion 880; five, eight or eleven expanding warps make no difference there, five beside many rows 360 against 342 us).  A tile of K ahead of the V before it: 434 us.  Denominators add the weights before their
 // rounding (with it, as the bf16 kernel has them: 392 against 342 us for two more instructions a pair).  Keys, values and weights are rounded to bf16 each, the roundings that reading the
 // pages as bf16 and attending the result would have: 4.0e-3 of the result's norm from the formula in 64 bits, of which the result's own rounding is 1.7e-3 (16 rows and fewer, where
-// only weights are rounded, 2.3e-3).  With fp16 operands, tiles and rows of q brought into its range by powers of two that another warp finds: 496 against 366 us, drafts 91 against 61.
+// only weights are rounded, 2.3e-3).  With fp16 operands, tiles and rows of q brought into its range by powers of two that another warp finds: 496 against 366 us, drafts 91 against 61;
+// with keys and q alone in fp16, the powers found by the expanding warps: 384 against 326 and 72 against 57.
 // Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
 #include <algorithm>
 
