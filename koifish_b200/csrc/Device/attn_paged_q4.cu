@@ -61,6 +61,13 @@ __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
         w[0] = v.x, w[1] = v.y;
     } else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
+// a pair of zeros times 2^-kZeroLog2: the zeros' sums, of weights of up to 2^68 times values of up to 2^50, stay within 32 bits' range over any number of positions
+constexpr int kZeroLog2 = 24;
+__device__ __forceinline__ uint32_t smaller(uint32_t zeros) {
+    constexpr uint32_t f = (127u - kZeroLog2) << 7;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(zeros) : "r"(zeros), "r"(f << 16 | f));
+    return zeros;
+}
 __device__ __forceinline__ float half_of(uint32_t w, int h) { return h ? bf16hi(w) : bf16lo(w); }
 // pairs of codes out of a word: nibbles (0, 4), (1, 5), (2, 6), (3, 7); the second and the fourth stand for 16 times their codes
 __device__ __forceinline__ void codes(uint32_t w, uint32_t (&c)[4]) { c[0] = w & 0x000f000fu, c[1] = w & 0x00f000f0u, c[2] = (w >> 8) & 0x000f000fu, c[3] = (w >> 8) & 0x00f000f0u; }
@@ -371,7 +378,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
                     for (int e = 0; e < 2; e++) {
                         const uint8_t* u = u0 + (2 * b + e) * UNIT;
                         words(u + un.v_code() + lane * 4 * G, vw[e]), words(u + un.v_step() + g * 2 * G, vs[e]);
-                        vz[e] = *reinterpret_cast<const uint32_t*>(u + un.v_zero() + (g % G) * 16 + t4 * 4);  // positions 2 t4, 2 t4 + 1 of group g
+                        vz[e] = smaller(*reinterpret_cast<const uint32_t*>(u + un.v_zero() + (g % G) * 16 + t4 * 4));  // positions 2 t4, 2 t4 + 1 of group g
                     }
                     if (ragged) {  // what no row sees need not be numbers
 #pragma unroll
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
                 if (g == 0) s_m[warp][r] = m[n][i], s_l[warp][r] = sum * 0x1p-60f;
 #pragma unroll
                 for (int j = 0; j < G; j++) {
-                    const float z = __shfl_sync(0xffffffffu, oz[n][i], j * 4 + t4) * -0x1p-60f;
+                    const float z = __shfl_sync(0xffffffffu, oz[n][i], j * 4 + t4) * -__uint_as_float((127u - 60u + kZeroLog2) << 23);
                     if (r < rows)
                         *reinterpret_cast<float4*>(s_o + ((size_t)warp * rb + r) * HD + 32 * j + 4 * g) =
                             make_float4(fmaf(o[n][j][0][i], 0x1p73f, z), fmaf(o[n][j][0][2 + i], 0x1p69f, z), fmaf(o[n][j][1][i], 0x1p73f, z), fmaf(o[n][j][1][2 + i], 0x1p69f, z));

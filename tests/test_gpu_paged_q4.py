@@ -969,3 +969,30 @@ def test_timed_calls_on_another_stream():
                 side.synchronize()
                 assert all(torch.equal(a, b) for a, b in zip(want, got))
         torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------------------------------------- the ends of what is allowed, in every kernel
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads", [8, 96])
+def test_long_sums_of_large_values(ctx, hd, heads):
+    """Values just below 2^50 whose zeros are some 2000 steps away, over a long sequence whose scores grow by less than what sums are rescaled for: weights of up to 2^7.75, 4096 of them
+    a warp.  Sequences that share their pages, more of them than there are teams of thread blocks, so that one block has a whole one."""
+    n, kv = 16384, 8
+    s = Step([1], [n], heads, kv, hd, 64, seed=heads)
+    n_seq = 60
+    t = torch.arange(n, device="cuda")
+    e, r = torch.from_numpy(s.table[0]).cuda()[t // 64], t % 64
+    codes, step, zero = read(s.pages, kv, hd, 64, 0, e, r)
+    codes[:] = 0
+    codes[128:, :, 0] = 5
+    s.put(0, e, r, codes, torch.ones_like(step).bfloat16(), torch.zeros_like(zero).bfloat16())
+    codes, step, zero = read(s.pages, kv, hd, 64, 1, e, r)
+    s.put(1, e, r, codes, torch.full_like(step, 2.0 ** 39).bfloat16(), torch.full_like(zero, -2000.0).bfloat16())
+    assert float(s.v.abs().max()) < 2.0 ** 50
+    s.new, s.length, s.rows, s.table = [1] * n_seq, [n] * n_seq, n_seq, np.repeat(s.table, n_seq, 0)
+    s.start = list(range(n_seq + 1))
+    s.q = torch.zeros(n_seq, heads * hd, device="cuda", dtype=torch.bfloat16)
+    s.q[:, ::hd] = 1
+    s.d = [i32(np.where(s.table > 2 ** 31 - 1, 0, s.table)), i32(s.start), i32(s.length)]
+    s.desc = s.describe()
+    s.check(ctx, scale=7.75 / (5 * math.log2(math.e)))
