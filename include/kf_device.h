@@ -281,8 +281,8 @@ int kf_paged_attention(kf_ctx* ctx, const kf_paged_kv* kv, void* out_dev, int ld
  *      row are a group with a step and a zero in bf16; a code c of 0 .. 15 stands for step * (c - zero):
  *        step = max((max - min) / 15, max |x| / 2048), rounded up to bf16; zero = -min / step, rounded to bf16 (0 where step is 0);
  *        c = x / step + zero, rounded to the nearest whole number (ties to even) and kept to 0 .. 15; all in fp32.
- *      So x comes back within step * (1/2 + |zero| / 256).  A group with an entry that is not finite comes back as NaN.  The attention is meant for keys, values and
- *      queries below 2^50.
+ *      So x comes back within step * (1/2 + |zero| / 256).  A group with an entry or a range (max - min, in fp32) that is not finite comes back as NaN.  The attention is
+ *      meant for keys, values and queries below 2^50; entries nearer to 0 than 2^-60 lose bits in it.
  *      0.625 bytes an entry, against 2 in bf16.
  *      A page holds for every kv head page_size / 8 units, one behind the other; a unit is 8 positions (10 * head_dim bytes, G = head_dim / 32):
  *        K codes [8][head_dim / 2] bytes | K steps [8][G] | K zeros [8][G] | V codes [8][4][2][head_dim / 16] bytes | V steps [8][G] | V zeros [G][8]   (bf16)

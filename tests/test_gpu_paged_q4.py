@@ -996,3 +996,22 @@ def test_long_sums_of_large_values(ctx, hd, heads):
     s.d = [i32(np.where(s.table > 2 ** 31 - 1, 0, s.table)), i32(s.start), i32(s.length)]
     s.desc = s.describe()
     s.check(ctx, scale=7.75 / (5 * math.log2(math.e)))
+
+
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+def test_append_of_the_largest_ranges(ctx, src):
+    """A group comes back within its bound as long as its range is a number of 32 bits; where the range is none it comes back as NaN, like one with an entry that is not finite."""
+    r = np.random.RandomState(1)
+    x = np.stack([1.69e38 * (2 * r.rand(32) - 1), np.r_[-1.69e38, 1.69e38, np.zeros(30)], 1e38 * (1 + 2 * r.rand(32)), np.r_[1.8e38, -1.8e38, np.zeros(30)]])
+    x = torch.tensor(x, dtype=torch.float32).to(src).cuda()
+    k = x.view(1, 128)
+    s = Step([1], [50], 1, 1, 128, 16, seed=1)
+    kf.paged_append_q4(ctx, s.desc, None, At(s.q if src == torch.bfloat16 else s.q.float()), At(k), At(k), 1, 1, out=At(torch.zeros_like(s.q)), src_f32=src == torch.float32)
+    back = [torch.zeros(1, 128, device="cuda") for _ in "kv"]
+    kf.paged_read_q4(ctx, s.desc, 1, k_out=At(back[0]), v_out=At(back[1]), out_f32=True)
+    torch.cuda.synchronize()
+    c, st, z = quantised(x[:3])
+    for b in back:
+        b = b.view(4, 32)
+        assert torch.all((b[:3].double() - x[:3].double()).abs() <= wide(st).double() * (0.5 + wide(z.abs()).double() / 256 + 2 ** -20))
+        assert torch.all(torch.isnan(b[3]))
