@@ -1015,3 +1015,70 @@ def test_append_of_the_largest_ranges(ctx, src):
         b = b.view(4, 32)
         assert torch.all((b[:3].double() - x[:3].double()).abs() <= wide(st).double() * (0.5 + wide(z.abs()).double() / 256 + 2 ** -20))
         assert torch.all(torch.isnan(b[3]))
+
+
+# heads of a kv head and new tokens of three sequences: 8, 12, 16 and 96 rows of a sequence and kv head
+ROWS = [(4, [1, 2, 1]), (6, [2, 1, 2]), (16, [1, 1, 1]), (24, [1, 4, 2])]
+
+
+def regroup(s, value, change):
+    """Steps and zeros of all cached rows of a Step by change(step, zero)."""
+    for i, n in enumerate(s.length):
+        t = torch.arange(n, device="cuda")
+        e, r = torch.from_numpy(s.table[i]).cuda()[t // s.page], t % s.page
+        codes, step, zero = read(s.pages, s.kv, s.hd, s.page, value, e, r)
+        s.put(value, e, r, codes, *(x.bfloat16() for x in change(step, zero)))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group,new", ROWS)
+def test_zeros_far_from_the_codes_in_every_kernel(ctx, hd, group, new):
+    """Zeros of hundreds of steps of both signs, a group beside the next."""
+    s = Step(new, [200, 60, 333], 2 * group, 2, hd, 16, seed=group + hd)
+    far = lambda step, zero: (step / 16, torch.where(torch.arange(hd // 32, device="cuda") % 2 == 1, -600.0, 900.0).expand_as(zero) + 8 * (zero - 7))  # noqa: E731
+    regroup(s, 0, far), regroup(s, 1, far)
+    s.check(ctx)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("key,value", [(-45, -58), (-40, 40), (-20, -20), (20, 44), (44, -40)])
+@pytest.mark.parametrize("group,new", ROWS)
+def test_sizes_of_values_in_every_kernel(ctx, hd, key, value, group, new):
+    """Steps from very small to very large, of keys against queries of the inverse size, and of values: entries of 2^-60 .. 2^50."""
+    s = Step(new, [300, 77, 130], 2 * group, 2, hd, 16, seed=group + hd)
+    regroup(s, 0, lambda step, zero: (step * 2.0 ** key, zero)), regroup(s, 1, lambda step, zero: (step * 2.0 ** value, zero))
+    s.q = (s.q.float() * 2.0 ** -key).bfloat16()
+    assert max(float(x.abs().max()) for x in (s.k, s.v, torch.nan_to_num(s.q.float()))) < 2.0 ** 50
+    s.check(ctx)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("max_q", [None, 0, 40])
+@pytest.mark.parametrize("group,new", ROWS)
+def test_how_near_the_result_is(ctx, hd, group, new, max_q):
+    """The roundings' errors are independent, so on the whole their squares add up.  Half a step of bf16 at most is 2^-8 / sqrt(3) = 2.26e-3 in the mean square where a number's bits are 1.0 ..,
+    and 1 / sqrt(E m^2) of that, 1.5e-3 .. 1.7e-3, over numbers of all sizes.  Few rows: the result and weight times step, 2.3e-3.  Many rows: the result, weights and values, 1.7e-3 each, and
+    keys, which change a score by 1.6e-3 of scale * sqrt(sum q^2 k^2) = 1.3 * 1.2 here, 2.5e-3: 3.9e-3.  Half as much again is allowed."""
+    s = Step(new, [700, 1000, 333], 2 * group, 2, hd, 16, seed=group + hd)
+    rows = max(max(new) if max_q is None else max_q, 1) * group
+    out = s.attend(ctx, hd ** -0.5, max_q=max_q)
+    ctx.sync()
+    ref, _ = s.expect(hd ** -0.5, 0)
+    assert float((out.double() - ref).norm() / ref.norm()) < (6e-3 if rows > 16 else 3.5e-3)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_seq,active,kv,past,few", [(33, 33, 2, 200, True), (40, 40, 4, 100, True), (1100, 60, 2, 250, True), (8192, 70, 2, 300, True), (200, 200, 4, 250, False), (8192, 300, 3, 300, False)])
+@pytest.mark.parametrize("window,first", [(0, 0), (60, 5)])
+def test_few_tiles_of_many_sequences(ctx, hd, n_seq, active, kv, past, few, window, first):
+    """More than 32 sequences with up to four tiles a thread block and with more: chunks of one and of two row tiles, drafts, single tokens, idle slots between them."""
+    r = np.random.RandomState(n_seq + active)
+    new = np.zeros(n_seq, dtype=int)
+    at = np.sort(r.choice(n_seq, active, replace=False))
+    new[at] = r.choice([1, 1, 1, 5, 20, 33, 90], active)
+    new[at[0]] = new[at[-1]] = 90
+    length = new + r.randint(0, past if n_seq < 1000 else 30, n_seq)
+    length[at] = new[at] + r.randint(0, past, active)
+    tiles = sum(-(-(e - n + min(n, b + 64)) // 128) for n, e in zip(new.tolist(), length.tolist()) for b in range(0, n, 64)) * kv  # 64 tokens of 4 heads are two row tiles
+    assert (tiles <= 4 * torch.cuda.get_device_properties(0).multi_processor_count) == few
+    Step(new, length, 4 * kv, kv, hd, 16, seed=active, pad=1).check(ctx, window=window, first=first)
