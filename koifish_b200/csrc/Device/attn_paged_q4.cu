@@ -30,10 +30,6 @@ namespace {
 constexpr int kWarps = 4, kSub = 2, kTok = 16 * kSub * kWarps, kMaxStages = 12;
 constexpr float kSlack = 8.f;  // growth of a maximum, log2, that sums are not rescaled for
 
-// bytes from global into shared memory, both at 16 bytes, a multiple of 16
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -50,17 +46,6 @@ __device__ __forceinline__ void mma_new(float (&c)[4], const uint32_t (&a)[4], u
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-// N words of shared memory, aligned to as many (up to four)
-template <int N>
-__device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
-    if constexpr (N == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x, w[1] = v.y;
-    } else w[0] = *reinterpret_cast<const uint32_t*>(p);
-}
 // a pair of zeros times 2^-kZeroLog2: the zeros' sums, of weights of up to 2^68 times values of up to 2^50, stay within 32 bits' range over any number of positions
 constexpr int kZeroLog2 = 24;
 __device__ __forceinline__ uint32_t smaller(uint32_t zeros) {
@@ -68,7 +53,6 @@ __device__ __forceinline__ uint32_t smaller(uint32_t zeros) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(zeros) : "r"(zeros), "r"(f << 16 | f));
     return zeros;
 }
-__device__ __forceinline__ float half_of(uint32_t w, int h) { return h ? bf16hi(w) : bf16lo(w); }
 // pairs of codes out of a word: nibbles (0, 4), (1, 5), (2, 6), (3, 7); the second and the fourth stand for 16 times their codes
 __device__ __forceinline__ void codes(uint32_t w, uint32_t (&c)[4]) { c[0] = w & 0x000f000fu, c[1] = w & 0x00f000f0u, c[2] = (w >> 8) & 0x000f000fu, c[3] = (w >> 8) & 0x00f000f0u; }
 

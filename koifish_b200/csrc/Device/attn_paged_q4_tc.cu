@@ -47,20 +47,6 @@ struct Q4TcArgs {  // kernel parameter
     const uint8_t* pool;
     long long page_stride;
 };
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
-    if constexpr (N == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x, w[1] = v.y;
-    } else w[0] = *reinterpret_cast<const uint32_t*>(p);
-}
-__device__ __forceinline__ float half_of(uint32_t w, int h) { return h ? bf16hi(w) : bf16lo(w); }
 // Keys or values of a unit and eight rows of a tile.  A lane takes the codes of one row that stand for eight dims of every group, as one word each: K dims 32 j + 8 t .. + 7, which it stores as
 // 16 bytes, V dims 32 j + 4 t .. + 3 and 32 j + 16 + 4 t .. + 3, half words of two words in the unit, stored as 8 bytes each.  Lanes of four are rows 0, 4, 2, 6, 1, 5, 3, 7: those that store
 // together meet all 32 banks.  The code is small for a reason: with two units unrolled beside one another, instructions had to be fetched again and again (2048 tokens behind 8192: 478 us

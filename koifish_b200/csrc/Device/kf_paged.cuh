@@ -42,6 +42,18 @@ __device__ __forceinline__ KfPaged behind_wait(KfPaged p) {
     p.table = behind_wait(p.table), p.q_start = behind_wait(p.q_start), p.len = behind_wait(p.len);
     return p;
 }
+// N words, aligned to as many (up to four)
+template <int N>
+__device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else w[0] = *reinterpret_cast<const uint32_t*>(p);
+}
+__device__ __forceinline__ float half_of(uint32_t w, int h) { return h ? bf16hi(w) : bf16lo(w); }
 // page of position p >= 0 of sequence s, -1: not there; row: of the position in its page
 __device__ __forceinline__ int paged_page(const KfPaged& pg, int s, int p, int& row) {
     const int c = (int)(__umulhi((uint32_t)p, pg.page_mul) >> pg.page_shift);

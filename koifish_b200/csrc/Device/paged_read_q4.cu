@@ -33,16 +33,6 @@ __device__ __forceinline__ void put4(float* p, float2 a, float2 b) {
     if (VEC) *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
     else p[0] = a.x, p[1] = a.y, p[2] = b.x, p[3] = b.y;
 }
-template <int N>
-__device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
-    if constexpr (N == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x, w[1] = v.y;
-    } else w[0] = *reinterpret_cast<const uint32_t*>(p);
-}
 
 // VEC: rows of the results are aligned to four entries
 template <int HD, typename Y, bool VEC>
