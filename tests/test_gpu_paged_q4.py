@@ -1082,3 +1082,27 @@ def test_few_tiles_of_many_sequences(ctx, hd, n_seq, active, kv, past, few, wind
     tiles = sum(-(-(e - n + min(n, b + 64)) // 128) for n, e in zip(new.tolist(), length.tolist()) for b in range(0, n, 64)) * kv  # 64 tokens of 4 heads are two row tiles
     assert (tiles <= 4 * torch.cuda.get_device_properties(0).multi_processor_count) == few
     Step(new, length, 4 * kv, kv, hd, 16, seed=active, pad=1).check(ctx, window=window, first=first)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [[1, 1, 2], [1, 40, 3]])
+def test_more_kv_heads_than_thread_blocks(ctx, hd, new):
+    """300 kv heads: one team of thread blocks in the kernel for few rows, runs of several heads of a sequence in the other."""
+    Step(new, [200, 77, 140], 300, 300, hd, 16, seed=hd).check(ctx)
+    Step(new, [200, 77, 140], 900, 300, hd, 8, seed=hd + 1).check(ctx, window=50, first=3, max_q=40)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("max_q", [2, 3, 40])
+def test_a_query_that_is_not_finite(ctx, hd, max_q):
+    """It makes the result of its own row and head NaN and nobody else's."""
+    s = Step([3, 1, 2], [90, 61, 20], 8, 2, hd, 16, seed=9)
+    bad = torch.zeros(6, 8, device="cuda", dtype=torch.bool)
+    for row, head in ((1, 2), (3, 7), (5, 0)):
+        s.q[row, head * hd + 5 * row] = float("nan")
+        bad[row, head] = True
+    out = s.attend(ctx, hd ** -0.5, max_q=max_q)
+    ctx.sync()
+    ref, tol = s.expect(hd ** -0.5, 0, many=max_q * 4 > 16)
+    off = (out.double() - ref).abs().view(6, 8, hd)
+    assert torch.all(torch.isnan(off[bad])) and torch.all(off[~bad] <= tol.view(6, 8, hd)[~bad])
