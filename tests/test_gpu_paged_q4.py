@@ -1106,3 +1106,14 @@ def test_a_query_that_is_not_finite(ctx, hd, max_q):
     ref, tol = s.expect(hd ** -0.5, 0, many=max_q * 4 > 16)
     off = (out.double() - ref).abs().view(6, 8, hd)
     assert torch.all(torch.isnan(off[bad])) and torch.all(off[~bad] <= tol.view(6, 8, hd)[~bad])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("max_q", [1, 2, 4])
+def test_the_nearer_kernel_by_choice(ctx, hd, max_q):
+    """With max_q for at most 16 rows of a sequence and kv head, drafts and chunks have the error of single tokens."""
+    s = Step([1, 30, 5], [700, 1000, 333], 8, 2, hd, 16, seed=hd)
+    out = s.attend(ctx, hd ** -0.5, max_q=max_q)
+    ctx.sync()
+    ref, _ = s.expect(hd ** -0.5, 0)
+    assert float((out.double() - ref).norm() / ref.norm()) < 3.5e-3
