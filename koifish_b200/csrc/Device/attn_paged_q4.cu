@@ -14,11 +14,13 @@
 //     fifth accumulator.
 //   * A warp takes 32 positions (four units) of a tile of 128; a unit is contiguous (Q4Unit), so a tile is a bulk copy per page (or part of 8 .. 128 positions of it).
 //   * A team of n_kv CTAs takes a run of tiles, a kv head each; runs are equal whatever the lengths are (PagedWalk), and a second kernel, launched behind, merges what several share.
-// For up to 16 rows of a sequence and kv head (new tokens x heads of the group); more go to attn_paged_q4_tc.cu, where single rows take longer (64 sequences with 12 heads to a kv head 106
-// us here, 186 there).
-// What bounds it: instructions.  16 positions of 128 dims and 8 rows take a warp 305 of them, 149 on the pipe of logic and shifts, 24 of matrix; beside loads that bring 5.7 TB/s alone
-// (43 us for the 64 sequences of 400 .. 4000 positions, 64 / 8 heads, 196 MB) they run at 3.1 TB/s.  Measured: these 62.6 us in a steady run, one sequence of 100000 positions (128 MB) 38 us, 3.3
-// TB/s, of which 7 are the start, 4 the end and the merge; one of 1300 9.3 us, as long as issuing two launches takes from Python; 40 with a window of 1000 and 4 first positions 28.5.
+// For up to 16 rows of a sequence and kv head (new tokens x heads of the group); more go to attn_paged_q4_tc.cu, where few rows take longer.  64 sequences of 400 .. 4000 positions, one
+// token each, us here / there: 128 dims, up to 8 rows 56 .. 62 / 154, 9 .. 16 rows 105 .. 111 / 154; 64 dims 38 .. 43 and 61 .. 64 / 124.
+// What bounds it: the computing warps' own way.  The 64 sequences (64 / 8 heads, 196 MB) take 62.5 us, 3.1 TB/s; 59.8 with nothing loaded, 45.6 with nothing computed.  16 positions of 128 dims and
+// 8 rows are 307 instructions of a warp, 149 of them on the pipe of logic and shifts, 24 products.  No pipe is full (1.8 instructions a clock of 4, logic 42 %, products 26 %): there are two
+// computing warps to a scheduler, and an instruction waits 1.2 clocks for the one before it and 0.9 for memory and barriers.  One sequence of 100000 positions (128 MB) 38.3 us, 3.3 TB/s (35.6, 30.0), of
+// which 7 are the start, 4 the end and the merge; one of 1300 9.3, as long as issuing two launches takes from Python; 40 with a window of 1000 and 4 first positions 28.7.
+// 9 .. 16 rows of 128 dims do not fit the 168 registers that ten warps on four schedulers leave a thread: 200 bytes of it are spilled; the other instances spill nothing.
 // Not kept: three CTAs per SM (62 us, and more pieces to merge: 42 for the one of 100000), one of eight computing warps (80 and 47), the merge by the CTA that arrives last (44 for the one of 100000:
 // a fence, an atomic and rounds of loads one behind the other).
 #include <algorithm>
@@ -444,8 +446,8 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, OCC)
     }
 }
 
-// Blocks that several CTAs share (256 threads for two rows: 39.6 us for the sequence of 100000 positions, 128 for one: 39.3; 512 for all: 40.2): thread block (n, y) takes rows kMergeRows y .. of the one that begins in run n and goes on behind it, if there is one.  A row's pieces are spread over as many
-// warps as there are for it, kAt on their way for each; these meet in order.
+// Blocks that several CTAs share: thread block (n, y) takes rows kMergeRows y .. of the one that begins in run n and goes on behind it, if there is one.  A row's pieces are spread over as many
+// warps as there are for it, kAt on their way for each; these meet in order.  One row to 128 threads: 39.3 us for the sequence of 100000 positions; two rows to 256 39.6, all rows to 512 40.2.
 constexpr int kMergeWarps = 4, kMergeRows = 1;
 template <int HD>
 __global__ void __launch_bounds__(kMergeWarps * 32) kf_attn_paged_q4_merge_kernel(const __grid_constant__ PagedPlan pl, const __grid_constant__ Q4Args a) {

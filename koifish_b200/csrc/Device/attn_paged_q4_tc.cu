@@ -12,14 +12,15 @@
 //   warp 10          the pieces
 //   warps 11-14      expansion: a unit of 8 positions at a time, K of a tile before V of it
 // Rows of V that no row of the block sees, or whose page is not there, are written as zeros.
-// What bounds it: the chains' way, as in attn_paged_tc.cu, and beside it instructions (2048 tokens behind 8192, 32 / 8 heads: 288 us with nothing stored by the expanding warps where 333 were taken in all, 326 now; 860
-// TFLOP/s in a steady run under the power cap, 359 us; bf16 335); where a tile has few rows, the expanding warps and shared memory (16 sequences of 500 .. 5000 positions with five drafted
-// tokens of 40 / 8 heads 57 us: a tile takes 1.85 us, K 0.64 of them, V 0.70 and where the softmax runs on the same scheduler 0.90; the matrix operands read 770 clocks' worth of shared
-// memory, the expansion 880; five, eight or eleven expanding warps make no difference there, five beside many rows 360 against 342 us).  A tile of K ahead of the V before it: 434 us.  Denominators add the weights before their
-// rounding (with it, as the bf16 kernel has them: 392 against 342 us for two more instructions a pair).  Keys, values and weights are rounded to bf16 each, the roundings that reading the
-// pages as bf16 and attending the result would have: 4.0e-3 of the result's norm from the formula in 64 bits, of which the result's own rounding is 1.7e-3 (16 rows and fewer, where
-// only weights are rounded, 2.3e-3).  With fp16 operands, tiles and rows of q brought into its range by powers of two that another warp finds: 496 against 366 us, drafts 91 against 61;
-// with keys and q alone in fp16, the powers found by the expanding warps: 384 against 326 and 72 against 57.
+// Roundings: keys, values and weights to bf16 each, the roundings that reading the pages as bf16 and attending the result would have; denominators add the weights before their rounding (the
+// rounded ones, as the bf16 kernel has them: 392 against 342 us for two more instructions a pair).  4.0e-3 of the result's norm from the formula in 64 bits, of which the result's own rounding is 1.7e-3
+// (attn_paged_q4.cu, where only weights times steps are rounded, 2.3e-3).  fp16 operands would be nearer, but have to be brought into range by powers of two: found for whole tiles by another
+// warp 496 against 366 us, drafts 91 against 61; for keys and q alone, found by the expanding warps, 384 against 326 and 72 against 57.
+// What bounds it: the chains' way, as in attn_paged_tc.cu, and the expansion beside it.
+//   * 2048 tokens behind 8192, 32 / 8 heads: 324 us, 870 TFLOP/s in a steady run under the power cap (354 us; bf16 335); 45 us less with nothing stored by the expanding warps.  A fifth of these 360
+//     against 342 us, a tile of K ahead of the V before it 434.
+//   * Where a tile has few rows, expansion and shared memory: 16 sequences of 500 .. 5000 positions with five drafted tokens of 40 / 8 heads 57 us, 1.85 a tile (K 0.64, V 0.70, 0.90 where the softmax
+//     runs on the same scheduler).  The matrix operands read 770 clocks' worth of shared memory, the expansion 880; five, eight or eleven expanding warps make no difference there.
 // Every wait is bounded: when one runs out, `dead` ends all roles, copies and matrix instructions in flight are awaited and tensor memory is freed.
 #include <algorithm>
 
@@ -37,7 +38,9 @@ struct Cfg {
 // What the runs are equal in.  A step of a block whose chains share their tiles (2.2 .. 2.7 us) is near two tiles of one whose chains take turns (1.6 .. 1.9 each), and what a block
 // takes beside its tiles, queries, first scores and sums, is about as much (3.7 us): 16 sequences with five drafted tokens 57.3 us, 62.1 with runs equal in tiles, 24 sequences with
 // three chunks and 64 dims 51.3 and 55.1.  A run must then be four units or more, which costs more than it gives where there are few tiles for all CTAs: 300 tokens of one
-// sequence alone 20.3 us, 28.5 by units.
+// sequence alone 20.3 us, 28.5 by units.  From 33 sequences on it is units in any case: how many tiles there are is known only behind the count, which adds up units, and counting both costs every
+// step of many sequences 1 .. 5 us (40 x 60 tokens behind 100 .. 600 of 64 / 8 heads 110 us, 115.6).  That is the worse choice for few tiles of like blocks (in tiles / by units: 40 x 5 tokens behind
+// 100 .. 250 of 40 / 8 heads 27.4 / 35.6, 33 x 30 behind 200 .. 500 of 16 / 4 29.3 / 32.0) and the better one where single tokens lie between them (27.9 / 25.7) or tiles are more (64 x 5 53.1 / 51.0).
 struct ChainTiles {
     static constexpr int kMost = 2, kBlock = 2, kFew = 4;
     static __device__ __forceinline__ int tile(int left, int tb) { return left > tb / 2; }

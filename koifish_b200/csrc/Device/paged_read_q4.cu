@@ -5,7 +5,7 @@
 // Every byte is read once and every entry written once, so HBM bounds it, and instructions are not far.  A warp takes eight positions that lie side by side in the panel, four lanes a row, and one of
 // K and V of one head at a time: a unit, where the positions are one, in whole.  A lane has one word of eight codes for every group.  A code at bits 16 .. 19 of a word is the fp32 number
 // code * 2^-133, at bits 20 .. 23 code * 2^-129 (subnormal numbers and the first normal ones are one ladder): a shift and an AND take the place of a conversion, and the multiply-add that brings
-// it back to size takes the zero off with the rounding of code - zero.  Measured: 50000 positions of 8 heads of 128 (64 MB of codes, 205 MB of rows) 52 us, 5.3 TB/s, 0.83 of the copy rate;
+// it back to size takes the zero off with the rounding of code - zero.  Measured: 52184 positions of 8 heads of 128 (67 MB of codes, 214 MB of rows) 51.6 us, 5.4 TB/s, 0.84 of the copy rate;
 // with conversions, a row a turn and sixteen tokens a block 80 us.
 #include <algorithm>
 
